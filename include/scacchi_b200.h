@@ -499,6 +499,45 @@ int scacchi_loss_input(const scacchi_loss_frames *frames, const scacchi_loss_out
                        int32_t legacy_reduction, void *stream);
 uint64_t scacchi_target_launch_count(void);
 
+/* ---- training operators after the loss input ---------------------------- */
+
+/* Rows of a clipped policy loss.  logits and reference_logits hold
+ * num_actions elements a row, rows `*_stride` elements apart; the others are
+ * dense.  At most one of reference_logits and reference_log_prob. */
+typedef struct {
+  const void *logits;                  /* [rows, actions] of `dtype` */
+  const void *reference_logits;        /* like logits, or NULL: the KL over the whole row */
+  const uint8_t *legal;                /* [rows, actions], or NULL: every action */
+  const int32_t *action;               /* [rows] */
+  const float *old_log_prob;           /* [rows] behaviour log-probability of `action` */
+  const float *advantage;              /* [rows] */
+  const float *weight;                 /* [rows] share of the loss, or NULL: 1 / rows */
+  const float *reference_log_prob;     /* [rows], or NULL: the KL estimated at `action` */
+  int64_t logits_stride, reference_stride;
+} scacchi_policy_rows;
+
+typedef struct {
+  float *loss;                         /* [1] */
+  float *log_prob;                     /* [rows] */
+  float *kl;                           /* [rows], or NULL where no reference is given */
+  uint8_t *clipped;                    /* [rows] 1 where the clip stops the surrogate's gradient */
+  void *grad_logits;                   /* dense [rows, actions] of `dtype`, or NULL: the loss alone */
+} scacchi_policy_out;
+
+/* loss = sum_i weight_i (-min(ratio A, clip(ratio, 1 - clip_low, 1 +
+ * clip_high) A) + kl_coefficient KL_i) over the legal actions, and its
+ * gradient in the logits.  dtype: 0 float32, 1 bfloat16, 2 float16;
+ * 1 <= num_actions <= 262144.  A row that does not count (weight 0, an
+ * action out of range, illegal or with a logit of -inf) adds nothing: its
+ * statistics and its gradient are 0, and with weight 0 its logits are not
+ * read.  workspace: scacchi_policy_loss_workspace_bytes() bytes, 8-byte
+ * aligned, of this call alone. */
+size_t scacchi_policy_loss_workspace_bytes(void);
+int scacchi_policy_loss(const scacchi_policy_rows *rows, const scacchi_policy_out *out, int64_t num_rows,
+                        int32_t num_actions, int32_t dtype, double clip_low, double clip_high, float kl_coefficient,
+                        void *workspace, void *stream);
+uint64_t scacchi_policy_loss_launch_count(void);
+
 /* ---- host-side jax.random key helpers (no device work) ---------------- */
 
 /* search.py:207-209 key chain: for i < num_simulations,

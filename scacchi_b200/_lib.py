@@ -73,6 +73,16 @@ class LossOut(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in FIELDS]
 
 
+class PolicyRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "reference_logits", "legal", "action", "old_log_prob",
+                                          "advantage", "weight", "reference_log_prob")] + [
+        ("logits_stride", C.c_int64), ("reference_stride", C.c_int64)]
+
+
+class PolicyOut(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("loss", "log_prob", "kl", "clipped", "grad_logits")]
+
+
 P = C.c_void_p
 I32 = C.c_int32
 F32 = C.c_float
@@ -120,6 +130,10 @@ SIGNATURES = {
     "scacchi_pack_targets": [I32, I32, P, P, P, P, P, I32, I32, P, P, P, P, P, P, P, P, P, P],
     "scacchi_loss_input": [C.POINTER(LossFrames), C.POINTER(LossOut), I32, I32, I32, I32, I32, I32, I32, I32, I32, P],
     "scacchi_target_launch_count": [],
+    "scacchi_policy_loss_workspace_bytes": [],
+    "scacchi_policy_loss": [C.POINTER(PolicyRows), C.POINTER(PolicyOut), C.c_int64, I32, I32, C.c_double, C.c_double,
+                            F32, P, P],
+    "scacchi_policy_loss_launch_count": [],
     "scacchi_tower_timing_read": [P, P],
     "scacchi_device_error": [P],
     "scacchi_launch_count": [],
@@ -127,7 +141,8 @@ SIGNATURES = {
 RESTYPES = {"scacchi_search_workspace_bytes": C.c_size_t, "scacchi_launch_count": C.c_uint64,
             "scacchi_tower_rows": C.c_uint64, "scacchi_tower_workspace_bytes": C.c_size_t,
             "scacchi_tower_launch_count": C.c_uint64, "scacchi_hex_launch_count": C.c_uint64,
-            "scacchi_target_launch_count": C.c_uint64}
+            "scacchi_target_launch_count": C.c_uint64, "scacchi_policy_loss_workspace_bytes": C.c_size_t,
+            "scacchi_policy_loss_launch_count": C.c_uint64}
 
 
 class ScacchiError(RuntimeError):
@@ -168,9 +183,11 @@ def device_error() -> int:
 
 
 def launch_count() -> int:
-    """Kernels this library launched since load (search + network + Hex)."""
+    """Kernels this library launched since load (search, network, Hex, targets and
+    training operators)."""
     return (int(lib().scacchi_launch_count()) + int(lib().scacchi_tower_launch_count())
-            + int(lib().scacchi_hex_launch_count()) + int(lib().scacchi_target_launch_count()))
+            + int(lib().scacchi_hex_launch_count()) + int(lib().scacchi_target_launch_count())
+            + int(lib().scacchi_policy_loss_launch_count()))
 
 
 def tower_error() -> int:
