@@ -538,6 +538,38 @@ int scacchi_policy_loss(const scacchi_policy_rows *rows, const scacchi_policy_ou
                         void *workspace, void *stream);
 uint64_t scacchi_policy_loss_launch_count(void);
 
+/* A stack of `batch` dense [rows, cols] matrices and the Newton-Schulz steps
+ * X <- a X + (b A + c A^2) X, A = X X^T on the narrow side, from
+ * X = U / (|U|_F + eps).  scale_exponent comes from
+ * scacchi_muon_scale_exponent. */
+#define SCACCHI_MUON_MAX_SIDE 131072
+typedef struct {
+  int32_t batch, rows, cols;
+  int32_t dtype;                       /* of the matrix or gradient: 0 float32, 1 bfloat16, 2 float16 */
+  int32_t steps;                       /* 1 to 64 */
+  int32_t scale_exponent;              /* operands are held as fp16 pairs of 2^scale_exponent times their value */
+  double a, b, c, eps;
+} scacchi_newton_schulz;
+
+/* The largest power of two that keeps the operands of these steps within
+ * fp16, or -1 where the steps diverge from singular values in [0, 1]. */
+int32_t scacchi_muon_scale_exponent(double a, double b, double c, int32_t steps);
+size_t scacchi_muon_workspace_bytes(int32_t batch, int32_t rows, int32_t cols);
+
+/* out = the orthogonalised stack, of the matrices' type.  workspace: 256-byte
+ * aligned, of this call alone. */
+int scacchi_orthogonalize(const scacchi_newton_schulz *params, const void *matrix, void *out, void *workspace,
+                          void *stream);
+
+/* Muon's step on float32 weights: momentum <- beta momentum + (1 - beta)
+ * gradient; u = nesterov ? (1 - beta) gradient + beta momentum : momentum;
+ * weight <- decay weight - step orthogonalize(u). */
+int scacchi_muon_update(const scacchi_newton_schulz *params, const void *gradient, float *momentum, float *weight,
+                        double beta, int32_t nesterov, float decay, float step, void *workspace, void *stream);
+/* Sticky flag of a product whose bounded wait ran out; reading clears it. */
+int scacchi_muon_error(uint32_t *flags);
+uint64_t scacchi_muon_launch_count(void);
+
 /* ---- host-side jax.random key helpers (no device work) ---------------- */
 
 /* search.py:207-209 key chain: for i < num_simulations,

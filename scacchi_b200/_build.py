@@ -15,9 +15,9 @@ LIB = os.path.join(HERE, "libscacchi_b200.so")
 # tolerance and keep contraction.
 UNITS = [(os.path.join(CSRC, "search.cu"), ["-fmad=false"]), (os.path.join(CSRC, "tower.cu"), []),
          (os.path.join(CSRC, "hex.cu"), ["-fmad=false"]), (os.path.join(CSRC, "targets.cu"), ["-fmad=false"]),
-         (os.path.join(CSRC, "policy_loss.cu"), [])]
+         (os.path.join(CSRC, "policy_loss.cu"), []), (os.path.join(CSRC, "muon.cu"), [])]
 SOURCES = [u[0] for u in UNITS]
-HEADERS = [os.path.join(CSRC, h) for h in ("smath.h", "threefry.h", "synthetic_env.h", "lane_cta.cuh")] + [
+HEADERS = [os.path.join(CSRC, h) for h in ("smath.h", "threefry.h", "synthetic_env.h", "lane_cta.cuh", "tc05.cuh")] + [
     os.path.join(ROOT, "include", "scacchi_b200.h")]
 
 NVCC_FLAGS = ["-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo"]

@@ -83,6 +83,11 @@ class PolicyOut(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("loss", "log_prob", "kl", "clipped", "grad_logits")]
 
 
+class NewtonSchulz(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "rows", "cols", "dtype", "steps", "scale_exponent")] + [
+        (n, C.c_double) for n in ("a", "b", "c", "eps")]
+
+
 P = C.c_void_p
 I32 = C.c_int32
 F32 = C.c_float
@@ -134,6 +139,12 @@ SIGNATURES = {
     "scacchi_policy_loss": [C.POINTER(PolicyRows), C.POINTER(PolicyOut), C.c_int64, I32, I32, C.c_double, C.c_double,
                             F32, P, P],
     "scacchi_policy_loss_launch_count": [],
+    "scacchi_muon_scale_exponent": [C.c_double, C.c_double, C.c_double, I32],
+    "scacchi_muon_workspace_bytes": [I32, I32, I32],
+    "scacchi_orthogonalize": [C.POINTER(NewtonSchulz), P, P, P, P],
+    "scacchi_muon_update": [C.POINTER(NewtonSchulz), P, P, P, C.c_double, I32, F32, F32, P, P],
+    "scacchi_muon_error": [P],
+    "scacchi_muon_launch_count": [],
     "scacchi_tower_timing_read": [P, P],
     "scacchi_device_error": [P],
     "scacchi_launch_count": [],
@@ -142,7 +153,8 @@ RESTYPES = {"scacchi_search_workspace_bytes": C.c_size_t, "scacchi_launch_count"
             "scacchi_tower_rows": C.c_uint64, "scacchi_tower_workspace_bytes": C.c_size_t,
             "scacchi_tower_launch_count": C.c_uint64, "scacchi_hex_launch_count": C.c_uint64,
             "scacchi_target_launch_count": C.c_uint64, "scacchi_policy_loss_workspace_bytes": C.c_size_t,
-            "scacchi_policy_loss_launch_count": C.c_uint64}
+            "scacchi_policy_loss_launch_count": C.c_uint64, "scacchi_muon_workspace_bytes": C.c_size_t,
+            "scacchi_muon_scale_exponent": C.c_int32, "scacchi_muon_launch_count": C.c_uint64}
 
 
 class ScacchiError(RuntimeError):
@@ -187,10 +199,16 @@ def launch_count() -> int:
     training operators)."""
     return (int(lib().scacchi_launch_count()) + int(lib().scacchi_tower_launch_count())
             + int(lib().scacchi_hex_launch_count()) + int(lib().scacchi_target_launch_count())
-            + int(lib().scacchi_policy_loss_launch_count()))
+            + int(lib().scacchi_policy_loss_launch_count()) + int(lib().scacchi_muon_launch_count()))
 
 
 def tower_error() -> int:
     flags = C.c_uint32(0)
     check(lib().scacchi_tower_error(C.byref(flags)), "scacchi_tower_error")
+    return int(flags.value)
+
+
+def muon_error() -> int:
+    flags = C.c_uint32(0)
+    check(lib().scacchi_muon_error(C.byref(flags)), "scacchi_muon_error")
     return int(flags.value)

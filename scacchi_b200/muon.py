@@ -1,0 +1,140 @@
+"""Muon for the network's matrices: the orthogonalised update and the
+weight's step (the reference trains with Muon and Adam; this is the part
+for matrices).
+
+A weight is a matrix [in, out] as flax stores it: the dense kernels of
+``AZDirichletParams`` as they are, a convolution kernel [3, 3, in, out] as
+its [9 in, out] reshape.  Leading axes stack matrices of one shape, which
+one call updates together.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import math
+
+import torch
+
+from . import _lib
+from .dirichlet_mctx.tree import ptr, stream_handle
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+MAX_SIDE = 131072
+MAX_STACK = 65535
+
+
+@functools.lru_cache(maxsize=64)
+def _scale_exponent(a: float, b: float, c: float, steps: int) -> int:
+    e = int(_lib.lib().scacchi_muon_scale_exponent(a, b, c, steps))
+    if e < 0:
+        raise ValueError(f"coefficients {(a, b, c)} diverge within {steps} steps from singular values in [0, 1]")
+    return e
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(batch: int, rows: int, cols: int) -> int:
+    return int(_lib.lib().scacchi_muon_workspace_bytes(batch, rows, cols))
+
+
+def _params(t: torch.Tensor, name: str, steps: int, coefficients, eps: float) -> _lib.NewtonSchulz:
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on a CUDA device, got {t.device}")
+    if t.dtype not in DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() < 2:
+        raise ValueError(f"{name} must be [..., rows, cols], got {tuple(t.shape)}")
+    rows, cols = t.shape[-2:]
+    batch = math.prod(t.shape[:-2])
+    if not (1 <= rows <= MAX_SIDE and 1 <= cols <= MAX_SIDE) or batch > MAX_STACK:
+        raise ValueError(f"{name} must stack at most {MAX_STACK} matrices with sides of 1 to {MAX_SIDE}, got "
+                         f"{tuple(t.shape)}")
+    if not 1 <= steps <= 64:
+        raise ValueError(f"steps must be in [1, 64], got {steps}")
+    a, b, c = (float(v) for v in coefficients)
+    if not all(math.isfinite(v) for v in (a, b, c)):
+        raise ValueError(f"coefficients must be finite, got {tuple(coefficients)}")
+    if not (0.0 <= eps < math.inf):
+        raise ValueError(f"eps must be finite and >= 0, got {eps}")
+    return _lib.NewtonSchulz(batch, rows, cols, DTYPES[t.dtype], int(steps), _scale_exponent(a, b, c, int(steps)),
+                             a, b, c, float(eps))
+
+
+def orthogonalize(matrix: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
+                  eps: float = 1e-8) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of each matrix of [..., rows, cols].
+
+    X = U / (|U|_F + eps), then ``steps`` times X <- a X + (b A + c A^2) X
+    with A = X X^T on the narrow side; returns X in the input's shape and
+    type (float32, bfloat16 or float16).  The products carry 32-bit
+    accuracy whatever the type, and round once at the end.  A matrix of
+    zeros gives zeros; one with an infinity or a NaN gives NaN, and leaves
+    the others of its stack alone.
+
+    The call launches on the current stream, does not synchronise and can
+    be captured into a CUDA graph.
+    """
+    matrix = matrix.detach()
+    params = _params(matrix, "matrix", steps, coefficients, eps)
+    dev = matrix.device
+    with torch.cuda.device(dev):
+        x = matrix.contiguous()
+        out = torch.empty_like(x)
+        if x.numel():
+            workspace = torch.empty((_workspace_bytes(params.batch, params.rows, params.cols),), dtype=torch.uint8,
+                                    device=dev)
+            _lib.check(_lib.lib().scacchi_orthogonalize(C.byref(params), ptr(x), ptr(out), ptr(workspace),
+                                                        stream_handle(dev)), "orthogonalize")
+    return out
+
+
+def muon_update(weight: torch.Tensor, gradient: torch.Tensor, momentum: torch.Tensor, *, learning_rate: float,
+                beta: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, scale: float | None = None,
+                steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-8) -> None:
+    """Muon's step, in place on ``weight`` and ``momentum``:
+
+        momentum <- beta momentum + (1 - beta) gradient
+        u = (1 - beta) gradient + beta momentum   (nesterov; else momentum)
+        weight <- (1 - learning_rate weight_decay) weight
+                  - learning_rate scale orthogonalize(u)
+
+    ``weight`` and ``momentum`` are contiguous float32 [..., in, out] of one
+    shape (state is kept in 32 bits); ``gradient`` has that shape in
+    float32, bfloat16 or float16.  ``scale`` defaults to
+    sqrt(max(1, out / in)).  The three may not overlap.
+
+    The call launches on the current stream, does not synchronise and can
+    be captured into a CUDA graph.
+    """
+    gradient = gradient.detach()
+    params = _params(gradient, "gradient", steps, coefficients, eps)
+    dev = gradient.device
+    for name, t in (("weight", weight), ("momentum", momentum)):
+        if t.dtype != torch.float32 or t.shape != gradient.shape or t.device != dev:
+            raise ValueError(f"{name} must be float32 {tuple(gradient.shape)} on {dev}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} is updated in place and must be contiguous")
+    g = gradient.contiguous()
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (weight, g, momentum))
+    if weight.numel() and any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("weight, gradient and momentum may not overlap")
+    if not 0.0 <= beta < 1.0:
+        raise ValueError(f"beta must be in [0, 1), got {beta}")
+    if scale is None:
+        scale = math.sqrt(max(1.0, params.cols / params.rows))
+    decay, step = 1.0 - learning_rate * weight_decay, learning_rate * scale
+    if not (math.isfinite(decay) and math.isfinite(step)):
+        raise ValueError(f"learning_rate, weight_decay and scale must be finite, got {learning_rate}, {weight_decay}, "
+                         f"{scale}")
+    if weight.numel() == 0:
+        return
+    with torch.cuda.device(dev):
+        workspace = torch.empty((_workspace_bytes(params.batch, params.rows, params.cols),), dtype=torch.uint8,
+                                device=dev)
+        _lib.check(_lib.lib().scacchi_muon_update(C.byref(params), ptr(g), ptr(momentum), ptr(weight), float(beta),
+                                                  int(bool(nesterov)), decay, step, ptr(workspace),
+                                                  stream_handle(dev)), "muon_update")
+    # a graph recorded before the step refuses to run backward through it
+    torch.autograd.graph.increment_version((weight, momentum))

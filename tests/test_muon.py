@@ -1,0 +1,83 @@
+"""The orthogonalised update and Muon's step refuse what they cannot
+compute, before any launch, and choose the operands' scale (no GPU needed)."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from scacchi_b200 import _lib
+from scacchi_b200.muon import COEFFICIENTS, MAX_SIDE, muon_update, orthogonalize
+
+A = 1 << 20  # a made-up aligned address: a refused call reads none
+
+
+def _params(**kw):
+    d = dict(batch=1, rows=8, cols=8, dtype=0, steps=5, scale_exponent=14, a=3.4445, b=-4.775, c=2.0315, eps=1e-8)
+    d.update(kw)
+    return _lib.NewtonSchulz(**d)
+
+
+BAD = [dict(batch=-1), dict(batch=65536), dict(rows=0), dict(cols=0), dict(rows=MAX_SIDE + 1),
+       dict(cols=MAX_SIDE + 1), dict(dtype=3), dict(dtype=-1), dict(steps=0), dict(steps=65),
+       dict(scale_exponent=-1), dict(scale_exponent=16), dict(a=float("nan")), dict(b=float("inf")),
+       dict(c=float("nan")), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf"))]
+
+
+@pytest.mark.parametrize("kw", BAD, ids=str)
+def test_library_rejects_bad_parameters(kw):
+    lib, p = _lib.lib(), _params(**kw)
+    before = lib.scacchi_muon_launch_count()
+    assert lib.scacchi_orthogonalize(C.byref(p), A, A, A, None) == _lib.EINVAL
+    assert lib.scacchi_muon_update(C.byref(p), A, A, A, 0.9, 1, 1.0, 0.1, A, None) == _lib.EINVAL
+    assert lib.scacchi_muon_launch_count() == before
+
+
+def test_library_rejects_bad_pointers():
+    lib, p, half = _lib.lib(), _params(), _params(dtype=1)
+    for args in ((None, A, A), (A, None, A), (A, A, None), (A + 2, A, A), (A, A + 1, A), (A, A, A + 128)):
+        assert lib.scacchi_orthogonalize(C.byref(p), *args, None) == _lib.EINVAL
+    assert lib.scacchi_orthogonalize(C.byref(half), A + 1, A, A, None) == _lib.EINVAL
+    assert lib.scacchi_orthogonalize(None, A, A, A, None) == _lib.EINVAL
+    for args in ((None, A, A), (A, None, A), (A, A, None), (A, A + 2, A), (A, A, A + 2)):
+        assert lib.scacchi_muon_update(C.byref(p), *args, 0.9, 1, 1.0, 0.1, A, None) == _lib.EINVAL
+    for beta, decay, step in ((1.0, 1.0, 0.1), (-0.1, 1.0, 0.1), (float("nan"), 1.0, 0.1),
+                              (0.9, float("nan"), 0.1), (0.9, 1.0, float("inf"))):
+        assert lib.scacchi_muon_update(C.byref(p), A, A, A, beta, 1, decay, step, A, None) == _lib.EINVAL
+    assert lib.scacchi_muon_update(C.byref(p), A, A, A, 0.9, 1, 1.0, 0.1, None, None) == _lib.EINVAL
+
+
+def test_python_rejects_cpu_tensors():
+    x = torch.zeros((4, 4))
+    with pytest.raises(ValueError, match="CUDA"):
+        orthogonalize(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        muon_update(x, x.clone(), x.clone(), learning_rate=0.1)
+
+
+def test_scale_keeps_operands_in_half_precision():
+    """Largest operand of every step, followed on a finer grid of singular
+    values, stays within fp16 at the scale; a doubled scale would not do or
+    is fp16's own exponent limit."""
+    f = _lib.lib().scacchi_muon_scale_exponent
+    for coefficients, steps in ((COEFFICIENTS, 5), (COEFFICIENTS, 64), ((1.5, -0.5, 0.0), 12), ((2.0, -1.5, 0.5), 9)):
+        e = f(*coefficients, steps)
+        a, b, c = coefficients
+        s = torch.linspace(0, 1, 100003, dtype=torch.float64)
+        most = 1.0
+        for _ in range(steps):
+            p = a + b * s ** 2 + c * s ** 4
+            most = max(most, float(s.abs().max()), float((s ** 2).max()), float(p.abs().max()))
+            s = s * p
+        assert 6 <= e <= 15 and most * 2 ** e < 65504
+        assert e == 15 or 1.11 * most * 2 ** (e + 1) > 65504
+    assert f(30.0, -1.5, 0.5, 5) == -1 and f(3.4445, -4.775, 2.0315, 0) == -1 and f(float("nan"), 0, 0, 5) == -1
+
+
+def test_workspace_size():
+    f = _lib.lib().scacchi_muon_workspace_bytes
+    assert f(0, 4, 4) == 0 and f(1, 0, 4) == 0
+    # two copies of the stack and two of its narrow square as fp16 pairs
+    assert f(12, 1152, 128) >= 12 * (2 * 1152 * 128 + 2 * 128 * 128) * 4
+    assert f(1, 3, 5) % 256 == 0
+    assert f(2, 65536, 65536) > 2 ** 36
