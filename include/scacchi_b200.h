@@ -552,7 +552,8 @@ typedef struct {
 } scacchi_newton_schulz;
 
 /* The largest power of two that keeps the operands of these steps within
- * fp16, or -1 where the steps diverge from singular values in [0, 1]. */
+ * fp16, or -1 where the steps diverge from singular values in [0, 1] or
+ * where 0 < 16 |c| < |b| (the quadratic's square is completed). */
 int32_t scacchi_muon_scale_exponent(double a, double b, double c, int32_t steps);
 size_t scacchi_muon_workspace_bytes(int32_t batch, int32_t rows, int32_t cols);
 

@@ -29,7 +29,8 @@ MAX_STACK = 65535
 def _scale_exponent(a: float, b: float, c: float, steps: int) -> int:
     e = int(_lib.lib().scacchi_muon_scale_exponent(a, b, c, steps))
     if e < 0:
-        raise ValueError(f"coefficients {(a, b, c)} diverge within {steps} steps from singular values in [0, 1]")
+        raise ValueError(f"coefficients {(a, b, c)} diverge within {steps} steps from singular values in [0, 1], or "
+                         "have 0 < 16 |c| < |b|")
     return e
 
 
