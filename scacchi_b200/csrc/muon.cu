@@ -14,10 +14,17 @@
 // five steps amplify 3.44^5 times (2e-2 of the result on a low-rank update
 // against 5e-6).
 //
-// A and A^2 are symmetric: their tiles on and below the diagonal are
-// computed and mirrored.  Rows and columns past a matrix's own are zeros
-// that TMA fills in, so any size works and nothing is padded in memory but
-// the row pitch (to 16 bytes).
+// Layout.  An operand is stored in panels of 64 columns, each row of a panel
+// 128 bytes with its 16-byte chunks already in the 128B-swizzled order of
+// shared memory (chunk c of row r at c ^ (r & 7)).  Any rows of a panel are
+// one contiguous piece, which serves as a K-major tile (the panel along K)
+// or an MN-major one (its rows along K) alike, and an epilogue warp's 32
+// rows leave as one 4 KB copy.  Rows are padded to 64 and columns to whole
+// panels with zeros, which every product keeps zero, so any size works.
+//
+// A and A^2 are symmetric: only blocks on and below the diagonal of 256 x 256
+// blocks are computed and stored; one above it is read as its mirror image,
+// MN-major for K-major.
 
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -40,23 +47,35 @@ using namespace tc05;
 namespace cg = cooperative_groups;
 
 constexpr int kBM = 128;           // rows of a CTA's output tile
-constexpr int kBK = 64;            // K of a stage: 128 bytes of fp16
+constexpr int kBK = 64;            // K of a stage: a panel
+constexpr int kSym = 256;          // blocks of a symmetric matrix that are stored whole
+constexpr int kBox = 64 * kBK * 2; // 64 rows of a panel
 constexpr int kEpiWarps = 8;       // two per TMEM lane quadrant, half the tile's columns each
-constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer, MMA issuer, epilogue
+constexpr int kThreads = 128 + 32 * kEpiWarps;  // producer, MMA issuer, two idle warps; epilogue
+// The pair kernel's registers per thread: kLaunchRegisters at launch (the
+// host checks that the build has them), shared out again for the sums:
+// 128 x 48 + 256 x 224 = 63488 of 384 x 168 = 64512.
+constexpr int kLaunchRegisters = 168, kFewRegisters = 48, kManyRegisters = 224;
+static_assert(128 * kFewRegisters + 32 * kEpiWarps * kManyRegisters <= kThreads * kLaunchRegisters,
+              "setmaxnreg would wait forever");
 constexpr int kMaxSplit = 8;       // CTAs of a cluster that share a tile's K
 constexpr int kNormBlocks = 128;   // most partial sums of squares per matrix
-constexpr int kPatch = 2 * 32 * 64;  // an epilogue warp's 32 x 32 block as two fp16 parts
+constexpr int kPatch = 32 * 32 * 4;  // an epilogue warp's 32 x 32 block in fp32
 
 __device__ uint32_t g_muon_error;
 std::atomic<uint64_t> g_muon_launches{0};
 
-enum Mode : int { kGram = 0, kSquare = 1, kUpdate = 2, kLast = 3 };
+enum Major : int { kAlongK = 0, kAlongMN = 1, kSymmetric = 2 };  // of an operand: K-, MN-major, or by the block
 
 struct Product {
-  int mode, sym;
+  int last, sym;                // the last update, and a symmetric output
+  int a_major, b_major;
+  int a_rows, b_rows;           // padded rows of the operands' panels
   int rows, cols, k;            // of the output, and the summed length
   int tiles_n, per_batch, tiles;
   float scale, diag;            // the output is scale acc + diag on the diagonal
+  __half *dst;                  // an operand of the next product: [batch][2][panel][dst_rows][64]
+  int dst_rows, dst_panels;
   // last: the result, or the weight's step w <- decay w - step x
   void *out;
   int dtype;                    // 0 float32, 1 bfloat16, 2 float16
@@ -64,8 +83,14 @@ struct Product {
   float decay, step;
 };
 
-// A tile's place: matrix, tile row (of BM rows), tile column.  Symmetric
-// outputs list, row by row, the tiles that touch the lower triangle.
+// Tiles of tile row i of a symmetric output: those that touch the stored blocks.
+template <int BM, int BN>
+__host__ __device__ __forceinline__ int row_tiles(int i, int tiles_n) {
+  const int n = ((i * BM) / kSym + 1) * (kSym / BN);
+  return n < tiles_n ? n : tiles_n;
+}
+
+// A tile's place: matrix, tile row (of BM rows), tile column.
 template <int BM, int BN>
 __device__ __forceinline__ void locate(const Product &q, int t, int &batch, int &i, int &j) {
   batch = t / q.per_batch;
@@ -76,118 +101,134 @@ __device__ __forceinline__ void locate(const Product &q, int t, int &batch, int 
     return;
   }
   i = 0;
-  for (;;) {
-    int n = (i * BM + BM - 1) / BN + 1;
-    n = n < q.tiles_n ? n : q.tiles_n;
-    if (u < n) break;
-    u -= n;
-    ++i;
-  }
+  for (int n; u >= (n = row_tiles<BM, BN>(i, q.tiles_n)); ++i) u -= n;
   j = u;
 }
 
-__device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn(v - __half2float(hi));
+// Whether the 64 K of stage kb are read MN-major for rows `at`.. of an operand
+__device__ __forceinline__ bool along_mn(int major, int at, int kb) {
+  return major == kAlongMN || (major == kSymmetric && kb / (kSym / kBK) > at / kSym);
 }
 
-// A warp's 32 x 32 block in the fragment layout (tmem_ld16x256_x4):
-// element (row 16 h + 8 u + t/4, column 8 j + 2 (t%4) + e) of thread t is
-// v[16 h + 4 j + 2 u + e].
+// one part of a stage's operand: `rows` of the output's rows or columns
+// (from `at`) by 64 of K, in boxes of 64 rows of a panel
+template <typename Load>
+__device__ __forceinline__ void load_operand(uint8_t *dst, int rows, int at, int kb, bool mn, int panel_rows,
+                                             Load load) {
+  for (int m = 0; m < rows; m += 64, dst += kBox)
+    load(dst, mn ? ((at + m) / 64) * panel_rows + kb * kBK : kb * panel_rows + at + m);
+}
+
+// Descriptors of a stage's operands: the first stage's, advanced by whole
+// 16-byte units (an address stays within the field's 14 bits).  The MMA
+// warp keeps its control flow uniform and elects a lane for the issue alone.
+struct StageDesc {
+  uint64_t a, b;
+  uint32_t a_part, b_part, a_step, b_step;
+  __device__ __forceinline__ StageDesc(uint32_t stage, uint32_t a_bytes, uint32_t b_bytes, bool a_mn, bool b_mn) {
+    a = desc_sw128(stage, a_mn);
+    b = desc_sw128(stage + 2 * a_bytes, b_mn);
+    a_part = a_bytes >> 4;
+    b_part = b_bytes >> 4;
+    a_step = a_mn ? 2048u >> 4 : 32u >> 4;
+    b_step = b_mn ? 2048u >> 4 : 32u >> 4;
+  }
+  // hi lo, lo hi, hi hi: the small products first
+  __device__ __forceinline__ uint64_t a_of(int term, int k) const { return a + (term == 1 ? a_part : 0u) + k * a_step; }
+  __device__ __forceinline__ uint64_t b_of(int term, int k) const { return b + (term == 0 ? b_part : 0u) + k * b_step; }
+};
+
+// Place of row `row`, 4-float chunk `chunk` in an epilogue patch: rows of
+// 32 floats, chunks swizzled so that a row per lane, eight columns of a row
+// per lane and a column per lane all spread over the banks.
+__device__ __forceinline__ int patch_at(int row, int chunk) {
+  return row * 32 + ((chunk ^ ((row ^ (row >> 3)) & 7)) << 2);
+}
+
+// What becomes of a warp's 32 rows (a row per lane) by COLS columns, 32
+// columns at a time: turned through the warp's patch of shared memory, then
+// written in whole pieces of rows, as hi + lo in the panels of the next
+// product's operand, or to the user's matrix.
 //
-// The last product's block goes to the user's matrix: four lanes write (or
-// update) 8 neighbouring columns of a row.
-__device__ __forceinline__ void emit_last(const Product &q, int batch, int r0, int c0, const float *v) {
-  const int lane = threadIdx.x & 31, row = r0 + (lane >> 2), col = c0 + 2 * (lane & 3);
-  const int64_t base = ((int64_t)batch * q.rows + row) * q.cols + col;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float w[16];
-    if (q.weight) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int dr = 16 * h + 8 * (i >> 1 & 1), dc = 8 * (i >> 2) + (i & 1);
-        if (row + dr < q.rows && col + dc < q.cols) w[i] = q.weight[base + (int64_t)dr * q.cols + dc];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int dr = 16 * h + 8 * (i >> 1 & 1), dc = 8 * (i >> 2) + (i & 1);
-      if (row + dr < q.rows && col + dc < q.cols) {
-        const int64_t at = base + (int64_t)dr * q.cols + dc;
-        const float y = v[16 * h + i] * q.scale;
-        if (q.weight)
-          q.weight[at] = fmaf(-q.step, y, q.decay * w[i]);
-        else if (q.dtype == 0)
-          static_cast<float *>(q.out)[at] = y;
-        else if (q.dtype == 1)
-          static_cast<__nv_bfloat16 *>(q.out)[at] = __float2bfloat16_rn(y);
-        else
-          static_cast<__half *>(q.out)[at] = __float2half_rn(y);
-      }
-    }
-  }
-}
-
-// The block of an operand of the next product: split into hi and lo, laid
-// out by stmatrix (rows of 64 bytes, 64B-swizzled) and stored by TMA, which
-// leaves out what lies past the matrix; for a symmetric output whose mirror
-// tile is not computed, once more transposed.  hi and lo have a patch each,
-// so one is filled while the other is read.
-__device__ __forceinline__ void emit_block(const Product &q, const CUtensorMap *map_d, int batch, int r0, int c0,
-                                           bool mirror, const float *v, uint8_t *patch) {
+// This code runs once per tile, so what it costs is mostly fetching it:
+// unrolled over the blocks (40 KB of code) it took 4 us a block, rolled
+// TODO.
+template <int COLS>
+__device__ __forceinline__ void emit(const Product &q, int batch, int r0, int c_first, const float (&sum)[COLS],
+                                     float *patch) {
   const int lane = threadIdx.x & 31;
-  uint32_t hi[16], lo[16];  // [row group 2 h + u][column group j]
-  const bool on_diagonal = r0 == c0;
+#pragma unroll 1
+  for (int g = 0; g < COLS / 32; ++g) {
+    const int c0 = c_first + 32 * g;
+    if (q.last ? r0 >= q.rows || c0 >= q.cols : r0 >= q.dst_rows || c0 >= q.dst_panels * 64) break;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int h = i >> 3, u = i >> 2 & 1, j = i & 3;
-    float x = v[16 * h + 4 * j + 2 * u] * q.scale, y = v[16 * h + 4 * j + 2 * u + 1] * q.scale;
-    if (on_diagonal) {
-      const int d = 16 * h + 8 * u + (lane >> 2) - (8 * j + 2 * (lane & 3));
-      if (d == 0) x += q.diag;
-      if (d == 1) y += q.diag;
-    }
-    const __half2 a = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(a);
-    const __half2 b = __floats2half2_rn(x - f.x, y - f.y);
-    hi[i] = *reinterpret_cast<const uint32_t *>(&a);
-    lo[i] = *reinterpret_cast<const uint32_t *>(&b);
-  }
-  const uint32_t base = smem_u32(patch);
-  const int sub = lane & 7, mat = lane >> 3;
+    for (int i = 0; i < COLS / 32; ++i)
+      if (i == g) {
 #pragma unroll
-  for (int turned = 0; turned < 2; ++turned) {
-    if (turned && !mirror) break;
-    const int x = turned ? r0 : c0, y = turned ? c0 : r0;
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const uint32_t(&p)[16] = part ? lo : hi;
-      if (lane == 0) tma_store_wait_read<1>();  // this part's patch is free
-      __syncwarp();
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int row = 8 * g + sub;
-        const uint32_t at = base + part * 2048 + row * 64 + ((mat ^ (row >> 1 & 3)) << 4);
-        if (turned)
-          stmatrix_x4_trans(at, p[g], p[4 + g], p[8 + g], p[12 + g]);
-        else
-          stmatrix_x4(at, p[4 * g], p[4 * g + 1], p[4 * g + 2], p[4 * g + 3]);
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<float4 *>(patch + patch_at(lane, k)) = make_float4(
+              sum[32 * i + 4 * k], sum[32 * i + 4 * k + 1], sum[32 * i + 4 * k + 2], sum[32 * i + 4 * k + 3]);
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_3d(map_d, patch + part * 2048, x, y, 2 * batch + part);
-        tma_store_commit();
+    __syncwarp();
+    if (q.last) {
+      // a column per lane
+      const int64_t base = ((int64_t)batch * q.rows + r0) * q.cols + c0 + lane;
+      const int n = q.rows - r0 < 32 ? q.rows - r0 : 32;
+      if (c0 + lane < q.cols) {
+#pragma unroll 1
+        for (int row = 0; row < n; row += 8) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            y[e] = patch[patch_at(row + e, lane >> 2) + (lane & 3)] * q.scale;
+            if (q.weight && row + e < n)
+              y[e] = fmaf(-q.step, y[e], q.decay * q.weight[base + (int64_t)(row + e) * q.cols]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int64_t at = base + (int64_t)(row + e) * q.cols;
+            if (row + e >= n) break;
+            if (q.weight)
+              q.weight[at] = y[e];
+            else if (q.dtype == 0)
+              static_cast<float *>(q.out)[at] = y[e];
+            else if (q.dtype == 1)
+              static_cast<__nv_bfloat16 *>(q.out)[at] = __float2bfloat16_rn(y[e]);
+            else
+              static_cast<__half *>(q.out)[at] = __float2half_rn(y[e]);
+          }
+        }
+      }
+    } else {
+      // eight columns of a row per lane: 64 bytes of eight rows at a time
+      const int64_t part = (int64_t)q.dst_panels * q.dst_rows * 64;
+      __half *to = q.dst + (int64_t)batch * 2 * part + ((int64_t)(c0 / 64) * q.dst_rows + r0) * 64;
+      const int oct = lane & 3, chunk = (c0 & 32) / 8 + oct;
+      const int diagonal = q.diag != 0.0f ? c0 + 8 * oct - r0 : 1 << 30;  // row - column offset of the diagonal
+#pragma unroll 2
+      for (int row = lane >> 2; row < 32; row += 8) {
+        float y[8];
+        *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(patch + patch_at(row, 2 * oct));
+        *reinterpret_cast<float4 *>(y + 4) = *reinterpret_cast<const float4 *>(patch + patch_at(row, 2 * oct + 1));
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          float u = y[e] * q.scale, v = y[e + 1] * q.scale;
+          if (row - diagonal == e && r0 + row < q.rows) u += q.diag;
+          if (row - diagonal == e + 1 && r0 + row < q.rows) v += q.diag;
+          const __half2 a = __floats2half2_rn(u, v);
+          const float2 f = __half22float2(a);
+          const __half2 b = __floats2half2_rn(u - f.x, v - f.y);
+          hi[e / 2] = *reinterpret_cast<const uint32_t *>(&a);
+          lo[e / 2] = *reinterpret_cast<const uint32_t *>(&b);
+        }
+        __half *at = to + row * 64 + ((chunk ^ (row & 7)) << 3);
+        *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(at + part) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
+    __syncwarp();
   }
-}
-
-// Whether the tile that holds (c, r) is absent from the symmetric list.
-template <int BM, int BN>
-__device__ __forceinline__ bool mirrored(const Product &q, int r, int c) {
-  return q.sym && r / BN * BN > c / BM * BM + BM - 1;
 }
 
 // The tensor core truncates each time it adds to a TMEM accumulator: about
@@ -202,42 +243,10 @@ __device__ __forceinline__ void add_stage(float (&sum)[COLS], uint32_t acc) {
 #pragma unroll
   for (int g = 0; g < COLS / 16; ++g) {
     uint32_t v[16];
-    tmem_ld16x256_x4(acc + ((uint32_t)(16 * (g & 1)) << 16) + (g >> 1) * 32, v);
+    tmem_ld16(acc + g * 16, v);
     tmem_wait_ld();
 #pragma unroll
     for (int e = 0; e < 16; ++e) sum[g * 16 + e] += __uint_as_float(v[e]);
-  }
-}
-
-// Descriptors of a stage's operands: the first stage's, advanced by whole
-// 16-byte units (an address stays within the field's 14 bits).  The MMA
-// warp keeps its control flow uniform and elects a lane for the issue
-// alone: with the loop inside `lane == 0` each MMA took 100 clocks to issue.
-template <bool kAMn, bool kBMn>
-struct StageDesc {
-  uint64_t a_hi, b_hi;
-  uint32_t a_part, b_part;
-  __device__ __forceinline__ StageDesc(uint32_t stage0, uint32_t a_bytes, uint32_t b_bytes) {
-    a_hi = desc_sw128(stage0, kAMn ? 64 * kBK * 2 : 16);
-    b_hi = desc_sw128(stage0 + 2 * a_bytes, kBMn ? 64 * kBK * 2 : 16);
-    a_part = a_bytes >> 4;
-    b_part = b_bytes >> 4;
-  }
-  __device__ __forceinline__ uint64_t a(bool lo, int k, uint32_t at) const {
-    return a_hi + (lo ? a_part : 0u) + at + (uint32_t)k * (kAMn ? 2048u >> 4 : 32u >> 4);
-  }
-  __device__ __forceinline__ uint64_t b(bool lo, int k, uint32_t at) const {
-    return b_hi + (lo ? b_part : 0u) + at + (uint32_t)k * (kBMn ? 2048u >> 4 : 32u >> 4);
-  }
-};
-
-// one operand part of a stage: `rows` rows of the tile (from `at`) by 64 of K
-template <bool kMn, typename Load>
-__device__ __forceinline__ void load_operand(uint8_t *dst, int rows, int at, int kb, Load load) {
-  if (kMn) {
-    for (int m = 0; m < rows; m += 64) load(dst + m * kBK * 2, at + m, kb * kBK);
-  } else {
-    load(dst, kb * kBK, at);
   }
 }
 
@@ -250,30 +259,31 @@ struct PairLayout {
   static constexpr int kA = kBM * kBK * 2, kB = BN / 2 * kBK * 2;  // one part of a stage's operands in one CTA
   static constexpr int kStage = 2 * (kA + kB);
   static constexpr int kStages = BN == 256 ? 3 : 4;
+  static constexpr int kSlots = 512 / BN;                          // accumulators in TMEM
   static constexpr int kPatches = kStages * kStage;
   static constexpr int kBars = kPatches + kEpiWarps * kPatch;
-  static constexpr int kBytes = kBars + 8 * (2 * kStages + 4) + 16 + 1024;  // + alignment slack
+  static constexpr int kBytes = kBars + 8 * (2 * kStages + 2 * kSlots) + 16 + 1024;  // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory budget");
 };
 
-// D[i, j] = A[i, k] B[j, k]; A and B are K-major (their rows run along k) or
-// MN-major (k counts rows).  Persistent over the tiles.
+// D[i, j] = A[i, k] B[j, k], persistent over the tiles.
 //
-// A single CTA's 128 x 256 tile needs 96 KB of operands per stage, and 148
-// of them drew 13 TB/s from L2, its limit here: 1.08 us a stage, against
-// 0.82 us of MMA.  A pair shares B, 64 KB a CTA.
-template <int BN, bool kAMn, bool kBMn>
+// A single CTA's 128 x 256 tile needs 96 KB of operands per stage, which
+// its shared memory cannot take in while the MMAs read theirs (240 KB of
+// 128 bytes a clock: 1.08 us a stage, against 0.82 us of MMA).  A pair
+// shares B: 64 KB a CTA.
+template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ns_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ CUtensorMap map_d, const __grid_constant__ Product q) {
+                   const __grid_constant__ Product q) {
   using L = PairLayout<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kBars);  // the even CTA's counts both CTAs' loads
   uint64_t *empty = full + L::kStages;
   uint64_t *acc_full = empty + L::kStages;
-  uint64_t *acc_empty = acc_full + 2;                              // the even CTA's counts both epilogues
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+  uint64_t *acc_empty = acc_full + L::kSlots;                      // the even CTA's counts both epilogues
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + L::kSlots);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int kblocks = (q.k + kBK - 1) / kBK;
@@ -287,7 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < L::kSlots; ++s) {
       mbar_init(&acc_full[s], 1);
       mbar_init(&acc_empty[s], 2 * kEpiWarps);
     }
@@ -296,7 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   __syncwarp();
   if (warp == 1) {
-    tmem_alloc_pair(tmem_slot, 2 * BN);
+    tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();
   }
   tc_fence_before();
@@ -306,14 +316,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    registers_dec<kFewRegisters>();
+    if (warp == 0 && lane == 0) {
       int stage = 0;
       uint32_t phase = 0, issued = 0, parity = 0;
       bool stop = false;
       for (int t = first; t < q.tiles && !stop; t += step) {
         int batch, i, j;
         locate<2 * kBM, BN>(q, t, batch, i, j);
+        const int a_at = (2 * i + rank) * kBM, b_at = j * BN + rank * (BN / 2);
         for (int kb = 0; kb < kblocks; ++kb) {
           if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_muon_error)) {
             stop = true;
@@ -322,15 +334,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint8_t *at = smem + stage * L::kStage;
           const uint32_t bar = cluster_addr(smem_u32(&full[stage]), 0);
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * L::kStage);
+          const bool a_mn = along_mn(q.a_major, a_at, kb), b_mn = along_mn(q.b_major, b_at, kb);
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
-            load_operand<kAMn>(at + part * L::kA, kBM, (2 * i + rank) * kBM, kb, [&](uint8_t *dst, int x, int y) {
-              tma_load_3d_pair(dst, &map_a, bar, x, y, 2 * batch + part);
-            });
-            load_operand<kBMn>(at + 2 * L::kA + part * L::kB, BN / 2, j * BN + rank * (BN / 2), kb,
-                               [&](uint8_t *dst, int x, int y) {
-                                 tma_load_3d_pair(dst, &map_b, bar, x, y, 2 * batch + part);
-                               });
+            load_operand(at + part * L::kA, kBM, a_at, kb, a_mn, q.a_rows,
+                         [&](uint8_t *dst, int y) { tma_load_3d_pair(dst, &map_a, bar, 0, y, 2 * batch + part); });
+            load_operand(at + 2 * L::kA + part * L::kB, BN / 2, b_at, kb, b_mn, q.b_rows,
+                         [&](uint8_t *dst, int y) { tma_load_3d_pair(dst, &map_b, bar, 0, y, 2 * batch + part); });
           }
           issued |= 1u << stage;
           parity = (parity & ~(1u << stage)) | (phase << stage);
@@ -345,27 +355,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (rank == 0)
         for (int s = 0; s < L::kStages; ++s)
           if (issued >> s & 1u) mbar_drain(&full[s], parity >> s & 1u);
-    }
-  } else if (warp == 1) {
-    if (rank == 0) {
+    } else if (warp == 1 && rank == 0) {
       int stage = 0, slot = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      const StageDesc<kAMn, kBMn> desc(smem_u32(smem), L::kA, L::kB);
       for (int t = first; t < q.tiles && ok; t += step) {
+        int batch, i, j;
+        locate<2 * kBM, BN>(q, t, batch, i, j);
         for (int kb = 0; kb < kblocks; ++kb) {
+          // one mode for the pair: its rows lie within one stored block
+          const bool a_mn = along_mn(q.a_major, 2 * i * kBM, kb), b_mn = along_mn(q.b_major, j * BN, kb);
+          const StageDesc desc(smem_u32(smem + stage * L::kStage), L::kA, L::kB, a_mn, b_mn);
+          const uint32_t idesc = idesc_f16(2 * kBM, BN, a_mn, b_mn), d = tmem + (uint32_t)(slot * BN);
           ok = mbar_wait_warp(&acc_empty[slot], acc_phase ^ 1u, abort_flag, &g_muon_error) &&
                mbar_wait_warp(&full[stage], phase, abort_flag, &g_muon_error);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            constexpr uint32_t idesc = idesc_f16(2 * kBM, BN, kAMn, kBMn);
-            const uint32_t d = tmem + (uint32_t)(slot * BN), at = (uint32_t)(stage * L::kStage) >> 4;
 #pragma unroll
             for (int term = 0; term < 3; ++term)
 #pragma unroll
               for (int k = 0; k < kBK / 16; ++k)
-                umma_f16_pair(d, desc.a(term == 1, k, at), desc.b(term == 0, k, at), idesc, (term | k) != 0);
+                umma_f16_pair(d, desc.a_of(term, k), desc.b_of(term, k), idesc, (term | k) != 0);
             umma_commit_pair(&empty[stage]);
             umma_commit_pair(&acc_full[slot]);
           }
@@ -374,7 +385,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             stage = 0;
             phase ^= 1u;
           }
-          if (++slot == 2) {
+          if (++slot == L::kSlots) {
             slot = 0;
             acc_phase ^= 1u;
           }
@@ -382,10 +393,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   } else {
+    registers_inc<kManyRegisters>();
     constexpr int kCols = BN / 2;              // columns of a warp
     const int quad = warp & 3;                 // the TMEM lanes this warp may read
-    const int half = (warp - 2) >> 2;
-    uint8_t *patch = smem + L::kPatches + (warp - 2) * kPatch;
+    const int half = (warp - 4) >> 2;
+    float *patch = reinterpret_cast<float *>(smem + L::kPatches + (warp - 4) * kPatch);
     int slot = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -403,7 +415,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&acc_empty[slot]), 0));
-        if (++slot == 2) {
+        if (++slot == L::kSlots) {
           slot = 0;
           acc_phase ^= 1u;
         }
@@ -411,24 +423,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok) break;
       int batch, i, j;
       locate<2 * kBM, BN>(q, t, batch, i, j);
-      const int r0 = (2 * i + rank) * kBM + quad * 32;
-#pragma unroll
-      for (int g = 0; g < kCols / 32; ++g) {
-        const int c0 = j * BN + half * kCols + g * 32;
-        if (r0 < q.rows && c0 < q.cols) {
-          if (q.mode == kLast)
-            emit_last(q, batch, r0, c0, sum + g * 32);
-          else
-            emit_block(q, &map_d, batch, r0, c0, mirrored<2 * kBM, BN>(q, r0, c0), sum + g * 32, patch);
-        }
-      }
+      emit<kCols>(q, batch, (2 * i + rank) * kBM + quad * 32, j * BN + half * kCols, sum, patch);
     }
-    if (lane == 0) tma_store_wait_all();
   }
   __syncwarp();
   tc_fence_before();
   cg::this_cluster().sync();
-  if (warp == 1) tmem_dealloc_pair(tmem, 2 * BN);
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -440,21 +441,21 @@ struct TileLayout {
   static constexpr int kA = kBM * kBK * 2, kB = kBN * kBK * 2;
   static constexpr int kStage = 2 * (kA + kB);
   static constexpr int kStages = 3;
+  static constexpr int kSlots = 4;
   static constexpr int kPatches = kStages * kStage;
   static constexpr int kBars = kPatches + kEpiWarps * kPatch;
-  static constexpr int kBytes = kBars + 8 * (2 * kStages + 4) + 16 + 1024;  // + alignment slack
+  static constexpr int kBytes = kBars + 8 * (2 * kStages + 2 * kSlots) + 16 + 1024;  // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory budget");
   static_assert(kBN * kBM * 4 <= kPatches, "the partial sums take the stages' place");
 };
 
 // The same product for outputs of few tiles: the CTAs of a cluster share one
-// tile's K, each reducing its share of the columns from all of them through
+// tile's K, each finishing its share of the columns from all of them through
 // distributed shared memory, so that a small output with a long sum does
 // not leave most SMs idle.
-template <bool kAMn, bool kBMn>
 __global__ void __launch_bounds__(kThreads, 1)
     ns_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ CUtensorMap map_d, const __grid_constant__ Product q) {
+                   const __grid_constant__ Product q) {
   using L = TileLayout;
   constexpr int BN = L::kBN;
   extern __shared__ uint8_t smem_raw[];
@@ -462,8 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kBars);
   uint64_t *empty = full + L::kStages;
   uint64_t *acc_full = empty + L::kStages;
-  uint64_t *acc_empty = acc_full + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+  uint64_t *acc_empty = acc_full + L::kSlots;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + L::kSlots);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int kblocks = (q.k + kBK - 1) / kBK;
@@ -479,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < L::kSlots; ++s) {
       mbar_init(&acc_full[s], 1);
       mbar_init(&acc_empty[s], kEpiWarps);
     }
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncwarp();
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 2 * BN);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -506,14 +507,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_muon_error)) break;
         uint8_t *at = smem + stage * L::kStage;
         mbar_expect_tx(&full[stage], L::kStage);
+        const bool a_mn = along_mn(q.a_major, i * kBM, kb), b_mn = along_mn(q.b_major, j * BN, kb);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          load_operand<kAMn>(at + part * L::kA, kBM, i * kBM, kb, [&](uint8_t *dst, int x, int y) {
-            tma_load_3d(dst, &map_a, &full[stage], x, y, 2 * batch + part);
-          });
-          load_operand<kBMn>(at + 2 * L::kA + part * L::kB, BN, j * BN, kb, [&](uint8_t *dst, int x, int y) {
-            tma_load_3d(dst, &map_b, &full[stage], x, y, 2 * batch + part);
-          });
+          load_operand(at + part * L::kA, kBM, i * kBM, kb, a_mn, q.a_rows,
+                       [&](uint8_t *dst, int y) { tma_load_3d(dst, &map_a, &full[stage], 0, y, 2 * batch + part); });
+          load_operand(at + 2 * L::kA + part * L::kB, BN, j * BN, kb, b_mn, q.b_rows,
+                       [&](uint8_t *dst, int y) { tma_load_3d(dst, &map_b, &full[stage], 0, y, 2 * batch + part); });
         }
         issued |= 1u << stage;
         parity = (parity & ~(1u << stage)) | (phase << stage);
@@ -529,20 +529,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     int stage = 0, slot = 0;
     uint32_t phase = 0, acc_phase = 0;
-    const StageDesc<kAMn, kBMn> desc(smem_u32(smem), L::kA, L::kB);
     for (int kb = kb0; kb < kb1; ++kb) {
+      const bool a_mn = along_mn(q.a_major, i * kBM, kb), b_mn = along_mn(q.b_major, j * BN, kb);
+      const StageDesc desc(smem_u32(smem + stage * L::kStage), L::kA, L::kB, a_mn, b_mn);
+      const uint32_t idesc = idesc_f16(kBM, BN, a_mn, b_mn), d = tmem + (uint32_t)(slot * BN);
       if (!mbar_wait_warp(&acc_empty[slot], acc_phase ^ 1u, abort_flag, &g_muon_error) ||
           !mbar_wait_warp(&full[stage], phase, abort_flag, &g_muon_error))
         break;
       tc_fence_after();
       if (elect_one()) {
-        constexpr uint32_t idesc = idesc_f16(kBM, BN, kAMn, kBMn);
-        const uint32_t d = tmem + (uint32_t)(slot * BN), at = (uint32_t)(stage * L::kStage) >> 4;
 #pragma unroll
         for (int term = 0; term < 3; ++term)
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k)
-            umma_f16(d, desc.a(term == 1, k, at), desc.b(term == 0, k, at), idesc, (term | k) != 0);
+            umma_f16(d, desc.a_of(term, k), desc.b_of(term, k), idesc, (term | k) != 0);
         umma_commit(&empty[stage]);
         umma_commit(&acc_full[slot]);
       }
@@ -551,17 +551,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         stage = 0;
         phase ^= 1u;
       }
-      if (++slot == 2) {
+      if (++slot == L::kSlots) {
         slot = 0;
         acc_phase ^= 1u;
       }
     }
-  } else {
-    constexpr int kCols = BN / 2;              // columns of a warp
+  } else if (warp >= 4) {
+    constexpr int kCols = BN / 2;              // columns of a warp: a panel
     const int quad = warp & 3;                 // the TMEM lanes this warp may read
-    const int half = (warp - 2) >> 2;
-    const int r0 = i * kBM + quad * 32;
-    uint8_t *patch = smem + L::kPatches + (warp - 2) * kPatch;
+    const int half = (warp - 4) >> 2;
+    float *patch = reinterpret_cast<float *>(smem + L::kPatches + (warp - 4) * kPatch);
     int slot = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -578,74 +577,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[slot]);
-      if (++slot == 2) {
+      if (++slot == L::kSlots) {
         slot = 0;
         acc_phase ^= 1u;
       }
     }
-    auto emit = [&](int c0, const float *v) {
-      if (r0 >= q.rows || c0 >= q.cols) return;
-      if (q.mode == kLast)
-        emit_last(q, batch, r0, c0, v);
-      else
-        emit_block(q, &map_d, batch, r0, c0, mirrored<kBM, BN>(q, r0, c0), v, patch);
-    };
-    if (ctas == 1) {
-      if (ok) {
-#pragma unroll
-        for (int g = 0; g < kCols / 32; ++g) emit(j * BN + half * kCols + g * 32, sum + g * 32);
-      }
-    } else {
-      // Each CTA finishes BN / ctas columns, as blocks of 32 x 32: its
-      // owner's warps take them in turn.  Partial sums arrive as [source]
-      // [block][element][lane], four elements at a time.
+    int unit = warp - 4;  // of the tile's eight units of 32 rows by a panel
+    if (ctas > 1) {
+      // Each CTA finishes 8 / ctas of them; the others' partial sums arrive
+      // as [source][unit][four elements][lane].
+      const int units = 8 / ctas;
       __syncwarp();
       cg::this_cluster().sync();  // every CTA is done with its stages
-      const int blocks = 16 / ctas;  // of this CTA: 4 quads x BN / 32 columns, shared out
+      float4 *to = cg::this_cluster().map_shared_rank(reinterpret_cast<float4 *>(smem), unit / units);
+      to += (rank * units + unit % units) * 512 + lane;
 #pragma unroll
-      for (int g = 0; g < kCols / 32; ++g) {
-        const int id = quad + 4 * (half * (kCols / 32) + g);  // block of the tile
-        float4 *buf = cg::this_cluster().map_shared_rank(reinterpret_cast<float4 *>(smem), id / blocks);
-        float4 *at = buf + (rank * blocks + id % blocks) * 256 + lane;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          at[e * 32] = make_float4(sum[g * 32 + 4 * e], sum[g * 32 + 4 * e + 1], sum[g * 32 + 4 * e + 2],
-                                   sum[g * 32 + 4 * e + 3]);
-      }
+      for (int e = 0; e < kCols / 4; ++e)
+        to[e * 32] = make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]);
       cg::this_cluster().sync();
-      if (warp - 2 < blocks && ok) {
-        const float4 *at = reinterpret_cast<const float4 *>(smem) + (warp - 2) * 256 + lane;
-        float v[32];
+      if (unit < units) {
+        const float4 *at = reinterpret_cast<const float4 *>(smem) + unit * 512 + lane;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+        for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
         for (int from = 0; from < ctas; ++from)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 f = at[from * blocks * 256 + e * 32];
-            v[4 * e] += f.x;
-            v[4 * e + 1] += f.y;
-            v[4 * e + 2] += f.z;
-            v[4 * e + 3] += f.w;
+          for (int e = 0; e < kCols / 4; ++e) {
+            const float4 f = at[from * units * 512 + e * 32];
+            sum[4 * e] += f.x;
+            sum[4 * e + 1] += f.y;
+            sum[4 * e + 2] += f.z;
+            sum[4 * e + 3] += f.w;
           }
-        const int id = rank * blocks + warp - 2, row = i * kBM + (id & 3) * 32, c0 = j * BN + (id >> 2) * 32;
-        if (row < q.rows && c0 < q.cols) {
-          if (q.mode == kLast)
-            emit_last(q, batch, row, c0, v);
-          else
-            emit_block(q, &map_d, batch, row, c0, mirrored<kBM, BN>(q, row, c0), v, patch);
-        }
+        unit += rank * units;
+      } else {
+        ok = false;
       }
     }
-    if (lane == 0) tma_store_wait_all();
+    if (ok) emit<kCols>(q, batch, i * kBM + (unit & 3) * 32, j * BN + (unit >> 2) * kCols, sum, patch);
   }
-  if (ctas > 1 && warp < 2) {  // the epilogue's two cluster barriers are everyone's
+  if (ctas > 1 && warp < 4) {  // the epilogue's two cluster barriers are everyone's
     __syncwarp();
     cg::this_cluster().sync();
     cg::this_cluster().sync();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 2 * BN);
+  if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -695,9 +672,14 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(Source s, int64_t elems, d
   }
 }
 
-// S u / (|u| + eps) as hi + lo, eight columns per thread
+__device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
+  hi = __float2half_rn(v);
+  lo = __float2half_rn(v - __half2float(hi));
+}
+
+// S u / (|u| + eps) as hi + lo in panels, a 16-byte chunk of each per thread
 __global__ void __launch_bounds__(256) ns_split_kernel(Source s, const double *partial, int blocks, int rows, int cols,
-                                                       int64_t pitch, int64_t part, double scale, double eps,
+                                                       int panel_rows, int panels, double scale, double eps,
                                                        __half *dst) {
   __shared__ double s_factor;
   cudaTriggerProgrammaticLaunchCompletion();
@@ -713,23 +695,25 @@ __global__ void __launch_bounds__(256) ns_split_kernel(Source s, const double *p
   const float f = (float)f64;
   const bool in_32 = f64 > 1e-30 && f64 < 1e30;  // a factor beyond is applied in 64 bits
   const int64_t base = (int64_t)blockIdx.y * rows * cols;
-  const int chunks = (int)(pitch / 8);
-  const int64_t total = (int64_t)rows * chunks;
+  const int chunks = panels * 8;
+  const int64_t total = (int64_t)panel_rows * chunks, part = (int64_t)panels * panel_rows * 64;
+  __half *out = dst + (int64_t)blockIdx.y * 2 * part;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / chunks;
-    const int c = (int)(i - r * chunks) * 8;
+    const int c8 = (int)(i - r * chunks), c = c8 * 8;
     __half hi[8], lo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float u = 0.0f;
-      if (c + e < cols) {
+      if (r < rows && c + e < cols) {
         const int64_t at = base + r * cols + c + e;
         u = load_any(s.in, s.dtype, at);
         if (s.momentum) u = muon_direction(s, u, s.momentum[at]);
+        u = in_32 ? u * f : (float)((double)u * f64);
       }
-      split_half(in_32 ? u * f : (float)((double)u * f64), hi[e], lo[e]);
+      split_half(u, hi[e], lo[e]);
     }
-    __half *at = dst + (int64_t)blockIdx.y * 2 * part + r * pitch + c;
+    __half *at = out + ((int64_t)(c8 >> 3) * panel_rows + r) * 64 + (((c8 & 7) ^ (int)(r & 7)) << 3);
     *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(hi);
     *reinterpret_cast<uint4 *>(at + part) = *reinterpret_cast<const uint4 *>(lo);
   }
@@ -779,48 +763,33 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cu
   return e;
 }
 
-// [batch][2][rows][pitch]
+// [batch][2][panels][panel_rows][64] of fp16, and the map that loads boxes
+// of 64 rows of it
 struct Stack {
   __half *p;
   int64_t batch;
-  int rows, cols;
-  int64_t pitch, part;
-};
+  int panel_rows, panels;
+  CUtensorMap map;
 
-int64_t pitch_of(int64_t cols) { return (cols + 7) / 8 * 8; }
-
-int64_t stack_bytes(int64_t batch, int64_t rows, int64_t cols) {
-  return (batch * 2 * rows * pitch_of(cols) * 2 + 255) / 256 * 256;
-}
-
-// Tensor maps of a call's stacks: [parts][rows][cols] of fp16, each encoded
-// once: boxes of 64 columns x box_rows rows to load, or (box_rows = 0) the
-// 32 x 32 blocks of an epilogue warp to store.
-struct Maps {
-  static constexpr int kMost = 20;
-  CUtensorMap map[kMost];
-  const __half *base[kMost];
-  int box[kMost], n = 0;
-
-  const CUtensorMap *get(const Stack &k, int box_rows) {
-    for (int i = 0; i < n; ++i)
-      if (base[i] == k.p && box[i] == box_rows) return &map[i];
-    auto fn = encode_fn();
-    if (!fn || n == kMost) return nullptr;
-    cuuint64_t dims[3] = {(cuuint64_t)k.cols, (cuuint64_t)k.rows, (cuuint64_t)k.batch * 2};
-    cuuint64_t strides[2] = {(cuuint64_t)k.pitch * 2, (cuuint64_t)k.part * 2};
-    const bool store = box_rows == 0;
-    cuuint32_t shape[3] = {store ? 32u : 64u, store ? 32u : (cuuint32_t)box_rows, 1};
+  bool place(uint8_t *at, int64_t matrices, int rows, int cols) {
+    p = reinterpret_cast<__half *>(at);
+    batch = matrices;
+    panel_rows = (rows + 63) / 64 * 64;
+    panels = (cols + 63) / 64;
+    const auto fn = encode_fn();
+    cuuint64_t dims[3] = {64, (cuuint64_t)panel_rows * panels, (cuuint64_t)batch * 2};
+    cuuint64_t strides[2] = {128, (cuuint64_t)panel_rows * panels * 128};
+    cuuint32_t box[3] = {64, 64, 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    if (fn(&map[n], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, k.p, dims, strides, shape, estr,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return nullptr;
-    base[n] = k.p;
-    box[n] = box_rows;
-    return &map[n++];
+    return fn && fn(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   }
 };
+
+int64_t stack_bytes(int64_t batch, int64_t rows, int64_t cols) {
+  return batch * 2 * ((rows + 63) / 64 * 64) * ((cols + 63) / 64) * 128;
+}
 
 // the device: its SMs, and how many clusters of 2, 4 and 8 CTAs of the tile
 // kernel it runs at once
@@ -830,17 +799,13 @@ struct Device {
 
 constexpr int kMaxDevices = 64;
 
-template <bool kAMn, bool kBMn>
-cudaError_t set_up() {
-  cudaError_t e = cudaFuncSetAttribute(ns_tile_kernel<kAMn, kBMn>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       TileLayout::kBytes);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(ns_pair_kernel<256, kAMn, kBMn>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             PairLayout<256>::kBytes);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(ns_pair_kernel<128, kAMn, kBMn>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             PairLayout<128>::kBytes);
-  return e;
+template <int BN>
+cudaError_t set_up_pair() {
+  cudaFuncAttributes a;
+  const cudaError_t e = cudaFuncGetAttributes(&a, ns_pair_kernel<BN>);
+  if (e != cudaSuccess) return e;
+  if (a.numRegs < kLaunchRegisters) return cudaErrorInvalidConfiguration;
+  return cudaFuncSetAttribute(ns_pair_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairLayout<BN>::kBytes);
 }
 
 // the current device's properties, read once (and its kernels' shared
@@ -856,8 +821,9 @@ const Device *device() {
   if (ready[dev].load(std::memory_order_relaxed)) return &known[dev];
   Device d = {};
   if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return nullptr;
-  if (set_up<false, false>() != cudaSuccess || set_up<true, true>() != cudaSuccess ||
-      set_up<false, true>() != cudaSuccess)
+  if (cudaFuncSetAttribute(ns_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileLayout::kBytes) !=
+          cudaSuccess ||
+      set_up_pair<256>() != cudaSuccess || set_up_pair<128>() != cudaSuccess)
     return nullptr;
   for (int z = 1; z < 4; ++z) {
     cudaLaunchConfig_t cfg = {};
@@ -870,51 +836,49 @@ const Device *device() {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&d.clusters[z], ns_tile_kernel<false, false>, &cfg) != cudaSuccess) return nullptr;
+    if (cudaOccupancyMaxActiveClusters(&d.clusters[z], ns_tile_kernel, &cfg) != cudaSuccess) return nullptr;
   }
   known[dev] = d;
   ready[dev].store(1, std::memory_order_release);
   return &known[dev];
 }
 
-int64_t tile_count(const Product &q, int64_t batch, int bm, int bn) {
-  const int64_t tm = (q.rows + bm - 1) / bm, tn = (q.cols + bn - 1) / bn;
-  if (!q.sym) return tm * tn * batch;
+template <int BM, int BN>
+int64_t tile_count(const Product &q, int64_t batch) {
+  const int tm = (q.rows + BM - 1) / BM, tn = (q.cols + BN - 1) / BN;
+  if (!q.sym) return (int64_t)tm * tn * batch;
   int64_t n = 0;
-  for (int64_t i = 0; i < tm; ++i) {
-    const int64_t w = (i * bm + bm - 1) / bn + 1;
-    n += w < tn ? w : tn;
-  }
+  for (int i = 0; i < tm; ++i) n += row_tiles<BM, BN>(i, tn);
   return n * batch;
 }
 
-template <int BN, bool kAMn, bool kBMn>
-cudaError_t run_pair(Product q, const Stack &a, const Stack &b, const Stack &to, Maps &maps, const Device &d, int64_t tiles,
-                     cudaStream_t st) {
-  const CUtensorMap *ma = maps.get(a, kAMn ? kBK : kBM), *mb = maps.get(b, kBMn ? kBK : BN / 2);
-  const CUtensorMap *md = maps.get(to, 0);
-  if (!ma || !mb || !md || tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
+template <int BN>
+cudaError_t run_pair(Product q, const Stack &a, const Stack &b, const Device &d, int64_t tiles, cudaStream_t st) {
+  if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
   q.tiles_n = (q.cols + BN - 1) / BN;
   q.tiles = (int)tiles;
   q.per_batch = (int)(tiles / a.batch);
   const int pairs = q.tiles < d.sms / 2 ? q.tiles : d.sms / 2;
-  return launch(ns_pair_kernel<BN, kAMn, kBMn>, dim3((unsigned)(2 * pairs)), kThreads,
-                (size_t)PairLayout<BN>::kBytes, st, true, 1, *ma, *mb, *md, q);
+  return launch(ns_pair_kernel<BN>, dim3((unsigned)(2 * pairs)), kThreads, (size_t)PairLayout<BN>::kBytes, st, true, 1,
+                a.map, b.map, q);
 }
 
 // The kernel and the CTAs that share a tile's K.  In units of one stage of a
-// 256 x 256 pair tile (0.82 us): a 256 x 128 pair tile's takes 0.6, a
-// 128 x 128 tile's 0.8 (it draws the most from L2 per product); splitting
+// 256 x 256 pair tile (0.87 us): a 256 x 128 pair tile's takes 0.57, a
+// 128 x 128 tile's 0.8 (it draws the most operands per product); splitting
 // K costs about 2 more.  What leaves SMs idle is a tile count below a wave,
 // or just above one.
-template <bool kAMn, bool kBMn>
-cudaError_t product(const Product &q, const Stack &a, const Stack &b, const Stack &to, Maps &maps, const Device &d,
-                    cudaStream_t st) {
+cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, const Device &d, cudaStream_t st) {
+  q.a_rows = a.panel_rows;
+  q.b_rows = b.panel_rows;
+  q.dst = to.p;
+  q.dst_rows = to.panel_rows;
+  q.dst_panels = to.panels;
   const int64_t kblocks = (q.k + kBK - 1) / kBK, pairs = d.sms / 2;
-  const int64_t p256 = tile_count(q, a.batch, 256, 256), p128 = tile_count(q, a.batch, 256, 128);
-  const int64_t t128 = tile_count(q, a.batch, 128, 128);
+  const int64_t p256 = tile_count<256, 256>(q, a.batch), p128 = tile_count<256, 128>(q, a.batch);
+  const int64_t t128 = tile_count<128, 128>(q, a.batch);
   const double cost256 = (double)((p256 + pairs - 1) / pairs * kblocks);
-  const double cost128 = 0.6 * (double)((p128 + pairs - 1) / pairs * kblocks);
+  const double cost128 = 0.57 * (double)((p128 + pairs - 1) / pairs * kblocks);
   double best = 0.8 * (double)((t128 + d.sms - 1) / d.sms * kblocks);
   int split = 1;
   for (int z = 1; z < 4 && (1 << z) <= kblocks; ++z) {
@@ -925,36 +889,30 @@ cudaError_t product(const Product &q, const Stack &a, const Stack &b, const Stac
       split = 1 << z;
     }
   }
-  if (cost256 <= cost128 && cost256 <= best) return run_pair<256, kAMn, kBMn>(q, a, b, to, maps, d, p256, st);
-  if (cost128 <= best) return run_pair<128, kAMn, kBMn>(q, a, b, to, maps, d, p128, st);
-  const CUtensorMap *ma = maps.get(a, kAMn ? kBK : kBM), *mb = maps.get(b, kBMn ? kBK : TileLayout::kBN);
-  const CUtensorMap *md = maps.get(to, 0);
-  if (!ma || !mb || !md || t128 * kMaxSplit > INT32_MAX) return cudaErrorInvalidValue;
-  Product t = q;
-  t.tiles_n = (q.cols + TileLayout::kBN - 1) / TileLayout::kBN;
-  t.tiles = (int)t128;
-  t.per_batch = (int)(t128 / a.batch);
-  return launch(ns_tile_kernel<kAMn, kBMn>, dim3((unsigned)(t.tiles * split)), kThreads, (size_t)TileLayout::kBytes, st,
-                true, split, *ma, *mb, *md, t);
+  if (cost256 <= cost128 && cost256 <= best) return run_pair<256>(q, a, b, d, p256, st);
+  if (cost128 <= best) return run_pair<128>(q, a, b, d, p128, st);
+  if (t128 * kMaxSplit > INT32_MAX) return cudaErrorInvalidValue;
+  q.tiles_n = (q.cols + TileLayout::kBN - 1) / TileLayout::kBN;
+  q.tiles = (int)t128;
+  q.per_batch = (int)(t128 / a.batch);
+  return launch(ns_tile_kernel, dim3((unsigned)(q.tiles * split)), kThreads, (size_t)TileLayout::kBytes, st, true,
+                split, a.map, b.map, q);
 }
 
 int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product last, void *workspace, cudaStream_t st) {
   const Device *dev = device();
   if (!dev) return SCACCHI_ECUDA;
   const int sms = dev->sms;
-  Maps maps;
   const int s = n.rows < n.cols ? n.rows : n.cols;
   const bool tall = n.rows > n.cols;
   uint8_t *at = static_cast<uint8_t *>(workspace);
   double *partial = reinterpret_cast<double *>(at);
   at += (size_t)n.batch * kNormBlocks * sizeof(double);
-  auto stack = [&](int rows, int cols) {
-    Stack k = {reinterpret_cast<__half *>(at), n.batch, rows, cols, pitch_of(cols), rows * pitch_of(cols)};
-    at += stack_bytes(n.batch, rows, cols);
-    return k;
-  };
-  Stack x = stack(n.rows, n.cols), y = stack(n.rows, n.cols);
-  const Stack gram = stack(s, s), poly = stack(s, s);
+  Stack x, y, gram, poly;
+  const int64_t wide = stack_bytes(n.batch, n.rows, n.cols), narrow = stack_bytes(n.batch, s, s);
+  if (!x.place(at, n.batch, n.rows, n.cols) || !y.place(at + wide, n.batch, n.rows, n.cols) ||
+      !gram.place(at + 2 * wide, n.batch, s, s) || !poly.place(at + 2 * wide + narrow, n.batch, s, s))
+    return SCACCHI_ECUDA;
   const double scale = ldexp(1.0, n.scale_exponent);
   const int64_t elems = (int64_t)n.rows * n.cols;
 
@@ -965,49 +923,47 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
   if (launch(ns_norm_kernel, dim3((unsigned)blocks, (unsigned)n.batch), 256, 0, st, false, 1, src, elems, partial) !=
       cudaSuccess)
     return SCACCHI_ECUDA;
-  const int64_t chunks = (int64_t)n.rows * (x.pitch / 8);
+  const int64_t chunks = (int64_t)x.panel_rows * x.panels * 8;
   int64_t split_blocks = (chunks + 255) / 256;
   const int64_t split_share = (8 * (int64_t)sms + n.batch - 1) / n.batch;
   split_blocks = split_blocks < split_share ? split_blocks : split_share;
   if (launch(ns_split_kernel, dim3((unsigned)split_blocks, (unsigned)n.batch), 256, 0, st, true, 1, src,
-             (const double *)partial, (int)blocks, n.rows, n.cols, x.pitch, x.part, scale, n.eps, x.p) != cudaSuccess)
+             (const double *)partial, (int)blocks, n.rows, n.cols, x.panel_rows, x.panels, scale, n.eps, x.p) != cudaSuccess)
     return SCACCHI_ECUDA;
 
   // M = c Z^2 + (a - b^2 / 4c) I with Z = A + (b / 2c) I: the square alone,
   // with shifted diagonals; without c, M = b A + a I takes no product
   const bool quintic = n.c != 0.0;
+  Stack *now = &x, *next = &y;
   for (int k = 0; k < n.steps; ++k) {
     Product q = {};
     q.sym = 1;
     q.rows = q.cols = s;
-    q.mode = kGram;
+    q.a_major = q.b_major = tall ? kAlongMN : kAlongK;
     q.k = tall ? n.rows : n.cols;
     q.scale = (float)((quintic ? 1.0 : n.b) / scale);
     q.diag = (float)((quintic ? n.b / (2.0 * n.c) : n.a) * scale);
-    const Stack &first = quintic ? gram : poly;
-    cudaError_t e = tall ? product<true, true>(q, x, x, first, maps, *dev, st)
-                         : product<false, false>(q, x, x, first, maps, *dev, st);
-    if (e != cudaSuccess) return SCACCHI_ECUDA;
+    if (product(q, *now, *now, quintic ? gram : poly, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
     if (quintic) {
-      q.mode = kSquare;
+      q.a_major = q.b_major = kSymmetric;
       q.k = s;
       q.scale = (float)(n.c / scale);
       q.diag = (float)((n.a - n.b * n.b / (4.0 * n.c)) * scale);
-      if (product<false, false>(q, gram, gram, poly, maps, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
+      if (product(q, gram, gram, poly, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
     }
     const bool final = k + 1 == n.steps;
     Product u = final ? last : Product{};
-    u.mode = final ? kLast : kUpdate;
+    u.last = final;
     u.scale = (float)(final ? 1.0 / (scale * scale) : 1.0 / scale);
     u.rows = n.rows;
     u.cols = n.cols;
     u.k = s;
-    e = tall ? product<false, false>(u, x, poly, y, maps, *dev, st)
-             : product<false, true>(u, poly, x, y, maps, *dev, st);
-    if (e != cudaSuccess) return SCACCHI_ECUDA;
-    const Stack t = x;
-    x = y;
-    y = t;
+    u.a_major = tall ? kAlongK : kSymmetric;
+    u.b_major = tall ? kSymmetric : kAlongMN;
+    if (product(u, tall ? *now : poly, tall ? poly : *now, *next, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
+    Stack *t = now;
+    now = next;
+    next = t;
   }
   return SCACCHI_OK;
 }

@@ -86,6 +86,17 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// A warpgroup's registers per thread: given back, and taken from what the
+// block was launched with.
+template <int N>
+__device__ __forceinline__ void registers_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // wait used while leaving: bounded by time only
 __device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return;
@@ -102,24 +113,10 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *smem_src, int c0, int c1, int c2) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2)
-               : "memory");
-}
-__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// at most N of this thread's store groups still read shared memory
-template <int N>
-__device__ __forceinline__ void tma_store_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_barrier_init() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
@@ -207,13 +204,11 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t *bar) {
       : "memory");
 }
 
-// 16 TMEM lanes x 32 columns in the mma fragment layout: for each eight
-// columns j, thread t receives lane t/4, columns 8 j + 2 (t%4) and the next
-// (r[4 j], r[4 j + 1]) and lane t/4 + 8, same columns (r[4 j + 2],
-// r[4 j + 3]).  Asynchronous until tmem_wait_ld().
-__device__ __forceinline__ void tmem_ld16x256_x4(uint32_t taddr, uint32_t (&r)[16]) {
+// 32 TMEM lanes x 16 columns: thread t receives lane t's columns.
+// Asynchronous until tmem_wait_ld().
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
       "[%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
@@ -221,31 +216,20 @@ __device__ __forceinline__ void tmem_ld16x256_x4(uint32_t taddr, uint32_t (&r)[1
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// four 8x8 16-bit matrices in the fragment layout to shared memory: thread
-// 8 i + r supplies the address of row r of matrix i (of its transpose)
-__device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
-               "r"(d)
-               : "memory");
-}
-__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
-               "r"(c), "r"(d)
-               : "memory");
-}
-
-// Shared-memory matrix descriptors, 128-byte swizzle, tiles 1024-aligned.
+// Shared-memory matrix descriptor of an operand tile, 128-byte swizzle,
+// 1024-byte aligned.  The same rows of 64 16-bit values (128 bytes) serve
+// both ways:
 //
-// K-major: rows of 64 16-bit values (128 bytes), 8-row groups 1024 bytes
-// apart; the leading offset is unused; K advances 32 bytes per 16 values.
+// K-major: rows of M or N, 8-row groups 1024 bytes apart; the leading offset
+// is unused; K advances 32 bytes per 16 values.
 //
-// MN-major: a block is 64 values of M or N (128 bytes) by `k` rows, 8-row
-// groups 1024 bytes apart (stride offset), the next 64 values of M or N
-// `block` bytes on (leading offset); K advances 2048 bytes per 16 rows.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, uint32_t leading) {
+// MN-major: blocks of 64 values of M or N by 64 rows of K, 8-row groups
+// 1024 bytes apart (stride offset), the next 64 values of M or N 8192 bytes
+// on (leading offset); K advances 2048 bytes per 16 rows.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, bool mn_major) {
   uint64_t d = 0;
   d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)((leading >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)(mn_major ? 8192u >> 4 : 1u) << 16;
   d |= (uint64_t)(1024u >> 4) << 32;
   d |= (uint64_t)1u << 46;  // descriptor version (sm_100)
   d |= (uint64_t)2u << 61;  // SWIZZLE_128B
