@@ -582,38 +582,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         acc_phase ^= 1u;
       }
     }
-    int unit = warp - 4;  // of the tile's eight units of 32 rows by a panel
-    if (ctas > 1) {
-      // Each CTA finishes 8 / ctas of them; the others' partial sums arrive
-      // as [source][unit][four elements][lane].
-      const int units = 8 / ctas;
+    if (ctas == 1) {
+      if (ok) emit<kCols>(q, batch, i * kBM + quad * 32, j * BN + half * kCols, sum, patch);
+    } else {
+      // Each CTA finishes 16 / ctas of the tile's 32 x 32 blocks, a warp
+      // each; the others' partial sums arrive as [source][block][four
+      // elements][lane].
+      const int blocks = 16 / ctas;
       __syncwarp();
       cg::this_cluster().sync();  // every CTA is done with its stages
-      float4 *to = cg::this_cluster().map_shared_rank(reinterpret_cast<float4 *>(smem), unit / units);
-      to += (rank * units + unit % units) * 512 + lane;
 #pragma unroll
-      for (int e = 0; e < kCols / 4; ++e)
-        to[e * 32] = make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]);
+      for (int g = 0; g < kCols / 32; ++g) {
+        const int id = (half * (kCols / 32) + g) * 4 + quad;
+        float4 *to = cg::this_cluster().map_shared_rank(reinterpret_cast<float4 *>(smem), id / blocks);
+        to += (rank * blocks + id % blocks) * 256 + lane;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          to[e * 32] = make_float4(sum[32 * g + 4 * e], sum[32 * g + 4 * e + 1], sum[32 * g + 4 * e + 2],
+                                   sum[32 * g + 4 * e + 3]);
+      }
       cg::this_cluster().sync();
-      if (unit < units) {
-        const float4 *at = reinterpret_cast<const float4 *>(smem) + unit * 512 + lane;
+      if (warp - 4 < blocks && ok) {
+        const float4 *at = reinterpret_cast<const float4 *>(smem) + (warp - 4) * 256 + lane;
+        float v[32];
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
+        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
         for (int from = 0; from < ctas; ++from)
 #pragma unroll
-          for (int e = 0; e < kCols / 4; ++e) {
-            const float4 f = at[from * units * 512 + e * 32];
-            sum[4 * e] += f.x;
-            sum[4 * e + 1] += f.y;
-            sum[4 * e + 2] += f.z;
-            sum[4 * e + 3] += f.w;
+          for (int e = 0; e < 8; ++e) {
+            const float4 f = at[from * blocks * 256 + e * 32];
+            v[4 * e] += f.x;
+            v[4 * e + 1] += f.y;
+            v[4 * e + 2] += f.z;
+            v[4 * e + 3] += f.w;
           }
-        unit += rank * units;
-      } else {
-        ok = false;
+        const int id = rank * blocks + warp - 4;
+        emit<32>(q, batch, i * kBM + (id & 3) * 32, j * BN + (id >> 2) * 32, v, patch);
       }
     }
-    if (ok) emit<kCols>(q, batch, i * kBM + (unit & 3) * 32, j * BN + (unit >> 2) * kCols, sum, patch);
   }
   if (ctas > 1 && warp < 4) {  // the epilogue's two cluster barriers are everyone's
     __syncwarp();
@@ -720,6 +726,352 @@ __global__ void __launch_bounds__(256) ns_split_kernel(Source s, const double *p
 }
 
 // ---------------------------------------------------------------------------
+// narrow sides up to 128: all steps in one launch, a cluster per matrix
+// ---------------------------------------------------------------------------
+
+struct Narrow {
+  Source src;
+  int rows, cols;          // the user's matrix
+  int side, length, tall;  // its narrow and long side, and which is which
+  int panels, steps;       // 64 along the long side each
+  int sub;                 // K of an accumulator: 32 or 64
+  int quintic;
+  double scale, eps;
+  float inv;               // 2^-e
+  float diag1, scale1;     // after X X^T
+  float diag2, scale2;     // after Z^2
+  void *out;
+  int dtype;
+  float *weight;
+  float decay, step;
+};
+
+struct NarrowLayout {
+  static constexpr int kMostPanels = 3;                          // of X in one CTA
+  static constexpr int kX = kMostPanels * kBM * 128;             // one part
+  static constexpr int kZ = 2 * kBM * 128;
+  static constexpr int kZAt = 2 * kX, kRAt = kZAt + 2 * kZ;      // Z (then M), and the partial sums
+  static constexpr int kBars = kRAt + kBM * kBM * 4;
+  static constexpr int kBytes = kBars + 64 + 8 * 8 + 1024;       // + alignment slack
+  static_assert(kBytes <= 227 * 1024, "shared memory budget");
+};
+constexpr int kNarrowThreads = 256;
+constexpr int kMostChunks = NarrowLayout::kMostPanels * 8 * kBM / kNarrowThreads;  // 8-element chunks of X per thread
+
+// byte of 8-column chunk `chunk` (of the slice) of row `row` in swizzled panels of 128 rows
+__device__ __forceinline__ int narrow_at(int row, int chunk) {
+  return (chunk >> 3) * (kBM * 128) + row * 128 + (((chunk ^ row) & 7) << 4);
+}
+
+// 64 columns of the summed accumulators of a row (TMEM lane) per thread
+__device__ __forceinline__ void read_sum(float (&sum)[64], uint32_t acc, int count, uint32_t stride) {
+#pragma unroll
+  for (int e = 0; e < 64; ++e) sum[e] = 0.0f;
+#pragma unroll 1
+  for (int a = 0; a < count; ++a, acc += stride) add_stage<64>(sum, acc);
+}
+
+__device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __half2 a = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+    const float2 f = __half22float2(a);
+    const __half2 b = __floats2half2_rn(v[2 * e] - f.x, v[2 * e + 1] - f.y);
+    h[e] = *reinterpret_cast<const uint32_t *>(&a);
+    l[e] = *reinterpret_cast<const uint32_t *>(&b);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// The last product's 32 rows (of the narrow side) by 64 of the long side, a
+// row per lane.  A tall matrix has the narrow side contiguous: a lane's
+// neighbours write with it; a wide one is turned through the warp's patch.
+__device__ __forceinline__ void narrow_out(const Narrow &q, int64_t base, int r0, int c0, const float (&v)[64],
+                                           float *patch) {
+  const int lane = threadIdx.x & 31;
+  const float inv2 = q.inv * q.inv;
+  auto put = [&](int64_t at, float y) {
+    if (q.weight)
+      q.weight[at] = fmaf(-q.step, y, q.decay * q.weight[at]);
+    else if (q.dtype == 0)
+      static_cast<float *>(q.out)[at] = y;
+    else if (q.dtype == 1)
+      static_cast<__nv_bfloat16 *>(q.out)[at] = __float2bfloat16_rn(y);
+    else
+      static_cast<__half *>(q.out)[at] = __float2half_rn(y);
+  };
+  if (q.tall) {
+    const int64_t at = base + (int64_t)c0 * q.side + r0 + lane;
+    if (r0 + lane < q.side) {
+      if (q.weight) {
+        float w[64];
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (c0 + e < q.length) w[e] = q.weight[at + (int64_t)e * q.side];
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (c0 + e < q.length) q.weight[at + (int64_t)e * q.side] = fmaf(-q.step, v[e] * inv2, q.decay * w[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (c0 + e < q.length) put(at + (int64_t)e * q.side, v[e] * inv2);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      *reinterpret_cast<float4 *>(patch + patch_at(lane, k)) = make_float4(
+          v[32 * g + 4 * k], v[32 * g + 4 * k + 1], v[32 * g + 4 * k + 2], v[32 * g + 4 * k + 3]);
+    __syncwarp();
+    const int c = c0 + 32 * g + lane;
+    if (c < q.length)
+      for (int row = 0; row < 32 && r0 + row < q.side; ++row)
+        put(base + (int64_t)(r0 + row) * q.length + c, patch[patch_at(row, lane >> 2) + (lane & 3)] * inv2);
+    __syncwarp();
+  }
+}
+
+// A matrix whose narrow side is at most 128 lives in the shared memory of a
+// cluster for all its steps: X [side <= 128][length], a slice of whole
+// panels per CTA (transposed on the way in and out if it is tall).  A step:
+// every CTA's product X X^T over its slice; the partial sums reduced, a
+// share of the rows per CTA, and Z = A + shift I handed to all through
+// distributed shared memory; M = c Z^2 + d I and X <- M X in every CTA for
+// its own slice.  Nothing but the matrix itself crosses global memory, and
+// seventeen launches of 6 us become one.
+//
+// What bounds it is latency: about ten dependent phases a step, each far
+// below the tensor cores' or shared memory's rate.
+__global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __grid_constant__ Narrow q) {
+  using L = NarrowLayout;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t *done = reinterpret_cast<uint64_t *>(smem + L::kBars);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  double *norms = reinterpret_cast<double *>(smem + L::kBars + 64);  // one per CTA of the cluster
+  __shared__ double s_part[kNarrowThreads / 32];
+  const auto cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int quad = warp & 3, half = warp >> 2;
+  const int64_t base = (int64_t)(blockIdx.x / ctas) * q.rows * q.cols;
+  const int panel0 = rank * q.panels / ctas, mine = (rank + 1) * q.panels / ctas - panel0;
+  const int side_panels = (q.side + 63) / 64;
+  const int per_panel = 64 / q.sub;
+
+  if (tid == 0) {
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+
+  // the slice, eight neighbours along the long side per chunk; lanes run
+  // along the axis that is contiguous in memory
+  float u[kMostChunks][8];
+  double sum = 0.0;
+  const int chunks = mine * 8;
+#pragma unroll
+  for (int i = 0; i < kMostChunks; ++i) {
+    const int id = i * kNarrowThreads + tid;
+    const int row = q.tall ? id & (kBM - 1) : id / (chunks > 0 ? chunks : 1);
+    const int chunk = q.tall ? id / kBM : id - row * chunks;
+    const int at = (panel0 * 8 + chunk) * 8;
+    const bool in = row < kBM && chunk < chunks && row < q.side;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      u[i][e] = 0.0f;
+      if (in && at + e < q.length) {
+        const int64_t g = base + (q.tall ? (int64_t)(at + e) * q.side + row : (int64_t)row * q.length + at + e);
+        u[i][e] = load_any(q.src.in, q.src.dtype, g);
+      }
+    }
+    if (q.src.momentum) {
+      float m[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = 0.0f;
+        if (in && at + e < q.length)
+          m[e] = q.src.momentum[base + (q.tall ? (int64_t)(at + e) * q.side + row : (int64_t)row * q.length + at + e)];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (in && at + e < q.length) {
+          m[e] = fmaf(q.src.beta, m[e], q.src.rest * u[i][e]);
+          q.src.momentum[base + (q.tall ? (int64_t)(at + e) * q.side + row : (int64_t)row * q.length + at + e)] = m[e];
+          u[i][e] = muon_direction(q.src, u[i][e], m[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fma((double)u[i][e], (double)u[i][e], sum);
+  }
+  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (lane == 0) s_part[warp] = sum;
+  __syncthreads();
+  cluster.sync();  // the other CTAs run: their shared memory may be written
+  if (tid < ctas) {
+    double total = 0.0;
+    for (int i = 0; i < kNarrowThreads / 32; ++i) total += s_part[i];
+    cluster.map_shared_rank(norms, tid)[rank] = total;
+  }
+  tc_fence_before();
+  cluster.sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  {
+    double total = 0.0;
+    for (int i = 0; i < ctas; ++i) total += norms[i];
+    const double f64 = q.scale / (sqrt(total) + q.eps);
+    const float f = (float)f64;
+    const bool in_32 = f64 > 1e-30 && f64 < 1e30;
+#pragma unroll
+    for (int i = 0; i < kMostChunks; ++i) {
+      const int id = i * kNarrowThreads + tid;
+      const int row = q.tall ? id & (kBM - 1) : id / (chunks > 0 ? chunks : 1);
+      const int chunk = q.tall ? id / kBM : id - row * chunks;
+      if (row >= kBM || chunk >= chunks) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[i][e] = in_32 ? u[i][e] * f : (float)((double)u[i][e] * f64);
+      uint4 hi, lo;
+      split8(u[i], hi, lo);
+      *reinterpret_cast<uint4 *>(smem + narrow_at(row, chunk)) = hi;
+      *reinterpret_cast<uint4 *>(smem + L::kX + narrow_at(row, chunk)) = lo;
+    }
+  }
+
+  uint32_t parity = 0;
+  const uint32_t x_at = smem_u32(smem), z_at = smem_u32(smem + L::kZAt);
+  // One product: `panels` of K, N columns; accumulators of q.sub of K each.
+  // b_mn: B's panels lie along N and K counts their rows.
+  auto product = [&](uint32_t a, uint32_t a_part, uint32_t b, uint32_t b_part, int panels, int n, bool b_mn) {
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t idesc = idesc_f16(kBM, n, false, b_mn);
+        // N along B's panels of 128 rows: the next 64 columns are a panel on
+        const uint64_t da = desc_sw128(a, false), db = desc_sw128(b, b_mn, kBM * 128);
+        const uint32_t b_step = b_mn ? 2048u >> 4 : 32u >> 4;
+        const int steps = q.sub / 16;
+        for (int p = 0; p < panels; ++p)
+          for (int h = 0; h < per_panel; ++h)
+            for (int term = 0; term < 3; ++term)
+              for (int k = 0; k < steps; ++k) {
+                const uint32_t kk = (uint32_t)(h * steps + k);
+                const uint32_t ao = (((term == 1 ? a_part : 0u) + (uint32_t)p * (kBM * 128)) >> 4) + kk * (32u >> 4);
+                const uint32_t bo = (((term == 0 ? b_part : 0u) + (uint32_t)p * (b_mn ? 8192u : kBM * 128)) >> 4) +
+                                    kk * b_step;
+                umma_f16(tmem + (uint32_t)((p * per_panel + h) * n), da + ao, db + bo, idesc, (term | k) != 0);
+              }
+        umma_commit(done);
+      }
+      __syncwarp();
+    }
+    mbar_wait(done, parity, abort_flag, &g_muon_error);
+    parity ^= 1u;
+    __syncwarp();
+    tc_fence_after();
+  };
+
+  const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+  const int row = quad * 32 + lane;
+  float v[64];
+  for (int step = 0; step < q.steps; ++step) {
+    // X X^T over this slice
+    product(x_at, L::kX, x_at, L::kX, mine, kBM, false);
+    read_sum(v, tmem + lanes + (uint32_t)(half * 64), mine * per_panel, kBM);
+    // partial sums to the CTA that owns the row: [source][4 columns][row]
+    const int own = kBM / ctas;
+    float4 *to = cluster.map_shared_rank(reinterpret_cast<float4 *>(smem + L::kRAt), row / own);
+    to += (rank * 32 + half * 16) * own + row % own;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) to[e * own] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+    cluster.sync();
+    const float4 *from = reinterpret_cast<const float4 *>(smem + L::kRAt);
+    for (int id = tid; id < own * 16; id += kNarrowThreads) {
+      const int r = id % own, c8 = id / own;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+      for (int c = 0; c < ctas; ++c) {
+        const float4 f0 = from[(c * 32 + 2 * c8) * own + r], f1 = from[(c * 32 + 2 * c8 + 1) * own + r];
+        y[0] += f0.x;
+        y[1] += f0.y;
+        y[2] += f0.z;
+        y[3] += f0.w;
+        y[4] += f1.x;
+        y[5] += f1.y;
+        y[6] += f1.z;
+        y[7] += f1.w;
+      }
+      const int at = rank * own + r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = y[e] * q.scale1 + (at == 8 * c8 + e && at < q.side ? q.diag1 : 0.0f);
+      uint4 hi, lo;
+      split8(y, hi, lo);
+      for (int c = 0; c < ctas; ++c) {
+        uint8_t *z = cluster.map_shared_rank(smem + L::kZAt, c);
+        *reinterpret_cast<uint4 *>(z + narrow_at(at, c8)) = hi;
+        *reinterpret_cast<uint4 *>(z + L::kZ + narrow_at(at, c8)) = lo;
+      }
+    }
+    cluster.sync();
+    if (q.quintic) {
+      product(z_at, L::kZ, z_at, L::kZ, side_panels, kBM, false);
+      read_sum(v, tmem + lanes + (uint32_t)(half * 64), side_panels * per_panel, kBM);
+#pragma unroll
+      for (int e = 0; e < 64; ++e) v[e] *= q.scale2;
+#pragma unroll
+      for (int e = 0; e < 64; ++e)
+        if (row == half * 64 + e && row < q.side) v[e] += q.diag2;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint4 hi, lo;
+        split8(v + 8 * c, hi, lo);
+        *reinterpret_cast<uint4 *>(smem + L::kZAt + narrow_at(row, half * 8 + c)) = hi;
+        *reinterpret_cast<uint4 *>(smem + L::kZAt + L::kZ + narrow_at(row, half * 8 + c)) = lo;
+      }
+    }
+    // X <- M X
+    const int n = mine * 64;
+    product(z_at, L::kZ, x_at, L::kX, side_panels, n, true);
+    const bool last = step + 1 == q.steps;
+#pragma unroll 1
+    for (int p = half; p < mine; p += 2) {
+      read_sum(v, tmem + lanes + (uint32_t)(p * 64), side_panels * per_panel, (uint32_t)n);
+      if (!last) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) v[e] *= q.inv;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint4 hi, lo;
+          split8(v + 8 * c, hi, lo);
+          *reinterpret_cast<uint4 *>(smem + narrow_at(row, p * 8 + c)) = hi;
+          *reinterpret_cast<uint4 *>(smem + L::kX + narrow_at(row, p * 8 + c)) = lo;
+        }
+      } else {
+        narrow_out(q, base, quad * 32, (panel0 + p) * 64, v, reinterpret_cast<float *>(smem + L::kRAt) + warp * 1024);
+      }
+    }
+  }
+  tc_fence_before();
+  cluster.sync();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
 
@@ -823,6 +1175,8 @@ const Device *device() {
   if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return nullptr;
   if (cudaFuncSetAttribute(ns_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileLayout::kBytes) !=
           cudaSuccess ||
+      cudaFuncSetAttribute(ns_narrow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NarrowLayout::kBytes) !=
+          cudaSuccess ||
       set_up_pair<256>() != cudaSuccess || set_up_pair<128>() != cudaSuccess)
     return nullptr;
   for (int z = 1; z < 4; ++z) {
@@ -863,11 +1217,13 @@ cudaError_t run_pair(Product q, const Stack &a, const Stack &b, const Device &d,
                 a.map, b.map, q);
 }
 
-// The kernel and the CTAs that share a tile's K.  In units of one stage of a
-// 256 x 256 pair tile (0.87 us): a 256 x 128 pair tile's takes 0.57, a
-// 128 x 128 tile's 0.8 (it draws the most operands per product); splitting
-// K costs about 2 more.  What leaves SMs idle is a tile count below a wave,
-// or just above one.
+// The kernel and the CTAs that share a tile's K, by their times in us: a
+// stage of a 256 x 256 pair tile takes 0.9 and its epilogue, which hides
+// less behind the next tile than a 256 x 128 one's, 3; a 256 x 128 pair
+// tile 0.53 and 0.5, the last one's 2; a 128 x 128 tile, which draws the
+// most operands per product, 0.7 and 4 to start and end; splitting its K
+// costs 2 more.  What leaves SMs idle is a tile count below a wave, or just
+// above one.
 cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, const Device &d, cudaStream_t st) {
   q.a_rows = a.panel_rows;
   q.b_rows = b.panel_rows;
@@ -877,19 +1233,19 @@ cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, 
   const int64_t kblocks = (q.k + kBK - 1) / kBK, pairs = d.sms / 2;
   const int64_t p256 = tile_count<256, 256>(q, a.batch), p128 = tile_count<256, 128>(q, a.batch);
   const int64_t t128 = tile_count<128, 128>(q, a.batch);
-  const double cost256 = (double)((p256 + pairs - 1) / pairs * kblocks);
-  const double cost128 = 0.57 * (double)((p128 + pairs - 1) / pairs * kblocks);
-  double best = 0.8 * (double)((t128 + d.sms - 1) / d.sms * kblocks);
+  const double cost256 = (double)((p256 + pairs - 1) / pairs) * (0.9 * (double)kblocks + 3.0) + 1.5;
+  const double cost128 = (double)((p128 + pairs - 1) / pairs) * (0.53 * (double)kblocks + 0.5) + 2.0;
+  double best = (double)((t128 + d.sms - 1) / d.sms) * (0.7 * (double)kblocks + 4.0) - 2.0;
   int split = 1;
   for (int z = 1; z < 4 && (1 << z) <= kblocks; ++z) {
     if (t128 > d.clusters[z]) break;
-    const double cost = 0.8 * (double)((kblocks + (1 << z) - 1) >> z) + 2.0;
+    const double cost = 0.7 * (double)((kblocks + (1 << z) - 1) >> z) + 4.0;
     if (cost < best) {
       best = cost;
       split = 1 << z;
     }
   }
-  if (cost256 <= cost128 && cost256 <= best) return run_pair<256>(q, a, b, d, p256, st);
+  if (cost256 < cost128 && cost256 <= best) return run_pair<256>(q, a, b, d, p256, st);
   if (cost128 <= best) return run_pair<128>(q, a, b, d, p128, st);
   if (t128 * kMaxSplit > INT32_MAX) return cudaErrorInvalidValue;
   q.tiles_n = (q.cols + TileLayout::kBN - 1) / TileLayout::kBN;
@@ -899,9 +1255,65 @@ cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, 
                 split, a.map, b.map, q);
 }
 
+// Narrow matrices: the CTAs of a matrix's cluster, 0 where it does not fit.
+// A cluster takes about 30 us and 4 more per panel of its longest slice
+// (time of the phases that grow with it), in as many waves as the device's
+// clusters of that size make of the stack.
+int narrow_ctas(const scacchi_newton_schulz &n, const Device &d) {
+  const int side = n.rows < n.cols ? n.rows : n.cols, panels = ((n.rows < n.cols ? n.cols : n.rows) + 63) / 64;
+  if (side > kBM) return 0;
+  int best = 0;
+  int64_t best_cost = 0;
+  for (int z = 0; z < 4; ++z) {
+    const int ctas = 1 << z, slice = (panels + ctas - 1) / ctas, at_once = z ? d.clusters[z] : d.sms;
+    if (slice > NarrowLayout::kMostPanels || ctas > panels) continue;
+    const int64_t cost = ((int64_t)n.batch + at_once - 1) / at_once * (30 + 4 * slice);
+    if (!best || cost < best_cost) {
+      best = ctas;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+int newton_schulz_narrow(const scacchi_newton_schulz &n, const Source &src, const Product &last, int ctas,
+                         cudaStream_t st) {
+  Narrow q = {};
+  q.src = src;
+  q.rows = n.rows;
+  q.cols = n.cols;
+  q.tall = n.rows > n.cols;
+  q.side = q.tall ? n.cols : n.rows;
+  q.length = q.tall ? n.rows : n.cols;
+  q.panels = (q.length + 63) / 64;
+  q.steps = n.steps;
+  // accumulators of 32 of K where they all fit into TMEM's 512 columns
+  q.sub = (q.panels + ctas - 1) / ctas <= 2 ? 32 : 64;
+  q.quintic = n.c != 0.0;
+  q.scale = ldexp(1.0, n.scale_exponent);
+  q.eps = n.eps;
+  q.inv = (float)(1.0 / q.scale);
+  q.scale1 = (float)((q.quintic ? 1.0 : n.b) / q.scale);
+  q.diag1 = (float)((q.quintic ? n.b / (2.0 * n.c) : n.a) * q.scale);
+  if (q.quintic) {
+    q.scale2 = (float)(n.c / q.scale);
+    q.diag2 = (float)((n.a - n.b * n.b / (4.0 * n.c)) * q.scale);
+  }
+  q.out = last.out;
+  q.dtype = last.dtype;
+  q.weight = last.weight;
+  q.decay = last.decay;
+  q.step = last.step;
+  return launch(ns_narrow_kernel, dim3((unsigned)(n.batch * ctas)), kNarrowThreads, (size_t)NarrowLayout::kBytes, st,
+                false, ctas, q) == cudaSuccess
+             ? SCACCHI_OK
+             : SCACCHI_ECUDA;
+}
+
 int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product last, void *workspace, cudaStream_t st) {
   const Device *dev = device();
   if (!dev) return SCACCHI_ECUDA;
+  if (const int ctas = narrow_ctas(n, *dev)) return newton_schulz_narrow(n, src, last, ctas, st);
   const int sms = dev->sms;
   const int s = n.rows < n.cols ? n.rows : n.cols;
   const bool tall = n.rows > n.cols;

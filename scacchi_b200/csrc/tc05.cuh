@@ -120,6 +120,7 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
 __device__ __forceinline__ void fence_barrier_init() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -224,12 +225,12 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 // is unused; K advances 32 bytes per 16 values.
 //
 // MN-major: blocks of 64 values of M or N by 64 rows of K, 8-row groups
-// 1024 bytes apart (stride offset), the next 64 values of M or N 8192 bytes
-// on (leading offset); K advances 2048 bytes per 16 rows.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, bool mn_major) {
+// 1024 bytes apart (stride offset), the next 64 values of M or N
+// `mn_block` bytes on (leading offset); K advances 2048 bytes per 16 rows.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, bool mn_major, uint32_t mn_block = 8192u) {
   uint64_t d = 0;
   d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(mn_major ? 8192u >> 4 : 1u) << 16;
+  d |= (uint64_t)(mn_major ? mn_block >> 4 : 1u) << 16;
   d |= (uint64_t)(1024u >> 4) << 32;
   d |= (uint64_t)1u << 46;  // descriptor version (sm_100)
   d |= (uint64_t)2u << 61;  // SWIZZLE_128B
