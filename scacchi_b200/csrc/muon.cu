@@ -643,6 +643,10 @@ struct Source {
   int nesterov;
 };
 
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+
 __device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
   if (dtype == 0) return static_cast<const float *>(p)[i];
   if (dtype == 1) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
@@ -683,6 +687,9 @@ __device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
   lo = __float2half_rn(v - __half2float(hi));
 }
 
+// kept out of line: as a select, its conversions run for every element
+__device__ __noinline__ float scale_in_64(float u, double f) { return (float)((double)u * f); }
+
 // S u / (|u| + eps) as hi + lo in panels, a 16-byte chunk of each per thread
 __global__ void __launch_bounds__(256) ns_split_kernel(Source s, const double *partial, int blocks, int rows, int cols,
                                                        int panel_rows, int panels, double scale, double eps,
@@ -715,7 +722,7 @@ __global__ void __launch_bounds__(256) ns_split_kernel(Source s, const double *p
         const int64_t at = base + r * cols + c + e;
         u = load_any(s.in, s.dtype, at);
         if (s.momentum) u = muon_direction(s, u, s.momentum[at]);
-        u = in_32 ? u * f : (float)((double)u * f64);
+        u = in_32 ? u * f : scale_in_64(u, f64);
       }
       split_half(u, hi[e], lo[e]);
     }
@@ -755,20 +762,20 @@ struct NarrowLayout {
   static constexpr int kBytes = kBars + 64 + 8 * 8 + 1024;       // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory budget");
 };
-constexpr int kNarrowThreads = 256;
-constexpr int kMostChunks = NarrowLayout::kMostPanels * 8 * kBM / kNarrowThreads;  // 8-element chunks of X per thread
+constexpr int kNarrowThreads = 512;  // a warp takes 32 rows by 32 columns of each result
+static_assert(NarrowLayout::kMostPanels * 64 * kBM * 4 <= NarrowLayout::kBars - NarrowLayout::kZAt, "scratch");
 
 // byte of 8-column chunk `chunk` (of the slice) of row `row` in swizzled panels of 128 rows
 __device__ __forceinline__ int narrow_at(int row, int chunk) {
   return (chunk >> 3) * (kBM * 128) + row * 128 + (((chunk ^ row) & 7) << 4);
 }
 
-// 64 columns of the summed accumulators of a row (TMEM lane) per thread
-__device__ __forceinline__ void read_sum(float (&sum)[64], uint32_t acc, int count, uint32_t stride) {
+// 32 columns of the summed accumulators of a row (TMEM lane) per thread
+__device__ __forceinline__ void read_sum(float (&sum)[32], uint32_t acc, int count, uint32_t stride) {
 #pragma unroll
-  for (int e = 0; e < 64; ++e) sum[e] = 0.0f;
+  for (int e = 0; e < 32; ++e) sum[e] = 0.0f;
 #pragma unroll 1
-  for (int a = 0; a < count; ++a, acc += stride) add_stage<64>(sum, acc);
+  for (int a = 0; a < count; ++a, acc += stride) add_stage<32>(sum, acc);
 }
 
 __device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
@@ -785,54 +792,139 @@ __device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// The last product's 32 rows (of the narrow side) by 64 of the long side, a
-// row per lane.  A tall matrix has the narrow side contiguous: a lane's
-// neighbours write with it; a wide one is turned through the warp's patch.
-__device__ __forceinline__ void narrow_out(const Narrow &q, int64_t base, int r0, int c0, const float (&v)[64],
+// The last product's 32 rows (of the narrow side) by 32 of the long side, a
+// row per lane, to the user's matrix: turned through the warp's patch, so
+// that lanes write along the axis that is contiguous there.
+__device__ __forceinline__ void narrow_out(const Narrow &q, int64_t base, int r0, int c0, const float (&v)[32],
                                            float *patch) {
   const int lane = threadIdx.x & 31;
   const float inv2 = q.inv * q.inv;
-  auto put = [&](int64_t at, float y) {
-    if (q.weight)
-      q.weight[at] = fmaf(-q.step, y, q.decay * q.weight[at]);
-    else if (q.dtype == 0)
-      static_cast<float *>(q.out)[at] = y;
-    else if (q.dtype == 1)
-      static_cast<__nv_bfloat16 *>(q.out)[at] = __float2bfloat16_rn(y);
-    else
-      static_cast<__half *>(q.out)[at] = __float2half_rn(y);
-  };
-  if (q.tall) {
-    const int64_t at = base + (int64_t)c0 * q.side + r0 + lane;
-    if (r0 + lane < q.side) {
-      if (q.weight) {
-        float w[64];
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (c0 + e < q.length) w[e] = q.weight[at + (int64_t)e * q.side];
+  for (int k = 0; k < 8; ++k)
+    *reinterpret_cast<float4 *>(patch + patch_at(lane, k)) =
+        make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+  __syncwarp();
+  const int fixed = q.tall ? r0 + lane : c0 + lane;
+  const int n = q.tall ? q.length - c0 : q.side - r0;  // of the other axis, one per iteration
+  const int64_t stride = q.tall ? q.side : q.length, at = base + (int64_t)(q.tall ? c0 : r0) * stride + fixed;
+  if (fixed < (q.tall ? q.side : q.length)) {
+#pragma unroll 1
+    for (int k = 0; k < 32 && k < n; k += 8) {
+      float y[8];
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (c0 + e < q.length) q.weight[at + (int64_t)e * q.side] = fmaf(-q.step, v[e] * inv2, q.decay * w[e]);
-      } else {
+      for (int e = 0; e < 8; ++e) {
+        const int row = q.tall ? lane : k + e, col = q.tall ? k + e : lane;
+        y[e] = patch[patch_at(row, col >> 2) + (col & 3)] * inv2;
+        if (q.weight && k + e < n) y[e] = fmaf(-q.step, y[e], q.decay * q.weight[at + (k + e) * stride]);
+      }
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (c0 + e < q.length) put(at + (int64_t)e * q.side, v[e] * inv2);
+      for (int e = 0; e < 8; ++e) {
+        if (k + e >= n) break;
+        if (q.weight)
+          q.weight[at + (k + e) * stride] = y[e];
+        else if (q.dtype == 0)
+          static_cast<float *>(q.out)[at + (k + e) * stride] = y[e];
+        else if (q.dtype == 1)
+          static_cast<__nv_bfloat16 *>(q.out)[at + (k + e) * stride] = __float2bfloat16_rn(y[e]);
+        else
+          static_cast<__half *>(q.out)[at + (k + e) * stride] = __float2half_rn(y[e]);
       }
     }
-    return;
   }
+  __syncwarp();
+}
+
+// Chunk `id` of a slice: its row (narrow side) and place along the slice.
+// Lanes run along the axis that is contiguous in memory.
+__device__ __forceinline__ void narrow_chunk(const Narrow &q, int id, int chunks, int &row, int &chunk) {
+  if (q.tall) {
+    row = id & (kBM - 1);
+    chunk = id / kBM;
+  } else {
+    row = id / chunks;
+    chunk = id - row * chunks;
+  }
+}
+
+// sum of eight squares, in 64 bits where 32 would lose them (a conversion
+// per element takes the time of the load)
+__device__ __forceinline__ double sum_of_squares(const float (&u)[8]) {
+  float s = 0.0f, most = 0.0f;
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  for (int e = 0; e < 8; ++e) {
+    s = fmaf(u[e], u[e], s);
+    most = fmaxf(most, fabsf(u[e]));
+  }
+  if (most == 0.0f || (most > 1e-15f && most < 1e18f)) return (double)s;  // NaN stays in s
+  double d = 0.0;
+  for (int e = 0; e < 8; ++e) d = fma((double)u[e], (double)u[e], d);
+  return d;
+}
+
+// The slice's update (and the momentum it leaves), eight neighbours along
+// the long side per chunk, into fp32 scratch; returns the sum of squares.
+template <typename T>
+__device__ __forceinline__ double narrow_load(const Narrow &q, int64_t base, int col0, int chunks, float *scratch) {
+  const T *in = static_cast<const T *>(q.src.in);
+  double sum = 0.0;
+  const int total = kBM * chunks;
+  const int64_t stride = q.tall ? q.side : 1;
+#pragma unroll 1
+  for (int id0 = threadIdx.x; id0 < total; id0 += 2 * kNarrowThreads) {
+    float u[2][8], m[2][8];
+    int64_t at[2];
+    int left[2];  // elements of the chunk that the matrix has
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      *reinterpret_cast<float4 *>(patch + patch_at(lane, k)) = make_float4(
-          v[32 * g + 4 * k], v[32 * g + 4 * k + 1], v[32 * g + 4 * k + 2], v[32 * g + 4 * k + 3]);
-    __syncwarp();
-    const int c = c0 + 32 * g + lane;
-    if (c < q.length)
-      for (int row = 0; row < 32 && r0 + row < q.side; ++row)
-        put(base + (int64_t)(r0 + row) * q.length + c, patch[patch_at(row, lane >> 2) + (lane & 3)] * inv2);
-    __syncwarp();
+    for (int i = 0; i < 2; ++i) {
+      const int id = id0 + i * kNarrowThreads;
+      int row, chunk;
+      narrow_chunk(q, id, chunks, row, chunk);
+      const int col = col0 + chunk * 8;
+      left[i] = id < total && row < q.side ? q.length - col : 0;
+      at[i] = base + (q.tall ? (int64_t)col * q.side + row : (int64_t)row * q.length + col);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        u[i][e] = e < left[i] ? to_f(in[at[i] + e * stride]) : 0.0f;
+        if (q.src.momentum) m[i][e] = e < left[i] ? q.src.momentum[at[i] + e * stride] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int id = id0 + i * kNarrowThreads;
+      if (id >= total) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (q.src.momentum) {
+          m[i][e] = fmaf(q.src.beta, m[i][e], q.src.rest * u[i][e]);
+          if (e < left[i]) q.src.momentum[at[i] + e * stride] = m[i][e];
+          u[i][e] = muon_direction(q.src, u[i][e], m[i][e]);
+        }
+      }
+      sum += sum_of_squares(u[i]);
+      float4 *to = reinterpret_cast<float4 *>(scratch + id * 8);
+      to[0] = make_float4(u[i][0], u[i][1], u[i][2], u[i][3]);
+      to[1] = make_float4(u[i][4], u[i][5], u[i][6], u[i][7]);
+    }
+  }
+  return sum;
+}
+
+// 32 columns of row `row` of Z or M, a row per lane: scale v + diag on the
+// diagonal, and zeros past the narrow side
+__device__ __forceinline__ void narrow_square(uint8_t *z, int part, int row, int col, int side, float scale, float diag,
+                                              const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = col + 8 * c + e;
+      y[e] = at < side ? v[8 * c + e] * scale + (row == at ? diag : 0.0f) : 0.0f;
+    }
+    uint4 hi, lo;
+    split8(y, hi, lo);
+    *reinterpret_cast<uint4 *>(z + narrow_at(row, col / 8 + c)) = hi;
+    *reinterpret_cast<uint4 *>(z + part + narrow_at(row, col / 8 + c)) = lo;
   }
 }
 
@@ -859,11 +951,9 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
   const auto cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int quad = warp & 3, half = warp >> 2;
+  const int quad = warp & 3;
   const int64_t base = (int64_t)(blockIdx.x / ctas) * q.rows * q.cols;
   const int panel0 = rank * q.panels / ctas, mine = (rank + 1) * q.panels / ctas - panel0;
-  const int side_panels = (q.side + 63) / 64;
-  const int per_panel = 64 / q.sub;
 
   if (tid == 0) {
     mbar_init(done, 1);
@@ -876,45 +966,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
     tmem_relinquish();
   }
 
-  // the slice, eight neighbours along the long side per chunk; lanes run
-  // along the axis that is contiguous in memory
-  float u[kMostChunks][8];
-  double sum = 0.0;
+  float *scratch = reinterpret_cast<float *>(smem + L::kZAt);  // 96 KB of what Z and the sums take later
   const int chunks = mine * 8;
-#pragma unroll
-  for (int i = 0; i < kMostChunks; ++i) {
-    const int id = i * kNarrowThreads + tid;
-    const int row = q.tall ? id & (kBM - 1) : id / (chunks > 0 ? chunks : 1);
-    const int chunk = q.tall ? id / kBM : id - row * chunks;
-    const int at = (panel0 * 8 + chunk) * 8;
-    const bool in = row < kBM && chunk < chunks && row < q.side;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      u[i][e] = 0.0f;
-      if (in && at + e < q.length) {
-        const int64_t g = base + (q.tall ? (int64_t)(at + e) * q.side + row : (int64_t)row * q.length + at + e);
-        u[i][e] = load_any(q.src.in, q.src.dtype, g);
-      }
-    }
-    if (q.src.momentum) {
-      float m[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        m[e] = 0.0f;
-        if (in && at + e < q.length)
-          m[e] = q.src.momentum[base + (q.tall ? (int64_t)(at + e) * q.side + row : (int64_t)row * q.length + at + e)];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (in && at + e < q.length) {
-          m[e] = fmaf(q.src.beta, m[e], q.src.rest * u[i][e]);
-          q.src.momentum[base + (q.tall ? (int64_t)(at + e) * q.side + row : (int64_t)row * q.length + at + e)] = m[e];
-          u[i][e] = muon_direction(q.src, u[i][e], m[e]);
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fma((double)u[i][e], (double)u[i][e], sum);
-  }
+  double sum = q.src.dtype == 0   ? narrow_load<float>(q, base, panel0 * 64, chunks, scratch)
+               : q.src.dtype == 1 ? narrow_load<__nv_bfloat16>(q, base, panel0 * 64, chunks, scratch)
+                                  : narrow_load<__half>(q, base, panel0 * 64, chunks, scratch);
   for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if (lane == 0) s_part[warp] = sum;
   __syncthreads();
@@ -933,27 +989,36 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
     for (int i = 0; i < ctas; ++i) total += norms[i];
     const double f64 = q.scale / (sqrt(total) + q.eps);
     const float f = (float)f64;
-    const bool in_32 = f64 > 1e-30 && f64 < 1e30;
+    auto split = [&](auto scaled) {
+#pragma unroll 2
+      for (int id = tid; id < kBM * chunks; id += kNarrowThreads) {
+        int row, chunk;
+        narrow_chunk(q, id, chunks, row, chunk);
+        float u[8];
+        *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(scratch + id * 8);
+        *reinterpret_cast<float4 *>(u + 4) = *reinterpret_cast<const float4 *>(scratch + id * 8 + 4);
 #pragma unroll
-    for (int i = 0; i < kMostChunks; ++i) {
-      const int id = i * kNarrowThreads + tid;
-      const int row = q.tall ? id & (kBM - 1) : id / (chunks > 0 ? chunks : 1);
-      const int chunk = q.tall ? id / kBM : id - row * chunks;
-      if (row >= kBM || chunk >= chunks) continue;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[i][e] = in_32 ? u[i][e] * f : (float)((double)u[i][e] * f64);
-      uint4 hi, lo;
-      split8(u[i], hi, lo);
-      *reinterpret_cast<uint4 *>(smem + narrow_at(row, chunk)) = hi;
-      *reinterpret_cast<uint4 *>(smem + L::kX + narrow_at(row, chunk)) = lo;
-    }
+        for (int e = 0; e < 8; ++e) u[e] = scaled(u[e]);
+        uint4 hi, lo;
+        split8(u, hi, lo);
+        *reinterpret_cast<uint4 *>(smem + narrow_at(row, chunk)) = hi;
+        *reinterpret_cast<uint4 *>(smem + L::kX + narrow_at(row, chunk)) = lo;
+      }
+    };
+    if (f64 > 1e-30 && f64 < 1e30)
+      split([=](float u) { return u * f; });
+    else
+      split([=](float u) { return (float)((double)u * f64); });  // a factor beyond is applied in 64 bits
   }
+
+  if (ctas > 1) cluster.sync();  // the scratch is read: partial sums may arrive in its place
 
   uint32_t parity = 0;
   const uint32_t x_at = smem_u32(smem), z_at = smem_u32(smem + L::kZAt);
-  // One product: `panels` of K, N columns; accumulators of q.sub of K each.
-  // b_mn: B's panels lie along N and K counts their rows.
-  auto product = [&](uint32_t a, uint32_t a_part, uint32_t b, uint32_t b_part, int panels, int n, bool b_mn) {
+  const int sub = q.sub / 16;  // K steps of 16 per accumulator
+  // One product: `ksteps` of 16, n columns.  b_mn: B's panels lie along N
+  // and K counts their rows.
+  auto product = [&](uint32_t a, uint32_t a_part, uint32_t b, uint32_t b_part, int ksteps, int n, bool b_mn) {
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
@@ -963,18 +1028,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
         const uint32_t idesc = idesc_f16(kBM, n, false, b_mn);
         // N along B's panels of 128 rows: the next 64 columns are a panel on
         const uint64_t da = desc_sw128(a, false), db = desc_sw128(b, b_mn, kBM * 128);
-        const uint32_t b_step = b_mn ? 2048u >> 4 : 32u >> 4;
-        const int steps = q.sub / 16;
-        for (int p = 0; p < panels; ++p)
-          for (int h = 0; h < per_panel; ++h)
-            for (int term = 0; term < 3; ++term)
-              for (int k = 0; k < steps; ++k) {
-                const uint32_t kk = (uint32_t)(h * steps + k);
-                const uint32_t ao = (((term == 1 ? a_part : 0u) + (uint32_t)p * (kBM * 128)) >> 4) + kk * (32u >> 4);
-                const uint32_t bo = (((term == 0 ? b_part : 0u) + (uint32_t)p * (b_mn ? 8192u : kBM * 128)) >> 4) +
-                                    kk * b_step;
-                umma_f16(tmem + (uint32_t)((p * per_panel + h) * n), da + ao, db + bo, idesc, (term | k) != 0);
-              }
+        for (int k0 = 0, acc = 0; k0 < ksteps; k0 += sub, acc += n)
+          for (int term = 0; term < 3; ++term)
+            for (int k = k0; k < k0 + sub && k < ksteps; ++k) {
+              const uint32_t along = (uint32_t)(k >> 2) * (kBM * 128) + (uint32_t)(k & 3) * 32;  // K-major
+              const uint32_t ao = (term == 1 ? a_part : 0u) + along;
+              const uint32_t bo = (term == 0 ? b_part : 0u) + (b_mn ? (uint32_t)k * 2048u : along);
+              umma_f16(tmem + (uint32_t)acc, da + (ao >> 4), db + (bo >> 4), idesc, term != 0 || k != k0);
+            }
         umma_commit(done);
       }
       __syncwarp();
@@ -985,84 +1046,85 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
     tc_fence_after();
   };
 
+  const int mine_steps = ((mine * 64 < q.length - panel0 * 64 ? mine * 64 : q.length - panel0 * 64) + 15) / 16;
+  const int side_steps = (q.side + 15) / 16, side_n = side_steps * 16;
+  const int mine_accs = (mine_steps + sub - 1) / sub, side_accs = (side_steps + sub - 1) / sub;
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-  const int row = quad * 32 + lane;
-  float v[64];
+  const int row = quad * 32 + lane, col = (warp >> 2) * 32;  // of this thread's 32 entries of Z and M
+  float v[32];
   for (int step = 0; step < q.steps; ++step) {
     // X X^T over this slice
-    product(x_at, L::kX, x_at, L::kX, mine, kBM, false);
-    read_sum(v, tmem + lanes + (uint32_t)(half * 64), mine * per_panel, kBM);
-    // partial sums to the CTA that owns the row: [source][4 columns][row]
-    const int own = kBM / ctas;
-    float4 *to = cluster.map_shared_rank(reinterpret_cast<float4 *>(smem + L::kRAt), row / own);
-    to += (rank * 32 + half * 16) * own + row % own;
+    product(x_at, L::kX, x_at, L::kX, mine_steps, side_n, false);
+    read_sum(v, tmem + lanes + (uint32_t)col, mine_accs, (uint32_t)side_n);
+    if (ctas == 1) {
+      narrow_square(smem + L::kZAt, L::kZ, row, col, q.side, q.scale1, q.diag1, v);
+    } else {
+      // partial sums to the CTA that owns the row, as [source][4 columns]
+      // [row], rows permuted so that the columns of a row spread over the
+      // banks; its rows of Z to all
+      const int own = kBM / ctas;
+      float4 *to = cluster.map_shared_rank(reinterpret_cast<float4 *>(smem + L::kRAt), row / own);
+      to += (rank * 32 + col / 4) * own;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) to[e * own] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-    cluster.sync();
-    const float4 *from = reinterpret_cast<const float4 *>(smem + L::kRAt);
-    for (int id = tid; id < own * 16; id += kNarrowThreads) {
-      const int r = id % own, c8 = id / own;
-      float y[8];
+      for (int e = 0; e < 8; ++e)
+        to[e * own + ((row % own) ^ ((col / 8 + e / 2) & 7))] =
+            make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+      cluster.sync();
+      const float4 *from = reinterpret_cast<const float4 *>(smem + L::kRAt);
+      for (int id = tid; id < own * 16; id += kNarrowThreads) {
+        const int r = id >> 4, c8 = id & 15, pos = r ^ (c8 & 7);
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-      for (int c = 0; c < ctas; ++c) {
-        const float4 f0 = from[(c * 32 + 2 * c8) * own + r], f1 = from[(c * 32 + 2 * c8 + 1) * own + r];
-        y[0] += f0.x;
-        y[1] += f0.y;
-        y[2] += f0.z;
-        y[3] += f0.w;
-        y[4] += f1.x;
-        y[5] += f1.y;
-        y[6] += f1.z;
-        y[7] += f1.w;
-      }
-      const int at = rank * own + r;
+        for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+        for (int c = 0; c < ctas; ++c) {
+          const float4 f0 = from[(c * 32 + 2 * c8) * own + pos], f1 = from[(c * 32 + 2 * c8 + 1) * own + pos];
+          y[0] += f0.x;
+          y[1] += f0.y;
+          y[2] += f0.z;
+          y[3] += f0.w;
+          y[4] += f1.x;
+          y[5] += f1.y;
+          y[6] += f1.z;
+          y[7] += f1.w;
+        }
+        const int at = rank * own + r;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] * q.scale1 + (at == 8 * c8 + e && at < q.side ? q.diag1 : 0.0f);
-      uint4 hi, lo;
-      split8(y, hi, lo);
-      for (int c = 0; c < ctas; ++c) {
-        uint8_t *z = cluster.map_shared_rank(smem + L::kZAt, c);
-        *reinterpret_cast<uint4 *>(z + narrow_at(at, c8)) = hi;
-        *reinterpret_cast<uint4 *>(z + L::kZ + narrow_at(at, c8)) = lo;
-      }
-    }
-    cluster.sync();
-    if (q.quintic) {
-      product(z_at, L::kZ, z_at, L::kZ, side_panels, kBM, false);
-      read_sum(v, tmem + lanes + (uint32_t)(half * 64), side_panels * per_panel, kBM);
-#pragma unroll
-      for (int e = 0; e < 64; ++e) v[e] *= q.scale2;
-#pragma unroll
-      for (int e = 0; e < 64; ++e)
-        if (row == half * 64 + e && row < q.side) v[e] += q.diag2;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
+        for (int e = 0; e < 8; ++e)
+          y[e] = 8 * c8 + e < q.side ? y[e] * q.scale1 + (at == 8 * c8 + e ? q.diag1 : 0.0f) : 0.0f;
         uint4 hi, lo;
-        split8(v + 8 * c, hi, lo);
-        *reinterpret_cast<uint4 *>(smem + L::kZAt + narrow_at(row, half * 8 + c)) = hi;
-        *reinterpret_cast<uint4 *>(smem + L::kZAt + L::kZ + narrow_at(row, half * 8 + c)) = lo;
+        split8(y, hi, lo);
+        for (int c = 0; c < ctas; ++c) {
+          uint8_t *z = cluster.map_shared_rank(smem + L::kZAt, c);
+          *reinterpret_cast<uint4 *>(z + narrow_at(at, c8)) = hi;
+          *reinterpret_cast<uint4 *>(z + L::kZ + narrow_at(at, c8)) = lo;
+        }
       }
+      cluster.sync();
+    }
+    if (q.quintic) {
+      product(z_at, L::kZ, z_at, L::kZ, side_steps, side_n, false);
+      read_sum(v, tmem + lanes + (uint32_t)col, side_accs, (uint32_t)side_n);
+      narrow_square(smem + L::kZAt, L::kZ, row, col, q.side, q.scale2, q.diag2, v);
     }
     // X <- M X
     const int n = mine * 64;
-    product(z_at, L::kZ, x_at, L::kX, side_panels, n, true);
+    product(z_at, L::kZ, x_at, L::kX, side_steps, n, true);
     const bool last = step + 1 == q.steps;
 #pragma unroll 1
-    for (int p = half; p < mine; p += 2) {
-      read_sum(v, tmem + lanes + (uint32_t)(p * 64), side_panels * per_panel, (uint32_t)n);
+    for (int c = col; c < n; c += 128) {
+      read_sum(v, tmem + lanes + (uint32_t)c, side_accs, (uint32_t)n);
       if (!last) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) v[e] *= q.inv;
+        for (int e = 0; e < 32; ++e) v[e] *= q.inv;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int k = 0; k < 4; ++k) {
           uint4 hi, lo;
-          split8(v + 8 * c, hi, lo);
-          *reinterpret_cast<uint4 *>(smem + narrow_at(row, p * 8 + c)) = hi;
-          *reinterpret_cast<uint4 *>(smem + L::kX + narrow_at(row, p * 8 + c)) = lo;
+          split8(v + 8 * k, hi, lo);
+          *reinterpret_cast<uint4 *>(smem + narrow_at(row, c / 8 + k)) = hi;
+          *reinterpret_cast<uint4 *>(smem + L::kX + narrow_at(row, c / 8 + k)) = lo;
         }
       } else {
-        narrow_out(q, base, quad * 32, (panel0 + p) * 64, v, reinterpret_cast<float *>(smem + L::kRAt) + warp * 1024);
+        narrow_out(q, base, quad * 32, panel0 * 64 + c, v, reinterpret_cast<float *>(smem + L::kRAt) + warp * 1024);
       }
     }
   }
@@ -1256,9 +1318,9 @@ cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, 
 }
 
 // Narrow matrices: the CTAs of a matrix's cluster, 0 where it does not fit.
-// A cluster takes about 30 us and 4 more per panel of its longest slice
-// (time of the phases that grow with it), in as many waves as the device's
-// clusters of that size make of the stack.
+// A single CTA takes about 30 us, a cluster's exchanges 25 more, and each
+// panel of the longest slice 4 (the phases that grow with it), in as many
+// waves as the device's clusters of that size make of the stack.
 int narrow_ctas(const scacchi_newton_schulz &n, const Device &d) {
   const int side = n.rows < n.cols ? n.rows : n.cols, panels = ((n.rows < n.cols ? n.cols : n.rows) + 63) / 64;
   if (side > kBM) return 0;
@@ -1267,7 +1329,7 @@ int narrow_ctas(const scacchi_newton_schulz &n, const Device &d) {
   for (int z = 0; z < 4; ++z) {
     const int ctas = 1 << z, slice = (panels + ctas - 1) / ctas, at_once = z ? d.clusters[z] : d.sms;
     if (slice > NarrowLayout::kMostPanels || ctas > panels) continue;
-    const int64_t cost = ((int64_t)n.batch + at_once - 1) / at_once * (30 + 4 * slice);
+    const int64_t cost = ((int64_t)n.batch + at_once - 1) / at_once * ((z ? 55 : 30) + 4 * slice);
     if (!best || cost < best_cost) {
       best = ctas;
       best_cost = cost;
