@@ -1028,14 +1028,23 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
         const uint32_t idesc = idesc_f16(kBM, n, false, b_mn);
         // N along B's panels of 128 rows: the next 64 columns are a panel on
         const uint64_t da = desc_sw128(a, false), db = desc_sw128(b, b_mn, kBM * 128);
-        for (int k0 = 0, acc = 0; k0 < ksteps; k0 += sub, acc += n)
-          for (int term = 0; term < 3; ++term)
-            for (int k = k0; k < k0 + sub && k < ksteps; ++k) {
-              const uint32_t along = (uint32_t)(k >> 2) * (kBM * 128) + (uint32_t)(k & 3) * 32;  // K-major
-              const uint32_t ao = (term == 1 ? a_part : 0u) + along;
-              const uint32_t bo = (term == 0 ? b_part : 0u) + (b_mn ? (uint32_t)k * 2048u : along);
-              umma_f16(tmem + (uint32_t)acc, da + (ao >> 4), db + (bo >> 4), idesc, term != 0 || k != k0);
-            }
+        // unrolled by accumulators of 32 of K: a loop over single MMAs took
+        // longer to issue than they run
+        const uint32_t a_lo = a_part >> 4, b_lo = b_part >> 4, b_step = b_mn ? 2048u >> 4 : 32u >> 4;
+        uint32_t d = tmem;
+        for (int k0 = 0; k0 < ksteps; k0 += 2) {
+          const uint32_t along = ((uint32_t)(k0 >> 2) * (kBM * 128) + (uint32_t)(k0 & 3) * 32) >> 4;  // K-major
+          const uint64_t ka = da + along, kb = db + (b_mn ? (uint32_t)k0 * b_step : along);
+          const bool two = k0 + 1 < ksteps;
+          const uint32_t more = sub == 4 ? (uint32_t)(k0 & 2) : 0u;  // the second half of a 64-wide accumulator
+          umma_f16(d, ka, kb + b_lo, idesc, more);
+          if (two) umma_f16(d, ka + 2, kb + b_step + b_lo, idesc, 1u);
+          umma_f16(d, ka + a_lo, kb, idesc, 1u);
+          if (two) umma_f16(d, ka + a_lo + 2, kb + b_step, idesc, 1u);
+          umma_f16(d, ka, kb, idesc, 1u);
+          if (two) umma_f16(d, ka + 2, kb + b_step, idesc, 1u);
+          if (sub == 2 || more) d += (uint32_t)n;
+        }
         umma_commit(done);
       }
       __syncwarp();

@@ -19,14 +19,17 @@
 // phi's form keeps the KL's leading digits when the two policies are near
 // each other, where sum p (log p - log q) in 32 bits loses them.
 //
-// One pass: a row's logits (and reference logits) are loaded once into the
-// registers of its group of threads, reduced there, and its gradient is
-// written from them, so the traffic is one read per input and one write
-// per output, and the kernel is bound by HBM on large batches.  Row sums
-// are held in 32 bits, the log-probability is finished in 64 from them and
+// One pass over memory: short rows live in the registers of a few lanes,
+// long ones in the shared memory of a CTA or of a cluster, so every input is
+// read once and every output written once.  Row sums are held in 32 bits, the log-probability is finished in 64 from them and
 // the loss is summed in 64.  A row whose ratio lies within kBorderTol of a
 // clip border is evaluated again in 64 bits, so the side it falls on does
 // not depend on 32-bit rounding.
+//
+// Exponentials are ex2.approx of (x - m) log2 e: the difference first, so
+// that only |x - m|, which p weights, is rounded and scaled; their errors
+// (2^-22, and |x - m| 2^-24) average out over a row's sum.  The accurate
+// expf() takes three times the instructions and made the kernel issue-bound.
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -46,17 +49,21 @@ namespace {
 std::atomic<uint64_t> g_policy_launches{0};
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kSubThreads = 256;   // CTA of the several-rows-per-warp kernel
-constexpr int kMaxWarps = 16;      // CTA of the row-per-CTA kernel: 512 threads
+constexpr int kShortThreads = 256;
+constexpr int kLongThreads = 512;
+constexpr int kMaxWarps = kLongThreads / 32;
 constexpr int kMaxCluster = 16;
-constexpr int kMaxSubActions = 512;
-constexpr int kMaxActions = kMaxCluster * 512 * 32;
+constexpr int kMaxShort = 512;     // actions of a short row
+constexpr int kMaxActions = 262144;
+constexpr int kLongShared = 224 * 1024;  // of an SM, for the slices of its CTAs
 constexpr int kMaxPartials = 148 * 16;
 // the 32-bit log-probability is within 3e-6 of the exact one: terms within
-// 2^-24 |x - m| + 2 ulp each weighted by p (sum p |x - m| <= 13 at 2^18
-// actions: 1e-6) and up to 32 rounded adds per thread plus the tree (2e-6)
+// 2^-24 |x - m| + 2^-22 each, weighted by p (sum p |x - m| <= 13 at 2^18
+// actions: 1e-6), and the adds of up to 64 values per thread, in eight
+// chains, plus the tree (2e-6)
 constexpr double kBorderTol = 8e-6;
 constexpr float kFarKl = 1.0e4f;   // sum p phi above this (KL > 9): the direct difference is exact enough
+constexpr float kLog2E = 1.44269504088896341f;
 
 struct Params {
   const void *logits, *reference;
@@ -68,7 +75,9 @@ struct Params {
   void *grad;
   double *partial;
   int64_t rows, stride, reference_stride;
-  int actions, group;
+  int actions;
+  int group;        // lanes of a short row
+  int slice_bytes;  // of a long row's logits in one CTA
   double clip_low, clip_high, log_low, log_high;  // borders of the ratio and their logarithms
   float beta, even_weight;
 };
@@ -111,6 +120,13 @@ __device__ __forceinline__ float phi_small(float y) {
   return c * y * y;
 }
 
+// e^u for u <= 0 or small (see above)
+__device__ __forceinline__ float exp_fast(float u) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(u * kLog2E));
+  return y;
+}
+
 // log of a positive finite float to 1e-9: s = 2^k f with f in [1/sqrt 2,
 // sqrt 2), log f = 2 atanh(q), q = (f - 1) / (f + 1), |q| < 0.172: the odd
 // series to q^11 in 64 bits (next term 2e-11).  Zero, infinity and NaN go
@@ -138,7 +154,7 @@ __device__ __forceinline__ double log_row_sum(float s) {
 }
 
 // ---------------------------------------------------------------------------
-// the threads of one row: G lanes of a warp, or the CTAs of a cluster
+// the threads of one row: some lanes of a warp, or the CTAs of a cluster
 // ---------------------------------------------------------------------------
 
 struct SumOp {
@@ -150,12 +166,20 @@ struct MaxOp {
   __device__ static U apply(U a, U b) { return a > b ? a : b; }
 };
 
-template <bool Cta>
-struct Group;
+// max, sum of e^{x - max} and of d e^{x - max}
+struct Stats {
+  float top, sum, mean;
+};
+
+__device__ __forceinline__ void rescale(Stats &v, float top) {
+  const float f = v.top == -INFINITY ? 0.0f : exp_fast(v.top - top);
+  v.sum *= f;
+  v.mean *= f;
+  v.top = top;
+}
 
 // every lane ends with the same bits: the butterfly adds the same pairs
-template <>
-struct Group<false> {
+struct Lanes {
   int lanes;
   unsigned mask;
   __device__ int index() const { return threadIdx.x & (lanes - 1); }
@@ -169,9 +193,9 @@ struct Group<false> {
 
 // warp butterflies, then the warps' results of every CTA of the cluster in
 // rank and warp order, which is the same for every thread
-template <>
-struct Group<true> {
-  double *slots;  // shared: two banks of kMaxWarps partials, alternating
+struct Ctas {
+  double *slots;      // shared: two banks of kMaxWarps partials, taken in turn
+  Stats *stat_slots;  // likewise
   int ctas, rank;
   mutable int bank;
   __device__ int index() const { return rank * blockDim.x + threadIdx.x; }
@@ -182,11 +206,11 @@ struct Group<true> {
     else
       __syncthreads();
   }
+  // A bank is written again two reductions later, and every thread has
+  // passed the barrier of the one between them, so its readers are done.
   template <typename Op, typename U>
   __device__ U reduce(U v) const {
     for (int off = 16; off; off >>= 1) v = Op::apply(v, __shfl_xor_sync(kFull, v, off));
-    // a bank is written again two reductions later, and every thread has
-    // passed the barrier between them, so its readers are done
     double *mine = slots + bank * kMaxWarps;
     bank ^= 1;
     if ((threadIdx.x & 31) == 0) *reinterpret_cast<U *>(mine + (threadIdx.x >> 5)) = v;
@@ -202,13 +226,49 @@ struct Group<true> {
     }
     return r;
   }
+  // One barrier for all three: each warp's maximum scales its sums; every
+  // lane then folds some of the warps' and a butterfly the rest.
+  __device__ Stats stats(Stats v) const {
+    float top = v.top;
+    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+    rescale(v, top);
+    for (int off = 16; off; off >>= 1) {
+      v.sum += __shfl_xor_sync(kFull, v.sum, off);
+      v.mean += __shfl_xor_sync(kFull, v.mean, off);
+    }
+    Stats *mine = stat_slots + bank * kMaxWarps;
+    bank ^= 1;
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, total = ctas * warps;
+    if (lane == 0) mine[threadIdx.x >> 5] = v;
+    sync();
+    Stats all = {-INFINITY, 0.0f, 0.0f};
+    for (int i = 0; i < total; i += 32) {
+      Stats u = {-INFINITY, 0.0f, 0.0f};
+      if (i + lane < total) {
+        const int c = (i + lane) / warps;
+        const Stats *from = ctas > 1 ? cg::this_cluster().map_shared_rank(mine, c) : mine;
+        u = from[i + lane - c * warps];
+      }
+      top = fmaxf(all.top, u.top);
+      for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+      rescale(all, top);
+      rescale(u, top);
+      all.sum += u.sum;
+      all.mean += u.mean;
+    }
+    for (int off = 16; off; off >>= 1) {
+      all.sum += __shfl_xor_sync(kFull, all.sum, off);
+      all.mean += __shfl_xor_sync(kFull, all.mean, off);
+    }
+    return all;
+  }
 };
 
 // A row in 64 bits, read again: log sum e^x over the kept actions, and
 // with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r).
 // Taken by the few rows next to a clip border or far from the reference.
-template <typename T, bool Cta>
-__device__ __noinline__ double2 row_in_64(const Group<Cta> &grp, const T *x, const T *r, const uint8_t *legal, int A,
+template <typename T, typename Grp>
+__device__ __noinline__ double2 row_in_64(const Grp &grp, const T *x, const T *r, const uint8_t *legal, int A,
                                           float top, bool want_kl) {
   double s = 0.0, sd = 0.0, rtop = -INFINITY;
   for (int a = grp.index(); a < A; a += grp.size()) {
@@ -243,22 +303,104 @@ __device__ __noinline__ double2 row_in_64(const Group<Cta> &grp, const T *x, con
 // one row
 // ---------------------------------------------------------------------------
 
+// A row's scalars, all requested with its logits: each met late would stall
+// the row for a memory latency of its own.
+struct RowIn {
+  float xk, old, adv, ref;
+  bool counts;
+};
+
+template <typename T>
+__device__ __forceinline__ RowIn row_in(const Params &p, int64_t row, const T *x, const uint8_t *legal, int k,
+                                        bool counts) {
+  RowIn in = {0.0f, 0.0f, 0.0f, 0.0f, counts};
+  if (counts) {
+    in.xk = to_f(x[k]);
+    const bool allowed = !legal || legal[k];
+    in.old = p.old_log_prob[row];
+    in.adv = p.advantage[row];
+    if (p.reference_log_prob) in.ref = p.reference_log_prob[row];
+    in.counts = allowed && in.xk != -INFINITY;
+  }
+  return in;
+}
+
+// What a row's gradient is made of: g_a = p_a ((d_a - mean) wb - wc), plus wc
+// at the action.
+struct RowOut {
+  double share;
+  float wc, wb;
+};
+
+// The row's statistics from its sums, by every thread alike; thread 0 of the
+// group writes them.
+template <typename T, bool Kl, typename Grp>
+__device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, int64_t row, float weight,
+                                             const RowIn &in, const T *x, const T *r, const uint8_t *legal, float top,
+                                             float sum, float kl_sum) {
+  double lp = ((double)in.xk - (double)top) - log_row_sum(sum), delta = lp - (double)in.old;
+  const bool far = Kl && !(kl_sum < kFarKl);
+  float kl = Kl ? log1pf(kl_sum) : 0.0f;
+  if (far || fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol) {
+    const double2 fine = row_in_64<T>(grp, x, r, legal, p.actions, top, far);
+    lp = (double)in.xk - fine.x;
+    delta = lp - (double)in.old;
+    if (far) kl = (float)fine.y;
+  }
+  const bool clipped = in.adv >= 0.0f ? delta > p.log_high : delta < p.log_low;
+  const float ratio = expf((float)delta);
+  // an advantage of 0 adds nothing, whatever the ratio overflows to
+  float c = clipped || in.adv == 0.0f ? 0.0f : -in.adv * ratio;
+  double term = clipped ? -(double)in.adv * (in.adv >= 0.0f ? p.clip_high : p.clip_low) : (double)c;
+  if (!Kl && p.reference_log_prob) {
+    const float y = (float)((double)in.ref - lp), em = expm1f(y);
+    kl = fabsf(y) < 1.0f ? phi_small(y) : em - y;
+    c = fmaf(-p.beta, em, c);
+  }
+  term += (double)p.beta * (double)kl;
+  if (grp.index() == 0) {
+    p.log_prob[row] = (float)lp;
+    p.clipped[row] = clipped;
+    if (p.kl) p.kl[row] = kl;
+  }
+  return RowOut{(double)weight * term, weight * c, weight * p.beta};
+}
+
+__device__ __forceinline__ void empty_row(const Params &p, int64_t row) {
+  p.log_prob[row] = 0.0f;
+  p.clipped[row] = 0;
+  if (p.kl) p.kl[row] = 0.0f;
+}
+
+// p phi(mean - d) of one action.  An e^y that overflows, or meets a p that
+// underflowed, makes the row a far one; an illegal place (p = 0, d = 0) has
+// no part.
+__device__ __forceinline__ float kl_part(float pa, float d, float mean) {
+  const float y = mean - d;
+  float part = pa * phi_small(y);
+  if (!(fabsf(y) < 1.0f))
+    part = pa > 0.0f ? fmaf(pa, expf(y), -pa * (1.0f + y)) : (y > 60.0f && d != 0.0f ? INFINITY : pa * 0.0f);
+  return part;
+}
+
+// ---------------------------------------------------------------------------
+// short rows: `group` lanes of a warp each, their elements in registers
+// ---------------------------------------------------------------------------
+
 // V vectors of W elements per thread; thread t of the group holds vectors
 // t, t + G, ... of the row.  Returns the row's share of the loss.
-template <typename T, int W, int V, bool Kl, bool Cta>
-__device__ __forceinline__ double one_row(const Params &p, const Group<Cta> &grp, int64_t row, float weight, int k) {
+template <typename T, int W, int V, bool Kl>
+__device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, int64_t row, float weight, int k) {
   const int A = p.actions, t = grp.index(), G = grp.size();
   const T *x = static_cast<const T *>(p.logits) + row * p.stride;
   const T *r = Kl ? static_cast<const T *>(p.reference) + row * p.reference_stride : nullptr;
   const uint8_t *legal = p.legal ? p.legal + row * A : nullptr;
   T *grad = p.grad ? static_cast<T *>(p.grad) + row * A : nullptr;
-  bool counts = weight != 0.0f && k >= 0 && k < A;
-  float xk = 0.0f;
   using Pack = Vec<T, W>;
   Pack xv[V], rv[Kl ? V : 1];
   Vec<uint8_t, W> lv[V];
-  if (counts) {
-    // every load of the row is issued before the first is used
+  const bool wanted = weight != 0.0f && k >= 0 && k < A;
+  if (wanted) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int a = (v * G + t) * W;
@@ -268,15 +410,10 @@ __device__ __forceinline__ double one_row(const Params &p, const Group<Cta> &grp
         if (legal) lv[v] = *reinterpret_cast<const Vec<uint8_t, W> *>(legal + a);
       }
     }
-    xk = to_f(x[k]);
-    counts = !(legal && !legal[k]) && xk != -INFINITY;
   }
-  if (!counts) {
-    if (t == 0) {
-      p.log_prob[row] = 0.0f;
-      p.clipped[row] = 0;
-      if (p.kl) p.kl[row] = 0.0f;
-    }
+  const RowIn in = row_in<T>(p, row, x, legal, k, wanted);
+  if (!in.counts) {
+    if (t == 0) empty_row(p, row);
     if (grad) {
       Pack z;
 #pragma unroll
@@ -290,106 +427,61 @@ __device__ __forceinline__ double one_row(const Params &p, const Group<Cta> &grp
     return 0.0;
   }
   // illegal actions become -inf, as places past the row are
-  float top = -INFINITY;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const bool in = (v * G + t) * W < A;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (!in || (legal && !lv[v].v[w])) xv[v].v[w] = from_f<T>(-INFINITY);
-      top = fmaxf(top, to_f(xv[v].v[w]));
-    }
-  }
-  top = grp.template reduce<MaxOp>(top);
-  float s = 0.0f, sd = 0.0f;
+  float e[V * W], d[Kl ? V * W : 1], top = -INFINITY;
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float xa = to_f(xv[v].v[w]);
-      const float e = expf(xa - top);
-      s += e;
-      if (Kl && xa != -INFINITY) sd = fmaf(e, xa - to_f(rv[Kl ? v : 0].v[w]), sd);
+      const int i = v * W + w;
+      const bool keep = (v * G + t) * W < A && (!legal || lv[v].v[w]);
+      e[i] = keep ? to_f(xv[v].v[w]) : -INFINITY;
+      top = fmaxf(top, e[i]);
+      if (Kl) d[Kl ? i : 0] = e[i] == -INFINITY ? 0.0f : e[i] - to_f(rv[Kl ? v : 0].v[w]);
     }
-  s = grp.template reduce<SumOp>(s);
-  const float inv = 1.0f / s;
-  double lp = ((double)xk - (double)top) - log_row_sum(s);
-  float kl = 0.0f, mean = 0.0f;
-  bool far = false;
+  top = grp.reduce<MaxOp>(top);
+  float sum = 0.0f, mean = 0.0f, kl = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V * W; ++i) {
+    e[i] = exp_fast(e[i] - top);
+    sum += e[i];
+    if (Kl) mean = fmaf(e[i], d[Kl ? i : 0], mean);
+  }
+  sum = grp.reduce<SumOp>(sum);
+  const float inv = 1.0f / sum;
   if (Kl) {
-    mean = grp.template reduce<SumOp>(sd) * inv;
-    float q = 0.0f;
+    mean = grp.reduce<SumOp>(mean) * inv;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float xa = to_f(xv[v].v[w]);
-        if (xa != -INFINITY) {
-          const float ra = to_f(rv[Kl ? v : 0].v[w]);
-          const float y = mean - (xa - ra), pa = expf(xa - top) * inv;
-          // p e^y = e^{r + mu - m} / s, which cannot overflow before the KL does
-          q += fabsf(y) < 1.0f ? pa * phi_small(y) : expf((ra + mean) - top) * inv - pa * (1.0f + y);
-        }
-      }
-    q = grp.template reduce<SumOp>(q);
-    far = !(q < kFarKl);
-    kl = log1pf(q);
+    for (int i = 0; i < V * W; ++i) kl += kl_part(e[i] * inv, d[Kl ? i : 0], mean);
+    kl = grp.reduce<SumOp>(kl);
   }
-  double delta = lp - (double)p.old_log_prob[row];
-  if (far || fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol) {
-    const double2 fine = row_in_64<T, Cta>(grp, x, r, legal, A, top, far);
-    lp = (double)xk - fine.x;
-    delta = lp - (double)p.old_log_prob[row];
-    if (far) kl = (float)fine.y;
-  }
-  const float adv = p.advantage[row];
-  const bool clipped = adv >= 0.0f ? delta > p.log_high : delta < p.log_low;
-  const float ratio = expf((float)delta);
-  // an advantage of 0 adds nothing, whatever the ratio overflows to
-  float c = clipped || adv == 0.0f ? 0.0f : -adv * ratio;
-  double term = clipped ? -(double)adv * (adv >= 0.0f ? p.clip_high : p.clip_low) : (double)c;
-  if (!Kl && p.reference_log_prob) {
-    const float y = (float)((double)p.reference_log_prob[row] - lp);
-    const float em = expm1f(y);
-    kl = fabsf(y) < 1.0f ? phi_small(y) : em - y;
-    c = fmaf(-p.beta, em, c);
-  }
-  term += (double)p.beta * (double)kl;
-  if (t == 0) {
-    p.log_prob[row] = (float)lp;
-    p.clipped[row] = clipped;
-    if (p.kl) p.kl[row] = kl;
-  }
+  const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, x, r, legal, top, sum, kl);
   if (grad) {
-    const float wc = weight * c, wb = weight * p.beta;
+    const float wc = -out.wc * inv, wb = out.wb * inv;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int a = (v * G + t) * W;
       Pack o;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float xa = to_f(xv[v].v[w]);
-        float g = -wc;
-        if (Kl && xa != -INFINITY) g = fmaf(wb, (xa - to_f(rv[Kl ? v : 0].v[w])) - mean, g);
-        g *= expf(xa - top) * inv;
-        if (a + w == k) g += wc;
-        o.v[w] = from_f<T>(xa == -INFINITY ? 0.0f : g);
+        const int i = v * W + w;
+        float g = (Kl ? fmaf(wb, d[Kl ? i : 0] - mean, wc) : wc) * e[i];
+        if (a + w == k) g += out.wc;
+        o.v[w] = from_f<T>(g);
       }
       if (a < A) *reinterpret_cast<Pack *>(grad + a) = o;
     }
   }
-  return (double)weight * term;
+  return out.share;
 }
 
-// Several rows per warp: `group` lanes each.
 template <typename T, int W, int V, bool Kl>
-__global__ void __launch_bounds__(kSubThreads) policy_loss_rows_kernel(Params p) {
-  __shared__ double s_part[kSubThreads / 32];
+__global__ void __launch_bounds__(kShortThreads, V * W <= 8 ? 4 : 2) policy_loss_short_kernel(Params p) {
+  __shared__ double s_part[kShortThreads / 32];
   const int lane = threadIdx.x & 31, G = p.group;
-  Group<false> grp;
+  Lanes grp;
   grp.lanes = G;
   grp.mask = G == 32 ? kFull : ((1u << G) - 1u) << (lane & ~(G - 1));
-  const int per_cta = kSubThreads / G;
+  const int per_cta = kShortThreads / G;
   double sum = 0.0;
   int64_t row = (int64_t)blockIdx.x * per_cta + threadIdx.x / G;
   const int64_t step = (int64_t)gridDim.x * per_cta;
@@ -407,7 +499,7 @@ __global__ void __launch_bounds__(kSubThreads) policy_loss_rows_kernel(Params p)
       w_next = p.weight ? p.weight[row + step] : p.even_weight;
       k_next = p.action[row + step];
     }
-    const double share = one_row<T, W, V, Kl, false>(p, grp, row, w, k);
+    const double share = short_row<T, W, V, Kl>(p, grp, row, w, k);
     if (grp.index() == 0) sum += share;
   }
   __syncwarp();
@@ -416,7 +508,7 @@ __global__ void __launch_bounds__(kSubThreads) policy_loss_rows_kernel(Params p)
   __syncthreads();
   if (threadIdx.x == 0) {
     double total = 0.0;
-    for (int i = 0; i < kSubThreads / 32; ++i) total += s_part[i];
+    for (int i = 0; i < kShortThreads / 32; ++i) total += s_part[i];
     if (gridDim.x == 1)
       p.loss[0] = (float)total;
     else
@@ -424,26 +516,177 @@ __global__ void __launch_bounds__(kSubThreads) policy_loss_rows_kernel(Params p)
   }
 }
 
-// One row per CTA, or per cluster of CTAs.
-template <typename T, int W, int V, bool Kl>
-__global__ void __launch_bounds__(512) policy_loss_cta_kernel(Params p) {
+// ---------------------------------------------------------------------------
+// long rows: a CTA each, or a cluster's slices, in shared memory
+// ---------------------------------------------------------------------------
+
+// the place of `from` within 16 bytes, in elements
+template <typename E>
+__device__ __forceinline__ int phase_of(const E *from) {
+  return (int)((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(E));
+}
+
+// Loads `count` elements to shared memory, at the same place within 16 bytes
+// as in global memory, so that whole vectors move at any alignment: 16-byte
+// asynchronous copies in the middle, elements at the ends.
+template <typename E>
+__device__ __forceinline__ void stage(E *to, const E *from, int count, int t, int threads) {
+  constexpr int kVec = 16 / (int)sizeof(E);
+  const int head = (kVec - phase_of(from)) % kVec;
+  const int first = head < count ? head : count, vecs = (count - first) / kVec, tail = first + vecs * kVec;
+  for (int i = t; i < vecs; i += threads) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to + first + i * kVec);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from + first + i * kVec) : "memory");
+  }
+  if (t < first) to[t] = from[t];
+  if (t < count - tail) to[tail + t] = from[tail + t];
+}
+
+// Passes over the slice's elements, W at a time where the row's arrays start
+// at the same place within a vector (vector v then holds elements v W -
+// lead.. of each), else by themselves (W = 1).
+//
+// Three passes read shared memory: the online maximum and sums, the KL's
+// sum, the gradient; each computes e^x again, which is cheaper than the
+// registers or the memory to keep it (and lets two to sixteen CTAs share an
+// SM, so that one loads while others compute).
+template <typename T, int W, bool Kl>
+__global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Params p) {
+  extern __shared__ __align__(16) uint8_t s_rows[];
   __shared__ double s_slots[2 * kMaxWarps];
-  Group<true> grp;
+  __shared__ Stats s_stats[2 * kMaxWarps];
+  using Pack = Vec<T, W>;
+  using Mask = Vec<uint8_t, W>;
+  Ctas grp;
   grp.slots = s_slots;
+  grp.stat_slots = s_stats;
   grp.ctas = (int)cg::this_cluster().num_blocks();
   grp.rank = (int)cg::this_cluster().block_rank();
   grp.bank = 0;
+  const int A = p.actions, t = threadIdx.x, threads = blockDim.x;
+  const int lo = (int)((int64_t)A * grp.rank / grp.ctas) / 16 * 16;
+  const int hi = grp.rank + 1 == grp.ctas ? A : (int)((int64_t)A * (grp.rank + 1) / grp.ctas) / 16 * 16;
+  const int n = hi - lo;
+  T *const sx_at = reinterpret_cast<T *>(s_rows);
+  T *const sr_at = reinterpret_cast<T *>(s_rows + p.slice_bytes);
+  uint8_t *const sl_at = s_rows + (Kl ? 2 : 1) * p.slice_bytes;
   const int64_t first = blockIdx.x / grp.ctas, step = gridDim.x / grp.ctas;
-  double sum = 0.0;
+  double share = 0.0;
   for (int64_t row = first; row < p.rows; row += step) {
-    const float w = p.weight ? p.weight[row] : p.even_weight;
-    sum += one_row<T, W, V, Kl, true>(p, grp, row, w, p.action[row]);
+    const float weight = p.weight ? p.weight[row] : p.even_weight;
+    const int k = p.action[row];
+    const T *x = static_cast<const T *>(p.logits) + row * p.stride;
+    const T *r = Kl ? static_cast<const T *>(p.reference) + row * p.reference_stride : nullptr;
+    const uint8_t *legal = p.legal ? p.legal + row * A : nullptr;
+    T *grad = p.grad ? static_cast<T *>(p.grad) + row * A + lo : nullptr;
+    const bool wanted = weight != 0.0f && k >= 0 && k < A;
+    T *sx = sx_at + phase_of(x + lo), *sr = sr_at;
+    uint8_t *sl = sl_at;
+    if (wanted) {
+      stage(sx, x + lo, n, t, threads);
+      if (Kl) {
+        sr += phase_of(r + lo);
+        stage(sr, r + lo, n, t, threads);
+      }
+      if (legal) {
+        sl += phase_of(legal + lo);
+        stage(sl, legal + lo, n, t, threads);
+      }
+    }
+    const RowIn in = row_in<T>(p, row, x, legal, k, wanted);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    if (!in.counts) {
+      if (grp.index() == 0) empty_row(p, row);
+      if (grad)
+        for (int i = t; i < n; i += threads) grad[i] = from_f<T>(0.0f);
+      __syncthreads();
+      continue;
+    }
+    // vector v covers elements v W - lead .. + W - 1
+    const int lead = phase_of(x + lo) % W, vecs = (n + lead + W - 1) / W;
+    // logits, and the difference to the reference, of one vector; -inf and 0
+    // where there is no kept action
+    auto load = [&](int v, float(&xa)[W], float(&da)[W]) {
+      const int a = v * W - lead;
+      const Pack xv = *reinterpret_cast<const Pack *>(sx + a);
+      Pack rv;
+      Mask lv;
+      if (Kl) rv = *reinterpret_cast<const Pack *>(sr + a);
+      if (legal) lv = *reinterpret_cast<const Mask *>(sl + a);
+      const bool whole = a >= 0 && a + W <= n;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        xa[w] = to_f(xv.v[w]);
+        if ((!whole && (a + w < 0 || a + w >= n)) || (legal && !lv.v[w])) xa[w] = -INFINITY;
+        da[w] = 0.0f;
+        if (Kl && xa[w] != -INFINITY) da[w] = xa[w] - to_f(rv.v[w]);
+      }
+    };
+    Stats st = {-INFINITY, 0.0f, 0.0f};
+    for (int v = t; v < vecs; v += threads) {
+      float xa[W], da[W], top = -INFINITY;
+      load(v, xa, da);
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, xa[w]);
+      if (top > st.top) rescale(st, top);
+      // without an action yet, only a NaN among them has a part in the sum
+      const float from = st.top == -INFINITY ? 0.0f : st.top;
+      float sum[2] = {0.0f, 0.0f}, mean[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float e = exp_fast(xa[w] - from);
+        sum[w & 1] += e;
+        if (Kl) mean[w & 1] = fmaf(e, da[w], mean[w & 1]);
+      }
+      st.sum += sum[0] + sum[1];
+      if (Kl) st.mean += mean[0] + mean[1];
+    }
+    st = grp.stats(st);
+    const float inv = 1.0f / st.sum, mean = st.mean * inv;
+    float kl = 0.0f;
+    if (Kl) {
+      for (int v = t; v < vecs; v += threads) {
+        float xa[W], da[W], part = 0.0f;
+        load(v, xa, da);
+#pragma unroll
+        for (int w = 0; w < W; ++w) part += kl_part(exp_fast(xa[w] - st.top) * inv, da[w], mean);
+        kl += part;
+      }
+      kl = grp.reduce<SumOp>(kl);
+    }
+    const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, x, r, legal, st.top, st.sum, kl);
+    share += out.share;
+    if (grad) {
+      const float wc = -out.wc * inv, wb = out.wb * inv;
+      const int at_k = k - lo;
+      for (int v = t; v < vecs; v += threads) {
+        float xa[W], da[W];
+        load(v, xa, da);
+        const int a = v * W - lead;
+        Pack o;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          float g = (Kl ? fmaf(wb, da[w] - mean, wc) : wc) * exp_fast(xa[w] - st.top);
+          if (a + w == at_k) g += out.wc;
+          o.v[w] = from_f<T>(g);
+        }
+        if (a >= 0 && a + W <= n) {
+          *reinterpret_cast<Pack *>(grad + a) = o;
+        } else {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (a + w >= 0 && a + w < n) grad[a + w] = o.v[w];
+        }
+      }
+    }
+    __syncthreads();  // the slice is read: the next row may take its place
   }
   if (grp.index() == 0) {
     if (step == 1)
-      p.loss[0] = (float)sum;
+      p.loss[0] = (float)share;
     else
-      p.partial[first] = sum;
+      p.partial[first] = share;
   }
   if (grp.ctas > 1) cg::this_cluster().sync();  // a CTA's slots outlive their readers
 }
@@ -477,23 +720,74 @@ int sm_count() {
 }
 
 template <typename T, int W, int V, bool Kl>
-cudaError_t launch_rows(const Params &p, int *ctas, cudaStream_t st) {
-  const int per_cta = kSubThreads / p.group;
+cudaError_t launch_short(const Params &p, int *ctas, cudaStream_t st) {
+  const int per_cta = kShortThreads / p.group;
   const int64_t need = (p.rows + per_cta - 1) / per_cta;
   const int most = sm_count() * 8 < kMaxPartials ? sm_count() * 8 : kMaxPartials;
   *ctas = (int)(need < most ? need : most);
-  policy_loss_rows_kernel<T, W, V, Kl><<<*ctas, kSubThreads, 0, st>>>(p);
+  policy_loss_short_kernel<T, W, V, Kl><<<*ctas, kShortThreads, 0, st>>>(p);
   return cudaPeekAtLastError();
 }
 
-template <typename T, int W, int V, bool Kl>
-cudaError_t launch_cta(const Params &p, int threads, int cluster, int *ctas, cudaStream_t st) {
-  const int most = sm_count() * 4 / cluster;
-  const int clusters = (int)(p.rows < most ? p.rows : most);
-  *ctas = clusters;
+// Lanes of a short row: 4 to 32, with 4 to 16 elements each: the split with
+// the fewest idle places, and among those the most lanes (fewer registers a
+// thread, more rows in flight an SM).
+template <typename T, int W, bool Kl>
+cudaError_t by_lanes(Params &p, int *ctas, cudaStream_t st) {
+  constexpr int kElems[] = {4, 6, 8, 12, 16};
+  int best = 0, elems = 0;
+  for (int e : kElems)
+    for (int g = 4; g <= 32; g *= 2)
+      if (g * e >= p.actions && (!best || g * e < best * elems || (g * e == best * elems && g > best))) {
+        best = g;
+        elems = e;
+      }
+  p.group = best;
+  if (elems == 4) return launch_short<T, W, 4 / W, Kl>(p, ctas, st);
+  if (elems == 6) return launch_short<T, W, 6 / W, Kl>(p, ctas, st);
+  if (elems == 8) return launch_short<T, W, 8 / W, Kl>(p, ctas, st);
+  if (elems == 12) return launch_short<T, W, 12 / W, Kl>(p, ctas, st);
+  return launch_short<T, W, 16 / W, Kl>(p, ctas, st);
+}
+
+// Long rows: a cluster where half an SM's shared memory does not hold the
+// row, or where the rows leave SMs idle (down to 4096 actions a CTA);
+// threads for some four vectors each; and as many CTAs an SM as its shared
+// memory holds.
+template <typename T, int W, bool Kl>
+cudaError_t by_cta(Params &p, int *ctas, cudaStream_t st) {
+  const int64_t sms = sm_count();
+  // a slice may begin 16 elements early, lie 15 bytes into its place, and be
+  // read to the end of its last vector
+  auto bytes = [&](int cluster) {
+    const int64_t slice = (p.actions + cluster - 1) / cluster + 16;
+    p.slice_bytes = (int)((slice * (int64_t)sizeof(T) + 47) / 16 * 16);
+    return (int64_t)(Kl ? 2 : 1) * p.slice_bytes + (p.legal ? (slice + 47) / 16 * 16 : 0);
+  };
+  int cluster = 1;
+  while (cluster < kMaxCluster && bytes(cluster) > kLongShared / 2) cluster *= 2;
+  while (cluster < kMaxCluster && p.rows * cluster * 2 <= sms && p.actions / cluster > 4096) cluster *= 2;
+  const int64_t smem = bytes(cluster);
+  if (smem > kLongShared) return cudaErrorInvalidValue;
+  const int vecs = (p.actions / cluster + W - 1) / W;
+  int threads = 64;
+  while (threads < kLongThreads && threads * 4 < vecs) threads *= 2;
+  cudaError_t e = cudaFuncSetAttribute(policy_loss_long_kernel<T, W, Kl>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kLongShared);
+  if (e == cudaSuccess && cluster > 8)
+    e = cudaFuncSetAttribute(policy_loss_long_kernel<T, W, Kl>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  int64_t resident = kLongShared / (smem + 2048);
+  if (resident > 1024 / threads) resident = 1024 / threads;  // the registers' limit
+  if (resident < 1) resident = 1;
+  int64_t most = sms * resident / cluster;
+  if (most > kMaxPartials) most = kMaxPartials;
+  if (most < 1) most = 1;
+  *ctas = (int)(p.rows < most ? p.rows : most);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * cluster));
+  cfg.gridDim = dim3((unsigned)(*ctas * cluster));
   cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -501,52 +795,7 @@ cudaError_t launch_cta(const Params &p, int threads, int cluster, int *ctas, cud
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cluster > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(policy_loss_cta_kernel<T, W, V, Kl>,
-                                               cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
-  return cudaLaunchKernelEx(&cfg, policy_loss_cta_kernel<T, W, V, Kl>, p);
-}
-
-// Threads per row.  Up to 512 actions a row is shared by 4 to 32 lanes of
-// a warp, 4 to 16 elements each: the split with the fewest idle places,
-// and among those the fewest lanes (shorter butterflies, more rows a warp).
-template <typename T, int W, bool Kl>
-cudaError_t by_rows(Params &p, int *ctas, cudaStream_t st) {
-  int best = 0, best_elems = 4;
-  for (int elems = 4; elems <= 16; elems += 4)
-    for (int g = 32; g >= 4; g >>= 1) {
-      const int places = g * elems;
-      if (places < p.actions) continue;
-      if (!best || places < best * best_elems || (places == best * best_elems && g < best)) {
-        best = g;
-        best_elems = elems;
-      }
-    }
-  p.group = best;
-  if (best_elems == 4) return launch_rows<T, W, 4 / W, Kl>(p, ctas, st);
-  if (best_elems == 8) return launch_rows<T, W, 8 / W, Kl>(p, ctas, st);
-  if (best_elems == 12) return launch_rows<T, W, 12 / W, Kl>(p, ctas, st);
-  return launch_rows<T, W, 16 / W, Kl>(p, ctas, st);
-}
-
-// Longer rows: 512 threads with up to 32 elements each, and as many CTAs
-// as the row needs; where the rows leave SMs idle the cluster grows to
-// share them.
-template <typename T, int W, bool Kl>
-cudaError_t by_cta(const Params &p, int *ctas, cudaStream_t st) {
-  const int64_t sms = sm_count();
-  int cluster = 1;
-  while (cluster < kMaxCluster && (int64_t)cluster * 512 * 32 < p.actions) cluster *= 2;
-  while (cluster < kMaxCluster && p.rows * cluster * 2 <= sms && (int64_t)cluster * 512 * 4 < p.actions) cluster *= 2;
-  int threads = 512;
-  const int per_cta = (p.actions + cluster - 1) / cluster;
-  while (threads > 128 && threads / 2 * 8 >= per_cta) threads /= 2;
-  const int elems = (per_cta + threads - 1) / threads;
-  if (elems <= 8) return launch_cta<T, W, 8 / W, Kl>(p, threads, cluster, ctas, st);
-  if (elems <= 16) return launch_cta<T, W, 16 / W, Kl>(p, threads, cluster, ctas, st);
-  return launch_cta<T, W, 32 / W, Kl>(p, threads, cluster, ctas, st);
+  return cudaLaunchKernelEx(&cfg, policy_loss_long_kernel<T, W, Kl>, p);
 }
 
 // vectors of W elements need every row of every array to start on one
@@ -557,12 +806,22 @@ bool rows_aligned(const Params &p, int w, size_t size) {
          (!p.legal || ok(p.legal, (size_t)w)) && (!p.grad || ok(p.grad, w * size));
 }
 
+// or, for the shared memory of long rows, all arrays' rows to start at the
+// same place within one
+bool same_phase(const Params &p, int w, size_t size) {
+  auto at = [&](const void *q, size_t s) { return (int)(reinterpret_cast<uintptr_t>(q) / s % (size_t)w); };
+  const int x = at(p.logits, size);
+  return (p.stride - p.actions) % w == 0 &&
+         (!p.reference || ((p.reference_stride - p.stride) % w == 0 && at(p.reference, size) == x)) &&
+         (!p.legal || at(p.legal, 1) == x) && (!p.grad || at(p.grad, size) == x);
+}
+
 template <typename T, bool Kl>
 cudaError_t by_type(Params &p, int *ctas, cudaStream_t st) {
-  if (p.actions <= kMaxSubActions)
-    return rows_aligned(p, 2, sizeof(T)) ? by_rows<T, 2, Kl>(p, ctas, st) : by_rows<T, 1, Kl>(p, ctas, st);
+  if (p.actions <= kMaxShort)
+    return rows_aligned(p, 2, sizeof(T)) ? by_lanes<T, 2, Kl>(p, ctas, st) : by_lanes<T, 1, Kl>(p, ctas, st);
   constexpr int kWide = 16 / (int)sizeof(T);
-  return rows_aligned(p, kWide, sizeof(T)) ? by_cta<T, kWide, Kl>(p, ctas, st) : by_cta<T, 1, Kl>(p, ctas, st);
+  return same_phase(p, kWide, sizeof(T)) ? by_cta<T, kWide, Kl>(p, ctas, st) : by_cta<T, 1, Kl>(p, ctas, st);
 }
 
 }  // namespace
