@@ -529,9 +529,9 @@ typedef struct {
  * gradient in the logits.  dtype: 0 float32, 1 bfloat16, 2 float16;
  * 1 <= num_actions <= 262144.  A row that does not count (weight 0, an
  * action out of range, illegal or with a logit of -inf) adds nothing: its
- * statistics and its gradient are 0, and with weight 0 its logits are not
- * read.  workspace: scacchi_policy_loss_workspace_bytes() bytes, 8-byte
- * aligned, of this call alone. */
+ * statistics and its gradient are 0, whatever its logits hold.  workspace:
+ * scacchi_policy_loss_workspace_bytes() bytes, 8-byte aligned, of this call
+ * alone. */
 size_t scacchi_policy_loss_workspace_bytes(void);
 int scacchi_policy_loss(const scacchi_policy_rows *rows, const scacchi_policy_out *out, int64_t num_rows,
                         int32_t num_actions, int32_t dtype, double clip_low, double clip_high, float kl_coefficient,

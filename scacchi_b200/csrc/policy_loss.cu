@@ -77,7 +77,8 @@ struct Params {
   int64_t rows, stride, reference_stride;
   int actions;
   int group;        // lanes of a short row
-  int slice_bytes;  // of a long row's logits in one CTA
+  int slice_bytes;  // of shared memory for a warp's batch, or a CTA's slice, of the logits
+  int mask_bytes, x_pitch, r_pitch;  // of a warp's batch: Batch
   double clip_low, clip_high, log_low, log_high;  // borders of the ratio and their logarithms
   float beta, even_weight;
 };
@@ -104,20 +105,17 @@ struct alignas(sizeof(T) * W) Vec {
   T v[W];
 };
 
-// e^y - 1 - y: its Taylor series for |y| < 1 (terms to y^11, 2 / 12! of the
-// leading one), the definition beyond, where it no longer cancels
+// e^y - 1 - y for |y| < 1 to 1.2e-7 of itself: y^2 times the Chebyshev
+// interpolant of degree 6 of (e^y - 1 - y) / y^2 on [-1, 1]
 __device__ __forceinline__ float phi_small(float y) {
-  float c = 1.0f / 39916800.0f;
-  c = fmaf(c, y, 1.0f / 3628800.0f);
-  c = fmaf(c, y, 1.0f / 362880.0f);
-  c = fmaf(c, y, 1.0f / 40320.0f);
-  c = fmaf(c, y, 1.0f / 5040.0f);
-  c = fmaf(c, y, 1.0f / 720.0f);
-  c = fmaf(c, y, 1.0f / 120.0f);
-  c = fmaf(c, y, 1.0f / 24.0f);
-  c = fmaf(c, y, 1.0f / 6.0f);
-  c = fmaf(c, y, 0.5f);
-  return c * y * y;
+  float c = 2.535864489e-05f;
+  c = fmaf(c, y, 2.032920127e-04f);
+  c = fmaf(c, y, 1.388539492e-03f);
+  c = fmaf(c, y, 8.330884178e-03f);
+  c = fmaf(c, y, 4.166673667e-02f);
+  c = fmaf(c, y, 1.666669734e-01f);
+  c = fmaf(c, y, 0.4999999978f);
+  return c * (y * y);
 }
 
 // e^u for u <= 0 or small (see above)
@@ -268,8 +266,11 @@ struct Ctas {
 // with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r).
 // Taken by the few rows next to a clip border or far from the reference.
 template <typename T, typename Grp>
-__device__ __noinline__ double2 row_in_64(const Grp &grp, const T *x, const T *r, const uint8_t *legal, int A,
-                                          float top, bool want_kl) {
+__device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64_t row, float top, bool want_kl) {
+  const int A = p.actions;
+  const T *x = static_cast<const T *>(p.logits) + row * p.stride;
+  const T *r = static_cast<const T *>(p.reference) + row * p.reference_stride;
+  const uint8_t *legal = p.legal ? p.legal + row * A : nullptr;
   double s = 0.0, sd = 0.0, rtop = -INFINITY;
   for (int a = grp.index(); a < A; a += grp.size()) {
     const float xa = to_f(x[a]);
@@ -336,13 +337,12 @@ struct RowOut {
 // group writes them.
 template <typename T, bool Kl, typename Grp>
 __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, int64_t row, float weight,
-                                             const RowIn &in, const T *x, const T *r, const uint8_t *legal, float top,
-                                             float sum, float kl_sum) {
+                                             const RowIn &in, float top, float sum, float kl_sum) {
   double lp = ((double)in.xk - (double)top) - log_row_sum(sum), delta = lp - (double)in.old;
   const bool far = Kl && !(kl_sum < kFarKl);
   float kl = Kl ? log1pf(kl_sum) : 0.0f;
   if (far || fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol) {
-    const double2 fine = row_in_64<T>(grp, x, r, legal, p.actions, top, far);
+    const double2 fine = row_in_64<T>(p, grp, row, top, far);
     lp = (double)in.xk - fine.x;
     delta = lp - (double)in.old;
     if (far) kl = (float)fine.y;
@@ -372,46 +372,152 @@ __device__ __forceinline__ void empty_row(const Params &p, int64_t row) {
   if (p.kl) p.kl[row] = 0.0f;
 }
 
-// p phi(mean - d) of one action.  An e^y that overflows, or meets a p that
-// underflowed, makes the row a far one; an illegal place (p = 0, d = 0) has
-// no part.
-__device__ __forceinline__ float kl_part(float pa, float d, float mean) {
+// p phi(mean - d) of one action whose y = mean - d is not within (-1, 1).  An
+// e^y that overflows, or meets a p that underflowed, makes
+// the row a far one; an illegal place (p = 0, d = 0) has no part.  Out of
+// line: few actions are that far, and e^y for all of them is a third of the
+// row's work.
+__device__ __noinline__ float kl_part_far(float pa, float d, float mean) {
   const float y = mean - d;
-  float part = pa * phi_small(y);
-  if (!(fabsf(y) < 1.0f))
-    part = pa > 0.0f ? fmaf(pa, expf(y), -pa * (1.0f + y)) : (y > 60.0f && d != 0.0f ? INFINITY : pa * 0.0f);
-  return part;
+  return pa > 0.0f ? fmaf(pa, expf(y), -pa * (1.0f + y)) : (y > 60.0f && d != 0.0f ? INFINITY : pa * 0.0f);
+}
+
+// ---------------------------------------------------------------------------
+// rows on their way to shared memory
+// ---------------------------------------------------------------------------
+
+// the place of `from` within 16 bytes, in elements
+template <typename E>
+__device__ __forceinline__ int phase_of(const E *from) {
+  return (int)((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(E));
+}
+
+template <int Bytes>
+__device__ __forceinline__ void copy_async(void *to, const void *from) {
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+  if (Bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(from) : "memory");
+}
+
+// Copies `count` elements, by `threads` threads, to the same place within 16
+// bytes as they have in global memory, so that whole vectors move at any
+// alignment: asynchronous copies of 16 bytes, of 4 at the ends, and where
+// even those do not fit, plain ones.
+template <typename E>
+__device__ __forceinline__ void stage(E *to, const E *from, int count, int t, int threads) {
+  constexpr int kVec = 16 / (int)sizeof(E), kWord = 4 / (int)sizeof(E);
+  const int phase = phase_of(from), head = (kVec - phase) % kVec;
+  const int first = head < count ? head : count, vecs = (count - first) / kVec, last = first + vecs * kVec;
+  for (int i = t; i < vecs; i += threads) copy_async<16>(to + first + i * kVec, from + first + i * kVec);
+  const int ends = first + count - last;
+  if (phase % kWord == 0 && first % kWord == 0 && count % kWord == 0) {
+    for (int i = t * kWord; i < ends; i += threads * kWord) {
+      const int at = i < first ? i : last + i - first;
+      copy_async<4>(to + at, from + at);
+    }
+  } else {
+    for (int i = t; i < ends; i += threads) {
+      const int at = i < first ? i : last + i - first;
+      to[at] = from[at];
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
 // short rows: `group` lanes of a warp each, their elements in registers
 // ---------------------------------------------------------------------------
 
+// CTAs an SM, as the registers of a thread's elements allow
+template <int Elems, bool Kl>
+constexpr int kShortCtas = Kl && Elems > 6 ? 2 : 3;
+
+// One array's rows of a warp's batch in shared memory.
+template <typename E>
+struct Batch {
+  E *at;      // of the warp's buffer
+  int pitch;  // elements between rows that are staged one by one, 0 if the rows are one piece
+
+  __device__ __forceinline__ void load(const E *first, int64_t stride, int rows, int A, int lane) const {
+    if (!pitch) {
+      stage(at + phase_of(first), first, rows * A, lane, 32);
+    } else {
+      for (int i = 0; i < rows; ++i)
+        stage(at + i * pitch + phase_of(first + i * stride), first + i * stride, A, lane, 32);
+    }
+  }
+  __device__ __forceinline__ const E *row(const E *first, int64_t stride, int i, int A) const {
+    return pitch ? at + i * pitch + phase_of(first + i * stride) : at + phase_of(first) + i * A;
+  }
+};
+
+// The copies of a batch whose rows are one piece of global memory: 16 bytes
+// each in the middle, 4 at the ends.
+struct Piece {
+  const uint8_t *from;  // of the first batch
+  int64_t step;         // bytes from batch to batch
+  int phase, first, vecs, words;
+  bool ok;              // the ends are whole words, and every batch is alike
+
+  __device__ __forceinline__ void copy(uint32_t to, int64_t turn, int lane) const {
+    const uint8_t *src = from + turn * step;
+    to += (uint32_t)phase;
+    for (int i = lane; i < vecs; i += 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + first + 16 * i), "l"(src + first + 16 * i)
+                   : "memory");
+    if (lane < words) {
+      const int at = 4 * lane < first ? 4 * lane : 4 * lane + 16 * vecs;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + at), "l"(src + at) : "memory");
+    }
+  }
+};
+
+__device__ __forceinline__ Piece piece_of(const void *from, int bytes, int64_t step) {
+  Piece p;
+  p.from = static_cast<const uint8_t *>(from);
+  p.step = step;
+  p.phase = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+  const int head = (16 - p.phase) & 15;
+  p.first = head < bytes ? head : bytes;
+  p.vecs = (bytes - p.first) / 16;
+  p.words = (bytes - 16 * p.vecs) / 4;  // at most 3 at each end
+  p.ok = p.phase % 4 == 0 && bytes % 4 == 0 && step % 16 == 0;
+  return p;
+}
+
+// A batch is the rows that a warp takes at once, one per lane group; while
+// it is computed the next one is on its way, its scalars in registers.
+struct Scalars {
+  float weight, old, adv, ref;
+  int action;
+};
+
+__device__ __forceinline__ Scalars scalars_of(const Params &p, int64_t row) {
+  Scalars s = {0.0f, 0.0f, 0.0f, 0.0f, -1};
+  if (row < p.rows) {
+    s.weight = p.weight ? p.weight[row] : p.even_weight;
+    s.action = p.action[row];
+    s.old = p.old_log_prob[row];
+    s.adv = p.advantage[row];
+    if (p.reference_log_prob) s.ref = p.reference_log_prob[row];
+  }
+  return s;
+}
+
 // V vectors of W elements per thread; thread t of the group holds vectors
 // t, t + G, ... of the row.  Returns the row's share of the loss.
 template <typename T, int W, int V, bool Kl>
-__device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, int64_t row, float weight, int k) {
-  const int A = p.actions, t = grp.index(), G = grp.size();
-  const T *x = static_cast<const T *>(p.logits) + row * p.stride;
-  const T *r = Kl ? static_cast<const T *>(p.reference) + row * p.reference_stride : nullptr;
-  const uint8_t *legal = p.legal ? p.legal + row * A : nullptr;
+__device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, int64_t row, const Scalars &s,
+                                            const T *sx, const T *sr, const uint8_t *sl) {
+  const int A = p.actions, t = grp.index(), G = grp.size(), k = s.action;
   T *grad = p.grad ? static_cast<T *>(p.grad) + row * A : nullptr;
   using Pack = Vec<T, W>;
-  Pack xv[V], rv[Kl ? V : 1];
-  Vec<uint8_t, W> lv[V];
-  const bool wanted = weight != 0.0f && k >= 0 && k < A;
-  if (wanted) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int a = (v * G + t) * W;
-      if (a < A) {
-        xv[v] = *reinterpret_cast<const Pack *>(x + a);
-        if (Kl) rv[Kl ? v : 0] = *reinterpret_cast<const Pack *>(r + a);
-        if (legal) lv[v] = *reinterpret_cast<const Vec<uint8_t, W> *>(legal + a);
-      }
-    }
+  RowIn in = {0.0f, s.old, s.adv, s.ref, s.weight != 0.0f && k >= 0 && k < A};
+  if (in.counts) {
+    in.xk = to_f(sx[k]);
+    in.counts = (!sl || sl[k]) && in.xk != -INFINITY;
   }
-  const RowIn in = row_in<T>(p, row, x, legal, k, wanted);
   if (!in.counts) {
     if (t == 0) empty_row(p, row);
     if (grad) {
@@ -426,18 +532,28 @@ __device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, i
     }
     return 0.0;
   }
-  // illegal actions become -inf, as places past the row are
+  // an action that is illegal, or has a logit of -inf, keeps x = -inf and
+  // d = 0, as places past the row do (the buffer goes on there)
   float e[V * W], d[Kl ? V * W : 1], top = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < V; ++v)
+  for (int v = 0; v < V; ++v) {
+    const int a = (v * G + t) * W;
+    const bool inside = a < A;
+    const Pack xv = *reinterpret_cast<const Pack *>(sx + a);
+    Pack rv;
+    Vec<uint8_t, W> lv;
+    if (Kl) rv = *reinterpret_cast<const Pack *>(sr + a);
+    if (sl) lv = *reinterpret_cast<const Vec<uint8_t, W> *>(sl + a);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const int i = v * W + w;
-      const bool keep = (v * G + t) * W < A && (!legal || lv[v].v[w]);
-      e[i] = keep ? to_f(xv[v].v[w]) : -INFINITY;
+      const float xa = to_f(xv.v[w]);
+      const bool keep = xa != -INFINITY && inside && (!sl || lv.v[w] != 0);
+      e[i] = keep ? xa : -INFINITY;
       top = fmaxf(top, e[i]);
-      if (Kl) d[Kl ? i : 0] = e[i] == -INFINITY ? 0.0f : e[i] - to_f(rv[Kl ? v : 0].v[w]);
+      if (Kl) d[Kl ? i : 0] = keep ? xa - to_f(rv.v[w]) : 0.0f;
     }
+  }
   top = grp.reduce<MaxOp>(top);
   float sum = 0.0f, mean = 0.0f, kl = 0.0f;
 #pragma unroll
@@ -450,11 +566,23 @@ __device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, i
   const float inv = 1.0f / sum;
   if (Kl) {
     mean = grp.reduce<SumOp>(mean) * inv;
+    bool some = false;
 #pragma unroll
-    for (int i = 0; i < V * W; ++i) kl += kl_part(e[i] * inv, d[Kl ? i : 0], mean);
+    for (int i = 0; i < V * W; ++i) {
+      const float y = mean - d[Kl ? i : 0];
+      const bool near = fabsf(y) < 1.0f;
+      some |= !near;
+      kl = fmaf(near ? e[i] : 0.0f, phi_small(near ? y : 0.0f), kl);
+    }
+    kl *= inv;
+    if (some) {
+#pragma unroll
+      for (int i = 0; i < V * W; ++i)
+        if (!(fabsf(mean - d[Kl ? i : 0]) < 1.0f)) kl += kl_part_far(e[i] * inv, d[Kl ? i : 0], mean);
+    }
     kl = grp.reduce<SumOp>(kl);
   }
-  const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, x, r, legal, top, sum, kl);
+  const RowOut out = finish_row<T, Kl>(p, grp, row, s.weight, in, top, sum, kl);
   if (grad) {
     const float wc = -out.wc * inv, wb = out.wb * inv;
 #pragma unroll
@@ -475,36 +603,81 @@ __device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, i
 }
 
 template <typename T, int W, int V, bool Kl>
-__global__ void __launch_bounds__(kShortThreads, V * W <= 8 ? 4 : 2) policy_loss_short_kernel(Params p) {
+__global__ void __launch_bounds__(kShortThreads, kShortCtas<V * W, Kl>) policy_loss_short_kernel(Params p) {
+  extern __shared__ __align__(16) uint8_t s_rows[];
   __shared__ double s_part[kShortThreads / 32];
-  const int lane = threadIdx.x & 31, G = p.group;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.group, A = p.actions;
   Lanes grp;
   grp.lanes = G;
   grp.mask = G == 32 ? kFull : ((1u << G) - 1u) << (lane & ~(G - 1));
-  const int per_cta = kShortThreads / G;
-  double sum = 0.0;
-  int64_t row = (int64_t)blockIdx.x * per_cta + threadIdx.x / G;
-  const int64_t step = (int64_t)gridDim.x * per_cta;
-  // the next row's weight and action are requested a row ahead
-  float w_next = 0.0f;
-  int k_next = 0;
-  if (row < p.rows) {
-    w_next = p.weight ? p.weight[row] : p.even_weight;
-    k_next = p.action[row];
-  }
-  for (; row < p.rows; row += step) {
-    const float w = w_next;
-    const int k = k_next;
-    if (row + step < p.rows) {
-      w_next = p.weight ? p.weight[row + step] : p.even_weight;
-      k_next = p.action[row + step];
+  const int per_warp = 32 / G;
+  const int64_t step = (int64_t)gridDim.x * (kShortThreads / 32) * per_warp;
+  int64_t first = ((int64_t)blockIdx.x * (kShortThreads / 32) + warp) * per_warp;
+  const T *x = static_cast<const T *>(p.logits), *r = static_cast<const T *>(p.reference);
+  const int buffer = (Kl ? 2 : 1) * p.slice_bytes + (p.legal ? p.mask_bytes : 0);
+  uint8_t *const base = s_rows + warp * 2 * buffer;
+  // A full batch of rows in one piece starts at the same place within 16
+  // bytes every time (the step is a multiple of 16 rows): its copies are
+  // worked out once.
+  const Piece px = piece_of(x + first * p.stride, per_warp * A * (int)sizeof(T), step * p.stride * (int)sizeof(T));
+  const Piece pr = piece_of(r + first * p.reference_stride, per_warp * A * (int)sizeof(T),
+                            step * p.reference_stride * (int)sizeof(T));
+  const Piece pl = piece_of(p.legal + first * A, per_warp * A, step * A);
+  const bool pieces = !p.x_pitch && px.ok && (!Kl || (!p.r_pitch && pr.ok)) && (!p.legal || pl.ok);
+  const uint32_t base_at = (uint32_t)__cvta_generic_to_shared(base);
+  int64_t turn = 0;
+  auto request = [&](int64_t at, int bank) {
+    if (pieces && at + per_warp <= p.rows) {
+      const uint32_t to = base_at + (uint32_t)(bank * buffer);
+      px.copy(to, turn, lane);
+      if (Kl) pr.copy(to + p.slice_bytes, turn, lane);
+      if (p.legal) pl.copy(to + (Kl ? 2 : 1) * p.slice_bytes, turn, lane);
+    } else if (at < p.rows) {
+      const int rows = p.rows - at < per_warp ? (int)(p.rows - at) : per_warp;
+      uint8_t *buf = base + bank * buffer;
+      Batch<T>{reinterpret_cast<T *>(buf), p.x_pitch}.load(x + at * p.stride, p.stride, rows, A, lane);
+      if (Kl)
+        Batch<T>{reinterpret_cast<T *>(buf + p.slice_bytes), p.r_pitch}.load(r + at * p.reference_stride,
+                                                                            p.reference_stride, rows, A, lane);
+      if (p.legal) Batch<uint8_t>{buf + (Kl ? 2 : 1) * p.slice_bytes, 0}.load(p.legal + at * A, A, rows, A, lane);
     }
-    const double share = short_row<T, W, V, Kl>(p, grp, row, w, k);
-    if (grp.index() == 0) sum += share;
+    ++turn;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  double sum = 0.0;
+  int bank = 0;
+  request(first, 0);
+  Scalars next = scalars_of(p, first + lane / G);
+  for (; first < p.rows; first += step, bank ^= 1) {
+    const Scalars now = next;
+    request(first + step, bank ^ 1);
+    next = scalars_of(p, first + step + lane / G);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const int64_t row = first + lane / G;
+    if (row < p.rows) {
+      uint8_t *buf = base + bank * buffer;
+      const T *sx, *sr = nullptr;
+      const uint8_t *sl = nullptr;
+      if (pieces) {
+        sx = reinterpret_cast<const T *>(buf + px.phase) + lane / G * A;
+        if (Kl) sr = reinterpret_cast<const T *>(buf + p.slice_bytes + pr.phase) + lane / G * A;
+        if (p.legal) sl = buf + (Kl ? 2 : 1) * p.slice_bytes + pl.phase + lane / G * A;
+      } else {
+        sx = Batch<T>{reinterpret_cast<T *>(buf), p.x_pitch}.row(x + first * p.stride, p.stride, lane / G, A);
+        if (Kl)
+          sr = Batch<T>{reinterpret_cast<T *>(buf + p.slice_bytes), p.r_pitch}.row(r + first * p.reference_stride,
+                                                                                   p.reference_stride, lane / G, A);
+        if (p.legal)
+          sl = Batch<uint8_t>{buf + (Kl ? 2 : 1) * p.slice_bytes, 0}.row(p.legal + first * A, A, lane / G, A);
+      }
+      const double share = short_row<T, W, V, Kl>(p, grp, row, now, sx, sr, sl);
+      if (grp.index() == 0) sum += share;
+    }
+    __syncwarp();  // the buffer is read: the batch after the next may take it
   }
-  __syncwarp();
   for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
-  if (lane == 0) s_part[threadIdx.x >> 5] = sum;
+  if (lane == 0) s_part[warp] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     double total = 0.0;
@@ -519,28 +692,6 @@ __global__ void __launch_bounds__(kShortThreads, V * W <= 8 ? 4 : 2) policy_loss
 // ---------------------------------------------------------------------------
 // long rows: a CTA each, or a cluster's slices, in shared memory
 // ---------------------------------------------------------------------------
-
-// the place of `from` within 16 bytes, in elements
-template <typename E>
-__device__ __forceinline__ int phase_of(const E *from) {
-  return (int)((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(E));
-}
-
-// Loads `count` elements to shared memory, at the same place within 16 bytes
-// as in global memory, so that whole vectors move at any alignment: 16-byte
-// asynchronous copies in the middle, elements at the ends.
-template <typename E>
-__device__ __forceinline__ void stage(E *to, const E *from, int count, int t, int threads) {
-  constexpr int kVec = 16 / (int)sizeof(E);
-  const int head = (kVec - phase_of(from)) % kVec;
-  const int first = head < count ? head : count, vecs = (count - first) / kVec, tail = first + vecs * kVec;
-  for (int i = t; i < vecs; i += threads) {
-    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to + first + i * kVec);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from + first + i * kVec) : "memory");
-  }
-  if (t < first) to[t] = from[t];
-  if (t < count - tail) to[tail + t] = from[tail + t];
-}
 
 // Passes over the slice's elements, W at a time where the row's arrays start
 // at the same place within a vector (vector v then holds elements v W -
@@ -648,14 +799,31 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Param
     if (Kl) {
       for (int v = t; v < vecs; v += threads) {
         float xa[W], da[W], part = 0.0f;
+        bool some = false;
         load(v, xa, da);
 #pragma unroll
-        for (int w = 0; w < W; ++w) part += kl_part(exp_fast(xa[w] - st.top) * inv, da[w], mean);
-        kl += part;
+        for (int w = 0; w < W; ++w) {
+          const float y = mean - da[w];
+          const bool near = fabsf(y) < 1.0f;
+          some |= !near;
+          part = fmaf(near ? exp_fast(xa[w] - st.top) : 0.0f, phi_small(near ? y : 0.0f), part);
+        }
+        kl = fmaf(part, inv, kl);
+        if (some) {
+#pragma unroll 1
+          for (int w = 0; w < W; ++w) {
+            // from shared memory again: registers are not indexed
+            const int a = v * W - lead + w;
+            if (a < 0 || a >= n || (legal && !sl[a])) continue;
+            const float xw = to_f(sx[a]);
+            const float dw = xw - to_f(sr[a]);
+            if (xw != -INFINITY && !(fabsf(mean - dw) < 1.0f)) kl += kl_part_far(exp_fast(xw - st.top) * inv, dw, mean);
+          }
+        }
       }
       kl = grp.reduce<SumOp>(kl);
     }
-    const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, x, r, legal, st.top, st.sum, kl);
+    const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, st.top, st.sum, kl);
     share += out.share;
     if (grad) {
       const float wc = -out.wc * inv, wb = out.wb * inv;
@@ -711,34 +879,68 @@ __global__ void policy_loss_sum_kernel(const double *partial, int n, float *loss
 // host
 // ---------------------------------------------------------------------------
 
+constexpr int kMaxDevices = 64;
+
+int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+
 int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-    return 148;
+  static std::atomic<int> known[kMaxDevices];
+  const int dev = current_device();
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
+// the kernel may use kLongShared bytes, and clusters above 8 CTAs if
+// `large`; asked once per kernel and device
+template <typename K>
+cudaError_t allow(K *kernel, std::atomic<uint64_t> &done, bool large) {
+  const uint64_t bit = 1ull << current_device();
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongShared);
+  if (e == cudaSuccess && large) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 template <typename T, int W, int V, bool Kl>
-cudaError_t launch_short(const Params &p, int *ctas, cudaStream_t st) {
-  const int per_cta = kShortThreads / p.group;
-  const int64_t need = (p.rows + per_cta - 1) / per_cta;
-  const int most = sm_count() * 8 < kMaxPartials ? sm_count() * 8 : kMaxPartials;
+cudaError_t launch_short(Params &p, int *ctas, cudaStream_t st) {
+  const int per_warp = 32 / p.group, warps = kShortThreads / 32;
+  // rows that follow one another are staged as one piece
+  const int pitch = (p.actions * (int)sizeof(T) + 31) / 16 * 16 / (int)sizeof(T);
+  p.x_pitch = p.stride == p.actions ? 0 : pitch;
+  p.r_pitch = !Kl || p.reference_stride == p.actions ? 0 : pitch;
+  // a lane's vectors past the last row are read too, and ignored
+  const int past = p.group * V * W;
+  p.slice_bytes = ((per_warp * pitch + past) * (int)sizeof(T) + 31) / 16 * 16;
+  p.mask_bytes = (per_warp * p.actions + past + 47) / 16 * 16;
+  const int smem = warps * 2 * ((Kl ? 2 : 1) * p.slice_bytes + (p.legal ? p.mask_bytes : 0));
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow(policy_loss_short_kernel<T, W, V, Kl>, allowed, false);
+  if (e != cudaSuccess) return e;
+  const int64_t need = (p.rows + per_warp * warps - 1) / (per_warp * warps);
+  const int most = sm_count() * kShortCtas<V * W, Kl>;
   *ctas = (int)(need < most ? need : most);
-  policy_loss_short_kernel<T, W, V, Kl><<<*ctas, kShortThreads, 0, st>>>(p);
+  policy_loss_short_kernel<T, W, V, Kl><<<*ctas, kShortThreads, smem, st>>>(p);
   return cudaPeekAtLastError();
 }
 
-// Lanes of a short row: 4 to 32, with 4 to 16 elements each: the split with
-// the fewest idle places, and among those the most lanes (fewer registers a
-// thread, more rows in flight an SM).
+// Lanes of a short row: 4 to 32, with 4 to 24 elements each: the split with
+// the fewest idle places, and among those the fewest lanes: a batch costs
+// some 550 instructions besides its elements' (its copies, its rows' ends),
+// which more rows share.
 template <typename T, int W, bool Kl>
 cudaError_t by_lanes(Params &p, int *ctas, cudaStream_t st) {
-  constexpr int kElems[] = {4, 6, 8, 12, 16};
+  constexpr int kElems[] = {4, 6, 8, 12, 16, 24};
   int best = 0, elems = 0;
   for (int e : kElems)
     for (int g = 4; g <= 32; g *= 2)
-      if (g * e >= p.actions && (!best || g * e < best * elems || (g * e == best * elems && g > best))) {
+      if (g * e >= p.actions && (!best || g * e < best * elems || (g * e == best * elems && g < best))) {
         best = g;
         elems = e;
       }
@@ -747,7 +949,8 @@ cudaError_t by_lanes(Params &p, int *ctas, cudaStream_t st) {
   if (elems == 6) return launch_short<T, W, 6 / W, Kl>(p, ctas, st);
   if (elems == 8) return launch_short<T, W, 8 / W, Kl>(p, ctas, st);
   if (elems == 12) return launch_short<T, W, 12 / W, Kl>(p, ctas, st);
-  return launch_short<T, W, 16 / W, Kl>(p, ctas, st);
+  if (elems == 16) return launch_short<T, W, 16 / W, Kl>(p, ctas, st);
+  return launch_short<T, W, 24 / W, Kl>(p, ctas, st);
 }
 
 // Long rows: a cluster where half an SM's shared memory does not hold the
@@ -772,10 +975,8 @@ cudaError_t by_cta(Params &p, int *ctas, cudaStream_t st) {
   const int vecs = (p.actions / cluster + W - 1) / W;
   int threads = 64;
   while (threads < kLongThreads && threads * 4 < vecs) threads *= 2;
-  cudaError_t e = cudaFuncSetAttribute(policy_loss_long_kernel<T, W, Kl>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kLongShared);
-  if (e == cudaSuccess && cluster > 8)
-    e = cudaFuncSetAttribute(policy_loss_long_kernel<T, W, Kl>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow(policy_loss_long_kernel<T, W, Kl>, allowed, true);
   if (e != cudaSuccess) return e;
   int64_t resident = kLongShared / (smem + 2048);
   if (resident > 1024 / threads) resident = 1024 / threads;  // the registers' limit

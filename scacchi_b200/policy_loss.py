@@ -10,13 +10,14 @@ loss is the cross-entropy to the search's policy.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from .dirichlet_mctx.tree import ptr, stream_handle
+from .dirichlet_mctx.tree import stream_handle
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_ACTIONS = 262144
@@ -36,6 +37,7 @@ class PolicyLoss(NamedTuple):
 
 def _rows(t: torch.Tensor, actions: int) -> torch.Tensor:
     """[..., A] as rows [N, A] of unit column stride, a view where it can be."""
+    t = t.detach()
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= actions:
         return t
     t = t.reshape(-1, actions)
@@ -86,64 +88,76 @@ def clipped_policy_loss(logits: torch.Tensor, action: torch.Tensor, old_log_prob
     if kl_coefficient != 0.0 and reference_logits is None and reference_log_prob is None:
         raise ValueError("a KL term needs reference_logits or reference_log_prob")
     dev, lead, A = logits.device, logits.shape[:-1], logits.shape[-1]
-
-    def per_row(t, name):
-        if t.shape != lead:
-            raise ValueError(f"{name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the logits on {dev}")
-        if not t.is_floating_point():
-            raise ValueError(f"{name} must be floating point, got {t.dtype}")
-        return t.to(torch.float32).contiguous()
-
     if action.shape != lead or action.device != dev or action.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"action must be int32 or int64 of shape {tuple(lead)} on {dev}, got {action.dtype} "
                          f"{tuple(action.shape)} on {action.device}")
+    if legal is not None and (legal.shape != logits.shape or legal.device != dev
+                              or legal.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"legal must be bool of shape {tuple(logits.shape)} on {dev}, got {legal.dtype} "
+                         f"{tuple(legal.shape)} on {legal.device}")
+    if reference_logits is not None and (reference_logits.shape != logits.shape or reference_logits.device != dev
+                                         or reference_logits.dtype != logits.dtype):
+        raise ValueError(f"reference_logits must match the logits ({logits.dtype} {tuple(logits.shape)} on {dev}), "
+                         f"got {reference_logits.dtype} {tuple(reference_logits.shape)} on "
+                         f"{reference_logits.device}")
+    old_log_prob = _per_row(old_log_prob, "old_log_prob", lead, dev)
+    advantage = _per_row(advantage, "advantage", lead, dev)
+    if weight is not None:
+        weight = _per_row(weight, "weight", lead, dev)
+    if reference_log_prob is not None:
+        reference_log_prob = _per_row(reference_log_prob, "reference_log_prob", lead, dev)
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _launch(logits, action, old_log_prob, advantage, legal, weight, reference_logits,
+                           reference_log_prob, clip_low, clip_high, kl_coefficient, gradient)
+    return _launch(logits, action, old_log_prob, advantage, legal, weight, reference_logits, reference_log_prob,
+                   clip_low, clip_high, kl_coefficient, gradient)
+
+
+def _per_row(t: torch.Tensor, name: str, lead: torch.Size, dev: torch.device) -> torch.Tensor:
+    if t.shape != lead:
+        raise ValueError(f"{name} must have shape {tuple(lead)}, got {tuple(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the logits on {dev}")
+    if t.dtype != torch.float32:
+        if not t.is_floating_point():
+            raise ValueError(f"{name} must be floating point, got {t.dtype}")
+        t = t.to(torch.float32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+@functools.lru_cache(maxsize=1)
+def _workspace_bytes() -> int:
+    return int(_lib.lib().scacchi_policy_loss_workspace_bytes())
+
+
+def _launch(logits, action, old_log_prob, advantage, legal, weight, reference_logits, reference_log_prob, clip_low,
+            clip_high, kl_coefficient, gradient) -> PolicyLoss:
+    dev, lead, A = logits.device, logits.shape[:-1], logits.shape[-1]
     if action.dtype == torch.int64:
         action = action.clamp(-1, A).to(torch.int32)  # an index past 32 bits stays out of range
-    action = action.contiguous()
-    old_log_prob, advantage = per_row(old_log_prob, "old_log_prob"), per_row(advantage, "advantage")
-    if weight is not None:
-        weight = per_row(weight, "weight")
-    if reference_log_prob is not None:
-        reference_log_prob = per_row(reference_log_prob, "reference_log_prob")
-    if legal is not None:
-        if legal.shape != logits.shape or legal.device != dev or legal.dtype not in (torch.bool, torch.uint8):
-            raise ValueError(f"legal must be bool of shape {tuple(logits.shape)} on {dev}, got {legal.dtype} "
-                             f"{tuple(legal.shape)} on {legal.device}")
+    if not action.is_contiguous():
+        action = action.contiguous()
+    if legal is not None and not legal.is_contiguous():
         legal = legal.contiguous()
-    if reference_logits is not None:
-        if (reference_logits.shape != logits.shape or reference_logits.device != dev
-                or reference_logits.dtype != logits.dtype):
-            raise ValueError(f"reference_logits must match the logits ({logits.dtype} {tuple(logits.shape)} on {dev}), "
-                             f"got {reference_logits.dtype} {tuple(reference_logits.shape)} on "
-                             f"{reference_logits.device}")
-        reference_logits = _rows(reference_logits.detach(), A)
-    x = _rows(logits.detach(), A)
+    x = _rows(logits, A)
+    ref = None if reference_logits is None else _rows(reference_logits, A)
     N = x.shape[0]
-    f32 = torch.float32
-    with_kl = reference_logits is not None or reference_log_prob is not None
-    with torch.cuda.device(dev):
-        loss = torch.empty((), dtype=f32, device=dev)
-        log_prob = torch.empty(lead, dtype=f32, device=dev)
-        clipped = torch.empty(lead, dtype=torch.bool, device=dev)
-        kl = torch.empty(lead, dtype=f32, device=dev) if with_kl else None
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if gradient else None
-        workspace = torch.empty((_workspace_bytes(),), dtype=torch.uint8, device=dev)
-        rows = _lib.PolicyRows(ptr(x), ptr(reference_logits), ptr(legal), ptr(action), ptr(old_log_prob),
-                               ptr(advantage), ptr(weight), ptr(reference_log_prob), max(x.stride(0), A),
-                               A if reference_logits is None else max(reference_logits.stride(0), A))
-        out = _lib.PolicyOut(ptr(loss), ptr(log_prob), ptr(kl), ptr(clipped), ptr(grad))
-        _lib.check(_lib.lib().scacchi_policy_loss(C.byref(rows), C.byref(out), N, A, DTYPES[logits.dtype],
-                                                  float(clip_low), float(clip_high), float(kl_coefficient),
-                                                  ptr(workspace), stream_handle(dev)), "policy_loss")
-    return PolicyLoss(loss=loss, log_prob=log_prob, clipped=clipped, kl=kl, grad_logits=grad)
+    with_kl = ref is not None or reference_log_prob is not None
+    new = functools.partial(torch.empty, device=dev)
+    loss, log_prob, clipped = new((), dtype=torch.float32), new(lead, dtype=torch.float32), new(lead, dtype=torch.bool)
+    kl = new(lead, dtype=torch.float32) if with_kl else None
+    grad = new(logits.shape, dtype=logits.dtype) if gradient else None
+    workspace = new((_workspace_bytes(),), dtype=torch.uint8)
 
+    def at(t):
+        return None if t is None else t.data_ptr()
 
-_workspace = []
-
-
-def _workspace_bytes() -> int:
-    if not _workspace:
-        _workspace.append(int(_lib.lib().scacchi_policy_loss_workspace_bytes()))
-    return _workspace[0]
+    rows = _lib.PolicyRows(x.data_ptr(), at(ref), at(legal), action.data_ptr(), old_log_prob.data_ptr(),
+                           advantage.data_ptr(), at(weight), at(reference_log_prob), max(x.stride(0), A),
+                           A if ref is None else max(ref.stride(0), A))
+    out = _lib.PolicyOut(loss.data_ptr(), log_prob.data_ptr(), at(kl), clipped.data_ptr(), at(grad))
+    _lib.check(_lib.lib().scacchi_policy_loss(C.byref(rows), C.byref(out), N, A, DTYPES[logits.dtype], clip_low,
+                                              clip_high, kl_coefficient, workspace.data_ptr(), stream_handle(dev)),
+               "policy_loss")
+    return PolicyLoss(loss, log_prob, clipped, kl, grad)
