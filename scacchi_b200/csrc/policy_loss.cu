@@ -158,14 +158,18 @@ __device__ __forceinline__ double log_row_sum(float s) {
 struct SumOp {
   template <typename U>
   __device__ static U apply(U a, U b) { return a + b; }
+  template <typename U>
+  __device__ static U none(U) { return U(0); }
 };
 struct MaxOp {
   template <typename U>
   __device__ static U apply(U a, U b) { return a > b ? a : b; }
+  template <typename U>
+  __device__ static U none(U) { return U(-INFINITY); }
 };
 
 // max, sum of e^{x - max} and of d e^{x - max}
-struct Stats {
+struct alignas(16) Stats {
   float top, sum, mean;
 };
 
@@ -189,76 +193,67 @@ struct Lanes {
   }
 };
 
-// warp butterflies, then the warps' results of every CTA of the cluster in
-// rank and warp order, which is the same for every thread
+// Three levels of butterflies: a warp's lanes, the CTA's warps, the
+// cluster's CTAs (each sends its own result to all).  Every thread ends with
+// the same bits.
 struct Ctas {
-  double *slots;      // shared: two banks of kMaxWarps partials, taken in turn
-  Stats *stat_slots;  // likewise
+  Stats *slots;  // shared: two banks of kMaxWarps of the warps', two of kMaxCluster of the CTAs'
   int ctas, rank;
   mutable int bank;
   __device__ int index() const { return rank * blockDim.x + threadIdx.x; }
   __device__ int size() const { return ctas * blockDim.x; }
-  __device__ void sync() const {
-    if (ctas > 1)
-      cg::this_cluster().sync();
-    else
-      __syncthreads();
+
+  template <typename U, typename Join>
+  __device__ static U butterfly(U v, int width, Join join) {
+    for (int off = width >> 1; off; off >>= 1) v = join(v, shuffle(v, off));
+    return v;
+  }
+  __device__ static float shuffle(float v, int off) { return __shfl_xor_sync(kFull, v, off); }
+  __device__ static double shuffle(double v, int off) { return __shfl_xor_sync(kFull, v, off); }
+  __device__ static Stats shuffle(Stats v, int off) {
+    return Stats{shuffle(v.top, off), shuffle(v.sum, off), shuffle(v.mean, off)};
   }
   // A bank is written again two reductions later, and every thread has
-  // passed the barrier of the one between them, so its readers are done.
+  // passed a barrier of the one between them, so its readers are done.
+  template <typename U, typename Join>
+  __device__ U all(U v, U none, Join join) const {
+    static_assert(sizeof(U) <= sizeof(Stats), "slot");
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    Stats *mine = slots + bank * kMaxWarps, *theirs = slots + 2 * kMaxWarps + bank * kMaxCluster;
+    bank ^= 1;
+    v = butterfly(v, 32, join);
+    if (warps > 1) {
+      if (lane == 0) *reinterpret_cast<U *>(mine + (threadIdx.x >> 5)) = v;
+      __syncthreads();
+      v = butterfly(lane < warps ? *reinterpret_cast<const U *>(mine + lane) : none, kMaxWarps, join);
+      v = broadcast(v);
+    }
+    if (ctas > 1) {
+      if ((int)threadIdx.x < ctas)
+        *reinterpret_cast<U *>(cg::this_cluster().map_shared_rank(theirs, threadIdx.x) + rank) = v;
+      cg::this_cluster().sync();
+      v = butterfly(lane < ctas ? *reinterpret_cast<const U *>(theirs + lane) : none, kMaxCluster, join);
+      v = broadcast(v);
+    }
+    return v;
+  }
+  // lanes beyond the butterfly's width hold another result
+  __device__ static float broadcast(float v) { return __shfl_sync(kFull, v, 0); }
+  __device__ static double broadcast(double v) { return __shfl_sync(kFull, v, 0); }
+  __device__ static Stats broadcast(Stats v) {
+    return Stats{broadcast(v.top), broadcast(v.sum), broadcast(v.mean)};
+  }
   template <typename Op, typename U>
   __device__ U reduce(U v) const {
-    for (int off = 16; off; off >>= 1) v = Op::apply(v, __shfl_xor_sync(kFull, v, off));
-    double *mine = slots + bank * kMaxWarps;
-    bank ^= 1;
-    if ((threadIdx.x & 31) == 0) *reinterpret_cast<U *>(mine + (threadIdx.x >> 5)) = v;
-    sync();
-    const int warps = blockDim.x >> 5;
-    U r{};
-    for (int c = 0; c < ctas; ++c) {
-      const double *from = ctas > 1 ? cg::this_cluster().map_shared_rank(mine, c) : mine;
-      for (int i = 0; i < warps; ++i) {
-        const U u = *reinterpret_cast<const U *>(from + i);
-        r = (c | i) ? Op::apply(r, u) : u;
-      }
-    }
-    return r;
+    return all(v, Op::none(U()), [](U a, U b) { return Op::apply(a, b); });
   }
-  // One barrier for all three: each warp's maximum scales its sums; every
-  // lane then folds some of the warps' and a butterfly the rest.
   __device__ Stats stats(Stats v) const {
-    float top = v.top;
-    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
-    rescale(v, top);
-    for (int off = 16; off; off >>= 1) {
-      v.sum += __shfl_xor_sync(kFull, v.sum, off);
-      v.mean += __shfl_xor_sync(kFull, v.mean, off);
-    }
-    Stats *mine = stat_slots + bank * kMaxWarps;
-    bank ^= 1;
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, total = ctas * warps;
-    if (lane == 0) mine[threadIdx.x >> 5] = v;
-    sync();
-    Stats all = {-INFINITY, 0.0f, 0.0f};
-    for (int i = 0; i < total; i += 32) {
-      Stats u = {-INFINITY, 0.0f, 0.0f};
-      if (i + lane < total) {
-        const int c = (i + lane) / warps;
-        const Stats *from = ctas > 1 ? cg::this_cluster().map_shared_rank(mine, c) : mine;
-        u = from[i + lane - c * warps];
-      }
-      top = fmaxf(all.top, u.top);
-      for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
-      rescale(all, top);
-      rescale(u, top);
-      all.sum += u.sum;
-      all.mean += u.mean;
-    }
-    for (int off = 16; off; off >>= 1) {
-      all.sum += __shfl_xor_sync(kFull, all.sum, off);
-      all.mean += __shfl_xor_sync(kFull, all.mean, off);
-    }
-    return all;
+    return all(v, Stats{-INFINITY, 0.0f, 0.0f}, [](Stats a, Stats b) {
+      const float top = fmaxf(a.top, b.top);
+      rescale(a, top);
+      rescale(b, top);
+      return Stats{top, a.sum + b.sum, a.mean + b.mean};
+    });
   }
 };
 
@@ -704,13 +699,11 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtas<V * W, Kl>) policy_l
 template <typename T, int W, bool Kl>
 __global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Params p) {
   extern __shared__ __align__(16) uint8_t s_rows[];
-  __shared__ double s_slots[2 * kMaxWarps];
-  __shared__ Stats s_stats[2 * kMaxWarps];
+  __shared__ __align__(16) Stats s_slots[2 * kMaxWarps + 2 * kMaxCluster];
   using Pack = Vec<T, W>;
   using Mask = Vec<uint8_t, W>;
   Ctas grp;
   grp.slots = s_slots;
-  grp.stat_slots = s_stats;
   grp.ctas = (int)cg::this_cluster().num_blocks();
   grp.rank = (int)cg::this_cluster().block_rank();
   grp.bank = 0;
