@@ -39,6 +39,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/scacchi_b200.h"
 
@@ -105,6 +106,44 @@ struct alignas(sizeof(T) * W) Vec {
   T v[W];
 };
 
+// a vector's elements as floats, and back; 16-bit ones two at a time
+template <typename T, int W>
+__device__ __forceinline__ void unpack(const Vec<T, W> &p, float (&f)[W]) {
+#pragma unroll
+  for (int w = 0; w < W; ++w) f[w] = to_f(p.v[w]);
+}
+template <int W>
+__device__ __forceinline__ void unpack(const Vec<__nv_bfloat16, W> &p, float (&f)[W]) {
+  if constexpr (W % 2 == 0) {
+    const uint32_t *u = reinterpret_cast<const uint32_t *>(&p);
+#pragma unroll
+    for (int w = 0; w < W; w += 2) {
+      f[w] = __uint_as_float(u[w / 2] << 16);
+      f[w + 1] = __uint_as_float(u[w / 2] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int w = 0; w < W; ++w) f[w] = to_f(p.v[w]);
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ Vec<T, W> pack(const float (&f)[W]) {
+  Vec<T, W> p;
+  if constexpr (sizeof(T) == 2 && W % 2 == 0) {
+#pragma unroll
+    for (int w = 0; w < W; w += 2) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        *reinterpret_cast<__nv_bfloat162 *>(p.v + w) = __floats2bfloat162_rn(f[w], f[w + 1]);
+      else
+        *reinterpret_cast<__half2 *>(p.v + w) = __floats2half2_rn(f[w], f[w + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int w = 0; w < W; ++w) p.v[w] = from_f<T>(f[w]);
+  }
+  return p;
+}
+
 // e^y - 1 - y for |y| < 1 to 1.2e-7 of itself: y^2 times the Chebyshev
 // interpolant of degree 6 of (e^y - 1 - y) / y^2 on [-1, 1]
 __device__ __forceinline__ float phi_small(float y) {
@@ -118,12 +157,14 @@ __device__ __forceinline__ float phi_small(float y) {
   return c * (y * y);
 }
 
-// e^u for u <= 0 or small (see above)
-__device__ __forceinline__ float exp_fast(float u) {
+__device__ __forceinline__ float exp2_fast(float t) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(u * kLog2E));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
   return y;
 }
+
+// e^u for u <= 0 or small (see above)
+__device__ __forceinline__ float exp_fast(float u) { return exp2_fast(u * kLog2E); }
 
 // log of a positive finite float to 1e-9: s = 2^k f with f in [1/sqrt 2,
 // sqrt 2), log f = 2 atanh(q), q = (f - 1) / (f + 1), |q| < 0.172: the odd
@@ -753,29 +794,36 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Param
     // where there is no kept action
     auto load = [&](int v, float(&xa)[W], float(&da)[W]) {
       const int a = v * W - lead;
-      const Pack xv = *reinterpret_cast<const Pack *>(sx + a);
-      Pack rv;
-      Mask lv;
-      if (Kl) rv = *reinterpret_cast<const Pack *>(sr + a);
-      if (legal) lv = *reinterpret_cast<const Mask *>(sl + a);
-      const bool whole = a >= 0 && a + W <= n;
+      unpack(*reinterpret_cast<const Pack *>(sx + a), xa);
+      if (a < 0 || a + W > n) {
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        xa[w] = to_f(xv.v[w]);
-        if ((!whole && (a + w < 0 || a + w >= n)) || (legal && !lv.v[w])) xa[w] = -INFINITY;
-        da[w] = 0.0f;
-        if (Kl && xa[w] != -INFINITY) da[w] = xa[w] - to_f(rv.v[w]);
+        for (int w = 0; w < W; ++w)
+          if (a + w < 0 || a + w >= n) xa[w] = -INFINITY;
+      }
+      if (legal) {
+        const Mask lv = *reinterpret_cast<const Mask *>(sl + a);
+#pragma unroll
+        for (int w = 0; w < W; ++w) xa[w] = lv.v[w] ? xa[w] : -INFINITY;
+      }
+      if (Kl) {
+        float ra[W];
+        unpack(*reinterpret_cast<const Pack *>(sr + a), ra);
+#pragma unroll
+        for (int w = 0; w < W; ++w) da[w] = xa[w] == -INFINITY ? 0.0f : xa[w] - ra[w];
       }
     };
     Stats st = {-INFINITY, 0.0f, 0.0f};
+    float from = 0.0f;  // st.top, or 0 without an action yet, when only a NaN has a part in the sum
     for (int v = t; v < vecs; v += threads) {
-      float xa[W], da[W], top = -INFINITY;
+      float xa[W], da[W];
       load(v, xa, da);
+      float top = xa[0];
 #pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, xa[w]);
-      if (top > st.top) rescale(st, top);
-      // without an action yet, only a NaN among them has a part in the sum
-      const float from = st.top == -INFINITY ? 0.0f : st.top;
+      for (int w = 1; w < W; ++w) top = fmaxf(top, xa[w]);
+      if (top > st.top) {
+        rescale(st, top);
+        from = top;
+      }
       float sum[2] = {0.0f, 0.0f}, mean[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < W; ++w) {
@@ -788,6 +836,8 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Param
     }
     st = grp.stats(st);
     const float inv = 1.0f / st.sum, mean = st.mean * inv;
+    // what the row's end does not judge: p to 2^-23 |m| is enough
+    const float shift = -st.top * kLog2E;
     float kl = 0.0f;
     if (Kl) {
       for (int v = t; v < vecs; v += threads) {
@@ -799,7 +849,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Param
           const float y = mean - da[w];
           const bool near = fabsf(y) < 1.0f;
           some |= !near;
-          part = fmaf(near ? exp_fast(xa[w] - st.top) : 0.0f, phi_small(near ? y : 0.0f), part);
+          part = fmaf(near ? exp2_fast(fmaf(xa[w], kLog2E, shift)) : 0.0f, phi_small(near ? y : 0.0f), part);
         }
         kl = fmaf(part, inv, kl);
         if (some) {
@@ -808,8 +858,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Param
             // from shared memory again: registers are not indexed
             const int a = v * W - lead + w;
             if (a < 0 || a >= n || (legal && !sl[a])) continue;
-            const float xw = to_f(sx[a]);
-            const float dw = xw - to_f(sr[a]);
+            const float xw = to_f(sx[a]), dw = xw - to_f(sr[a]);
             if (xw != -INFINITY && !(fabsf(mean - dw) < 1.0f)) kl += kl_part_far(exp_fast(xw - st.top) * inv, dw, mean);
           }
         }
@@ -820,18 +869,22 @@ __global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Param
     share += out.share;
     if (grad) {
       const float wc = -out.wc * inv, wb = out.wb * inv;
-      const int at_k = k - lo;
+      const int at_k = k - lo + lead;  // the action, counted from vector 0
       for (int v = t; v < vecs; v += threads) {
         float xa[W], da[W];
         load(v, xa, da);
         const int a = v * W - lead;
-        Pack o;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          float g = (Kl ? fmaf(wb, da[w] - mean, wc) : wc) * exp_fast(xa[w] - st.top);
-          if (a + w == at_k) g += out.wc;
-          o.v[w] = from_f<T>(g);
+          const float e = exp2_fast(fmaf(xa[w], kLog2E, shift));
+          xa[w] = (Kl ? fmaf(wb, da[w] - mean, wc) : wc) * e;
         }
+        if (at_k / W == v && at_k >= 0) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (v * W + w == at_k) xa[w] += out.wc;
+        }
+        const Pack o = pack<T, W>(xa);
         if (a >= 0 && a + W <= n) {
           *reinterpret_cast<Pack *>(grad + a) = o;
         } else {
