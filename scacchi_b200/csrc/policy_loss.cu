@@ -51,8 +51,9 @@ std::atomic<uint64_t> g_policy_launches{0};
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kShortThreads = 256;
-constexpr int kLongThreads = 512;
-constexpr int kMaxWarps = kLongThreads / 32;
+constexpr int kLongThreads = 256;
+constexpr int kMaxWarps = 8;  // of a long row's CTA
+static_assert(kLongThreads == 32 * kMaxWarps, "warps");
 constexpr int kMaxCluster = 16;
 constexpr int kMaxShort = 512;     // actions of a short row
 constexpr int kMaxActions = 262144;
@@ -738,7 +739,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtas<V * W, Kl>) policy_l
 // registers or the memory to keep it (and lets two to sixteen CTAs share an
 // SM, so that one loads while others compute).
 template <typename T, int W, bool Kl>
-__global__ void __launch_bounds__(kLongThreads, 2) policy_loss_long_kernel(Params p) {
+__global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(Params p) {
   extern __shared__ __align__(16) uint8_t s_rows[];
   __shared__ __align__(16) Stats s_slots[2 * kMaxWarps + 2 * kMaxCluster];
   using Pack = Vec<T, W>;
@@ -1001,7 +1002,8 @@ cudaError_t by_lanes(Params &p, int *ctas, cudaStream_t st) {
 
 // Long rows: a cluster where half an SM's shared memory does not hold the
 // row, or where the rows leave SMs idle (down to 4096 actions a CTA);
-// threads for some four vectors each; and as many CTAs an SM as its shared
+// threads for four vectors or more each (256 at most: 512 took 166 us for
+// 4096 x 32000 bf16 where 256 take 145); and as many CTAs an SM as its shared
 // memory holds.
 template <typename T, int W, bool Kl>
 cudaError_t by_cta(Params &p, int *ctas, cudaStream_t st) {

@@ -9,7 +9,6 @@ loss is the cross-entropy to the search's policy.
 
 from __future__ import annotations
 
-import ctypes as C
 import functools
 import math
 from typing import NamedTuple
@@ -37,7 +36,8 @@ class PolicyLoss(NamedTuple):
 
 def _rows(t: torch.Tensor, actions: int) -> torch.Tensor:
     """[..., A] as rows [N, A] of unit column stride, a view where it can be."""
-    t = t.detach()
+    if t.requires_grad:
+        t = t.detach()
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= actions:
         return t
     t = t.reshape(-1, actions)
@@ -127,8 +127,8 @@ def _per_row(t: torch.Tensor, name: str, lead: torch.Size, dev: torch.device) ->
 
 
 @functools.lru_cache(maxsize=1)
-def _workspace_bytes() -> int:
-    return int(_lib.lib().scacchi_policy_loss_workspace_bytes())
+def _workspace_floats() -> int:
+    return -(-int(_lib.lib().scacchi_policy_loss_workspace_bytes()) // 4)
 
 
 def _launch(logits, action, old_log_prob, advantage, legal, weight, reference_logits, reference_log_prob, clip_low,
@@ -143,12 +143,14 @@ def _launch(logits, action, old_log_prob, advantage, legal, weight, reference_lo
     x = _rows(logits, A)
     ref = None if reference_logits is None else _rows(reference_logits, A)
     N = x.shape[0]
-    with_kl = ref is not None or reference_log_prob is not None
-    new = functools.partial(torch.empty, device=dev)
-    loss, log_prob, clipped = new((), dtype=torch.float32), new(lead, dtype=torch.float32), new(lead, dtype=torch.bool)
-    kl = new(lead, dtype=torch.float32) if with_kl else None
-    grad = new(logits.shape, dtype=logits.dtype) if gradient else None
-    workspace = new((_workspace_bytes(),), dtype=torch.uint8)
+    # (empty_like and new_empty cost the host half of what torch.empty does)
+    loss, log_prob = old_log_prob.new_empty(()), torch.empty_like(old_log_prob)
+    clipped = torch.empty_like(action, dtype=torch.bool)
+    kl = None if ref is None and reference_log_prob is None else torch.empty_like(old_log_prob)
+    grad = None
+    if gradient:
+        grad = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
+    workspace = old_log_prob.new_empty((_workspace_floats(),))
 
     def at(t):
         return None if t is None else t.data_ptr()
@@ -157,7 +159,7 @@ def _launch(logits, action, old_log_prob, advantage, legal, weight, reference_lo
                            advantage.data_ptr(), at(weight), at(reference_log_prob), max(x.stride(0), A),
                            A if ref is None else max(ref.stride(0), A))
     out = _lib.PolicyOut(loss.data_ptr(), log_prob.data_ptr(), at(kl), clipped.data_ptr(), at(grad))
-    _lib.check(_lib.lib().scacchi_policy_loss(C.byref(rows), C.byref(out), N, A, DTYPES[logits.dtype], clip_low,
-                                              clip_high, kl_coefficient, workspace.data_ptr(), stream_handle(dev)),
+    _lib.check(_lib.lib().scacchi_policy_loss(rows, out, N, A, DTYPES[logits.dtype], clip_low, clip_high,
+                                              kl_coefficient, workspace.data_ptr(), stream_handle(dev)),
                "policy_loss")
     return PolicyLoss(loss, log_prob, clipped, kl, grad)
