@@ -83,10 +83,11 @@ struct Product {
   float decay, step;
 };
 
-// Tiles of tile row i of a symmetric output: those that touch the stored blocks.
+// Tiles of tile row i of a symmetric output: those of the stored blocks, of
+// which 128 x 128 tiles leave out the one that its neighbour writes turned.
 template <int BM, int BN>
 __host__ __device__ __forceinline__ int row_tiles(int i, int tiles_n) {
-  const int n = ((i * BM) / kSym + 1) * (kSym / BN);
+  const int n = BM == BN && BM < kSym ? i + 1 : ((i * BM) / kSym + 1) * (kSym / BN);
   return n < tiles_n ? n : tiles_n;
 }
 
@@ -138,6 +139,21 @@ struct StageDesc {
   __device__ __forceinline__ uint64_t b_of(int term, int k) const { return b + (term == 0 ? b_part : 0u) + k * b_step; }
 };
 
+// eight values as hi and lo halves
+__device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __half2 a = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+    const float2 f = __half22float2(a);
+    const __half2 b = __floats2half2_rn(v[2 * e] - f.x, v[2 * e + 1] - f.y);
+    h[e] = *reinterpret_cast<const uint32_t *>(&a);
+    l[e] = *reinterpret_cast<const uint32_t *>(&b);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
 // Place of row `row`, 4-float chunk `chunk` in an epilogue patch: rows of
 // 32 floats, chunks swizzled so that a row per lane, eight columns of a row
 // per lane and a column per lane all spread over the banks.
@@ -150,12 +166,15 @@ __device__ __forceinline__ int patch_at(int row, int chunk) {
 // written in whole pieces of rows, as hi + lo in the panels of the next
 // product's operand, or to the user's matrix.
 //
+// `mirror`: written turned as well, in the place of a tile that is not
+// computed.
+//
 // This code runs once per tile, so what it costs is mostly fetching it:
-// unrolled over the blocks (40 KB of code) it took 4 us a block, rolled
-// TODO.
+// unrolled over the blocks (some 40 KB of instructions) it took 4 us for a
+// warp's 32 columns, rolled 1 us.
 template <int COLS>
-__device__ __forceinline__ void emit(const Product &q, int batch, int r0, int c_first, const float (&sum)[COLS],
-                                     float *patch) {
+__device__ __forceinline__ void emit(const Product &q, int batch, int r0, int c_first, bool mirror,
+                                     const float (&sum)[COLS], float *patch) {
   const int lane = threadIdx.x & 31;
 #pragma unroll 1
   for (int g = 0; g < COLS / 32; ++g) {
@@ -200,31 +219,36 @@ __device__ __forceinline__ void emit(const Product &q, int batch, int r0, int c_
         }
       }
     } else {
-      // eight columns of a row per lane: 64 bytes of eight rows at a time
+      // eight columns of a row per lane: 64 bytes of eight rows at a time;
+      // turned, eight rows of a column
       const int64_t part = (int64_t)q.dst_panels * q.dst_rows * 64;
-      __half *to = q.dst + (int64_t)batch * 2 * part + ((int64_t)(c0 / 64) * q.dst_rows + r0) * 64;
-      const int oct = lane & 3, chunk = (c0 & 32) / 8 + oct;
-      const int diagonal = q.diag != 0.0f ? c0 + 8 * oct - r0 : 1 << 30;  // row - column offset of the diagonal
+      const int oct = lane & 3;
+#pragma unroll 1
+      for (int turned = 0; turned <= (int)mirror; ++turned) {
+        const int rows_at = turned ? c0 : r0, cols_at = turned ? r0 : c0, chunk = (cols_at & 32) / 8 + oct;
+        if (rows_at >= q.dst_rows || cols_at >= q.dst_panels * 64) break;
+        __half *to = q.dst + (int64_t)batch * 2 * part + ((int64_t)(cols_at / 64) * q.dst_rows + rows_at) * 64;
+        // row - column offset of the diagonal
+        const int diagonal = q.diag != 0.0f ? cols_at + 8 * oct - rows_at : 1 << 30;
 #pragma unroll 2
-      for (int row = lane >> 2; row < 32; row += 8) {
-        float y[8];
-        *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(patch + patch_at(row, 2 * oct));
-        *reinterpret_cast<float4 *>(y + 4) = *reinterpret_cast<const float4 *>(patch + patch_at(row, 2 * oct + 1));
-        uint32_t hi[4], lo[4];
+        for (int row = lane >> 2; row < 32; row += 8) {
+          float y[8];
+          if (turned) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          float u = y[e] * q.scale, v = y[e + 1] * q.scale;
-          if (row - diagonal == e && r0 + row < q.rows) u += q.diag;
-          if (row - diagonal == e + 1 && r0 + row < q.rows) v += q.diag;
-          const __half2 a = __floats2half2_rn(u, v);
-          const float2 f = __half22float2(a);
-          const __half2 b = __floats2half2_rn(u - f.x, v - f.y);
-          hi[e / 2] = *reinterpret_cast<const uint32_t *>(&a);
-          lo[e / 2] = *reinterpret_cast<const uint32_t *>(&b);
+            for (int e = 0; e < 8; ++e) y[e] = patch[patch_at(8 * oct + e, row >> 2) + (row & 3)];
+          } else {
+            *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(patch + patch_at(row, 2 * oct));
+            *reinterpret_cast<float4 *>(y + 4) = *reinterpret_cast<const float4 *>(patch + patch_at(row, 2 * oct + 1));
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            y[e] = y[e] * q.scale + (row - diagonal == e && rows_at + row < q.rows ? q.diag : 0.0f);
+          uint4 hi, lo;
+          split8(y, hi, lo);
+          __half *at = to + row * 64 + ((chunk ^ (row & 7)) << 3);
+          *reinterpret_cast<uint4 *>(at) = hi;
+          *reinterpret_cast<uint4 *>(at + part) = lo;
         }
-        __half *at = to + row * 64 + ((chunk ^ (row & 7)) << 3);
-        *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(at + part) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     __syncwarp();
@@ -423,7 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok) break;
       int batch, i, j;
       locate<2 * kBM, BN>(q, t, batch, i, j);
-      emit<kCols>(q, batch, (2 * i + rank) * kBM + quad * 32, j * BN + half * kCols, sum, patch);
+      emit<kCols>(q, batch, (2 * i + rank) * kBM + quad * 32, j * BN + half * kCols, false, sum, patch);
     }
   }
   __syncwarp();
@@ -446,7 +470,7 @@ struct TileLayout {
   static constexpr int kBars = kPatches + kEpiWarps * kPatch;
   static constexpr int kBytes = kBars + 8 * (2 * kStages + 2 * kSlots) + 16 + 1024;  // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory budget");
-  static_assert(kBN * kBM * 4 <= kPatches, "the partial sums take the stages' place");
+  static_assert((16 + kMaxSplit) * 32 * 32 * 4 <= kPatches, "the partial sums take the stages' place");
 };
 
 // The same product for outputs of few tiles: the CTAs of a cluster share one
@@ -582,27 +606,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         acc_phase ^= 1u;
       }
     }
+    // the tile right of it in the diagonal's 256 x 256 block is its mirror image
+    const bool mirror = q.sym && (i & 1) && j == i - 1;
     if (ctas == 1) {
-      if (ok) emit<kCols>(q, batch, i * kBM + quad * 32, j * BN + half * kCols, sum, patch);
+      if (ok) emit<kCols>(q, batch, i * kBM + quad * 32, j * BN + half * kCols, mirror, sum, patch);
     } else {
-      // Each CTA finishes 16 / ctas of the tile's 32 x 32 blocks, a warp
+      // The CTAs finish the tile's sixteen 32 x 32 blocks in turn, a warp
       // each; the others' partial sums arrive as [source][block][four
       // elements][lane].
-      const int blocks = 16 / ctas;
+      const int most = (16 + ctas - 1) / ctas;
       __syncwarp();
       cg::this_cluster().sync();  // every CTA is done with its stages
 #pragma unroll
       for (int g = 0; g < kCols / 32; ++g) {
         const int id = (half * (kCols / 32) + g) * 4 + quad;
-        float4 *to = cg::this_cluster().map_shared_rank(reinterpret_cast<float4 *>(smem), id / blocks);
-        to += (rank * blocks + id % blocks) * 256 + lane;
+        float4 *to = cg::this_cluster().map_shared_rank(reinterpret_cast<float4 *>(smem), id % ctas);
+        to += (rank * most + id / ctas) * 256 + lane;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           to[e * 32] = make_float4(sum[32 * g + 4 * e], sum[32 * g + 4 * e + 1], sum[32 * g + 4 * e + 2],
                                    sum[32 * g + 4 * e + 3]);
       }
       cg::this_cluster().sync();
-      if (warp - 4 < blocks && ok) {
+      const int id = (warp - 4) * ctas + rank;
+      if (warp - 4 < most && id < 16 && ok) {
         const float4 *at = reinterpret_cast<const float4 *>(smem) + (warp - 4) * 256 + lane;
         float v[32];
 #pragma unroll
@@ -610,14 +637,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int from = 0; from < ctas; ++from)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float4 f = at[from * blocks * 256 + e * 32];
+            const float4 f = at[from * most * 256 + e * 32];
             v[4 * e] += f.x;
             v[4 * e + 1] += f.y;
             v[4 * e + 2] += f.z;
             v[4 * e + 3] += f.w;
           }
-        const int id = rank * blocks + warp - 4;
-        emit<32>(q, batch, i * kBM + (id & 3) * 32, j * BN + (id >> 2) * 32, v, patch);
+        emit<32>(q, batch, i * kBM + (id & 3) * 32, j * BN + (id >> 2) * 32, mirror, v, patch);
       }
     }
   }
@@ -741,7 +767,6 @@ struct Narrow {
   int rows, cols;          // the user's matrix
   int side, length, tall;  // its narrow and long side, and which is which
   int panels, steps;       // 64 along the long side each
-  int sub;                 // K of an accumulator: 32 or 64
   int quintic;
   double scale, eps;
   float inv;               // 2^-e
@@ -770,26 +795,14 @@ __device__ __forceinline__ int narrow_at(int row, int chunk) {
   return (chunk >> 3) * (kBM * 128) + row * 128 + (((chunk ^ row) & 7) << 4);
 }
 
-// 32 columns of the summed accumulators of a row (TMEM lane) per thread
+// 32 columns of the summed accumulators of a row (TMEM lane) per thread.
+// The last one's may reach 16 columns past the accumulators, not past TMEM:
+// at most six of them are narrower than 96.
 __device__ __forceinline__ void read_sum(float (&sum)[32], uint32_t acc, int count, uint32_t stride) {
 #pragma unroll
   for (int e = 0; e < 32; ++e) sum[e] = 0.0f;
 #pragma unroll 1
   for (int a = 0; a < count; ++a, acc += stride) add_stage<32>(sum, acc);
-}
-
-__device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const __half2 a = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-    const float2 f = __half22float2(a);
-    const __half2 b = __floats2half2_rn(v[2 * e] - f.x, v[2 * e + 1] - f.y);
-    h[e] = *reinterpret_cast<const uint32_t *>(&a);
-    l[e] = *reinterpret_cast<const uint32_t *>(&b);
-  }
-  hi = make_uint4(h[0], h[1], h[2], h[3]);
-  lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
 // The last product's 32 rows (of the narrow side) by 32 of the long side, a
@@ -1015,10 +1028,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
 
   uint32_t parity = 0;
   const uint32_t x_at = smem_u32(smem), z_at = smem_u32(smem + L::kZAt);
-  const int sub = q.sub / 16;  // K steps of 16 per accumulator
-  // One product: `ksteps` of 16, n columns.  b_mn: B's panels lie along N
-  // and K counts their rows.
-  auto product = [&](uint32_t a, uint32_t a_part, uint32_t b, uint32_t b_part, int ksteps, int n, bool b_mn) {
+  // One product: `ksteps` of 16, `sub` of them per accumulator of n columns
+  // (of the 512 that there are).  b_mn: B's panels lie along N and K counts
+  // their rows.
+  auto product = [&](uint32_t a, uint32_t a_part, uint32_t b, uint32_t b_part, int ksteps, int sub, int n,
+                     bool b_mn) {
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
@@ -1028,23 +1042,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
         const uint32_t idesc = idesc_f16(kBM, n, false, b_mn);
         // N along B's panels of 128 rows: the next 64 columns are a panel on
         const uint64_t da = desc_sw128(a, false), db = desc_sw128(b, b_mn, kBM * 128);
-        // unrolled by accumulators of 32 of K: a loop over single MMAs took
-        // longer to issue than they run
-        const uint32_t a_lo = a_part >> 4, b_lo = b_part >> 4, b_step = b_mn ? 2048u >> 4 : 32u >> 4;
-        uint32_t d = tmem;
-        for (int k0 = 0; k0 < ksteps; k0 += 2) {
-          const uint32_t along = ((uint32_t)(k0 >> 2) * (kBM * 128) + (uint32_t)(k0 & 3) * 32) >> 4;  // K-major
-          const uint64_t ka = da + along, kb = db + (b_mn ? (uint32_t)k0 * b_step : along);
-          const bool two = k0 + 1 < ksteps;
-          const uint32_t more = sub == 4 ? (uint32_t)(k0 & 2) : 0u;  // the second half of a 64-wide accumulator
-          umma_f16(d, ka, kb + b_lo, idesc, more);
-          if (two) umma_f16(d, ka + 2, kb + b_step + b_lo, idesc, 1u);
-          umma_f16(d, ka + a_lo, kb, idesc, 1u);
-          if (two) umma_f16(d, ka + a_lo + 2, kb + b_step, idesc, 1u);
-          umma_f16(d, ka, kb, idesc, 1u);
-          if (two) umma_f16(d, ka + 2, kb + b_step, idesc, 1u);
-          if (sub == 2 || more) d += (uint32_t)n;
-        }
+        for (int k0 = 0, acc = 0; k0 < ksteps; k0 += sub, acc += n)
+          for (int term = 0; term < 3; ++term)
+            for (int k = k0; k < k0 + sub && k < ksteps; ++k) {
+              const uint32_t along = (uint32_t)(k >> 2) * (kBM * 128) + (uint32_t)(k & 3) * 32;  // K-major
+              const uint32_t ao = (term == 1 ? a_part : 0u) + along;
+              const uint32_t bo = (term == 0 ? b_part : 0u) + (b_mn ? (uint32_t)k * 2048u : along);
+              umma_f16(tmem + (uint32_t)acc, da + (ao >> 4), db + (bo >> 4), idesc, term != 0 || k != k0);
+            }
         umma_commit(done);
       }
       __syncwarp();
@@ -1057,14 +1062,23 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
 
   const int mine_steps = ((mine * 64 < q.length - panel0 * 64 ? mine * 64 : q.length - panel0 * 64) + 15) / 16;
   const int side_steps = (q.side + 15) / 16, side_n = side_steps * 16;
-  const int mine_accs = (mine_steps + sub - 1) / sub, side_accs = (side_steps + sub - 1) / sub;
+  // K steps per accumulator: two, or as many as TMEM's columns make it
+  auto sub_of = [](int ksteps, int n) {
+    const int accs = 512 / n, sub = (ksteps + accs - 1) / accs;
+    return sub < 2 ? 2 : sub;
+  };
+  const int n_update = mine * 64;
+  const int gram_sub = sub_of(mine_steps, side_n), square_sub = sub_of(side_steps, side_n);
+  const int update_sub = sub_of(side_steps, n_update);
+  const int gram_accs = (mine_steps + gram_sub - 1) / gram_sub, square_accs = (side_steps + square_sub - 1) / square_sub;
+  const int update_accs = (side_steps + update_sub - 1) / update_sub;
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
   const int row = quad * 32 + lane, col = (warp >> 2) * 32;  // of this thread's 32 entries of Z and M
   float v[32];
   for (int step = 0; step < q.steps; ++step) {
     // X X^T over this slice
-    product(x_at, L::kX, x_at, L::kX, mine_steps, side_n, false);
-    read_sum(v, tmem + lanes + (uint32_t)col, mine_accs, (uint32_t)side_n);
+    product(x_at, L::kX, x_at, L::kX, mine_steps, gram_sub, side_n, false);
+    read_sum(v, tmem + lanes + (uint32_t)col, col < side_n ? gram_accs : 0, (uint32_t)side_n);
     if (ctas == 1) {
       narrow_square(smem + L::kZAt, L::kZ, row, col, q.side, q.scale1, q.diag1, v);
     } else {
@@ -1111,17 +1125,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
       cluster.sync();
     }
     if (q.quintic) {
-      product(z_at, L::kZ, z_at, L::kZ, side_steps, side_n, false);
-      read_sum(v, tmem + lanes + (uint32_t)col, side_accs, (uint32_t)side_n);
+      product(z_at, L::kZ, z_at, L::kZ, side_steps, square_sub, side_n, false);
+      read_sum(v, tmem + lanes + (uint32_t)col, col < side_n ? square_accs : 0, (uint32_t)side_n);
       narrow_square(smem + L::kZAt, L::kZ, row, col, q.side, q.scale2, q.diag2, v);
     }
     // X <- M X
-    const int n = mine * 64;
-    product(z_at, L::kZ, x_at, L::kX, side_steps, n, true);
+    product(z_at, L::kZ, x_at, L::kX, side_steps, update_sub, n_update, true);
     const bool last = step + 1 == q.steps;
 #pragma unroll 1
-    for (int c = col; c < n; c += 128) {
-      read_sum(v, tmem + lanes + (uint32_t)c, side_accs, (uint32_t)n);
+    for (int c = col; c < n_update; c += 128) {
+      read_sum(v, tmem + lanes + (uint32_t)c, update_accs, (uint32_t)n_update);
       if (!last) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] *= q.inv;
@@ -1214,10 +1227,10 @@ int64_t stack_bytes(int64_t batch, int64_t rows, int64_t cols) {
   return batch * 2 * ((rows + 63) / 64 * 64) * ((cols + 63) / 64) * 128;
 }
 
-// the device: its SMs, and how many clusters of 2, 4 and 8 CTAs of the tile
+// the device: its SMs, and how many clusters of 2 to 8 CTAs of the tile
 // kernel it runs at once
 struct Device {
-  int sms, clusters[4];
+  int sms, clusters[kMaxSplit + 1];
 };
 
 constexpr int kMaxDevices = 64;
@@ -1250,14 +1263,15 @@ const Device *device() {
           cudaSuccess ||
       set_up_pair<256>() != cudaSuccess || set_up_pair<128>() != cudaSuccess)
     return nullptr;
-  for (int z = 1; z < 4; ++z) {
+  d.clusters[1] = d.sms;
+  for (int z = 2; z <= kMaxSplit; ++z) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1u << z);
+    cfg.gridDim = dim3((unsigned)z);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = TileLayout::kBytes;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 1u << z;
+    attr.val.clusterDim.x = (unsigned)z;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
@@ -1288,13 +1302,14 @@ cudaError_t run_pair(Product q, const Stack &a, const Stack &b, const Device &d,
                 a.map, b.map, q);
 }
 
-// The kernel and the CTAs that share a tile's K, by their times in us: a
-// stage of a 256 x 256 pair tile takes 0.9 and its epilogue, which hides
-// less behind the next tile than a 256 x 128 one's, 3; a 256 x 128 pair
-// tile 0.53 and 0.5, the last one's 2; a 128 x 128 tile, which draws the
-// most operands per product, 0.7 and 4 to start and end; splitting its K
-// costs 2 more.  What leaves SMs idle is a tile count below a wave, or just
-// above one.
+// The kernel and the CTAs that share a tile's K, by their measured times in
+// us beyond what every launch takes: a stage of a 256 x 256 pair tile 0.9 and
+// its epilogue, which hides less behind the next tile than a 256 x 128
+// one's, 3; a 256 x 128 pair tile 0.53 and 0.5, the last one's 2; a 128 x
+// 128 tile, which draws the most operands per product, 0.65 and 1.5 (3.5
+// where a symmetric one is written twice), or with its K split 4.2 (two
+// cluster barriers and the exchange).  What leaves SMs idle is a tile count
+// below a wave, or just above one.
 cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, const Device &d, cudaStream_t st) {
   q.a_rows = a.panel_rows;
   q.b_rows = b.panel_rows;
@@ -1304,16 +1319,16 @@ cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, 
   const int64_t kblocks = (q.k + kBK - 1) / kBK, pairs = d.sms / 2;
   const int64_t p256 = tile_count<256, 256>(q, a.batch), p128 = tile_count<256, 128>(q, a.batch);
   const int64_t t128 = tile_count<128, 128>(q, a.batch);
-  const double cost256 = (double)((p256 + pairs - 1) / pairs) * (0.9 * (double)kblocks + 3.0) + 1.5;
+  const double cost256 = (double)((p256 + pairs - 1) / pairs) * (0.9 * (double)kblocks + 3.0) + 2.2;
   const double cost128 = (double)((p128 + pairs - 1) / pairs) * (0.53 * (double)kblocks + 0.5) + 2.0;
-  double best = (double)((t128 + d.sms - 1) / d.sms) * (0.7 * (double)kblocks + 4.0) - 2.0;
+  double best = (double)((t128 + d.sms - 1) / d.sms) * (0.65 * (double)kblocks + (q.sym ? 3.5 : 1.5));
   int split = 1;
-  for (int z = 1; z < 4 && (1 << z) <= kblocks; ++z) {
-    if (t128 > d.clusters[z]) break;
-    const double cost = 0.7 * (double)((kblocks + (1 << z) - 1) >> z) + 4.0;
+  for (int z = 2; z <= kMaxSplit && z <= kblocks; ++z) {
+    if (t128 > d.clusters[z]) continue;
+    const double cost = 0.65 * (double)((kblocks + z - 1) / z) + 4.2;
     if (cost < best) {
       best = cost;
-      split = 1 << z;
+      split = z;
     }
   }
   if (cost256 < cost128 && cost256 <= best) return run_pair<256>(q, a, b, d, p256, st);
@@ -1336,8 +1351,8 @@ int narrow_ctas(const scacchi_newton_schulz &n, const Device &d) {
   int best = 0;
   int64_t best_cost = 0;
   for (int z = 0; z < 4; ++z) {
-    const int ctas = 1 << z, slice = (panels + ctas - 1) / ctas, at_once = z ? d.clusters[z] : d.sms;
-    if (slice > NarrowLayout::kMostPanels || ctas > panels) continue;
+    const int ctas = 1 << z, slice = (panels + ctas - 1) / ctas, at_once = d.clusters[ctas];
+    if (slice > NarrowLayout::kMostPanels || ctas > panels || at_once < 1) continue;
     const int64_t cost = ((int64_t)n.batch + at_once - 1) / at_once * ((z ? 55 : 30) + 4 * slice);
     if (!best || cost < best_cost) {
       best = ctas;
@@ -1358,8 +1373,6 @@ int newton_schulz_narrow(const scacchi_newton_schulz &n, const Source &src, cons
   q.length = q.tall ? n.rows : n.cols;
   q.panels = (q.length + 63) / 64;
   q.steps = n.steps;
-  // accumulators of 32 of K where they all fit into TMEM's 512 columns
-  q.sub = (q.panels + ctas - 1) / ctas <= 2 ? 32 : 64;
   q.quintic = n.c != 0.0;
   q.scale = ldexp(1.0, n.scale_exponent);
   q.eps = n.eps;
