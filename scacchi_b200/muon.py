@@ -6,18 +6,25 @@ A weight is a matrix [in, out] as flax stores it: the dense kernels of
 ``AZDirichletParams`` as they are, a convolution kernel [3, 3, in, out] as
 its [9 in, out] reshape.  Leading axes stack matrices of one shape, which
 one call updates together.
+
+``NetworkMuon`` holds the network's matrices in that form (the blocks'
+convolutions as one stack), steps them, and gives back the parameters that
+``AZDirichletNet`` evaluates.
 """
 
 from __future__ import annotations
 
 import ctypes as C
+import dataclasses
 import functools
 import math
 
+import numpy as np
 import torch
 
 from . import _lib
 from .dirichlet_mctx.tree import ptr, stream_handle
+from .network import AZDirichletParams
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -139,3 +146,46 @@ def muon_update(weight: torch.Tensor, gradient: torch.Tensor, momentum: torch.Te
                                                   stream_handle(dev)), "muon_update")
     # a graph recorded before the step refuses to run backward through it
     torch.autograd.graph.increment_version((weight, momentum))
+
+
+# the dense kernels; the blocks' convolutions are the stack "convs"
+DENSE = ("policy_w", "value_w", "q_dir_w", "q_dir_out_w", "q_conc_w", "q_conc_out_w")
+
+
+class NetworkMuon:
+    """Muon over the matrices of ``AZDirichletParams``: the blocks'
+    convolutions as one stack ``convs`` [2 blocks, 9 channels, channels] (in
+    order: block 0's first, its second, block 1's first, ...) and the dense
+    kernels of DENSE by their names.
+
+    ``step`` takes gradients of any of them, in their shapes; ``params``
+    gives the updated parameters.  The stem, the 1x1 convolutions, the
+    output vectors, biases and BatchNorm are not matrices to orthogonalise
+    and stay as they were given (train them with Adam beside it).
+    """
+
+    def __init__(self, params: AZDirichletParams, *, learning_rate: float, beta: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-8,
+                 device="cuda"):
+        self._params = params
+        self.settings = dict(learning_rate=learning_rate, beta=beta, nesterov=nesterov, weight_decay=weight_decay,
+                             steps=steps, coefficients=coefficients, eps=eps)
+        convs = np.stack([blk[k].reshape(-1, blk[k].shape[-1]) for blk in params.blocks for k in ("conv1_w", "conv2_w")])
+        host = {"convs": convs, **{name: getattr(params, name) for name in DENSE}}
+        self.matrices = {k: torch.tensor(np.asarray(v, np.float32), device=device) for k, v in host.items()}
+        self.momentum = {k: torch.zeros_like(v) for k, v in self.matrices.items()}
+
+    def step(self, gradients: dict) -> None:
+        unknown = sorted(set(gradients) - set(self.matrices))
+        if unknown:
+            raise ValueError(f"no such matrices: {unknown}; expected some of {sorted(self.matrices)}")
+        for name, gradient in gradients.items():
+            muon_update(self.matrices[name], gradient, self.momentum[name], **self.settings)
+
+    def params(self) -> AZDirichletParams:
+        host = {k: v.cpu().numpy() for k, v in self.matrices.items()}
+        blocks = [dict(blk) for blk in self._params.blocks]
+        for i, blk in enumerate(blocks):
+            for j, k in enumerate(("conv1_w", "conv2_w")):
+                blk[k] = host["convs"][2 * i + j].reshape(blk[k].shape)
+        return dataclasses.replace(self._params, blocks=blocks, **{name: host[name] for name in DENSE})
