@@ -77,7 +77,7 @@ def orthogonalize(matrix: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     with A = X X^T on the narrow side; returns X in the input's shape and
     type (float32, bfloat16 or float16).  The products carry 32-bit
     accuracy whatever the type, and round once at the end.  A matrix of
-    zeros gives zeros; one with an infinity or a NaN gives NaN, and leaves
+    zeros gives zeros (NaN where ``eps`` is 0); one with an infinity or a NaN gives NaN, and leaves
     the others of its stack alone.
 
     The call launches on the current stream, does not synchronise and can

@@ -12,6 +12,9 @@ eps / 2 of it (and half the smallest subnormal).
 """
 
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -281,6 +284,72 @@ def test_strided_rows_and_leading_shape(cuda):
     assert torch.equal(one.grad_logits[0], one.grad_logits[3])
     scalar = clipped_policy_loss(logits[0], action[0].long(), kw["old_log_prob"][0], kw["advantage"][0])
     assert scalar.log_prob.shape == () and torch.equal(scalar.grad_logits, one.grad_logits[0] * 4)
+
+
+def _moved(t, offset, pad):
+    """`t` as rows `pad` elements further apart, from an odd place of a buffer of NaN (of ones, for a mask)."""
+    N, A = t.shape
+    fill = 1 if t.dtype == torch.bool else math.nan
+    buf = torch.full((offset + N * (A + pad) + 64,), fill, dtype=t.dtype, device="cuda")
+    view = buf[offset:offset + N * (A + pad)].view(N, A + pad)[:, :A]
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("kl", ["none", "full"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(37, 82), (37, 81), (21, 600), (21, 601), (5, 20003), (2, 70001)], ids=str)
+def test_rows_at_any_alignment(cuda, size, dtype, kl):
+    """Bases and strides off every vector's alignment, together and each by
+    itself, with masks likewise."""
+    logits, action, kw = _inputs(*size, dtype, True, kl, seed=15)
+    for x_at, r_at, m_at in (((1, 0), (1, 0), (1, 0)), ((0, 3), (0, 3), (0, 0)), ((3, 1), (2, 5), (7, 0)),
+                             ((0, 0), (1, 0), (0, 0)), ((2, 8), (2, 8), (2, 0)), ((5, 0), (5, 0), (3, 0))):
+        moved = dict(kw, legal=_moved(kw["legal"], *m_at))
+        if kl == "full":
+            moved["reference_logits"] = _moved(kw["reference_logits"], *r_at)
+        _check(_moved(logits, *x_at), action, moved, beta=0.0 if kl == "none" else 0.1)
+
+
+@pytest.mark.parametrize("A", [82, 3000])
+def test_a_nan_stays_in_its_row(cuda, A):
+    logits, action, kw = _inputs(12, A, "fp32", False, "full", seed=16)
+    clean = clipped_policy_loss(logits, action, kl_coefficient=0.1, **kw)
+    logits[5, (int(action[5]) + 1) % A] = math.nan
+    out = clipped_policy_loss(logits, action, kl_coefficient=0.1, **kw)
+    others = torch.arange(12, device="cuda") != 5
+    assert math.isnan(float(out.loss)) and bool(torch.isnan(out.log_prob[5])) and bool(torch.isnan(out.grad_logits[5]).any())
+    for name in ("log_prob", "kl", "grad_logits", "clipped"):
+        assert torch.equal(getattr(out, name)[others], getattr(clean, name)[others]), name
+
+
+def test_first_call_under_capture(cuda):
+    """A process whose first calls are captured, not run."""
+    code = """
+import torch
+from scacchi_b200.policy_loss import clipped_policy_loss
+from scacchi_b200.muon import orthogonalize
+g = torch.Generator(device="cuda").manual_seed(0)
+x = [torch.randn(s, generator=g, device="cuda") for s in ((40, 82), (3, 5000), (90, 70), (300, 400))]
+z = torch.zeros(40, device="cuda")
+k = z.int()
+torch.cuda.synchronize()
+def work():
+    a = clipped_policy_loss(x[0], k, z, z + 1)
+    b = clipped_policy_loss(x[1], k[:3], z[:3], z[:3] + 1)
+    return [a.grad_logits, b.grad_logits, orthogonalize(x[2]), orthogonalize(x[3])]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = work()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(held, work()):
+    assert torch.equal(a, b) and bool(a.any())
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
 
 
 def test_rows_past_32_bits(cuda):
