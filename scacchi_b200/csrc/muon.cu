@@ -59,7 +59,7 @@ constexpr int kLaunchRegisters = 168, kFewRegisters = 48, kManyRegisters = 224;
 static_assert(128 * kFewRegisters + 32 * kEpiWarps * kManyRegisters <= kThreads * kLaunchRegisters,
               "setmaxnreg would wait forever");
 constexpr int kMaxSplit = 8;       // CTAs of a cluster that share a tile's K
-constexpr int kNormBlocks = 128;   // most partial sums of squares per matrix
+constexpr int kNormBlocks = 1024;  // most partial sums of squares per matrix
 constexpr int kPatch = 32 * 32 * 4;  // an epilogue warp's 32 x 32 block in fp32
 
 __device__ uint32_t g_muon_error;
@@ -194,27 +194,31 @@ __device__ __forceinline__ void emit(const Product &q, int batch, int r0, int c_
       const int64_t base = ((int64_t)batch * q.rows + r0) * q.cols + c0 + lane;
       const int n = q.rows - r0 < 32 ? q.rows - r0 : 32;
       if (c0 + lane < q.cols) {
+        if (q.weight) {
+          // half of the block's weights are requested before the first is used
 #pragma unroll 1
-        for (int row = 0; row < n; row += 8) {
-          float y[8];
+          for (int half = 0; half < n; half += 16) {
+            float w[16];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            y[e] = patch[patch_at(row + e, lane >> 2) + (lane & 3)] * q.scale;
-            if (q.weight && row + e < n)
-              y[e] = fmaf(-q.step, y[e], q.decay * q.weight[base + (int64_t)(row + e) * q.cols]);
+            for (int e = 0; e < 16; ++e)
+              if (half + e < n) w[e] = q.weight[base + (int64_t)(half + e) * q.cols];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (half + e < n)
+                q.weight[base + (int64_t)(half + e) * q.cols] =
+                    fmaf(-q.step, patch[patch_at(half + e, lane >> 2) + (lane & 3)] * q.scale, q.decay * w[e]);
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int64_t at = base + (int64_t)(row + e) * q.cols;
-            if (row + e >= n) break;
-            if (q.weight)
-              q.weight[at] = y[e];
-            else if (q.dtype == 0)
-              static_cast<float *>(q.out)[at] = y[e];
+        } else {
+#pragma unroll 8
+          for (int row = 0; row < n; ++row) {
+            const float y = patch[patch_at(row, lane >> 2) + (lane & 3)] * q.scale;
+            const int64_t at = base + (int64_t)row * q.cols;
+            if (q.dtype == 0)
+              static_cast<float *>(q.out)[at] = y;
             else if (q.dtype == 1)
-              static_cast<__nv_bfloat16 *>(q.out)[at] = __float2bfloat16_rn(y[e]);
+              static_cast<__nv_bfloat16 *>(q.out)[at] = __float2bfloat16_rn(y);
             else
-              static_cast<__half *>(q.out)[at] = __float2half_rn(y[e]);
+              static_cast<__half *>(q.out)[at] = __float2half_rn(y);
           }
         }
       }
@@ -673,59 +677,102 @@ __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 
-__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
-  if (dtype == 0) return static_cast<const float *>(p)[i];
-  if (dtype == 1) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-  return __half2float(static_cast<const __half *>(p)[i]);
-}
-
 __device__ __forceinline__ float muon_direction(const Source &s, float g, float m) {
   return s.nesterov ? fmaf(s.beta, m, s.rest * g) : m;
 }
 
-// sum of squares of each matrix in 64 bits (an update may be small enough
-// that its squares leave fp32), one partial per block
-__global__ void __launch_bounds__(256) ns_norm_kernel(Source s, int64_t elems, double *partial) {
+// sum of eight squares, in 64 bits where 32 would lose them (a conversion
+// per element takes the time of the load)
+__device__ __forceinline__ double sum_of_squares(const float (&u)[8]) {
+  float s = 0.0f, most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    s = fmaf(u[e], u[e], s);
+    most = fmaxf(most, fabsf(u[e]));
+  }
+  if (most == 0.0f || (most > 1e-15f && most < 1e18f)) return (double)s;  // NaN stays in s
+  double d = 0.0;
+  for (int e = 0; e < 8; ++e) d = fma((double)u[e], (double)u[e], d);
+  return d;
+}
+
+// eight neighbouring elements as floats; `vec`: they start on 16 bytes
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, bool vec, int left, float (&f)[8]) {
+  if (vec) {
+    constexpr int kWords = 8 * (int)sizeof(T) / 16;
+    uint4 raw[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
+    const T *v = reinterpret_cast<const T *>(raw);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = to_f(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = e < left ? to_f(p[e]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ double norm_part(const Source &s, int64_t base, int64_t elems, bool vec) {
+  const T *in = static_cast<const T *>(s.in) + base;
+  float *momentum = s.momentum ? s.momentum + base : nullptr;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x * 8;
+  double sum = 0.0;
+#pragma unroll 2
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; i < elems; i += stride) {
+    const int left = elems - i < 8 ? (int)(elems - i) : 8;
+    float u[8], m[8];
+    load8(in + i, vec, left, u);
+    if (momentum) {
+      load8(momentum + i, vec, left, m);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = fmaf(s.beta, m[e], s.rest * u[e]);
+        u[e] = muon_direction(s, u[e], m[e]);
+      }
+      if (vec) {
+        *reinterpret_cast<float4 *>(momentum + i) = make_float4(m[0], m[1], m[2], m[3]);
+        *reinterpret_cast<float4 *>(momentum + i + 4) = make_float4(m[4], m[5], m[6], m[7]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) momentum[i + e] = m[e];
+      }
+    }
+    sum += sum_of_squares(u);
+  }
+  return sum;
+}
+
+// sum of squares of each matrix (in 64 bits: an update may be small enough
+// that its squares leave fp32), one partial per block, and Muon's momentum
+__global__ void __launch_bounds__(256) ns_norm_kernel(Source s, int64_t elems, int vec, double *partial) {
   __shared__ double part[8];
   const int64_t base = (int64_t)blockIdx.y * elems;
-  double sum = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < elems; i += (int64_t)gridDim.x * blockDim.x) {
-    float u = load_any(s.in, s.dtype, base + i);
-    if (s.momentum) {
-      const float m = fmaf(s.beta, s.momentum[base + i], s.rest * u);
-      s.momentum[base + i] = m;
-      u = muon_direction(s, u, m);
-    }
-    sum = fma((double)u, (double)u, sum);
-  }
+  double sum = s.dtype == 0   ? norm_part<float>(s, base, elems, vec)
+               : s.dtype == 1 ? norm_part<__nv_bfloat16>(s, base, elems, vec)
+                              : norm_part<__half>(s, base, elems, vec);
   for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     double total = 0.0;
     for (int i = 0; i < 8; ++i) total += part[i];
-    partial[blockIdx.y * kNormBlocks + blockIdx.x] = total;
+    partial[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = total;
   }
 }
 
-__device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn(v - __half2float(hi));
-}
-
-// kept out of line: as a select, its conversions run for every element
-__device__ __noinline__ float scale_in_64(float u, double f) { return (float)((double)u * f); }
-
 // S u / (|u| + eps) as hi + lo in panels, a 16-byte chunk of each per thread
 __global__ void __launch_bounds__(256) ns_split_kernel(Source s, const double *partial, int blocks, int rows, int cols,
-                                                       int panel_rows, int panels, double scale, double eps,
+                                                       int panel_rows, int panels, int vec, double scale, double eps,
                                                        __half *dst) {
   __shared__ double s_factor;
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   if (threadIdx.x < 32) {
     double sum = 0.0;
-    for (int i = threadIdx.x; i < blocks; i += 32) sum += partial[blockIdx.y * kNormBlocks + i];
+    for (int i = threadIdx.x; i < blocks; i += 32) sum += partial[(int64_t)blockIdx.y * blocks + i];
     for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (threadIdx.x == 0) s_factor = scale / (sqrt(sum) + eps);
   }
@@ -740,21 +787,36 @@ __global__ void __launch_bounds__(256) ns_split_kernel(Source s, const double *p
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / chunks;
     const int c8 = (int)(i - r * chunks), c = c8 * 8;
-    __half hi[8], lo[8];
+    float u[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float u = 0.0f;
-      if (r < rows && c + e < cols) {
-        const int64_t at = base + r * cols + c + e;
-        u = load_any(s.in, s.dtype, at);
-        if (s.momentum) u = muon_direction(s, u, s.momentum[at]);
-        u = in_32 ? u * f : scale_in_64(u, f64);
+    for (int e = 0; e < 8; ++e) u[e] = 0.0f;
+    const int left = r < rows ? (cols - c < 8 ? cols - c : 8) : 0;
+    if (left > 0) {
+      const int64_t at = base + r * cols + c;
+      if (s.dtype == 0)
+        load8(static_cast<const float *>(s.in) + at, vec, left, u);
+      else if (s.dtype == 1)
+        load8(static_cast<const __nv_bfloat16 *>(s.in) + at, vec, left, u);
+      else
+        load8(static_cast<const __half *>(s.in) + at, vec, left, u);
+      if (s.momentum) {
+        float m[8];
+        load8(s.momentum + at, vec, left, m);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = muon_direction(s, u[e], m[e]);
       }
-      split_half(u, hi[e], lo[e]);
+      if (in_32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] *= f;
+      } else {
+        for (int e = 0; e < 8; ++e) u[e] = (float)((double)u[e] * f64);
+      }
     }
+    uint4 hi, lo;
+    split8(u, hi, lo);
     __half *at = out + ((int64_t)(c8 >> 3) * panel_rows + r) * 64 + (((c8 & 7) ^ (int)(r & 7)) << 3);
-    *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(hi);
-    *reinterpret_cast<uint4 *>(at + part) = *reinterpret_cast<const uint4 *>(lo);
+    *reinterpret_cast<uint4 *>(at) = hi;
+    *reinterpret_cast<uint4 *>(at + part) = lo;
   }
 }
 
@@ -857,21 +919,6 @@ __device__ __forceinline__ void narrow_chunk(const Narrow &q, int id, int chunks
     row = id / chunks;
     chunk = id - row * chunks;
   }
-}
-
-// sum of eight squares, in 64 bits where 32 would lose them (a conversion
-// per element takes the time of the load)
-__device__ __forceinline__ double sum_of_squares(const float (&u)[8]) {
-  float s = 0.0f, most = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    s = fmaf(u[e], u[e], s);
-    most = fmaxf(most, fabsf(u[e]));
-  }
-  if (most == 0.0f || (most > 1e-15f && most < 1e18f)) return (double)s;  // NaN stays in s
-  double d = 0.0;
-  for (int e = 0; e < 8; ++e) d = fma((double)u[e], (double)u[e], d);
-  return d;
 }
 
 // The slice's update (and the momentum it leaves), eight neighbours along
@@ -1223,6 +1270,16 @@ struct Stack {
   }
 };
 
+// partial sums of squares of a matrix, at most
+int64_t norm_blocks(int64_t rows, int64_t cols) {
+  const int64_t blocks = (rows * cols + 2047) / 2048;
+  return blocks < kNormBlocks ? blocks : kNormBlocks;
+}
+
+int64_t norm_bytes(int64_t batch, int64_t rows, int64_t cols) {
+  return (batch * norm_blocks(rows, cols) * (int64_t)sizeof(double) + 255) / 256 * 256;
+}
+
 int64_t stack_bytes(int64_t batch, int64_t rows, int64_t cols) {
   return batch * 2 * ((rows + 63) / 64 * 64) * ((cols + 63) / 64) * 128;
 }
@@ -1403,7 +1460,7 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
   const bool tall = n.rows > n.cols;
   uint8_t *at = static_cast<uint8_t *>(workspace);
   double *partial = reinterpret_cast<double *>(at);
-  at += (size_t)n.batch * kNormBlocks * sizeof(double);
+  at += norm_bytes(n.batch, n.rows, n.cols);
   Stack x, y, gram, poly;
   const int64_t wide = stack_bytes(n.batch, n.rows, n.cols), narrow = stack_bytes(n.batch, s, s);
   if (!x.place(at, n.batch, n.rows, n.cols) || !y.place(at + wide, n.batch, n.rows, n.cols) ||
@@ -1412,19 +1469,22 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
   const double scale = ldexp(1.0, n.scale_exponent);
   const int64_t elems = (int64_t)n.rows * n.cols;
 
-  int64_t blocks = (elems + 4095) / 4096;
-  const int64_t share = (4 * (int64_t)sms + n.batch - 1) / n.batch;
+  // 16-byte vectors where every matrix starts on one
+  auto on_16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const int vec = elems % 8 == 0 && on_16(src.in) && (!src.momentum || on_16(src.momentum));
+  int64_t blocks = norm_blocks(n.rows, n.cols);
+  const int64_t share = (8 * (int64_t)sms + n.batch - 1) / n.batch;
   blocks = blocks < share ? blocks : share;
-  blocks = blocks < kNormBlocks ? blocks : kNormBlocks;
-  if (launch(ns_norm_kernel, dim3((unsigned)blocks, (unsigned)n.batch), 256, 0, st, false, 1, src, elems, partial) !=
-      cudaSuccess)
+  if (launch(ns_norm_kernel, dim3((unsigned)blocks, (unsigned)n.batch), 256, 0, st, false, 1, src, elems, vec,
+             partial) != cudaSuccess)
     return SCACCHI_ECUDA;
   const int64_t chunks = (int64_t)x.panel_rows * x.panels * 8;
+  const int split_vec = vec && n.cols % 8 == 0;  // rows too
   int64_t split_blocks = (chunks + 255) / 256;
   const int64_t split_share = (8 * (int64_t)sms + n.batch - 1) / n.batch;
   split_blocks = split_blocks < split_share ? split_blocks : split_share;
   if (launch(ns_split_kernel, dim3((unsigned)split_blocks, (unsigned)n.batch), 256, 0, st, true, 1, src,
-             (const double *)partial, (int)blocks, n.rows, n.cols, x.panel_rows, x.panels, scale, n.eps, x.p) != cudaSuccess)
+             (const double *)partial, (int)blocks, n.rows, n.cols, x.panel_rows, x.panels, split_vec, scale, n.eps, x.p) != cudaSuccess)
     return SCACCHI_ECUDA;
 
   // M = c Z^2 + (a - b^2 / 4c) I with Z = A + (b / 2c) I: the square alone,
@@ -1508,8 +1568,7 @@ int32_t scacchi_muon_scale_exponent(double a, double b, double c, int32_t steps)
 size_t scacchi_muon_workspace_bytes(int32_t batch, int32_t rows, int32_t cols) {
   if (batch < 1 || rows < 1 || cols < 1) return 0;
   const int64_t s = rows < cols ? rows : cols;
-  return (size_t)batch * kNormBlocks * sizeof(double) + 2 * (size_t)stack_bytes(batch, rows, cols) +
-         2 * (size_t)stack_bytes(batch, s, s);
+  return (size_t)(norm_bytes(batch, rows, cols) + 2 * stack_bytes(batch, rows, cols) + 2 * stack_bytes(batch, s, s));
 }
 
 int scacchi_orthogonalize(const scacchi_newton_schulz *params, const void *matrix, void *out, void *workspace,
