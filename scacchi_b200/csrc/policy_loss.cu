@@ -21,10 +21,17 @@
 //
 // One pass over memory: short rows live in the registers of a few lanes,
 // long ones in the shared memory of a CTA or of a cluster, so every input is
-// read once and every output written once.  Row sums are held in 32 bits, the log-probability is finished in 64 from them and
-// the loss is summed in 64.  A row whose ratio lies within kBorderTol of a
-// clip border is evaluated again in 64 bits, so the side it falls on does
-// not depend on 32-bit rounding.
+// read once and every output written once.  Row sums are held in 32 bits,
+// the log-probability is finished in 64 from them and the loss is summed in
+// 64.  A row whose ratio lies within kBorderTol of a clip border is evaluated
+// again in 64 bits, so the side it falls on does not depend on 32-bit
+// rounding.
+//
+// What bounds it is the instructions an action costs (some 57 with the full
+// KL, 25 without), not memory: 262144 rows of 82 fp32 actions with the full
+// KL take 102 us (2.8 TB/s, 44 % of a copy's rate), with a sampled KL 60 us
+// (3.3 TB/s); 4096 rows of 32000 bf16 138 us (3.8 TB/s); 8 rows of 131071
+// fp32 19 us, which is latency: one row's phases across a cluster.
 //
 // Exponentials are ex2.approx of (x - m) log2 e: the difference first, so
 // that only |x - m|, which p weights, is rounded and scaled; their errors
@@ -468,7 +475,7 @@ __device__ __forceinline__ void stage(E *to, const E *from, int count, int t, in
 
 // CTAs an SM, as the registers of a thread's elements allow
 template <int Elems, bool Kl>
-constexpr int kShortCtas = Kl && Elems > 6 ? 2 : 3;
+constexpr int kShortCtas = Kl && Elems > 12 ? 2 : 3;
 
 // One array's rows of a warp's batch in shared memory.
 template <typename E>
@@ -498,13 +505,15 @@ struct Piece {
   bool ok;              // the ends are whole words, and every batch is alike
 
   __device__ __forceinline__ void copy(uint32_t to, int64_t turn, int lane) const {
+    // (read once: nothing in shared memory is kept across an asm)
+    const int head = first, n = vecs, ends = words;
     const uint8_t *src = from + turn * step;
     to += (uint32_t)phase;
-    for (int i = lane; i < vecs; i += 32)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + first + 16 * i), "l"(src + first + 16 * i)
+    for (int i = lane; i < n; i += 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + head + 16 * i), "l"(src + head + 16 * i)
                    : "memory");
-    if (lane < words) {
-      const int at = 4 * lane < first ? 4 * lane : 4 * lane + 16 * vecs;
+    if (lane < ends) {
+      const int at = 4 * lane < head ? 4 * lane : 4 * lane + 16 * n;
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + at), "l"(src + at) : "memory");
     }
   }
@@ -655,11 +664,17 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtas<V * W, Kl>) policy_l
   uint8_t *const base = s_rows + warp * 2 * buffer;
   // A full batch of rows in one piece starts at the same place within 16
   // bytes every time (the step is a multiple of 16 rows): its copies are
-  // worked out once.
-  const Piece px = piece_of(x + first * p.stride, per_warp * A * (int)sizeof(T), step * p.stride * (int)sizeof(T));
-  const Piece pr = piece_of(r + first * p.reference_stride, per_warp * A * (int)sizeof(T),
-                            step * p.reference_stride * (int)sizeof(T));
-  const Piece pl = piece_of(p.legal + first * A, per_warp * A, step * A);
+  // worked out once, and kept in shared memory, not in the registers that
+  // the elements need (262144 x 82 fp32 with a sampled KL 69 us, now 60).
+  __shared__ Piece s_pieces[kShortThreads / 32][3];
+  const Piece &px = s_pieces[warp][0], &pr = s_pieces[warp][1], &pl = s_pieces[warp][2];
+  if (lane == 0) {
+    s_pieces[warp][0] = piece_of(x + first * p.stride, per_warp * A * (int)sizeof(T), step * p.stride * (int)sizeof(T));
+    s_pieces[warp][1] = piece_of(r + first * p.reference_stride, per_warp * A * (int)sizeof(T),
+                                 step * p.reference_stride * (int)sizeof(T));
+    s_pieces[warp][2] = piece_of(p.legal + first * A, per_warp * A, step * A);
+  }
+  __syncwarp();
   const bool pieces = !p.x_pitch && px.ok && (!Kl || (!p.r_pitch && pr.ok)) && (!p.legal || pl.ok);
   const uint32_t base_at = (uint32_t)__cvta_generic_to_shared(base);
   int64_t turn = 0;
@@ -964,7 +979,8 @@ cudaError_t launch_short(Params &p, int *ctas, cudaStream_t st) {
   p.r_pitch = !Kl || p.reference_stride == p.actions ? 0 : pitch;
   // a lane's vectors past the last row are read too, and ignored
   const int past = p.group * V * W;
-  p.slice_bytes = ((per_warp * pitch + past) * (int)sizeof(T) + 31) / 16 * 16;
+  const int row = p.x_pitch || p.r_pitch ? pitch : p.actions;
+  p.slice_bytes = ((per_warp * row + past) * (int)sizeof(T) + 31) / 16 * 16;
   p.mask_bytes = (per_warp * p.actions + past + 47) / 16 * 16;
   const int smem = warps * 2 * ((Kl ? 2 : 1) * p.slice_bytes + (p.legal ? p.mask_bytes : 0));
   static std::atomic<uint64_t> allowed{0};
