@@ -1495,7 +1495,8 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
   const int64_t split_share = (8 * (int64_t)sms + n.batch - 1) / n.batch;
   split_blocks = split_blocks < split_share ? split_blocks : split_share;
   if (launch(ns_split_kernel, dim3((unsigned)split_blocks, (unsigned)n.batch), 256, 0, st, true, 1, src,
-             (const double *)partial, (int)blocks, n.rows, n.cols, x.panel_rows, x.panels, split_vec, scale, n.eps, x.p) != cudaSuccess)
+             (const double *)partial, (int)blocks, n.rows, n.cols, x.panel_rows, x.panels, split_vec, scale, n.eps,
+             x.p) != cudaSuccess)
     return SCACCHI_ECUDA;
 
   // M = c Z^2 + (a - b^2 / 4c) I with Z = A + (b / 2c) I: the square alone,

@@ -649,7 +649,8 @@ __device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, i
 }
 
 template <typename T, int W, int V, bool Kl>
-__global__ void __launch_bounds__(kShortThreads, kShortCtas<V * W, Kl>) policy_loss_short_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kShortThreads, kShortCtas<V * W, Kl>)
+    policy_loss_short_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint8_t s_rows[];
   __shared__ double s_part[kShortThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.group, A = p.actions;

@@ -77,8 +77,9 @@ def orthogonalize(matrix: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     with A = X X^T on the narrow side; returns X in the input's shape and
     type (float32, bfloat16 or float16).  The products carry 32-bit
     accuracy whatever the type, and round once at the end.  A matrix of
-    zeros gives zeros (NaN where ``eps`` is 0); one with an infinity or a NaN gives NaN, and leaves
-    the others of its stack alone.
+    zeros gives zeros (NaN where ``eps`` is 0); one with an infinity or a
+    NaN gives NaN, and leaves the others of its stack alone.  The result is
+    outside autograd.
 
     The call launches on the current stream, does not synchronise and can
     be captured into a CUDA graph.
@@ -170,7 +171,8 @@ class NetworkMuon:
         self._params = params
         self.settings = dict(learning_rate=learning_rate, beta=beta, nesterov=nesterov, weight_decay=weight_decay,
                              steps=steps, coefficients=coefficients, eps=eps)
-        convs = np.stack([blk[k].reshape(-1, blk[k].shape[-1]) for blk in params.blocks for k in ("conv1_w", "conv2_w")])
+        kernels = [blk[k] for blk in params.blocks for k in ("conv1_w", "conv2_w")]
+        convs = np.stack([k.reshape(-1, k.shape[-1]) for k in kernels])
         host = {"convs": convs, **{name: getattr(params, name) for name in DENSE}}
         self.matrices = {k: torch.tensor(np.asarray(v, np.float32), device=device) for k, v in host.items()}
         self.momentum = {k: torch.zeros_like(v) for k, v in self.matrices.items()}
@@ -179,6 +181,11 @@ class NetworkMuon:
         unknown = sorted(set(gradients) - set(self.matrices))
         if unknown:
             raise ValueError(f"no such matrices: {unknown}; expected some of {sorted(self.matrices)}")
+        for name, gradient in gradients.items():  # all of them before the first is applied
+            m = self.matrices[name]
+            if gradient.shape != m.shape or gradient.device != m.device or gradient.dtype not in DTYPES:
+                raise ValueError(f"the gradient of {name} must be float32, bfloat16 or float16 {tuple(m.shape)} on "
+                                 f"{m.device}, got {gradient.dtype} {tuple(gradient.shape)} on {gradient.device}")
         for name, gradient in gradients.items():
             muon_update(self.matrices[name], gradient, self.momentum[name], **self.settings)
 

@@ -266,3 +266,23 @@ def test_refusals(cuda):
         with pytest.raises(ValueError):
             muon_update(**{**good, **kw})
     assert _lib.launch_count() == before
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(2, 264, 304), (2, 160, 301), (3, 129, 131), (2, 72, 96)], ids=str)
+def test_muon_at_any_alignment(cuda, shape, dtype):
+    """Tensors that start on their element alone give the bits of aligned ones."""
+    def odd(t):
+        at = torch.full((t.numel() + 2,), 7.0, dtype=t.dtype, device="cuda")
+        at[1:-1].view(t.shape).copy_(t)
+        return at
+
+    w, m = _matrix(shape, "fp32", "normal", seed=21), _matrix(shape, "fp32", "normal", seed=22)
+    g = _matrix(shape, dtype, "normal", seed=23)
+    w2, m2, g2 = odd(w), odd(m), odd(g)
+    view = lambda t: t[1:-1].view(shape)
+    muon_update(w, g, m, learning_rate=0.05, weight_decay=0.1)
+    muon_update(view(w2), view(g2), view(m2), learning_rate=0.05, weight_decay=0.1)
+    assert torch.equal(view(w2), w) and torch.equal(view(m2), m)
+    for t in (w2, m2, g2):  # and nothing beside them is written
+        assert float(t[0]) == 7.0 and float(t[-1]) == 7.0

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from scacchi_b200 import _lib
-from scacchi_b200.muon import COEFFICIENTS, MAX_SIDE, muon_update, orthogonalize
+from scacchi_b200.muon import COEFFICIENTS, MAX_SIDE, NetworkMuon, muon_update, orthogonalize
+from scacchi_b200.network import init_params
 
 A = 1 << 20  # a made-up aligned address: a refused call reads none
 
@@ -81,3 +82,17 @@ def test_workspace_size():
     assert f(12, 1152, 128) >= 12 * (2 * 1152 * 128 + 2 * 128 * 128) * 4
     assert f(1, 3, 5) % 256 == 0
     assert f(2, 65536, 65536) > 2 ** 36
+
+
+def test_network_muon_refuses_a_step_as_a_whole():
+    """One bad gradient, and no matrix has moved."""
+    opt = NetworkMuon(init_params(4, num_blocks=1), learning_rate=0.1, device="cpu")
+    before = {k: v.clone() for k, v in opt.matrices.items()}
+    good = {k: torch.ones_like(v) for k, v in opt.matrices.items()}
+    for bad in (torch.ones((3, 3)), torch.ones_like(good["value_w"], dtype=torch.int32),
+                torch.ones_like(good["value_w"]).double()):
+        with pytest.raises(ValueError, match="gradient of value_w"):
+            opt.step({**good, "value_w": bad})
+    with pytest.raises(ValueError, match="no such matrices"):
+        opt.step({**good, "stem_w": torch.ones((3, 3))})
+    assert all(torch.equal(v, before[k]) for k, v in opt.matrices.items())
