@@ -29,9 +29,9 @@
 //
 // What bounds it is the instructions an action costs (some 57 with the full
 // KL, 25 without), not memory: 262144 rows of 82 fp32 actions with the full
-// KL take 102 us (2.8 TB/s, 44 % of a copy's rate), with a sampled KL 60 us
-// (3.3 TB/s); 4096 rows of 32000 bf16 138 us (3.8 TB/s); 8 rows of 131071
-// fp32 19 us, which is latency: one row's phases across a cluster.
+// KL take 104 us (2.7 TB/s, 43 % of a copy's rate), with a sampled KL 62 us
+// (3.2 TB/s); 4096 rows of 32000 bf16 141 us (3.7 TB/s); 8 rows of 131071
+// fp32 25 us, which is latency: one row's phases across a cluster.
 //
 // Exponentials are ex2.approx of (x - m) log2 e: the difference first, so
 // that only |x - m|, which p weights, is rounded and scaled; their errors
@@ -71,6 +71,11 @@ constexpr int kMaxPartials = 148 * 16;
 // actions: 1e-6), and the adds of up to 64 values per thread, in eight
 // chains, plus the tree (2e-6)
 constexpr double kBorderTol = 8e-6;
+// Up to this many logits every row's log-probability is evaluated in 64 bits:
+// the terms of a few rows may cancel to a loss that shows the 1e-7 of each.
+// The host needs 25 us for a call, and the kernels stay below that: 64 x 82
+// fp32 14 us (6 without), 8 x 131071 fp32 25 us (19 without).
+constexpr int64_t kFineLogits = 1 << 20;
 constexpr float kFarKl = 1.0e4f;   // sum p phi above this (KL > 9): the direct difference is exact enough
 constexpr float kLog2E = 1.44269504088896341f;
 
@@ -90,6 +95,7 @@ struct Params {
   int mask_bytes, x_pitch, r_pitch;  // of a warp's batch: Batch
   double clip_low, clip_high, log_low, log_high;  // borders of the ratio and their logarithms
   float beta, even_weight;
+  bool fine;  // every row's log-probability in 64 bits
 };
 
 template <typename T>
@@ -198,6 +204,18 @@ __device__ __forceinline__ double log_row_sum(float s) {
   c = fma(c, q2, 1.0 / 3.0);
   c = fma(c, q2, 1.0);
   return fma(2.0 * q, c, (double)k * 0.693147180559945309417);
+}
+
+// e^u for u <= 0 to 1e-11 of itself, without a branch: u = k ln 2 + r, |r| <=
+// ln 2 / 2, the exponential series to r^9 (next term 7e-12), and 2^k.  Below
+// e^-700, and for minus infinity, 1e-304; NaN stays.
+__device__ __forceinline__ double exp_64(double u) {
+  u = u < -700.0 ? -700.0 : u;
+  const double k = rint(u * 1.44269504088896340736), r = fma(k, -0.693147180559945309417, u), r2 = r * r;
+  const double a = fma(r, 1.0 / 362880, 1.0 / 40320), b = fma(r, 1.0 / 5040, 1.0 / 720);
+  const double c = fma(r, 1.0 / 120, 1.0 / 24), d = fma(r, 1.0 / 6, 0.5);
+  const double p = fma(fma(fma(fma(a, r2, b), r2, c), r2, d), r2, 1.0 + r);
+  return p * __hiloint2double((1023 + (int)k) << 20, 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -381,21 +399,22 @@ struct RowOut {
 // group writes them.
 template <typename T, bool Kl, typename Grp>
 __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, int64_t row, float weight,
-                                             const RowIn &in, float top, float sum, float kl_sum) {
-  double lp = ((double)in.xk - (double)top) - log_row_sum(sum), delta = lp - (double)in.old;
+                                             const RowIn &in, float top, double log_sum, bool fine, float kl_sum) {
+  double lp = ((double)in.xk - (double)top) - log_sum, delta = lp - (double)in.old;
   const bool far = Kl && !(kl_sum < kFarKl);
   float kl = Kl ? log1pf(kl_sum) : 0.0f;
-  if (far || fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol) {
+  if (fine || far || fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol) {
     const double2 fine = row_in_64<T>(p, grp, row, top, far);
     lp = (double)in.xk - fine.x;
     delta = lp - (double)in.old;
     if (far) kl = (float)fine.y;
   }
   const bool clipped = in.adv >= 0.0f ? delta > p.log_high : delta < p.log_low;
-  const float ratio = expf((float)delta);
-  // an advantage of 0 adds nothing, whatever the ratio overflows to
-  float c = clipped || in.adv == 0.0f ? 0.0f : -in.adv * ratio;
-  double term = clipped ? -(double)in.adv * (in.adv >= 0.0f ? p.clip_high : p.clip_low) : (double)c;
+  // (in 64 bits: the rows' terms cancel in the loss.)  An advantage of 0 adds
+  // nothing, whatever the ratio overflows to
+  double term = clipped || in.adv == 0.0f ? 0.0 : -(double)in.adv * exp(delta);
+  float c = (float)term;
+  if (clipped) term = -(double)in.adv * (in.adv >= 0.0f ? p.clip_high : p.clip_low);
   if (!Kl && p.reference_log_prob) {
     const float y = (float)((double)in.ref - lp), em = expm1f(y);
     kl = fabsf(y) < 1.0f ? phi_small(y) : em - y;
@@ -628,7 +647,7 @@ __device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, i
     }
     kl = grp.reduce<SumOp>(kl);
   }
-  const RowOut out = finish_row<T, Kl>(p, grp, row, s.weight, in, top, sum, kl);
+  const RowOut out = finish_row<T, Kl>(p, grp, row, s.weight, in, top, log_row_sum(sum), p.fine, kl);
   if (grad) {
     const float wc = -out.wc * inv, wb = out.wb * inv;
 #pragma unroll
@@ -666,7 +685,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtas<V * W, Kl>)
   // A full batch of rows in one piece starts at the same place within 16
   // bytes every time (the step is a multiple of 16 rows): its copies are
   // worked out once, and kept in shared memory, not in the registers that
-  // the elements need (262144 x 82 fp32 with a sampled KL 69 us, now 60).
+  // the elements need (262144 x 82 fp32 with a sampled KL 60 us for 69).
   __shared__ Piece s_pieces[kShortThreads / 32][3];
   const Piece &px = s_pieces[warp][0], &pr = s_pieces[warp][1], &pl = s_pieces[warp][2];
   if (lane == 0) {
@@ -882,7 +901,20 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
       }
       kl = grp.reduce<SumOp>(kl);
     }
-    const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, st.top, st.sum, kl);
+    double log_sum;
+    if (p.fine) {  // as row_in_64 does, from shared memory
+      double s = 0.0;
+      for (int v = t; v < vecs; v += threads) {
+        float xa[W], da[W];
+        load(v, xa, da);
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += exp_64((double)xa[w] - (double)st.top);
+      }
+      log_sum = log(grp.reduce<SumOp>(s));
+    } else {
+      log_sum = log_row_sum(st.sum);
+    }
+    const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, st.top, log_sum, false, kl);
     share += out.share;
     if (grad) {
       const float wc = -out.wc * inv, wb = out.wb * inv;
@@ -1143,6 +1175,7 @@ int scacchi_policy_loss(const scacchi_policy_rows *rows, const scacchi_policy_ou
   p.log_high = log1p(clip_high);
   p.beta = kl_coefficient;
   p.even_weight = (float)(1.0 / (double)num_rows);
+  p.fine = num_rows <= kFineLogits / num_actions;
   int ctas = 0;
   cudaError_t err;
   if (dtype == 0)

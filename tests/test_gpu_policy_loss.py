@@ -443,3 +443,23 @@ def test_refusals(cuda):
             clipped_policy_loss(args.pop("logits"), args.pop("action"), args.pop("old_log_prob"),
                                 args.pop("advantage"), **args)
     assert _lib.launch_count() == before
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(64, 82), (1, 5), (33, 511), (7, 520), (3, 70001), (4, 262144)], ids=str)
+def test_few_rows_in_64_bits(cuda, size, dtype):
+    """Few rows' terms may cancel: their sum is taken before any rounding to
+    32 bits.  Exponentials to 1e-11 and 64-bit sums leave 1e-10 of each term;
+    the results round once, by 2^-24."""
+    for seed in range(4):
+        logits, action, kw = _inputs(*size, dtype, size[1] < 1000, "none", seed=40 + seed)
+        got = clipped_policy_loss(logits, action, **kw)
+        x = logits.double()
+        if kw["legal"] is not None:
+            x = x.masked_fill(~kw["legal"], -math.inf)
+        lp = torch.log_softmax(x, -1).gather(-1, action.long()[:, None])[:, 0]
+        ratio, adv = torch.exp(lp - kw["old_log_prob"].double()), kw["advantage"].double()
+        term = -torch.minimum(ratio * adv, ratio.clamp(1 - 0.2, 1 + 0.2) * adv) * kw["weight"].double()
+        tol = U * abs(float(term.sum())) + 1e-10 * float(term.abs().sum())
+        assert abs(float(got.loss) - float(term.sum())) <= tol
+        assert bool(((got.log_prob.double() - lp).abs() <= U * lp.abs() + 1e-10).all())
