@@ -30,7 +30,7 @@
 // What bounds it is the instructions an action costs (some 57 with the full
 // KL, 25 without), not memory: 262144 rows of 82 fp32 actions with the full
 // KL take 104 us (2.7 TB/s, 43 % of a copy's rate), with a sampled KL 62 us
-// (3.2 TB/s); 4096 rows of 32000 bf16 141 us (3.7 TB/s); 8 rows of 131071
+// (3.2 TB/s); 4096 rows of 32000 bf16 140 us (3.7 TB/s); 8 rows of 131071
 // fp32 25 us, which is latency: one row's phases across a cluster.
 //
 // Exponentials are ex2.approx of (x - m) log2 e: the difference first, so
@@ -326,7 +326,8 @@ struct Ctas {
 
 // A row in 64 bits, read again: log sum e^x over the kept actions, and
 // with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r).
-// Taken by the few rows next to a clip border or far from the reference.
+// Taken by rows far from the reference, and by short rows next to a clip
+// border or of a small call (kFineLogits).
 template <typename T, typename Grp>
 __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64_t row, float top, bool want_kl) {
   const int A = p.actions;
@@ -395,15 +396,20 @@ struct RowOut {
   float wc, wb;
 };
 
+// a log-ratio that 32-bit sums may have put on the wrong side of the clip
+__device__ __forceinline__ bool near_border(const Params &p, double delta) {
+  return fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol;
+}
+
 // The row's statistics from its sums, by every thread alike; thread 0 of the
-// group writes them.
+// group writes them.  `settled`: log_sum is in 64 bits where it has to be.
 template <typename T, bool Kl, typename Grp>
 __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, int64_t row, float weight,
-                                             const RowIn &in, float top, double log_sum, bool fine, float kl_sum) {
+                                             const RowIn &in, float top, double log_sum, bool settled, float kl_sum) {
   double lp = ((double)in.xk - (double)top) - log_sum, delta = lp - (double)in.old;
   const bool far = Kl && !(kl_sum < kFarKl);
   float kl = Kl ? log1pf(kl_sum) : 0.0f;
-  if (fine || far || fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol) {
+  if (far || (!settled && (p.fine || near_border(p, delta)))) {
     const double2 fine = row_in_64<T>(p, grp, row, top, far);
     lp = (double)in.xk - fine.x;
     delta = lp - (double)in.old;
@@ -647,7 +653,7 @@ __device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, i
     }
     kl = grp.reduce<SumOp>(kl);
   }
-  const RowOut out = finish_row<T, Kl>(p, grp, row, s.weight, in, top, log_row_sum(sum), p.fine, kl);
+  const RowOut out = finish_row<T, Kl>(p, grp, row, s.weight, in, top, log_row_sum(sum), false, kl);
   if (grad) {
     const float wc = -out.wc * inv, wb = out.wb * inv;
 #pragma unroll
@@ -872,7 +878,7 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
     }
     st = grp.stats(st);
     const float inv = 1.0f / st.sum, mean = st.mean * inv;
-    // what the row's end does not judge: p to 2^-23 |m| is enough
+    // for sums and gradients p to 2^-23 |m| is enough
     const float shift = -st.top * kLog2E;
     float kl = 0.0f;
     if (Kl) {
@@ -901,8 +907,9 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
       }
       kl = grp.reduce<SumOp>(kl);
     }
-    double log_sum;
-    if (p.fine) {  // as row_in_64 does, from shared memory
+    double log_sum = log_row_sum(st.sum);
+    const bool fine = p.fine || near_border(p, ((double)in.xk - (double)st.top) - log_sum - (double)in.old);
+    if (fine) {  // as row_in_64, from shared memory (out of line it was slower)
       double s = 0.0;
       for (int v = t; v < vecs; v += threads) {
         float xa[W], da[W];
@@ -911,10 +918,8 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
         for (int w = 0; w < W; ++w) s += exp_64((double)xa[w] - (double)st.top);
       }
       log_sum = log(grp.reduce<SumOp>(s));
-    } else {
-      log_sum = log_row_sum(st.sum);
     }
-    const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, st.top, log_sum, false, kl);
+    const RowOut out = finish_row<T, Kl>(p, grp, row, weight, in, st.top, log_sum, true, kl);
     share += out.share;
     if (grad) {
       const float wc = -out.wc * inv, wb = out.wb * inv;
