@@ -1120,10 +1120,10 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
 
   const int mine_steps = ((mine * 64 < q.length - panel0 * 64 ? mine * 64 : q.length - panel0 * 64) + 15) / 16;
   const int side_steps = (q.side + 15) / 16, side_n = side_steps * 16;
-  // K steps per accumulator: two, or as many as TMEM's columns make it
+  // K steps per accumulator: as few as TMEM's columns allow
   auto sub_of = [](int ksteps, int n) {
-    const int accs = 512 / n, sub = (ksteps + accs - 1) / accs;
-    return sub < 2 ? 2 : sub;
+    const int accs = 512 / n;
+    return (ksteps + accs - 1) / accs;
   };
   const int n_update = mine * 64;
   const int gram_sub = sub_of(mine_steps, side_n), square_sub = sub_of(side_steps, side_n);
