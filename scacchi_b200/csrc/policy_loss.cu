@@ -799,6 +799,10 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
   uint8_t *const sl_at = s_rows + (Kl ? 2 : 1) * p.slice_bytes;
   const int64_t first = blockIdx.x / grp.ctas, step = gridDim.x / grp.ctas;
   double share = 0.0;
+  // A CTA's shared memory may be written by the others only once it runs:
+  // each arrives here, and waits after its first row is requested (every
+  // cluster has one), so that the row's latency hides the barrier's.
+  if (grp.ctas > 1) cg::this_cluster().barrier_arrive();
   for (int64_t row = first; row < p.rows; row += step) {
     const float weight = p.weight ? p.weight[row] : p.even_weight;
     const int k = p.action[row];
@@ -821,6 +825,7 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
       }
     }
     const RowIn in = row_in<T>(p, row, x, legal, k, wanted);
+    if (grp.ctas > 1 && row == first) cg::this_cluster().barrier_wait();
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     if (!in.counts) {

@@ -463,3 +463,19 @@ def test_few_rows_in_64_bits(cuda, size, dtype):
         tol = U * abs(float(term.sum())) + 1e-10 * float(term.abs().sum())
         assert abs(float(got.loss) - float(term.sum())) <= tol
         assert bool(((got.log_prob.double() - lp).abs() <= U * lp.abs() + 1e-10).all())
+
+
+@pytest.mark.parametrize("kl", ["none", "sampled", "full"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(3, 40000), (9, 131071), (74, 9001), (160, 60001)], ids=str)
+def test_clusters_whose_first_rows_do_not_count(cuda, size, dtype, kl):
+    """Rows in clusters of 2 to 16 CTAs: the first ones, every other one, or
+    all of them without a part in the loss."""
+    logits, action, kw = _inputs(*size, dtype, False, kl, seed=60)
+    beta = 0.0 if kl == "none" else 0.1
+    every = kw["weight"].clone()
+    for off in (slice(0, 2), slice(0, None, 2), slice(0, None)):
+        kw["weight"] = every.clone()
+        kw["weight"][off] = 0.0
+        out = _check(logits, action, kw, beta=beta)
+        assert not out.grad_logits[off].any() and not out.log_prob[off].any()

@@ -2,6 +2,7 @@
 launch (no GPU needed)."""
 
 import ctypes as C
+from pathlib import Path
 
 import pytest
 import torch
@@ -51,3 +52,20 @@ def test_library_rejects_without_launching(kw):
 def test_null_structs_are_rejected():
     out = _lib.PolicyOut(*[1 << 20] * 5)
     assert _lib.lib().scacchi_policy_loss(None, C.byref(out), 1, 2, 0, 0.2, 0.2, 0.0, 8, None) == _lib.EINVAL
+
+
+def test_clusters_meet_before_the_first_remote_write():
+    """A CTA may write another's shared memory only once that one runs: the
+    long rows' kernel arrives on the cluster's barrier before its first row
+    and waits for it before the first reduction across CTAs, also where the
+    first row does not count.  Read from the source: on a GPU the row's
+    latency hides a missing barrier."""
+    source = (Path(__file__).parents[1] / "scacchi_b200" / "csrc" / "policy_loss.cu").read_text()
+    kernel = source[source.index("policy_loss_long_kernel(const"):]
+    kernel = kernel[:kernel.index("\n}\n")]
+    rows = kernel.index("for (int64_t row = first")
+    arrive, wait = kernel.find("barrier_arrive()"), kernel.find("barrier_wait()")
+    assert 0 <= arrive < rows < wait
+    assert "row == first" in kernel[kernel.rindex("\n", 0, wait):wait]  # once, by every thread
+    for later in ("grp.stats(", "grp.reduce<", "finish_row<", "continue;", "map_shared_rank"):
+        assert kernel.find(later) == -1 or wait < kernel.index(later), later
