@@ -1084,7 +1084,10 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
 
   if (ctas > 1) cluster.sync();  // the scratch is read: partial sums may arrive in its place
 
-  uint32_t parity = 0;
+  // A warp whose wait ran out takes no further part: it issues and reads no
+  // product, tells the cluster, and goes on to the barriers alone.
+  bool alive = true;
+  uint32_t parity = 0, issued = 0;
   const uint32_t x_at = smem_u32(smem), z_at = smem_u32(smem + L::kZAt);
   // One product: `ksteps` of 16, `sub` of them per accumulator of n columns
   // (of the 512 that there are).  b_mn: B's panels lie along N and K counts
@@ -1094,7 +1097,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 0 && alive) {
       tc_fence_after();
       if (elect_one()) {
         const uint32_t idesc = idesc_f16(kBM, n, false, b_mn);
@@ -1110,9 +1113,13 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
             }
         umma_commit(done);
       }
+      issued = parity;
       __syncwarp();
     }
-    mbar_wait(done, parity, abort_flag, &g_muon_error);
+    if (alive && !mbar_wait_warp(done, parity, abort_flag, &g_muon_error)) {
+      alive = false;
+      if (lane < ctas) *cluster.map_shared_rank(const_cast<int *>(abort_flag), lane) = 1;
+    }
     parity ^= 1u;
     __syncwarp();
     tc_fence_after();
@@ -1136,7 +1143,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
   for (int step = 0; step < q.steps; ++step) {
     // X X^T over this slice
     product(x_at, L::kX, x_at, L::kX, mine_steps, gram_sub, side_n, false);
-    read_sum(v, tmem + lanes + (uint32_t)col, col < side_n ? gram_accs : 0, (uint32_t)side_n);
+    read_sum(v, tmem + lanes + (uint32_t)col, alive && col < side_n ? gram_accs : 0, (uint32_t)side_n);
     if (ctas == 1) {
       narrow_square(smem + L::kZAt, L::kZ, row, col, q.side, q.scale1, q.diag1, v);
     } else {
@@ -1184,15 +1191,20 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
     }
     if (q.quintic) {
       product(z_at, L::kZ, z_at, L::kZ, side_steps, square_sub, side_n, false);
-      read_sum(v, tmem + lanes + (uint32_t)col, col < side_n ? square_accs : 0, (uint32_t)side_n);
+      read_sum(v, tmem + lanes + (uint32_t)col, alive && col < side_n ? square_accs : 0, (uint32_t)side_n);
       narrow_square(smem + L::kZAt, L::kZ, row, col, q.side, q.scale2, q.diag2, v);
     }
     // X <- M X
     product(z_at, L::kZ, x_at, L::kX, side_steps, update_sub, n_update, true);
     const bool last = step + 1 == q.steps;
+    if (last) {
+      // a matrix is written whole or, where a wait of any CTA ran out, not at all
+      cluster.sync();
+      if (*abort_flag) break;
+    }
 #pragma unroll 1
     for (int c = col; c < n_update; c += 128) {
-      read_sum(v, tmem + lanes + (uint32_t)c, update_accs, (uint32_t)n_update);
+      read_sum(v, tmem + lanes + (uint32_t)c, alive ? update_accs : 0, (uint32_t)n_update);
       if (!last) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] *= q.inv;
@@ -1208,8 +1220,10 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ns_narrow_kernel(const __gr
       }
     }
   }
+  // (the last access to another CTA's memory lies before the last step's barrier)
+  if (warp == 0 && !alive) mbar_drain(done, issued);
   tc_fence_before();
-  cluster.sync();
+  __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 

@@ -2,6 +2,8 @@
 compute, before any launch, and choose the operands' scale (no GPU needed)."""
 
 import ctypes as C
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -96,3 +98,30 @@ def test_network_muon_refuses_a_step_as_a_whole():
     with pytest.raises(ValueError, match="no such matrices"):
         opt.step({**good, "stem_w": torch.ones((3, 3))})
     assert all(torch.equal(v, before[k]) for k, v in opt.matrices.items())
+
+
+def _kernel(name):
+    source = (Path(__file__).parents[1] / "scacchi_b200" / "csrc" / "muon.cu").read_text()
+    kernel = source[source.index(name + "(const __grid_constant__"):]
+    return kernel[:kernel.index("\n}\n")]
+
+
+def test_no_wait_goes_unheeded():
+    """A bounded wait that ran out leaves a product unfinished, so every
+    kernel looks at what its waits return.  Read from the source: no input
+    makes a wait run out."""
+    for name in ("ns_pair_kernel", "ns_tile_kernel", "ns_narrow_kernel"):
+        statements = [text.strip() for text in re.split("[;{}]", _kernel(name))]
+        assert any("mbar_wait" in text for text in statements)
+        assert not [text for text in statements if text.startswith("mbar_wait")], name
+
+
+def test_a_narrow_matrix_is_written_whole_or_not_at_all():
+    """In the last step the cluster's CTAs meet, and none writes where a wait
+    of any of them ran out; an unfinished product is drained before TMEM goes."""
+    kernel = _kernel("ns_narrow_kernel")
+    update = kernel[kernel.index("// X <- M X"):]
+    meet, leave, write = update.find("cluster.sync()"), update.find("if (*abort_flag) break;"), update.index("narrow_out(")
+    assert 0 <= meet < leave < write
+    assert "map_shared_rank(const_cast<int *>(abort_flag)" in kernel
+    assert update.index("mbar_drain(") < update.index("tmem_dealloc(")
