@@ -88,7 +88,12 @@ struct Product {
   int dtype;                    // 0 float32, 1 bfloat16, 2 float16
   float *weight;
   float decay, step;
+  uint32_t *failed;             // of this call: a wait of one of its products ran out
 };
+
+// Whether a product's output is written: the user's matrix is not once an
+// earlier product of the call was left unfinished.
+__device__ __forceinline__ bool may_write(const Product &q) { return !q.last || __ldcg(q.failed) == 0u; }
 
 // Tiles of tile row i of a symmetric output: those of the stored blocks, of
 // which 128 x 128 tiles leave out the one that its neighbour writes turned.
@@ -362,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         locate<2 * kBM, BN>(q, t, batch, i, j);
         const int a_at = (2 * i + rank) * kBM, b_at = j * BN + rank * (BN / 2);
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_muon_error)) {
+          if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_muon_error, q.failed)) {
             stop = true;
             break;
           }
@@ -402,8 +407,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const bool a_mn = along_mn(q.a_major, 2 * i * kBM, kb), b_mn = along_mn(q.b_major, j * BN, kb);
           const StageDesc desc(smem_u32(smem + stage * L::kStage), L::kA, L::kB, a_mn, b_mn);
           const uint32_t idesc = idesc_f16(2 * kBM, BN, a_mn, b_mn), d = tmem + (uint32_t)(slot * BN);
-          ok = mbar_wait_warp(&acc_empty[slot], acc_phase ^ 1u, abort_flag, &g_muon_error) &&
-               mbar_wait_warp(&full[stage], phase, abort_flag, &g_muon_error);
+          ok = mbar_wait_warp(&acc_empty[slot], acc_phase ^ 1u, abort_flag, &g_muon_error, q.failed) &&
+               mbar_wait_warp(&full[stage], phase, abort_flag, &g_muon_error, q.failed);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -442,7 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
       for (int kb = 0; kb < kblocks; ++kb) {
         int go = 0;
-        if (lane == 0) go = !*abort_flag && mbar_wait(&acc_full[slot], acc_phase, abort_flag, &g_muon_error);
+        if (lane == 0) go = !*abort_flag && mbar_wait(&acc_full[slot], acc_phase, abort_flag, &g_muon_error, q.failed);
         ok = __shfl_sync(0xffffffffu, go, 0) != 0;
         if (!ok) break;
         tc_fence_after();
@@ -458,7 +463,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok) break;
       int batch, i, j;
       locate<2 * kBM, BN>(q, t, batch, i, j);
-      emit<kCols>(q, batch, (2 * i + rank) * kBM + quad * 32, j * BN + half * kCols, false, sum, patch);
+      if (may_write(q))
+        emit<kCols>(q, batch, (2 * i + rank) * kBM + quad * 32, j * BN + half * kCols, false, sum, patch);
     }
   }
   __syncwarp();
@@ -539,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0, issued = 0, parity = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_muon_error)) break;
+        if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_muon_error, q.failed)) break;
         uint8_t *at = smem + stage * L::kStage;
         mbar_expect_tx(&full[stage], L::kStage);
         const bool a_mn = along_mn(q.a_major, i * kBM, kb), b_mn = along_mn(q.b_major, j * BN, kb);
@@ -568,8 +574,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool a_mn = along_mn(q.a_major, i * kBM, kb), b_mn = along_mn(q.b_major, j * BN, kb);
       const StageDesc desc(smem_u32(smem + stage * L::kStage), L::kA, L::kB, a_mn, b_mn);
       const uint32_t idesc = idesc_f16(kBM, BN, a_mn, b_mn), d = tmem + (uint32_t)(slot * BN);
-      if (!mbar_wait_warp(&acc_empty[slot], acc_phase ^ 1u, abort_flag, &g_muon_error) ||
-          !mbar_wait_warp(&full[stage], phase, abort_flag, &g_muon_error))
+      if (!mbar_wait_warp(&acc_empty[slot], acc_phase ^ 1u, abort_flag, &g_muon_error, q.failed) ||
+          !mbar_wait_warp(&full[stage], phase, abort_flag, &g_muon_error, q.failed))
         break;
       tc_fence_after();
       if (elect_one()) {
@@ -604,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int e = 0; e < kCols; ++e) sum[e] = 0.0f;
     for (int kb = kb0; kb < kb1; ++kb) {
       int go = 0;
-      if (lane == 0) go = !*abort_flag && mbar_wait(&acc_full[slot], acc_phase, abort_flag, &g_muon_error);
+      if (lane == 0) go = !*abort_flag && mbar_wait(&acc_full[slot], acc_phase, abort_flag, &g_muon_error, q.failed);
       ok = __shfl_sync(0xffffffffu, go, 0) != 0;
       if (!ok) break;
       tc_fence_after();
@@ -620,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the tile right of it in the diagonal's 256 x 256 block is its mirror image
     const bool mirror = q.sym && (i & 1) && j == i - 1;
     if (ctas == 1) {
-      if (ok) emit<kCols>(q, batch, i * kBM + quad * 32, j * BN + half * kCols, mirror, sum, patch);
+      if (ok && may_write(q)) emit<kCols>(q, batch, i * kBM + quad * 32, j * BN + half * kCols, mirror, sum, patch);
     } else {
       // The CTAs finish the tile's sixteen 32 x 32 blocks in turn, a warp
       // each; the others' partial sums arrive as [source][block][four
@@ -640,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       cg::this_cluster().sync();
       const int id = (warp - 4) * ctas + rank;
-      if (warp - 4 < most && id < 16 && ok) {
+      if (warp - 4 < most && id < 16 && ok && may_write(q)) {
         const float4 *at = reinterpret_cast<const float4 *>(smem) + (warp - 4) * 256 + lane;
         float v[32];
 #pragma unroll
@@ -756,8 +762,10 @@ __device__ __forceinline__ double norm_part(const Source &s, int64_t base, int64
 // that its squares leave fp32), one partial per block, and Muon's momentum.
 // Bound by memory: 8192 x 2048 bf16 14 us (2.4 TB/s; 70 with 128 blocks of
 // single elements)
-__global__ void __launch_bounds__(256) ns_norm_kernel(Source s, int64_t elems, int vec, double *partial) {
+__global__ void __launch_bounds__(256) ns_norm_kernel(Source s, int64_t elems, int vec, double *partial,
+                                                      uint32_t *failed) {
   __shared__ double part[8];
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *failed = 0;
   const int64_t base = (int64_t)blockIdx.y * elems;
   double sum = s.dtype == 0   ? norm_part<float>(s, base, elems, vec)
                : s.dtype == 1 ? norm_part<__nv_bfloat16>(s, base, elems, vec)
@@ -1301,6 +1309,8 @@ int64_t norm_blocks(int64_t rows, int64_t cols) {
   return blocks < kNormBlocks ? blocks : kNormBlocks;
 }
 
+constexpr int64_t kFlagBytes = 256;  // a call's flag, at the start of its workspace
+
 int64_t norm_bytes(int64_t batch, int64_t rows, int64_t cols) {
   return (batch * norm_blocks(rows, cols) * (int64_t)sizeof(double) + 255) / 256 * 256;
 }
@@ -1392,7 +1402,9 @@ cudaError_t run_pair(Product q, const Stack &a, const Stack &b, const Device &d,
 // where a symmetric one is written twice), or with its K split 4.2 (two
 // cluster barriers and the exchange).  What leaves SMs idle is a tile count
 // below a wave, or just above one.
-cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, const Device &d, cudaStream_t st) {
+cudaError_t product(Product q, const Stack &a, const Stack &b, const Stack &to, uint32_t *failed, const Device &d,
+                    cudaStream_t st) {
+  q.failed = failed;
   q.a_rows = a.panel_rows;
   q.b_rows = b.panel_rows;
   q.dst = to.p;
@@ -1484,8 +1496,9 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
   const int s = n.rows < n.cols ? n.rows : n.cols;
   const bool tall = n.rows > n.cols;
   uint8_t *at = static_cast<uint8_t *>(workspace);
-  double *partial = reinterpret_cast<double *>(at);
-  at += norm_bytes(n.batch, n.rows, n.cols);
+  uint32_t *failed = reinterpret_cast<uint32_t *>(at);
+  double *partial = reinterpret_cast<double *>(at + kFlagBytes);
+  at += kFlagBytes + norm_bytes(n.batch, n.rows, n.cols);
   Stack x, y, gram, poly;
   const int64_t wide = stack_bytes(n.batch, n.rows, n.cols), narrow = stack_bytes(n.batch, s, s);
   if (!x.place(at, n.batch, n.rows, n.cols) || !y.place(at + wide, n.batch, n.rows, n.cols) ||
@@ -1501,7 +1514,7 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
   const int64_t share = (8 * (int64_t)sms + n.batch - 1) / n.batch;
   blocks = blocks < share ? blocks : share;
   if (launch(ns_norm_kernel, dim3((unsigned)blocks, (unsigned)n.batch), 256, 0, st, false, 1, src, elems, vec,
-             partial) != cudaSuccess)
+             partial, failed) != cudaSuccess)
     return SCACCHI_ECUDA;
   const int64_t chunks = (int64_t)x.panel_rows * x.panels * 8;
   const int split_vec = vec && n.cols % 8 == 0;  // rows too
@@ -1525,13 +1538,13 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
     q.k = tall ? n.rows : n.cols;
     q.scale = (float)((quintic ? 1.0 : n.b) / scale);
     q.diag = (float)((quintic ? n.b / (2.0 * n.c) : n.a) * scale);
-    if (product(q, *now, *now, quintic ? gram : poly, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
+    if (product(q, *now, *now, quintic ? gram : poly, failed, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
     if (quintic) {
       q.a_major = q.b_major = kSymmetric;
       q.k = s;
       q.scale = (float)(n.c / scale);
       q.diag = (float)((n.a - n.b * n.b / (4.0 * n.c)) * scale);
-      if (product(q, gram, gram, poly, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
+      if (product(q, gram, gram, poly, failed, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
     }
     const bool final = k + 1 == n.steps;
     Product u = final ? last : Product{};
@@ -1542,7 +1555,8 @@ int newton_schulz(const scacchi_newton_schulz &n, const Source &src, Product las
     u.k = s;
     u.a_major = tall ? kAlongK : kSymmetric;
     u.b_major = tall ? kSymmetric : kAlongMN;
-    if (product(u, tall ? *now : poly, tall ? poly : *now, *next, *dev, st) != cudaSuccess) return SCACCHI_ECUDA;
+    if (product(u, tall ? *now : poly, tall ? poly : *now, *next, failed, *dev, st) != cudaSuccess)
+      return SCACCHI_ECUDA;
     Stack *t = now;
     now = next;
     next = t;
@@ -1594,7 +1608,8 @@ int32_t scacchi_muon_scale_exponent(double a, double b, double c, int32_t steps)
 size_t scacchi_muon_workspace_bytes(int32_t batch, int32_t rows, int32_t cols) {
   if (batch < 1 || rows < 1 || cols < 1) return 0;
   const int64_t s = rows < cols ? rows : cols;
-  return (size_t)(norm_bytes(batch, rows, cols) + 2 * stack_bytes(batch, rows, cols) + 2 * stack_bytes(batch, s, s));
+  return (size_t)(kFlagBytes + norm_bytes(batch, rows, cols) + 2 * stack_bytes(batch, rows, cols) +
+                  2 * stack_bytes(batch, s, s));
 }
 
 int scacchi_orthogonalize(const scacchi_newton_schulz *params, const void *matrix, void *out, void *workspace,

@@ -48,11 +48,12 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 }
 
 // Bounded wait: gives up after kWaitNs (or when another role gave up),
-// raises the flags and returns whether the phase completed.  The clock is
+// raises the flags (`call_flag`: that of the launch's call, if it has one)
+// and returns whether the phase completed.  The clock is
 // read only after some hundred tries: a read of %globaltimer takes most of
 // a microsecond, which every wait would pay.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
-                                          uint32_t *error_flag) {
+                                          uint32_t *error_flag, uint32_t *call_flag = nullptr) {
   uint64_t start = 0;
   for (uint32_t i = 1; i < (1u << 30); ++i) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -64,14 +65,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volati
     }
   }
   atomicOr(error_flag, 1u);
+  if (call_flag) atomicOr(call_flag, 1u);
   *abort_flag = 1;
   return false;
 }
 
 // the same by a whole warp, whose lanes agree on the result
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
-                                               uint32_t *error_flag) {
-  const bool ok = mbar_wait(bar, parity, abort_flag, error_flag);
+                                               uint32_t *error_flag, uint32_t *call_flag = nullptr) {
+  const bool ok = mbar_wait(bar, parity, abort_flag, error_flag, call_flag);
   return __all_sync(0xffffffffu, ok) != 0;
 }
 

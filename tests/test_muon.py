@@ -125,3 +125,19 @@ def test_a_narrow_matrix_is_written_whole_or_not_at_all():
     assert 0 <= meet < leave < write
     assert "map_shared_rank(const_cast<int *>(abort_flag)" in kernel
     assert update.index("mbar_drain(") < update.index("tmem_dealloc(")
+
+
+def test_products_after_an_unfinished_one_write_no_weights():
+    """A call's products are launched in a row, so the last one has to learn
+    that an earlier one gave up: a wait that runs out raises the call's flag,
+    the first kernel clears it, and nothing is written to the user's matrix
+    where it stands."""
+    for name in ("ns_pair_kernel", "ns_tile_kernel"):
+        kernel = _kernel(name)
+        for wait in re.findall(r"mbar_wait\w*\((.*?)\)", kernel):
+            assert wait.endswith("q.failed"), (name, wait)
+        for at in re.finditer("emit<", kernel):
+            assert "may_write(q)" in kernel[kernel.rindex("if (", 0, at.start()):at.start()], name
+    source = (Path(__file__).parents[1] / "scacchi_b200" / "csrc" / "muon.cu").read_text()
+    norm = source[source.index("ns_norm_kernel(Source"):]
+    assert "*failed = 0" in norm[:norm.index("\n}\n")]
