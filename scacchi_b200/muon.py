@@ -46,6 +46,16 @@ def _workspace_bytes(batch: int, rows: int, cols: int) -> int:
     return int(_lib.lib().scacchi_muon_workspace_bytes(batch, rows, cols))
 
 
+def check_waits(device=None) -> None:
+    """Raises ScacchiError where a wait of these operators ran out on
+    ``device`` (the current one if absent) since the last call, so that
+    their results are not to be trusted.  Speaks of the work that is
+    complete: synchronise first."""
+    with torch.cuda.device(device):
+        if _lib.muon_error():
+            raise _lib.ScacchiError("a wait of an orthogonalised update ran out: its results are incomplete")
+
+
 def _params(t: torch.Tensor, name: str, steps: int, coefficients, eps: float) -> _lib.NewtonSchulz:
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be on a CUDA device, got {t.device}")
@@ -82,7 +92,9 @@ def orthogonalize(matrix: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     outside autograd.
 
     The call launches on the current stream, does not synchronise and can
-    be captured into a CUDA graph.
+    be captured into a CUDA graph.  It cannot report a product whose wait
+    ran out (2 s): the output then stays unwritten in part or as a whole,
+    and ``check_waits``, at a point where the program synchronises, raises.
     """
     matrix = matrix.detach()
     params = _params(matrix, "matrix", steps, coefficients, eps)
@@ -114,7 +126,10 @@ def muon_update(weight: torch.Tensor, gradient: torch.Tensor, momentum: torch.Te
     sqrt(max(1, out / in)).  The three may not overlap.
 
     The call launches on the current stream, does not synchronise and can
-    be captured into a CUDA graph.
+    be captured into a CUDA graph.  It cannot report a product whose wait
+    ran out (2 s): ``momentum`` is then the step's, ``weight`` unwritten in
+    part or as a whole, and ``check_waits``, at a point where the program
+    synchronises, raises.
     """
     gradient = gradient.detach()
     params = _params(gradient, "gradient", steps, coefficients, eps)
@@ -160,7 +175,8 @@ class NetworkMuon:
     kernels of DENSE by their names.
 
     ``step`` takes gradients of any of them, in their shapes; ``params``
-    gives the updated parameters.  The stem, the 1x1 convolutions, the
+    gives the updated parameters, and raises ScacchiError where a wait of a
+    step ran out (``check_waits``).  The stem, the 1x1 convolutions, the
     output vectors, biases and BatchNorm are not matrices to orthogonalise
     and stay as they were given (train them with Adam beside it).
     """
@@ -191,6 +207,9 @@ class NetworkMuon:
 
     def params(self) -> AZDirichletParams:
         host = {k: v.cpu().numpy() for k, v in self.matrices.items()}
+        device = self.matrices["convs"].device
+        if device.type == "cuda":
+            check_waits(device)  # after the copies, which waited for the steps
         blocks = [dict(blk) for blk in self._params.blocks]
         for i, blk in enumerate(blocks):
             for j, k in enumerate(("conv1_w", "conv2_w")):

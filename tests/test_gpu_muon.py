@@ -286,3 +286,20 @@ def test_muon_at_any_alignment(cuda, shape, dtype):
     assert torch.equal(view(w2), w) and torch.equal(view(m2), m)
     for t in (w2, m2, g2):  # and nothing beside them is written
         assert float(t[0]) == 7.0 and float(t[-1]) == 7.0
+
+
+def test_a_wait_that_ran_out_is_reported(cuda, monkeypatch):
+    """The flag of the device in question, once the steps are complete."""
+    from scacchi_b200 import muon
+    from scacchi_b200.network import init_params
+
+    opt = muon.NetworkMuon(init_params(5, num_blocks=1), learning_rate=0.1)
+    opt.step({k: torch.ones_like(v) for k, v in opt.matrices.items()})
+    opt.params()
+    muon.check_waits()
+    asked = []
+    monkeypatch.setattr(_lib, "muon_error", lambda: asked.append(torch.cuda.current_device()) or 1)
+    for report in (opt.params, muon.check_waits, lambda: muon.check_waits("cuda:0")):
+        with pytest.raises(_lib.ScacchiError, match="wait"):
+            report()
+    assert asked == [0, 0, 0]
