@@ -479,3 +479,26 @@ def test_clusters_whose_first_rows_do_not_count(cuda, size, dtype, kl):
         kw["weight"][off] = 0.0
         out = _check(logits, action, kw, beta=beta)
         assert not out.grad_logits[off].any() and not out.log_prob[off].any()
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("A", [2, 82, 301, 700, 40000])
+def test_kl_of_actions_whose_logits_are_equal(cuda, A, masked):
+    """Actions of p = e^-100 whose logits are the reference's (d = 0) carry
+    the KL where the one of p = 1 has d = 120: log of the others' share of
+    the reference, in 64 bits and rounded once."""
+    N = 9
+    x, r = torch.full((N, A), -100.0, device="cuda"), torch.full((N, A), -100.0, device="cuda")
+    x[:, 0], r[:, 0] = 0.0, -120.0
+    legal, others = None, A - 1
+    if masked:
+        legal = torch.ones((N, A), dtype=torch.bool, device="cuda")
+        legal[:, 2::3] = False
+        others = int(legal[0].sum()) - 1
+    z = torch.zeros(N, device="cuda")
+    out = clipped_policy_loss(x, z.int(), z, z, legal=legal, reference_logits=r, kl_coefficient=0.25)
+    want = math.log1p(others * math.exp(20.0))
+    assert float((out.kl.double() - want).abs().max()) <= 2 * U * want
+    assert abs(float(out.loss) - 0.25 * want) <= 4 * U * want
+    # p = 1 and d = mean there; p = 0 elsewhere
+    assert not out.grad_logits.any()
