@@ -324,9 +324,10 @@ struct Ctas {
   }
 };
 
-// A row in 64 bits, read again: log sum e^x over the kept actions, and
-// with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r).
-// Taken by rows far from the reference, and by short rows next to a clip
+// A row in 64 bits, read again: log sum e^{x - top} over the kept actions,
+// and with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r).
+// The maxima are subtracted from one another first: at 1e38 a sum's logarithm
+// is lost beside them.  Taken by rows far from the reference, and by short rows next to a clip
 // border or of a small call (kFineLogits).
 template <typename T, typename Grp>
 __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64_t row, float top, bool want_kl) {
@@ -347,7 +348,7 @@ __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64
     }
   }
   s = grp.template reduce<SumOp>(s);
-  const double lse = (double)top + log(s);
+  const double log_sum = log(s);
   double kl = 0.0;
   if (want_kl) {
     sd = grp.template reduce<SumOp>(sd);
@@ -358,9 +359,9 @@ __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64
       sr += exp((double)to_f(r[a]) - rtop);
     }
     sr = grp.template reduce<SumOp>(sr);
-    kl = sd / s - lse + rtop + log(sr);
+    kl = (sd / s - ((double)top - rtop)) + (log(sr) - log_sum);
   }
-  return make_double2(lse, kl);
+  return make_double2(log_sum, kl);
 }
 
 // ---------------------------------------------------------------------------
@@ -411,7 +412,7 @@ __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, in
   float kl = Kl ? log1pf(kl_sum) : 0.0f;
   if (far || (!settled && (p.fine || near_border(p, delta)))) {
     const double2 fine = row_in_64<T>(p, grp, row, top, far);
-    lp = (double)in.xk - fine.x;
+    lp = ((double)in.xk - (double)top) - fine.x;
     delta = lp - (double)in.old;
     if (far) kl = (float)fine.y;
   }

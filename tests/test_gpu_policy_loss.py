@@ -502,3 +502,23 @@ def test_kl_of_actions_whose_logits_are_equal(cuda, A, masked):
     assert abs(float(out.loss) - 0.25 * want) <= 4 * U * want
     # p = 1 and d = mean there; p = 0 elsewhere
     assert not out.grad_logits.any()
+
+
+@pytest.mark.parametrize("kl", ["none", "sampled", "full"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("A", [2, 82, 512])
+def test_rows_of_the_lowest_value(cuda, A, dtype, kl):
+    """A mask that leaves nothing, written as the type's lowest value: the
+    uniform policy, the logits being equal."""
+    _lowest_rows(A, dtype, kl)
+
+
+def _lowest_rows(A, dtype, kl):
+    logits, action, kw = _inputs(6, A, dtype, False, kl, seed=62)
+    logits[::2] = torch.finfo(DT[dtype]).min
+    kw["old_log_prob"][::2] = 0.1 - math.log(A)
+    if kl == "full":
+        kw["reference_logits"][::2] = torch.finfo(DT[dtype]).min
+    if kl == "sampled":
+        kw["reference_log_prob"][::2] = 0.2 - math.log(A)
+    _check(logits, action, kw, beta=0.0 if kl == "none" else 0.07)
