@@ -180,6 +180,24 @@ __device__ __forceinline__ float exp2_fast(float t) {
 // e^u for u <= 0 or small (see above)
 __device__ __forceinline__ float exp_fast(float u) { return exp2_fast(u * kLog2E); }
 
+// e^{x - top} of a vector's elements, the same bits: differences and
+// products two at a time (4096 x 32000 bf16 140 us, 143 one at a time)
+template <int W>
+__device__ __forceinline__ void exps(const float (&x)[W], float top, float (&e)[W]) {
+  if constexpr (W % 2 == 0) {
+#pragma unroll
+    for (int w = 0; w < W; w += 2) {
+      const float2 u = __fmul2_rn(__fadd2_rn(make_float2(x[w], x[w + 1]), make_float2(-top, -top)),
+                                  make_float2(kLog2E, kLog2E));
+      e[w] = exp2_fast(u.x);
+      e[w + 1] = exp2_fast(u.y);
+    }
+  } else {
+#pragma unroll
+    for (int w = 0; w < W; ++w) e[w] = exp_fast(x[w] - top);
+  }
+}
+
 // log of a positive finite float to 1e-9: s = 2^k f with f in [1/sqrt 2,
 // sqrt 2), log f = 2 atanh(q), q = (f - 1) / (f + 1), |q| < 0.172: the odd
 // series to q^11 in 64 bits (next term 2e-11).  Zero, infinity and NaN go
@@ -895,20 +913,19 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
     }
     st = grp.stats(st);
     const float inv = 1.0f / st.sum, mean = st.mean * inv;
-    // for sums and gradients p to 2^-23 |m| is enough
-    const float shift = -st.top * kLog2E;
     float kl = 0.0f;
     if (Kl) {
       for (int v = t; v < vecs; v += threads) {
-        float xa[W], da[W], part = 0.0f;
+        float xa[W], da[W], e[W], part = 0.0f;
         bool some = false;
         load(v, xa, da);
+        exps(xa, st.top, e);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const float y = mean - da[w];
           const bool near = fabsf(y) < 1.0f;
           some |= !near;
-          part = fmaf(near ? exp2_fast(fmaf(xa[w], kLog2E, shift)) : 0.0f, phi_small(near ? y : 0.0f), part);
+          part = fmaf(near ? e[w] : 0.0f, phi_small(near ? y : 0.0f), part);
         }
         kl = fmaf(part, inv, kl);
         if (some) {
@@ -944,14 +961,12 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
       const float wc = -out.wc * inv, wb = out.wb * inv;
       const int at_k = k - lo + lead;  // the action, counted from vector 0
       for (int v = t; v < vecs; v += threads) {
-        float xa[W], da[W];
+        float xa[W], da[W], e[W];
         load(v, xa, da);
+        exps(xa, st.top, e);
         const int a = v * W - lead;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float e = exp2_fast(fmaf(xa[w], kLog2E, shift));
-          xa[w] = (Kl ? fmaf(wb, da[w] - mean, wc) : wc) * e;
-        }
+        for (int w = 0; w < W; ++w) xa[w] = (Kl ? fmaf(wb, da[w] - mean, wc) : wc) * e[w];
         if (at_k / W == v && at_k >= 0) {
 #pragma unroll
           for (int w = 0; w < W; ++w)

@@ -522,3 +522,50 @@ def _lowest_rows(A, dtype, kl):
     if kl == "sampled":
         kw["reference_log_prob"][::2] = 0.2 - math.log(A)
     _check(logits, action, kw, beta=0.0 if kl == "none" else 0.07)
+
+
+@pytest.mark.parametrize("kl", ["none", "sampled", "full"])
+@pytest.mark.parametrize("m", [1e2, 1e3, 1e4, -6e4, 6e4])
+@pytest.mark.parametrize("A", [82, 700, 5001, 33000])
+def test_logits_around_a_large_value(cuda, A, m, kl):
+    """A constant added to a row's logits changes p by nothing but what the
+    logits' own type rounds: x - m is taken first, and is as exact as it was."""
+    N = 100 if A < 5000 else 40
+    logits, action, kw = _inputs(N, A, "fp32", True, kl, seed=61)
+    logits = logits + m
+    x = logits.double().masked_fill(~kw["legal"], -math.inf)
+    lp = torch.log_softmax(x, -1).gather(-1, action.long()[:, None])[:, 0]
+    kw["old_log_prob"] = lp.float() + 0.3 * torch.sin(torch.arange(N, device="cuda"))
+    if kl == "sampled":
+        kw["reference_log_prob"] = lp.float() + 0.2 * torch.cos(torch.arange(N, device="cuda"))
+    if kl == "full":
+        kw["reference_logits"] = kw["reference_logits"] + m
+    _check(logits, action, kw, beta=0.0 if kl == "none" else 0.07)
+
+
+@pytest.mark.parametrize("kl", ["none", "sampled"])
+@pytest.mark.parametrize("dtype,m", [("bf16", 1e4), ("bf16", 1e30), ("fp16", 1e3), ("fp16", 6e4), ("fp16", -6e4)])
+@pytest.mark.parametrize("A", [82, 700, 33000])
+def test_ties_at_a_large_value(cuda, A, dtype, m, kl):
+    """Half of a row's logits at m, the others one step of the type below
+    (p of m is 2 / A, or a little less where the step is small)."""
+    N = 40
+    _, action, kw = _inputs(N, A, dtype, False, kl, seed=63)
+    top = torch.tensor(m, dtype=DT[dtype], device="cuda")
+    below = torch.nextafter(top, torch.full_like(top, -math.inf))
+    logits = torch.where(torch.arange(A, device="cuda") % 2 == 0, top, below).expand(N, A).contiguous()
+    action = action // 2 * 2
+    lp = torch.log_softmax(logits.double(), -1).gather(-1, action.long()[:, None])[:, 0]
+    kw["old_log_prob"] = lp.float() + 0.3 * torch.sin(torch.arange(N, device="cuda"))
+    if kl == "sampled":
+        kw["reference_log_prob"] = lp.float() + 0.2 * torch.cos(torch.arange(N, device="cuda"))
+    # weights that the gradients stay normal numbers of the type with
+    kw["weight"] = torch.full((N,), 256.0, device="cuda")
+    _check(logits, action, kw, beta=0.0 if kl == "none" else 0.07)
+
+
+@pytest.mark.parametrize("kl", ["none", "sampled", "full"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("A", [700, 40000])
+def test_long_rows_of_the_lowest_value(cuda, A, dtype, kl):
+    _lowest_rows(A, dtype, kl)
