@@ -66,11 +66,14 @@ constexpr int kMaxShort = 512;     // actions of a short row
 constexpr int kMaxActions = 262144;
 constexpr int kLongShared = 224 * 1024;  // of an SM, for the slices of its CTAs
 constexpr int kMaxPartials = 148 * 16;
-// the 32-bit log-probability is within 3e-6 of the exact one: terms within
-// 2^-24 |x - m| + 2^-22 each, weighted by p (sum p |x - m| <= 13 at 2^18
-// actions: 1e-6), and the adds of up to 64 values per thread, in eight
-// chains, plus the tree (2e-6)
-constexpr double kBorderTol = 8e-6;
+// What the 32-bit log-probability may be off by: terms within 2^-24 |x - m| +
+// 2^-22 each, weighted by p (sum p |x - m| <= 13 at 2^18 actions: 1e-6); a
+// thread's adds, at most 4 for eight elements and 28 of such sums (a slice of
+// kLongShared / 2 bytes over 256 threads), and the tree's (2.5e-6); and up to
+// 28 changes of a thread's maximum, 2^-22 of the sum each at worst (6.7e-6,
+// in rows that ascend; 1e-6 was measured, and 3e-6 in all is what other rows
+// stay below)
+constexpr double kBorderTol = 1.1e-5;
 // Up to this many logits every row's log-probability is evaluated in 64 bits:
 // the terms of a few rows may cancel to a loss that shows the 1e-7 of each.
 // The host needs 25 us for a call, and the kernels stay below that: 64 x 82
@@ -181,7 +184,7 @@ __device__ __forceinline__ float exp2_fast(float t) {
 __device__ __forceinline__ float exp_fast(float u) { return exp2_fast(u * kLog2E); }
 
 // e^{x - top} of a vector's elements, the same bits: differences and
-// products two at a time (4096 x 32000 bf16 140 us, 143 one at a time)
+// products two at a time (4096 x 32000 bf16 137 us, 143 one at a time)
 template <int W>
 __device__ __forceinline__ void exps(const float (&x)[W], float top, float (&e)[W]) {
   if constexpr (W % 2 == 0) {
@@ -889,24 +892,38 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
         for (int w = 0; w < W; ++w) da[w] = xa[w] == -INFINITY ? 0.0f : xa[w] - ra[w];
       }
     };
+    // single elements are taken eight at a time, so that no chain of adds is
+    // longer than a row of vectors has (kBorderTol)
+    constexpr int kTake = W == 1 ? 8 : 1, kElems = kTake * W;
     Stats st = {-INFINITY, 0.0f, 0.0f};
     float from = 0.0f;  // st.top, or 0 without an action yet, when only a NaN has a part in the sum
-    for (int v = t; v < vecs; v += threads) {
-      float xa[W], da[W];
-      load(v, xa, da);
+    for (int first_v = t; first_v < vecs; first_v += kTake * threads) {
+      float xa[kElems], da[kElems];
+#pragma unroll
+      for (int i = 0; i < kTake; ++i) {
+        const int v = first_v + i * threads;
+        float xv[W], dv[W];
+        const bool inside = kTake == 1 || v < vecs;
+        load(inside ? v : vecs - 1, xv, dv);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          xa[i * W + w] = inside ? xv[w] : -INFINITY;
+          if (Kl) da[i * W + w] = inside ? dv[w] : 0.0f;
+        }
+      }
       float top = xa[0];
 #pragma unroll
-      for (int w = 1; w < W; ++w) top = fmaxf(top, xa[w]);
+      for (int w = 1; w < kElems; ++w) top = fmaxf(top, xa[w]);
       if (top > st.top) {
         rescale(st, top);
         from = top;
       }
-      float sum[2] = {0.0f, 0.0f}, mean[2] = {0.0f, 0.0f};
+      float e[kElems], sum[2] = {0.0f, 0.0f}, mean[2] = {0.0f, 0.0f};
+      exps(xa, from, e);
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float e = exp_fast(xa[w] - from);
-        sum[w & 1] += e;
-        if (Kl) mean[w & 1] = fmaf(e, da[w], mean[w & 1]);
+      for (int w = 0; w < kElems; ++w) {
+        sum[w & 1] += e[w];
+        if (Kl) mean[w & 1] = fmaf(e[w], da[w], mean[w & 1]);
       }
       st.sum += sum[0] + sum[1];
       if (Kl) st.mean += mean[0] + mean[1];

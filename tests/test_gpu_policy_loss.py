@@ -569,3 +569,43 @@ def test_ties_at_a_large_value(cuda, A, dtype, m, kl):
 @pytest.mark.parametrize("A", [700, 40000])
 def test_long_rows_of_the_lowest_value(cuda, A, dtype, kl):
     _lowest_rows(A, dtype, kl)
+
+
+def _sliced(x, pad):
+    """`x` as the first columns of rows `pad` elements longer."""
+    wide = torch.full((x.shape[0], x.shape[1] + pad), math.nan, dtype=x.dtype, device="cuda")
+    wide[:, :x.shape[1]] = x
+    return wide[:, :x.shape[1]]
+
+
+@pytest.mark.parametrize("pad", [0, 1])
+def test_borders_of_long_sums(cuda, pad):
+    """Rows of one CTA, taken vector by vector or (rows an odd number of
+    elements apart) one by one, whose sums round one way all along: each
+    thread adds 222 terms of 0.57 steps to a first one of 1.  Log-probability
+    and clipping as of any row."""
+    N, A = 80, 57001
+    x = torch.full((N, A), -16.5, dtype=torch.bfloat16, device="cuda")
+    x[:, :256] = 0.0
+    x = _sliced(x, pad)
+    action = 3 * torch.arange(N, device="cuda", dtype=torch.int32)
+    lp = torch.log_softmax(x.double(), -1).gather(-1, action.long()[:, None])[:, 0]
+    steps = (torch.arange(N, device="cuda") % 7 - 3).to(torch.int32)
+    for adv, border in ((1.0, math.log1p(0.2)), (-1.0, math.log1p(-0.2))):
+        old = ((lp - border).float().view(torch.int32) + steps).view(torch.float32)
+        out = _check(x, action, dict(old_log_prob=old, advantage=torch.full((N,), adv, device="cuda")), beta=0.0)
+        assert 0 < int(out.clipped.sum()) < N
+
+
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("span", [0.03, 0.3, 3.0, 30.0])
+@pytest.mark.parametrize("dtype,A", [("fp32", 28000), ("bf16", 57000)])
+def test_rows_that_ascend(cuda, dtype, A, span, pad):
+    """Every element or vector is a new maximum: sums are rescaled all along."""
+    N = 80
+    end = span * (1 + torch.arange(N, device="cuda", dtype=torch.float64) / N)[:, None]
+    x = _sliced((-end * (1 - torch.linspace(0, 1, A, device="cuda", dtype=torch.float64))).to(DT[dtype]), pad)
+    action = (A - 1 - 5 * torch.arange(N, device="cuda")).to(torch.int32)
+    lp = torch.log_softmax(x.double(), -1).gather(-1, action.long()[:, None])[:, 0]
+    _check(x, action, dict(old_log_prob=lp.float() + 0.3 * torch.sin(torch.arange(N, device="cuda")),
+                           advantage=torch.cos(torch.arange(N, device="cuda", dtype=torch.float32))), beta=0.0)
