@@ -446,9 +446,10 @@ __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, in
   if (!Kl && p.reference_log_prob) {
     const float y = (float)((double)in.ref - lp), em = expm1f(y);
     kl = fabsf(y) < 1.0f ? phi_small(y) : em - y;
-    c = fmaf(-p.beta, em, c);
+    if (p.beta != 0.0f) c = fmaf(-p.beta, em, c);
   }
-  term += (double)p.beta * (double)kl;
+  // (without a coefficient the KL is a statistic alone, and may be infinite)
+  if (p.beta != 0.0f) term += (double)p.beta * (double)kl;
   if (grp.index() == 0) {
     p.log_prob[row] = (float)lp;
     p.clipped[row] = clipped;

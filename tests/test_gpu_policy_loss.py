@@ -609,3 +609,18 @@ def test_rows_that_ascend(cuda, dtype, A, span, pad):
     lp = torch.log_softmax(x.double(), -1).gather(-1, action.long()[:, None])[:, 0]
     _check(x, action, dict(old_log_prob=lp.float() + 0.3 * torch.sin(torch.arange(N, device="cuda")),
                            advantage=torch.cos(torch.arange(N, device="cuda", dtype=torch.float32))), beta=0.0)
+
+
+@pytest.mark.parametrize("A", [82, 2000])
+def test_kl_without_a_coefficient_is_a_statistic(cuda, A):
+    """References whose estimate overflows, or that exclude the action: the
+    KL is infinite, and loss and gradient are those of a call without one."""
+    logits, action, kw = _inputs(20, A, "fp32", True, "sampled", seed=66)
+    reference = kw.pop("reference_log_prob")
+    want = clipped_policy_loss(logits, action, **kw)
+    reference[:5] += 300.0
+    reference[5:9] = -math.inf
+    got = clipped_policy_loss(logits, action, reference_log_prob=reference, **kw)
+    assert torch.isposinf(got.kl[:9]).all() and torch.isfinite(got.kl[9:]).all()
+    for name in ("loss", "log_prob", "clipped", "grad_logits"):
+        assert torch.equal(getattr(got, name), getattr(want, name)), name
