@@ -74,6 +74,10 @@ constexpr int kMaxPartials = 148 * 16;
 // in rows that ascend; 1e-6 was measured, and 3e-6 in all is what other rows
 // stay below)
 constexpr double kBorderTol = 1.1e-5;
+// and of a short row: sum p |x - m| <= 6.3, 24 adds and the tree's, no changes
+// of the maximum (2.4e-6).  (A row next to a border holds its warp up: 262144
+// x 82 fp32 with a sampled KL 62 us at 8e-6, 64 at 1.1e-5)
+constexpr double kShortBorderTol = 4e-6;
 // Up to this many logits every row's log-probability is evaluated in 64 bits:
 // the terms of a few rows may cancel to a loss that shows the 1e-7 of each.
 // The host needs 25 us for a call, and the kernels stay below that: 64 x 82
@@ -419,8 +423,8 @@ struct RowOut {
 };
 
 // a log-ratio that 32-bit sums may have put on the wrong side of the clip
-__device__ __forceinline__ bool near_border(const Params &p, double delta) {
-  return fabs(delta - p.log_high) < kBorderTol || fabs(delta - p.log_low) < kBorderTol;
+__device__ __forceinline__ bool near_border(const Params &p, double delta, double tol) {
+  return fabs(delta - p.log_high) < tol || fabs(delta - p.log_low) < tol;
 }
 
 // The row's statistics from its sums, by every thread alike; thread 0 of the
@@ -431,7 +435,7 @@ __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, in
   double lp = ((double)in.xk - (double)top) - log_sum, delta = lp - (double)in.old;
   const bool far = Kl && !(kl_sum < kFarKl);
   float kl = Kl ? log1pf(kl_sum) : 0.0f;
-  if (far || (!settled && (p.fine || near_border(p, delta)))) {
+  if (far || (!settled && (p.fine || near_border(p, delta, kShortBorderTol)))) {
     const double2 fine = row_in_64<T>(p, grp, row, top, far);
     lp = ((double)in.xk - (double)top) - fine.x;
     delta = lp - (double)in.old;
@@ -962,7 +966,8 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
       kl = grp.reduce<SumOp>(kl);
     }
     double log_sum = log_row_sum(st.sum);
-    const bool fine = p.fine || near_border(p, ((double)in.xk - (double)st.top) - log_sum - (double)in.old);
+    const bool fine =
+        p.fine || near_border(p, ((double)in.xk - (double)st.top) - log_sum - (double)in.old, kBorderTol);
     if (fine) {  // as row_in_64, from shared memory (out of line it was slower)
       double s = 0.0;
       for (int v = t; v < vecs; v += threads) {
