@@ -84,6 +84,7 @@ constexpr double kShortBorderTol = 4e-6;
 // fp32 14 us (6 without), 8 x 131071 fp32 25 us (19 without).
 constexpr int64_t kFineLogits = 1 << 20;
 constexpr float kFarKl = 1.0e4f;   // sum p phi above this (KL > 9): the direct difference is exact enough
+constexpr float kLowest = -1.0e30f;  // what is below is a mask's value where the row has any above
 constexpr float kLog2E = 1.44269504088896341f;
 
 struct Params {
@@ -468,14 +469,12 @@ __device__ __forceinline__ void empty_row(const Params &p, int64_t row) {
   if (p.kl) p.kl[row] = 0.0f;
 }
 
-// p phi(mean - d) of one action whose y = mean - d is not within (-1, 1).  An
-// e^y that overflows, or meets a p that underflowed, makes the row a far one.
-// A place with p = 0 and d = 0 has no part here: it may be one that is not
-// kept, so an action of that kind is the caller's to find.  Out of line: few
-// actions are that far, and e^y for all of them is a third of the row's work.
-__device__ __noinline__ float kl_part_far(float pa, float d, float mean) {
-  const float y = mean - d;
-  return pa > 0.0f ? fmaf(pa, expf(y), -pa * (1.0f + y)) : (y > 60.0f && d != 0.0f ? INFINITY : pa * 0.0f);
+// p phi(y) of one action whose y = mean - d is not within (-1, 1).  An e^y
+// that overflows, or meets a p that underflowed, makes the row a far one.  Out
+// of line: few actions are that far, and e^y for all of them is a third of the
+// row's work.
+__device__ __noinline__ float kl_part_far(float pa, float y) {
+  return pa > 0.0f ? fmaf(pa, expf(y), -pa * (1.0f + y)) : (y > 60.0f ? INFINITY : pa * 0.0f);
 }
 
 // ---------------------------------------------------------------------------
@@ -676,7 +675,16 @@ __device__ __forceinline__ double short_row(const Params &p, const Lanes &grp, i
     if (some) {
 #pragma unroll
       for (int i = 0; i < V * W; ++i)
-        if (!(fabsf(mean - d[Kl ? i : 0]) < 1.0f)) kl += kl_part_far(e[i] * inv, d[Kl ? i : 0], mean);
+        if (const float y = mean - d[Kl ? i : 0]; !(fabsf(y) < 1.0f)) {
+          if (e[i] != 0.0f) {
+            kl += kl_part_far(e[i] * inv, y);
+          } else {
+            // (a place that is not kept has d = 0.)  The gradient is 0, where
+            // a logit of the type's lowest value leaves a d that overflows
+            if (y > 60.0f && d[Kl ? i : 0] != 0.0f) kl = INFINITY;
+            d[Kl ? i : 0] = mean;
+          }
+        }
     }
     // actions with p = 0 whose logits are equal (d = 0) count above 60, and
     // are looked up there alone (telling them from places that are not kept
@@ -900,40 +908,48 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
     // single elements are taken eight at a time, so that no chain of adds is
     // longer than a row of vectors has (kBorderTol)
     constexpr int kTake = W == 1 ? 8 : 1, kElems = kTake * W;
-    Stats st = {-INFINITY, 0.0f, 0.0f};
-    float from = 0.0f;  // st.top, or 0 without an action yet, when only a NaN has a part in the sum
-    for (int first_v = t; first_v < vecs; first_v += kTake * threads) {
-      float xa[kElems], da[kElems];
+    // The maximum starts at kLowest, so that logits of the type's lowest value
+    // have no part before a larger one is met: their differences to the
+    // reference would overflow the mean.  A row without one starts from -inf.
+    Stats st;
+    for (float least = Kl ? kLowest : -INFINITY;; least = -INFINITY) {
+      st = {least, 0.0f, 0.0f};
+      // st.top, or 0 without an action yet, when only a NaN has a part in the sum
+      float from = least == -INFINITY ? 0.0f : least;
+      for (int first_v = t; first_v < vecs; first_v += kTake * threads) {
+        float xa[kElems], da[kElems];
 #pragma unroll
-      for (int i = 0; i < kTake; ++i) {
-        const int v = first_v + i * threads;
-        float xv[W], dv[W];
-        const bool inside = kTake == 1 || v < vecs;
-        load(inside ? v : vecs - 1, xv, dv);
+        for (int i = 0; i < kTake; ++i) {
+          const int v = first_v + i * threads;
+          float xv[W], dv[W];
+          const bool inside = kTake == 1 || v < vecs;
+          load(inside ? v : vecs - 1, xv, dv);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          xa[i * W + w] = inside ? xv[w] : -INFINITY;
-          if (Kl) da[i * W + w] = inside ? dv[w] : 0.0f;
+          for (int w = 0; w < W; ++w) {
+            xa[i * W + w] = inside ? xv[w] : -INFINITY;
+            if (Kl) da[i * W + w] = inside ? dv[w] : 0.0f;
+          }
         }
-      }
-      float top = xa[0];
+        float top = xa[0];
 #pragma unroll
-      for (int w = 1; w < kElems; ++w) top = fmaxf(top, xa[w]);
-      if (top > st.top) {
-        rescale(st, top);
-        from = top;
-      }
-      float e[kElems], sum[2] = {0.0f, 0.0f}, mean[2] = {0.0f, 0.0f};
-      exps(xa, from, e);
+        for (int w = 1; w < kElems; ++w) top = fmaxf(top, xa[w]);
+        if (top > st.top) {
+          rescale(st, top);
+          from = top;
+        }
+        float e[kElems], sum[2] = {0.0f, 0.0f}, mean[2] = {0.0f, 0.0f};
+        exps(xa, from, e);
 #pragma unroll
-      for (int w = 0; w < kElems; ++w) {
-        sum[w & 1] += e[w];
-        if (Kl) mean[w & 1] = fmaf(e[w], da[w], mean[w & 1]);
+        for (int w = 0; w < kElems; ++w) {
+          sum[w & 1] += e[w];
+          if (Kl) mean[w & 1] = fmaf(e[w], da[w], mean[w & 1]);
+        }
+        st.sum += sum[0] + sum[1];
+        if (Kl) st.mean += mean[0] + mean[1];
       }
-      st.sum += sum[0] + sum[1];
-      if (Kl) st.mean += mean[0] + mean[1];
+      st = grp.stats(st);
+      if (st.sum != 0.0f || least == -INFINITY) break;
     }
-    st = grp.stats(st);
     const float inv = 1.0f / st.sum, mean = st.mean * inv;
     float kl = 0.0f;
     if (Kl) {
@@ -958,8 +974,7 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
             if (a < 0 || a >= n || (legal && !sl[a])) continue;
             const float xw = to_f(sx[a]), dw = xw - to_f(sr[a]);
             if (xw == -INFINITY || fabsf(mean - dw) < 1.0f) continue;
-            const float pw = exp_fast(xw - st.top) * inv;
-            kl += pw == 0.0f && mean - dw > 60.0f ? INFINITY : kl_part_far(pw, dw, mean);
+            kl += kl_part_far(exp_fast(xw - st.top) * inv, mean - dw);
           }
         }
       }
@@ -983,6 +998,15 @@ __global__ void __launch_bounds__(kLongThreads, 4) policy_loss_long_kernel(const
     if (grad) {
       const float wc = -out.wc * inv, wb = out.wb * inv;
       const int at_k = k - lo + lead;  // the action, counted from vector 0
+      if (Kl && !(fabsf(wb) <= 1.0f)) {
+        // p = 0 has no gradient, where a logit of the type's lowest value
+        // leaves a d that overflows once multiplied by wb.  (Each thread
+        // writes the elements that it reads.)
+        for (int v = t; v < vecs; v += threads)
+#pragma unroll 1
+          for (int a = max(v * W - lead, 0); a < min(v * W - lead + W, n); ++a)
+            if (exp_fast(to_f(sx[a]) - st.top) == 0.0f) sr[a] = sx[a];
+      }
       for (int v = t; v < vecs; v += threads) {
         float xa[W], da[W], e[W];
         load(v, xa, da);

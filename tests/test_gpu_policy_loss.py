@@ -624,3 +624,24 @@ def test_kl_without_a_coefficient_is_a_statistic(cuda, A):
     assert torch.isposinf(got.kl[:9]).all() and torch.isfinite(got.kl[9:]).all()
     for name in ("loss", "log_prob", "clipped", "grad_logits"):
         assert torch.equal(getattr(got, name), getattr(want, name)), name
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("A", [82, 81, 2000, 2001, 40000])
+def test_lowest_value_in_the_logits_alone(cuda, A, dtype):
+    """Actions masked by the type's lowest value where the reference is not:
+    their differences are of 1e38, their p and gradients 0.  A weight 2^12
+    times larger gives 2^12 times the gradient, bit for bit."""
+    logits, action, kw = _inputs(30, A, dtype, True, "full", seed=64)
+    legal = kw.pop("legal")
+    logits = logits.masked_fill(~legal, torch.finfo(DT[dtype]).min)
+    grads = []
+    for weight in (2.0 ** -6, 2.0 ** 6):
+        kw["weight"] = torch.full((30,), weight, device="cuda")
+        out = clipped_policy_loss(logits, action, kl_coefficient=4.0, **kw)
+        assert torch.isfinite(out.loss) and torch.isfinite(out.kl).all() and not out.grad_logits[~legal].any()
+        grads.append(out.grad_logits.float())
+    # (the smallest normal number itself may be the rounding of a subnormal one, in coarser steps)
+    normal = grads[0].abs() > torch.finfo(DT[dtype]).smallest_normal
+    assert bool(normal.any()) and torch.equal((grads[0] * 2.0 ** 12)[normal], grads[1][normal])
+    assert torch.isfinite(grads[1]).all()
