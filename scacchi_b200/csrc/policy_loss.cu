@@ -444,8 +444,8 @@ __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, in
   }
   const bool clipped = in.adv >= 0.0f ? delta > p.log_high : delta < p.log_low;
   // (in 64 bits: the rows' terms cancel in the loss.)  An advantage of 0 adds
-  // nothing, whatever the ratio overflows to
-  double term = clipped || in.adv == 0.0f ? 0.0 : -(double)in.adv * exp(delta);
+  // nothing, whatever the ratio overflows to, unless that is NaN
+  double term = clipped || (in.adv == 0.0f && delta == delta) ? 0.0 : -(double)in.adv * exp(delta);
   float c = (float)term;
   if (clipped) term = -(double)in.adv * (in.adv >= 0.0f ? p.clip_high : p.clip_low);
   if (!Kl && p.reference_log_prob) {

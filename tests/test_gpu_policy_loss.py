@@ -645,3 +645,19 @@ def test_lowest_value_in_the_logits_alone(cuda, A, dtype):
     normal = grads[0].abs() > torch.finfo(DT[dtype]).smallest_normal
     assert bool(normal.any()) and torch.equal((grads[0] * 2.0 ** 12)[normal], grads[1][normal])
     assert torch.isfinite(grads[1]).all()
+
+
+@pytest.mark.parametrize("A", [82, 2000])
+def test_a_nan_meets_an_advantage_of_zero(cuda, A):
+    """0 times a ratio that overflows is 0, times one that is NaN is NaN: a
+    check of the loss sees the row whose gradient is NaN."""
+    logits, action, kw = _inputs(8, A, "fp32", False, "none", seed=65)
+    kw["advantage"][3] = 0.0
+    assert math.isfinite(float(clipped_policy_loss(logits, action, **kw).loss))
+    bad = logits.clone()
+    bad[3, 5] = math.nan
+    out = clipped_policy_loss(bad, action, **kw)
+    assert math.isnan(float(out.loss)) and bool(torch.isnan(out.grad_logits[3]).any())
+    kw["old_log_prob"][3] = math.nan
+    out = clipped_policy_loss(logits, action, **kw)
+    assert math.isnan(float(out.loss)) and bool(torch.isnan(out.grad_logits[3]).any())
