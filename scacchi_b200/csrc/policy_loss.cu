@@ -445,22 +445,24 @@ __device__ __forceinline__ RowOut finish_row(const Params &p, const Grp &grp, in
   const bool clipped = in.adv >= 0.0f ? delta > p.log_high : delta < p.log_low;
   // (in 64 bits: the rows' terms cancel in the loss.)  An advantage of 0 adds
   // nothing, whatever the ratio overflows to, unless that is NaN
-  double term = clipped || (in.adv == 0.0f && delta == delta) ? 0.0 : -(double)in.adv * exp(delta);
-  float c = (float)term;
-  if (clipped) term = -(double)in.adv * (in.adv >= 0.0f ? p.clip_high : p.clip_low);
+  // (weighted first: a ratio may leave 32 bits where the row's share does not)
+  const double gain = (double)weight * (double)in.adv;
+  double term = clipped || (in.adv == 0.0f && delta == delta) ? 0.0 : -gain * exp(delta);
+  float wc = (float)term;
+  if (clipped) term = -gain * (in.adv >= 0.0f ? p.clip_high : p.clip_low);
   if (!Kl && p.reference_log_prob) {
     const float y = (float)((double)in.ref - lp), em = expm1f(y);
     kl = fabsf(y) < 1.0f ? phi_small(y) : em - y;
-    if (p.beta != 0.0f) c = fmaf(-p.beta, em, c);
+    if (p.beta != 0.0f) wc = fmaf(-weight * p.beta, em, wc);
   }
   // (without a coefficient the KL is a statistic alone, and may be infinite)
-  if (p.beta != 0.0f) term += (double)p.beta * (double)kl;
+  if (p.beta != 0.0f) term += (double)weight * ((double)p.beta * (double)kl);
   if (grp.index() == 0) {
     p.log_prob[row] = (float)lp;
     p.clipped[row] = clipped;
     if (p.kl) p.kl[row] = kl;
   }
-  return RowOut{(double)weight * term, weight * c, weight * p.beta};
+  return RowOut{term, wc, weight * p.beta};
 }
 
 __device__ __forceinline__ void empty_row(const Params &p, int64_t row) {

@@ -661,3 +661,15 @@ def test_a_nan_meets_an_advantage_of_zero(cuda, A):
     kw["old_log_prob"][3] = math.nan
     out = clipped_policy_loss(logits, action, **kw)
     assert math.isnan(float(out.loss)) and bool(torch.isnan(out.grad_logits[3]).any())
+
+
+@pytest.mark.parametrize("kl", ["none", "sampled"])
+@pytest.mark.parametrize("A", [82, 2000])
+def test_a_ratio_beyond_32_bits_with_a_small_weight(cuda, A, kl):
+    """e^90 leaves fp32, 1e-5 of it does not: the gradient is as finite as
+    the loss."""
+    logits, action, kw = _inputs(20, A, "fp32", True, kl, seed=67)
+    kw["old_log_prob"] = kw["old_log_prob"] - 90.0
+    kw["advantage"] = -1.0 - kw["advantage"].abs()
+    kw["weight"] = torch.full((20,), 1e-5, device="cuda")
+    _check(logits, action, kw, beta=0.0 if kl == "none" else 0.1)
