@@ -110,6 +110,19 @@ def orthogonalize(matrix: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     return out
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two dense tensors share memory."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size()
+            and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
+def _span(t: torch.Tensor) -> torch.Tensor:
+    """All memory from a tensor's first element to its last, as a dense one."""
+    return t if t.is_contiguous() else t.as_strided((1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())),), (1,))
+
+
 def muon_update(weight: torch.Tensor, gradient: torch.Tensor, momentum: torch.Tensor, *, learning_rate: float,
                 beta: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, scale: float | None = None,
                 steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-8) -> None:
@@ -141,8 +154,7 @@ def muon_update(weight: torch.Tensor, gradient: torch.Tensor, momentum: torch.Te
         if not t.is_contiguous():
             raise ValueError(f"{name} is updated in place and must be contiguous")
     g = gradient.contiguous()
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (weight, g, momentum))
-    if weight.numel() and any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+    if _overlap(weight, g) or _overlap(weight, momentum) or _overlap(g, momentum):
         raise ValueError("weight, gradient and momentum may not overlap")
     if not 0.0 <= beta < 1.0:
         raise ValueError(f"beta must be in [0, 1), got {beta}")
@@ -202,6 +214,9 @@ class NetworkMuon:
             if gradient.shape != m.shape or gradient.device != m.device or gradient.dtype not in DTYPES:
                 raise ValueError(f"the gradient of {name} must be float32, bfloat16 or float16 {tuple(m.shape)} on "
                                  f"{m.device}, got {gradient.dtype} {tuple(gradient.shape)} on {gradient.device}")
+            # (a strided one is copied before its update, but after the others')
+            if any(_overlap(_span(gradient), t) for t in (*self.matrices.values(), *self.momentum.values())):
+                raise ValueError(f"the gradient of {name} overlaps a matrix or a momentum, which the step changes")
         for name, gradient in gradients.items():
             muon_update(self.matrices[name], gradient, self.momentum[name], **self.settings)
 

@@ -141,3 +141,21 @@ def test_products_after_an_unfinished_one_write_no_weights():
     source = (Path(__file__).parents[1] / "scacchi_b200" / "csrc" / "muon.cu").read_text()
     norm = source[source.index("ns_norm_kernel(Source"):]
     assert "*failed = 0" in norm[:norm.index("\n}\n")]
+
+
+def test_network_muon_refuses_gradients_that_the_step_changes():
+    """A gradient that lies in a matrix or a momentum, its own or another's,
+    would change between the updates: refused before the first of them."""
+    opt = NetworkMuon(init_params(4, num_blocks=1), learning_rate=0.1, device="cpu")
+    before = {k: v.clone() for k, v in opt.matrices.items()}
+    good = {k: torch.ones_like(v) for k, v in opt.matrices.items()}
+    square = opt.matrices["convs"].shape[-1]
+    strided = opt.matrices["convs"][0, :square].T  # of no matrix's shape but its own
+    for name, bad in (("value_w", opt.matrices["value_w"]), ("policy_w", opt.momentum["policy_w"]),
+                      ("convs", opt.matrices["convs"].detach())):
+        with pytest.raises(ValueError, match=f"gradient of {name} overlaps"):
+            opt.step({**good, name: bad})
+    opt.matrices["policy_w"], opt.momentum["policy_w"] = torch.zeros((square, square)), torch.zeros((square, square))
+    with pytest.raises(ValueError, match="gradient of policy_w overlaps"):
+        opt.step({"convs": good["convs"], "policy_w": strided})
+    assert all(torch.equal(opt.matrices[k], v) for k, v in before.items() if k != "policy_w")
