@@ -564,10 +564,13 @@ int scacchi_orthogonalize(const scacchi_newton_schulz *params, const void *matri
 
 /* Muon's step on float32 weights: momentum <- beta momentum + (1 - beta)
  * gradient; u = nesterov ? (1 - beta) gradient + beta momentum : momentum;
- * weight <- decay weight - step orthogonalize(u). */
+ * weight <- decay weight - step orthogonalize(u).  Either call's waits are
+ * bounded: where one runs out, out or weight stays unwritten in part or as a
+ * whole, and the flag below is raised. */
 int scacchi_muon_update(const scacchi_newton_schulz *params, const void *gradient, float *momentum, float *weight,
                         double beta, int32_t nesterov, float decay, float step, void *workspace, void *stream);
-/* Sticky flag of a product whose bounded wait ran out; reading clears it. */
+/* Sticky flag, of the current device, of a product whose bounded wait ran
+ * out; reading clears it.  Speaks of the work that is complete. */
 int scacchi_muon_error(uint32_t *flags);
 uint64_t scacchi_muon_launch_count(void);
 

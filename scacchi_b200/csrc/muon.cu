@@ -26,12 +26,16 @@
 // blocks are computed and stored; one above it is read as its mirror image,
 // MN-major for K-major.
 //
-// What bounds it: at 2048 x 2048 and above the tensor cores, three products
-// for one, at 1.1 to 1.2 PFLOP/s (2048 x 2048 fp32 461 us back to back for
-// 515 GFLOP issued; the pair kernel keeps the tensor pipe busy for 73 % of
-// a CTA's time); below, latency: seventeen dependent launches of 7 us or
-// more (300 x 300 117 us), or for narrow matrices one launch's phases
+// What bounds it (device times, by graph replays): at 2048 x 2048 and above
+// the tensor cores, three products for one, at 1.1 PFLOP/s (2048 x 2048 fp32
+// 452 us for 515 GFLOP issued; the pair kernel keeps the tensor pipe busy for
+// 73 % of a CTA's time); below, latency: seventeen dependent launches of 7 us
+// or more (300 x 300 117 us), or for narrow matrices one launch's phases
 // (162 x 82 49 us).
+//
+// Every wait is bounded (2 s).  One that runs out raises g_muon_error and, in
+// the kernels of one product, the call's flag in its workspace; a narrow
+// matrix, or any whose flag stands before the last product, is not written.
 
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -876,8 +880,9 @@ __device__ __forceinline__ int narrow_at(int row, int chunk) {
 }
 
 // 32 columns of the summed accumulators of a row (TMEM lane) per thread.
-// The last one's may reach 16 columns past the accumulators, not past TMEM:
-// at most six of them are narrower than 96.
+// The last one's may reach 16 columns past the accumulators where their width
+// is an odd multiple of 16, but not past TMEM's 512: such accumulators fill
+// 512 columns only at a width of 16, and at most 12 of those are in use.
 __device__ __forceinline__ void read_sum(float (&sum)[32], uint32_t acc, int count, uint32_t stride) {
 #pragma unroll
   for (int e = 0; e < 32; ++e) sum[e] = 0.0f;
@@ -1014,7 +1019,7 @@ __device__ __forceinline__ void narrow_square(uint8_t *z, int part, int row, int
 // distributed shared memory; M = c Z^2 + d I and X <- M X in every CTA for
 // its own slice.  Nothing but the matrix itself crosses global memory, and
 // seventeen launches of 7 us become one (162 x 82 49 us, 12 matrices of
-// 1152 x 128 82 us; one launch per product took 94 and 125).
+// 1152 x 128 82 us, 86 as Muon's step; one launch per product took 94 and 125).
 //
 // What bounds it is latency: about ten dependent phases a step, each far
 // below the tensor cores' or shared memory's rate.

@@ -23,18 +23,25 @@
 // long ones in the shared memory of a CTA or of a cluster, so every input is
 // read once and every output written once.  Row sums are held in 32 bits,
 // the log-probability is finished in 64 from them and the loss is summed in
-// 64.  A row whose ratio lies within kBorderTol of a clip border is evaluated
-// again in 64 bits, so the side it falls on does not depend on 32-bit
-// rounding.
+// 64.  A row whose ratio lies within kBorderTol (kShortBorderTol) of a clip
+// border is evaluated again in 64 bits, so the side it falls on does not
+// depend on 32-bit rounding.
 //
-// What bounds it is the instructions an action costs (some 57 with the full
-// KL, 25 without), not memory: 262144 rows of 82 fp32 actions with the full
-// KL take 104 us (2.7 TB/s, 43 % of a copy's rate), with a sampled KL 62 us
-// (3.2 TB/s); 4096 rows of 32000 bf16 140 us (3.7 TB/s); 8 rows of 131071
-// fp32 25 us, which is latency: one row's phases across a cluster.
+// Device times, by graph replays: 262144 rows of 82 fp32 actions with the
+// full KL 105 us (2.7 TB/s, 43 % of a copy's rate), with a sampled KL 62 us
+// (3.2 TB/s); 4096 rows of 32000 bf16 137 us (3.8 TB/s), with the full KL 445
+// us; 8 rows of 131071 fp32 24 us.
 //
-// Exponentials are ex2.approx of (x - m) log2 e: the difference first, so
-// that only |x - m|, which p weights, is rounded and scaled; their errors
+// What bounds it is not memory (30 to 41 % of DRAM's rate).  Short rows with
+// the full KL issue 96 instructions an action on 58 % of the cycles: 128
+// registers leave 16 warps an SM, which wait on their own results and on
+// instruction fetch.  Long rows issue 23 an action without it on 67 %, with
+// the exponentials' pipe at 52 % and shared memory at 47 %.  A few rows are
+// latency: one row's phases across a cluster.
+//
+// Exponentials are ex2.approx of (x - m) log2 e: the difference first, in
+// every pass, so that only |x - m|, which p weights, is rounded and scaled
+// (a fused x log2 e - m log2 e loses digits as m grows); their errors
 // (2^-22, and |x - m| 2^-24) average out over a row's sum.  The accurate
 // expf() takes three times the instructions and made the kernel issue-bound.
 

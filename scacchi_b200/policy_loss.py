@@ -57,20 +57,25 @@ def clipped_policy_loss(logits: torch.Tensor, action: torch.Tensor, old_log_prob
     vocabulary).  ``action`` (int32 or int64), ``old_log_prob``,
     ``advantage`` and ``weight`` have the leading shape; ``weight`` is a
     row's share of the loss (a mask over its sum, say; 1 / rows if absent).
+    Floating point of another type is rounded to float32 first.
     ``legal`` (bool) has the logits' shape; absent, every action is legal.
 
     The KL term is KL(pi || reference) over the legal actions where
     ``reference_logits`` (the logits' shape and type, finite where legal) is
     given, and its estimate exp(y) - 1 - y, y = reference - log pi(action),
-    where ``reference_log_prob`` is.
+    where ``reference_log_prob`` is; with a coefficient of 0 the KL is a
+    statistic alone.  A row whose logits are all masked by the type's lowest
+    value has to have its reference masked likewise, or weight 0.
 
     A row of weight 0, or whose action is out of range, illegal or has a
     logit of -inf, adds nothing: its statistics and gradient are 0.  An
     illegal action's logit may hold anything; its gradient is 0.
 
     The gradient is returned, not recorded: ``logits.backward(grad_logits)``
-    continues it.  The call launches on the current stream, does not
-    synchronise and can be captured into a CUDA graph.
+    continues it.  It has the logits' type, and float16 ends at 6e-8: put a
+    loss scale into ``weight`` where rows are many.  The call launches on the
+    current stream, does not synchronise and can be captured into a CUDA
+    graph.
     """
     if logits.device.type != "cuda":
         raise ValueError("clipped_policy_loss runs on the GPU: pass logits on a CUDA device")
