@@ -358,9 +358,8 @@ struct Ctas {
 };
 
 // A row in 64 bits, read again: log sum e^{x - top} over the kept actions,
-// and with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r).
-// The maxima are subtracted from one another first: at 1e38 a sum's logarithm
-// is lost beside them.  Taken by rows far from the reference, and by short rows next to a clip
+// and with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r),
+// of x - top throughout: beside 1e38 the rest is lost.  Taken by rows far from the reference, and by short rows next to a clip
 // border or of a small call (kFineLogits).
 template <typename T, typename Grp>
 __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64_t row, float top, bool want_kl) {
@@ -376,7 +375,7 @@ __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64
     s += e;
     if (want_kl) {
       const double ra = to_f(r[a]);
-      sd += e * ((double)xa - ra);
+      sd += e * (((double)xa - (double)top) - ra);
       rtop = ra > rtop ? ra : rtop;
     }
   }
@@ -392,7 +391,7 @@ __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64
       sr += exp((double)to_f(r[a]) - rtop);
     }
     sr = grp.template reduce<SumOp>(sr);
-    kl = (sd / s - ((double)top - rtop)) + (log(sr) - log_sum);
+    kl = (sd / s + rtop) + (log(sr) - log_sum);
   }
   return make_double2(log_sum, kl);
 }

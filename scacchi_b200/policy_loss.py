@@ -64,8 +64,10 @@ def clipped_policy_loss(logits: torch.Tensor, action: torch.Tensor, old_log_prob
     ``reference_logits`` (the logits' shape and type, finite where legal) is
     given, and its estimate exp(y) - 1 - y, y = reference - log pi(action),
     where ``reference_log_prob`` is; with a coefficient of 0 the KL is a
-    statistic alone.  A row whose logits are all masked by the type's lowest
-    value has to have its reference masked likewise, or weight 0.
+    statistic alone.  Rows without a legal action belong into ``legal``: one
+    whose logits are all masked by the type's lowest value is the uniform
+    policy, and where its reference is not masked likewise, fp32 and bfloat16
+    have no gradient of the KL (NaN).
 
     A row of weight 0, or whose action is out of range, illegal or has a
     logit of -inf, adds nothing: its statistics and gradient are 0.  An

@@ -673,3 +673,28 @@ def test_a_ratio_beyond_32_bits_with_a_small_weight(cuda, A, kl):
     kw["advantage"] = -1.0 - kw["advantage"].abs()
     kw["weight"] = torch.full((20,), 1e-5, device="cuda")
     _check(logits, action, kw, beta=0.0 if kl == "none" else 0.1)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("size", [(40, 3), (40, 82), (40, 81), (20, 512), (12, 700), (12, 701), (3, 40000), (90, 20003)],
+                         ids=str)
+def test_rows_of_the_lowest_value_against_a_reference_that_is_not(cuda, size, dtype):
+    """The uniform policy again: loss and statistics as of rows of zeros (in
+    fp16, where 2^-24 of the value is no more than 4e-3, as of rows of that
+    value)."""
+    N, A = size
+    logits, action, kw = _inputs(N, A, dtype, True, "full", seed=68)
+    logits[::2] = torch.finfo(torch.float16).min if dtype == "fp16" else 0.0
+    kw["old_log_prob"][::2] = 0.1 - torch.log(kw["legal"][::2].sum(-1).float())
+    kw["weight"] = torch.full((N,), 3.0, device="cuda")
+    want, clipped = _plain(logits, action, kl_coefficient=0.7, **kw)
+    logits[::2] = torch.finfo(DT[dtype]).min
+    for pad in (0, 1):
+        out = clipped_policy_loss(_sliced(logits, pad), action, kl_coefficient=0.7, **kw)
+        assert torch.equal(out.clipped, clipped)
+        for name in ("loss", "log_prob", "kl"):
+            value, tol = want[name]
+            err = (getattr(out, name).double() - value).abs()
+            assert float((err - tol).max()) <= 0, f"{name}: off by {float(err.max()):.3g}"
+        err = (out.grad_logits[1::2].double() - want["grad_logits"][0][1::2]).abs()
+        assert float((err - want["grad_logits"][1][1::2]).max()) <= 0
