@@ -42,7 +42,7 @@
 // Exponentials are ex2.approx of (x - m) log2 e: the difference first, in
 // every pass, so that only |x - m|, which p weights, is rounded and scaled
 // (a fused x log2 e - m log2 e loses digits as m grows); their errors
-// (2^-22, and |x - m| 2^-24) average out over a row's sum.  The accurate
+// (2^-22, and |x - m| 2^-23) average out over a row's sum.  The accurate
 // expf() takes three times the instructions and made the kernel issue-bound.
 
 #include <cooperative_groups.h>
@@ -73,16 +73,17 @@ constexpr int kMaxShort = 512;     // actions of a short row
 constexpr int kMaxActions = 262144;
 constexpr int kLongShared = 224 * 1024;  // of an SM, for the slices of its CTAs
 constexpr int kMaxPartials = 148 * 16;
-// What the 32-bit log-probability may be off by: terms within 2^-24 |x - m| +
-// 2^-22 each, weighted by p (sum p |x - m| <= 13 at 2^18 actions: 1e-6); a
-// thread's adds, at most 4 for eight elements and 28 of such sums (a slice of
-// kLongShared / 2 bytes over 256 threads), and the tree's (2.5e-6); and up to
-// 28 changes of a thread's maximum, 2^-22 of the sum each at worst (6.7e-6,
-// in rows that ascend; 1e-6 was measured, and 3e-6 in all is what other rows
+// What the 32-bit log-probability may be off by: terms within 2^-22 + 2.3 x
+// 2^-24 |x - m| each (the difference, the product and log2 e), weighted by p
+// (sum p |x - m| <= log of the actions, 11 for a slice of kLongShared / 2
+// bytes: 1.8e-6); a thread's adds, at most 4 for eight elements and 28 of such
+// sums (that slice over 256 threads), and the tree's (2.5e-6); and up to 28
+// changes of a thread's maximum, 2^-22 of the sum each at worst (6.7e-6, in
+// rows that ascend; 1e-6 was measured, and 3e-6 in all is what other rows
 // stay below)
 constexpr double kBorderTol = 1.1e-5;
 // and of a short row: sum p |x - m| <= 6.3, 24 adds and the tree's, no changes
-// of the maximum (2.4e-6).  (A row next to a border holds its warp up: 262144
+// of the maximum (2.9e-6).  (A row next to a border holds its warp up: 262144
 // x 82 fp32 with a sampled KL 62 us at 8e-6, 64 at 1.1e-5)
 constexpr double kShortBorderTol = 4e-6;
 // Up to this many logits every row's log-probability is evaluated in 64 bits:
@@ -359,8 +360,9 @@ struct Ctas {
 
 // A row in 64 bits, read again: log sum e^{x - top} over the kept actions,
 // and with `want_kl` the KL as the difference mean(x - r) - lse(x) + lse(r),
-// of x - top throughout: beside 1e38 the rest is lost.  Taken by rows far from the reference, and by short rows next to a clip
-// border or of a small call (kFineLogits).
+// of x - top throughout: beside 1e38 the rest is lost.  Taken by rows far
+// from the reference, and by short rows next to a clip border or of a small
+// call (kFineLogits).
 template <typename T, typename Grp>
 __device__ __noinline__ double2 row_in_64(const Params &p, const Grp &grp, int64_t row, float top, bool want_kl) {
   const int A = p.actions;
