@@ -574,6 +574,90 @@ int scacchi_muon_update(const scacchi_newton_schulz *params, const void *gradien
 int scacchi_muon_error(uint32_t *flags);
 uint64_t scacchi_muon_launch_count(void);
 
+/* Rows of logits and one action each.  logits hold num_actions elements a
+ * row, rows `stride` elements apart; the others are dense. */
+typedef struct {
+  const void *logits;                  /* [rows, actions] of `dtype` */
+  const uint8_t *legal;                /* [rows, actions], or NULL: every action */
+  const int32_t *action;               /* [rows] */
+  int64_t stride;
+} scacchi_log_prob_rows;
+
+typedef struct {
+  float *log_prob;                     /* [rows] 0 where the action is out of range, -inf where it is not kept */
+  float *entropy;                      /* [rows] */
+  float *max_logit;                    /* [rows] of the kept actions, -inf where there is none */
+  float *log_sum;                      /* [rows] log sum e^((x - max_logit) / temperature) */
+  float *top_log_prob;                 /* [rows, top], or NULL where top is 0 */
+  int32_t *top_action;                 /* [rows, top] -1 beyond the kept actions */
+} scacchi_log_prob_out;
+
+/* Over the kept actions (legal, logit above -inf) of softmax(logits /
+ * temperature): the action's log-probability, the entropy and the `top`
+ * (0 to 32) likeliest, the lower index first among equals.  dtype: 0 float32,
+ * 1 bfloat16, 2 float16; 1 <= num_actions <= 262144; 1e-3 <= temperature <=
+ * 1e3.  A NaN or +inf among the kept logits makes a row's numbers NaN. */
+int scacchi_log_probs(const scacchi_log_prob_rows *rows, const scacchi_log_prob_out *out, int64_t num_rows,
+                      int32_t num_actions, int32_t dtype, double temperature, int32_t top, void *stream);
+/* The gradient in the logits, dense [rows, actions] of `dtype`, from
+ * gradients of log_prob and entropy (either may be NULL: 0) and what
+ * scacchi_log_probs gave for the same rows.  Actions that are not kept have
+ * 0, and log_prob of an action that is not kept or out of range has none. */
+int scacchi_log_probs_gradient(const scacchi_log_prob_rows *rows, const float *max_logit, const float *log_sum,
+                               const float *entropy, const float *grad_log_prob, const float *grad_entropy,
+                               int64_t num_rows, int32_t num_actions, int32_t dtype, double temperature,
+                               void *grad_logits, void *stream);
+uint64_t scacchi_log_probs_launch_count(void);
+
+/* A tensor of an AdamW step, or (gradient, count and gradient_dtype alone) of
+ * a gradient norm.  All are dense. */
+typedef struct {
+  void *weight;
+  const void *gradient;                /* NULL: no gradient in this step, the tensor stays as it is */
+  int64_t count;                       /* elements */
+  int64_t offset;                      /* of its moments: a multiple of 256, ascending from tensor to tensor */
+  double weight_decay;
+  int32_t weight_dtype;                /* 0 float32, 1 bfloat16 */
+  int32_t gradient_dtype;              /* 0 float32, 1 bfloat16, 2 float16 */
+} scacchi_adamw_tensor;
+
+/* norm[0] = sqrt(sum of squares) over all tensors, summed in 64 bits in a
+ * fixed order.  workspace: scacchi_gradient_norm_workspace_bytes(num_tensors)
+ * bytes, 8-byte aligned, of this call alone. */
+size_t scacchi_gradient_norm_workspace_bytes(int32_t num_tensors);
+int scacchi_gradient_norm(const scacchi_adamw_tensor *tensors, int32_t num_tensors, float *norm, void *workspace,
+                          void *stream);
+
+#define SCACCHI_ADAMW_STATE_BYTES 64   /* the step's count and scalars */
+#define SCACCHI_ADAMW_BLOCK 256        /* elements that share an exponent */
+typedef struct {
+  int32_t state_bits;                  /* of the moments: 32 (float) or 8 (codes, a byte of exponent a block) */
+  int32_t stochastic;                  /* bfloat16 weights by random bits (must be set where state_bits is 8) */
+  double learning_rate, beta1, beta2, max_norm;
+  float eps;
+  uint32_t key0, key1;                 /* threefry key of the random bits */
+  int64_t moments;                     /* elements of each moment, a multiple of 256 */
+  void *first, *second;                /* [moments]; of 8 bits the second holds its root */
+  uint8_t *first_exponent, *second_exponent; /* [moments / 256], or NULL */
+  void *state;                         /* SCACCHI_ADAMW_STATE_BYTES, 8-byte aligned; begins with the int64 step count */
+  const float *norm;                   /* of all gradients, or NULL: no clipping */
+  const float *learning_rate_at;       /* read on the device in place of learning_rate, or NULL */
+} scacchi_adamw;
+
+/* state.step += 1; g = gradient max_norm / max(norm, max_norm); first <-
+ * beta1 first + (1 - beta1) g; second <- beta2 second + (1 - beta2) g^2;
+ * weight <- (1 - learning_rate weight_decay) weight - learning_rate
+ * (first / (1 - beta1^step)) / (sqrt(second / (1 - beta2^step)) + eps).
+ * A norm that is not finite skips the step: nothing is written.  Weights,
+ * moments and state may not overlap each other nor the gradients. */
+int scacchi_adamw_step(const scacchi_adamw *params, const scacchi_adamw_tensor *tensors, int32_t num_tensors,
+                       void *stream);
+/* The values that 8-bit moments stand for, exact in bfloat16 [moments]. */
+int scacchi_adamw_moments(const uint8_t *first, const uint8_t *second, const uint8_t *first_exponent,
+                          const uint8_t *second_exponent, int64_t moments, void *first_out, void *root_out,
+                          void *stream);
+uint64_t scacchi_adamw_launch_count(void);
+
 /* ---- host-side jax.random key helpers (no device work) ---------------- */
 
 /* search.py:207-209 key chain: for i < num_simulations,

@@ -11,11 +11,13 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libscacchi_b200.so")
 # (source, extra flags).  The search kernels are bit-reproducible against
 # the oracle: no implicit multiply-add contraction (they call fmaf()
-# explicitly where they want one).  The network kernels are checked to a
+# explicitly where they want one), and the AdamW step's 8-bit codes against
+# their definition.  The network kernels are checked to a
 # tolerance and keep contraction.
 UNITS = [(os.path.join(CSRC, "search.cu"), ["-fmad=false"]), (os.path.join(CSRC, "tower.cu"), []),
          (os.path.join(CSRC, "hex.cu"), ["-fmad=false"]), (os.path.join(CSRC, "targets.cu"), ["-fmad=false"]),
-         (os.path.join(CSRC, "policy_loss.cu"), []), (os.path.join(CSRC, "muon.cu"), [])]
+         (os.path.join(CSRC, "policy_loss.cu"), []), (os.path.join(CSRC, "muon.cu"), []),
+         (os.path.join(CSRC, "adamw.cu"), ["-fmad=false"]), (os.path.join(CSRC, "log_probs.cu"), [])]
 SOURCES = [u[0] for u in UNITS]
 HEADERS = [os.path.join(CSRC, h) for h in ("smath.h", "threefry.h", "synthetic_env.h", "lane_cta.cuh", "tc05.cuh")] + [
     os.path.join(ROOT, "include", "scacchi_b200.h")]

@@ -88,6 +88,23 @@ class NewtonSchulz(C.Structure):
         (n, C.c_double) for n in ("a", "b", "c", "eps")]
 
 
+class LogProbRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "legal", "action")] + [("stride", C.c_int64)]
+
+
+class LogProbOut(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("log_prob", "entropy", "max_logit", "log_sum", "top_log_prob",
+                                          "top_action")]
+
+
+class AdamWStep(C.Structure):
+    _fields_ = [("state_bits", C.c_int32), ("stochastic", C.c_int32)] + [
+        (n, C.c_double) for n in ("learning_rate", "beta1", "beta2", "max_norm")] + [
+        ("eps", C.c_float), ("key0", C.c_uint32), ("key1", C.c_uint32), ("moments", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("first", "second", "first_exponent", "second_exponent", "state", "norm",
+                                  "learning_rate_at")]
+
+
 P = C.c_void_p
 I32 = C.c_int32
 F32 = C.c_float
@@ -145,6 +162,14 @@ SIGNATURES = {
     "scacchi_muon_update": [C.POINTER(NewtonSchulz), P, P, P, C.c_double, I32, F32, F32, P, P],
     "scacchi_muon_error": [P],
     "scacchi_muon_launch_count": [],
+    "scacchi_log_probs": [C.POINTER(LogProbRows), C.POINTER(LogProbOut), C.c_int64, I32, I32, C.c_double, I32, P],
+    "scacchi_log_probs_gradient": [C.POINTER(LogProbRows), P, P, P, P, P, C.c_int64, I32, I32, C.c_double, P, P],
+    "scacchi_log_probs_launch_count": [],
+    "scacchi_gradient_norm_workspace_bytes": [I32],
+    "scacchi_gradient_norm": [P, I32, P, P, P],
+    "scacchi_adamw_step": [C.POINTER(AdamWStep), P, I32, P],
+    "scacchi_adamw_moments": [P, P, P, P, C.c_int64, P, P, P],
+    "scacchi_adamw_launch_count": [],
     "scacchi_tower_timing_read": [P, P],
     "scacchi_device_error": [P],
     "scacchi_launch_count": [],
@@ -154,7 +179,9 @@ RESTYPES = {"scacchi_search_workspace_bytes": C.c_size_t, "scacchi_launch_count"
             "scacchi_tower_launch_count": C.c_uint64, "scacchi_hex_launch_count": C.c_uint64,
             "scacchi_target_launch_count": C.c_uint64, "scacchi_policy_loss_workspace_bytes": C.c_size_t,
             "scacchi_policy_loss_launch_count": C.c_uint64, "scacchi_muon_workspace_bytes": C.c_size_t,
-            "scacchi_muon_scale_exponent": C.c_int32, "scacchi_muon_launch_count": C.c_uint64}
+            "scacchi_muon_scale_exponent": C.c_int32, "scacchi_muon_launch_count": C.c_uint64,
+            "scacchi_gradient_norm_workspace_bytes": C.c_size_t, "scacchi_adamw_launch_count": C.c_uint64,
+            "scacchi_log_probs_launch_count": C.c_uint64}
 
 
 class ScacchiError(RuntimeError):
@@ -199,7 +226,8 @@ def launch_count() -> int:
     training operators)."""
     return (int(lib().scacchi_launch_count()) + int(lib().scacchi_tower_launch_count())
             + int(lib().scacchi_hex_launch_count()) + int(lib().scacchi_target_launch_count())
-            + int(lib().scacchi_policy_loss_launch_count()) + int(lib().scacchi_muon_launch_count()))
+            + int(lib().scacchi_policy_loss_launch_count()) + int(lib().scacchi_muon_launch_count())
+            + int(lib().scacchi_adamw_launch_count()) + int(lib().scacchi_log_probs_launch_count()))
 
 
 def tower_error() -> int:

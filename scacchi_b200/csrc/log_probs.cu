@@ -1,0 +1,688 @@
+// Log-probabilities of one action per row of logits, with the row's entropy
+// and its best actions, and the gradient of both in the logits.
+//
+// Over the kept actions (legal, logit above -inf), with M = max x,
+// u = (x - M) / T, s = sum e^u and t = sum u e^u:
+//
+//   log_sum  = log s            log_prob = u_a - log s
+//   entropy  = log s - t / s    top k by x, the lower index first among equals
+//   dx_i     = (g ([i = a] - p_i) - h p_i (log p_i + entropy)) / T,
+//              p_i = e^(u_i - log s), for gradients g of log_prob, h of entropy
+//
+// Logits are read once.  Rows of up to 512 actions lie in the registers of a
+// few lanes.  Longer ones go through a CTA, or a cluster of them where rows
+// are few: every thread keeps the maximum of what it has seen and s and t
+// relative to it, and they are joined at the row's end.
+//
+// The best k come from the same maxima.  Split the row's threads into at least
+// 64 groups: of the groups' maxima the k-th largest, L, has k elements at or
+// above it, so the best k are among the elements >= L, and only threads whose
+// own maximum reaches L look at their elements again: for 64 groups of
+// independent logits 64 ln(64 / (64 - k)) elements, 24 for k = 20.  They are
+// ranked by counting.  Where more than kCandidates elements reach L (many equal
+// ones) the CTA takes the maximum below the last one k times.
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "../../include/scacchi_b200.h"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+std::atomic<uint64_t> g_log_probs_launches{0};
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxShort = 512;      // actions of a short row
+constexpr int kMaxActions = 262144;
+constexpr int kMaxTop = 32;
+constexpr int kMaxCluster = 16;
+constexpr int kMaxGroups = 128;
+constexpr int kCandidates = 512;
+constexpr float kLog2E = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kNothing = -1.0e4f;  // 2^kNothing is 0, and 0 times it is 0
+
+struct Params {
+  const void *logits;
+  const uint8_t *legal;
+  const int32_t *action;
+  float *log_prob, *entropy, *max_logit, *log_sum, *top_log_prob;
+  int32_t *top_action;
+  // of the gradient: max_logit, log_sum and entropy are inputs
+  const float *grad_log_prob, *grad_entropy;
+  void *grad;
+  int64_t rows, stride;
+  int actions, top;
+  int group;     // lanes of a short row
+  float scale;   // log2(e) / T
+  float inverse; // 1 / T
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
+  if constexpr (std::is_same_v<T, __half>) return __half2float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f(float v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+  if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+}
+
+template <typename T, int W>
+struct alignas(sizeof(T) * W) Vec {
+  T v[W];
+};
+
+__device__ __forceinline__ float exp2_fast(float t) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+  return y;
+}
+// the larger one, NaN where either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// u log2 e of a logit relative to the row's maximum (0 where the row has
+// none): the difference first, so that a row's offset costs no digits
+__device__ __forceinline__ float exponent_of(float x, float top, float scale) {
+  return max_nan((x - top) * scale, kNothing);
+}
+
+// Logits in their order, as whole numbers: -0 and 0 are equal
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t order) {
+  return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+// by value, then by the lower index; 0 is below every element
+__device__ __forceinline__ uint64_t key_of(float x, int a) {
+  return (uint64_t)order_of(x) << 32 | (uint32_t)~a;
+}
+
+struct Row {
+  float top, log_sum, entropy;
+};
+
+__device__ __forceinline__ Row finish_row(float top, float s, float t) {
+  Row r;
+  r.top = top;
+  r.log_sum = logf(s);
+  r.entropy = s == 0.0f ? 0.0f : r.log_sum - kLn2 * t / s;
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_row(const Params &p, int64_t row, const Row &r) {
+  const int a = p.action[row];
+  float lp = 0.0f;
+  if (a >= 0 && a < p.actions) {
+    const float x = to_f(static_cast<const T *>(p.logits)[row * p.stride + a]);
+    const bool keep = (!p.legal || p.legal[row * p.actions + a]) && x != -INFINITY;
+    lp = keep ? (x - r.top) * p.inverse - r.log_sum : -INFINITY;
+  }
+  p.log_prob[row] = lp;
+  p.entropy[row] = r.entropy;
+  p.max_logit[row] = r.top;
+  p.log_sum[row] = r.log_sum;
+}
+
+__device__ __forceinline__ void write_top(const Params &p, int64_t row, const Row &r, int rank, float x, int a) {
+  p.top_action[row * p.top + rank] = a;
+  p.top_log_prob[row * p.top + rank] = a < 0 ? -INFINITY : (x - r.top) * p.inverse - r.log_sum;
+}
+
+// ---------------------------------------------------------------------------
+// short rows: p.group lanes each, V vectors of W elements a lane
+// ---------------------------------------------------------------------------
+
+template <typename T, int W, int V>
+__device__ __forceinline__ void load_short(const Params &p, int64_t row, int lane, bool live, float (&x)[V * W]) {
+  const T *logits = static_cast<const T *>(p.logits) + row * p.stride;
+  const uint8_t *legal = p.legal ? p.legal + row * p.actions : nullptr;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int a = (v * p.group + lane) * W;
+    if (live && a < p.actions) {
+      const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(logits + a);
+      Vec<uint8_t, W> keep;
+      if (legal) keep = *reinterpret_cast<const Vec<uint8_t, W> *>(legal + a);
+#pragma unroll
+      for (int w = 0; w < W; ++w) x[v * W + w] = !legal || keep.v[w] ? to_f(q.v[w]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int w = 0; w < W; ++w) x[v * W + w] = -INFINITY;
+    }
+  }
+}
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kThreads) short_kernel(const __grid_constant__ Params p) {
+  constexpr int E = V * W;
+  const int group = p.group, lane = threadIdx.x & (group - 1);
+  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / group;
+  const bool live = row < p.rows;
+  float x[E];
+  load_short<T, W, V>(p, row, lane, live, x);
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < E; ++j) top = fmaxf(top, x[j]);
+  for (int off = group >> 1; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float s = 0.0f, t = 0.0f;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const float u = exponent_of(x[j], base, p.scale), e = exp2_fast(u);
+    s += e;
+    t = fmaf(e, u, t);
+  }
+  for (int off = group >> 1; off; off >>= 1) {
+    s += __shfl_xor_sync(kFull, s, off);
+    t += __shfl_xor_sync(kFull, t, off);
+  }
+  const Row r = finish_row(top, s, t);
+  if (live && lane == 0) write_row<T>(p, row, r);
+  if (!p.top) return;
+  // a lane's best: the first of its largest, since its indices ascend
+  int removed = -1;
+  for (int rank = 0; rank < p.top; ++rank) {
+    float best = -INFINITY;
+    int at = -1;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      if (j == removed) x[j] = -INFINITY;
+      if (x[j] > best) {
+        best = x[j];
+        at = j;
+      }
+    }
+    int a = at < 0 ? 0x7fffffff : ((at / W) * group + lane) * W + at % W;
+    const int mine = a;
+    for (int off = group >> 1; off; off >>= 1) {
+      const float other = __shfl_xor_sync(kFull, best, off);
+      const int oa = __shfl_xor_sync(kFull, a, off);
+      if (other > best || (other == best && oa < a)) {
+        best = other;
+        a = oa;
+      }
+    }
+    removed = a == mine ? at : -1;
+    if (live && lane == 0) write_top(p, row, r, rank, best, a == 0x7fffffff ? -1 : a);
+  }
+}
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kThreads) short_gradient_kernel(const __grid_constant__ Params p) {
+  const int group = p.group, lane = threadIdx.x & (group - 1);
+  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / group;
+  if (row >= p.rows) return;
+  float x[V * W];
+  load_short<T, W, V>(p, row, lane, true, x);
+  const float top = p.max_logit[row], base = top == -INFINITY ? 0.0f : top;
+  const float log_sum = p.log_sum[row] * kLog2E;
+  const int a = p.action[row];
+  float g = 0.0f;
+  const bool inside = a >= 0 && a < p.actions;
+  if (p.grad_log_prob && inside && (!p.legal || p.legal[row * p.actions + a]) &&
+      to_f(static_cast<const T *>(p.logits)[row * p.stride + a]) != -INFINITY)
+    g = p.grad_log_prob[row] * p.inverse;
+  const float h = p.grad_entropy ? p.grad_entropy[row] * p.inverse : 0.0f;
+  const float offset = g + (h == 0.0f ? 0.0f : h * p.entropy[row]), slope = h * kLn2;
+  T *grad = static_cast<T *>(p.grad) + row * p.actions;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int first = (v * group + lane) * W;
+    if (first >= p.actions) continue;
+    Vec<T, W> out;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float u = max_nan((x[v * W + w] - base) * p.scale - log_sum, kNothing);
+      float d = -exp2_fast(u) * fmaf(slope, u, offset);
+      if (first + w == a) d += g;
+      out.v[w] = from_f<T>(x[v * W + w] == -INFINITY ? 0.0f : d);
+    }
+    *reinterpret_cast<Vec<T, W> *>(grad + first) = out;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// long rows: a cluster each
+// ---------------------------------------------------------------------------
+
+// A row's elements by thread: vectors of W from the first 16-byte boundary
+// on, the head and the tail one by one, thread after thread across the
+// cluster.
+template <typename T, int W, typename F>
+__device__ __forceinline__ void each(const T *x, const uint8_t *legal, int actions, int index, int threads,
+                                     const F &f) {
+  const int head = min(actions, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+  const int vectors = (actions - head) / W, tail = head + vectors * W;
+  auto one = [&](int a) {
+    float v[1] = {!legal || legal[a] ? to_f(x[a]) : -INFINITY};
+    f(v, a);
+  };
+  // the head's and tail's elements go to the last threads, which may have a vector less
+  const int back = threads - 1 - index;
+  if (back < head) one(back);
+  if (back < actions - tail) one(tail + back);
+  constexpr int U = 4;
+  int v = index;
+  for (; v + (U - 1) * threads < vectors; v += U * threads) {
+    Vec<T, W> q[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) q[k] = *reinterpret_cast<const Vec<T, W> *>(x + head + (v + k * threads) * W);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int a = head + (v + k * threads) * W;
+      float y[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) y[w] = !legal || legal[a + w] ? to_f(q[k].v[w]) : -INFINITY;
+      f(y, a);
+    }
+  }
+  for (; v < vectors; v += threads) {
+    const int a = head + v * W;
+    const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(x + a);
+    float y[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) y[w] = !legal || legal[a + w] ? to_f(q.v[w]) : -INFINITY;
+    f(y, a);
+  }
+}
+
+struct Shared {
+  float maxima[kMaxGroups];
+  float2 sums[kMaxCluster * kWarps];
+  uint64_t keys[kCandidates];
+  int count;
+  float limit;
+  uint64_t best[kWarps];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) long_kernel(const __grid_constant__ Params p) {
+  constexpr int W = 16 / sizeof(T);
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int64_t row = blockIdx.x / ctas;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T *x = static_cast<const T *>(p.logits) + row * p.stride;
+  const uint8_t *legal = p.legal ? p.legal + row * p.actions : nullptr;
+  const int index = rank * kThreads + threadIdx.x, threads = ctas * kThreads;
+  if (threadIdx.x == 0) sh.count = 0;
+  // the cluster's CTAs have begun, and counts are set, before the first write into another's memory
+  if (ctas > 1) cluster.barrier_arrive();
+
+  float top = -INFINITY, s = 0.0f, t = 0.0f;
+  each<T, W>(x, legal, p.actions, index, threads, [&](auto &y, int) {
+    constexpr int N = sizeof(y) / sizeof(float);
+    float most = y[0];
+#pragma unroll
+    for (int w = 1; w < N; ++w) most = fmaxf(most, y[w]);
+    if (most > top) {
+      if (s != 0.0f) {
+        const float d = (top - most) * p.scale, f = exp2_fast(d);
+        t = f == 0.0f ? 0.0f : f * fmaf(d, s, t);
+        s *= f;
+      }
+      top = most;
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < N; ++w) {
+      const float u = exponent_of(y[w], base, p.scale), e = exp2_fast(u);
+      s += e;
+      t = fmaf(e, u, t);
+    }
+  });
+
+  // groups' maxima, to every CTA
+  const int width = ctas >= 8 ? 32 : 4 * ctas;  // threads of a group
+  const int per_cta = kThreads / width, groups = per_cta * ctas;
+  float most = top;
+  for (int off = width >> 1; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, off));
+  if (ctas > 1) cluster.barrier_wait();
+  if ((threadIdx.x & (width - 1)) == 0) {
+    const int g = rank * per_cta + threadIdx.x / width;
+    if (ctas == 1)
+      sh.maxima[g] = most;
+    else
+      for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&sh, c)->maxima[g] = most;
+  }
+  if (ctas == 1)
+    __syncthreads();
+  else
+    cluster.sync();
+  float largest = -INFINITY;
+  for (int g = lane; g < groups; g += 32) largest = fmaxf(largest, sh.maxima[g]);
+#pragma unroll
+  for (int off = 16; off; off >>= 1) largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, off));
+
+  Shared *home = ctas == 1 ? &sh : cluster.map_shared_rank(&sh, 0);
+  if (p.top) {
+    // the top-th largest of the maxima, equal ones by their place
+    if (threadIdx.x < groups) {
+      const float mine = sh.maxima[threadIdx.x];
+      int above = 0;
+      for (int g = 0; g < groups; ++g) {
+        const float other = sh.maxima[g];
+        above += other > mine || (other == mine && g < (int)threadIdx.x);
+      }
+      if (above == p.top - 1) sh.limit = mine;
+    }
+    __syncthreads();
+    const float limit = sh.limit;
+    if (top >= limit && top > -INFINITY)
+      each<T, W>(x, legal, p.actions, index, threads, [&](auto &y, int a) {
+        constexpr int N = sizeof(y) / sizeof(float);
+#pragma unroll
+        for (int w = 0; w < N; ++w)
+          if (y[w] >= limit && y[w] > -INFINITY) {
+            const int at = atomicAdd(&home->count, 1);
+            if (at < kCandidates) home->keys[at] = key_of(y[w], a + w);
+          }
+      });
+  }
+  // sums relative to the row's maximum, warp by warp
+  if (s != 0.0f) {
+    const float d = (top - largest) * p.scale, f = exp2_fast(d);
+    t = f == 0.0f ? 0.0f : f * fmaf(d, s, t);
+    s *= f;
+  }
+#pragma unroll
+  for (int off = 16; off; off >>= 1) {
+    s += __shfl_xor_sync(kFull, s, off);
+    t += __shfl_xor_sync(kFull, t, off);
+  }
+  if (lane == 0) home->sums[rank * kWarps + warp] = make_float2(s, t);
+  if (ctas == 1)
+    __syncthreads();
+  else
+    cluster.sync();
+  if (rank) return;
+
+  s = t = 0.0f;
+  for (int i = lane; i < ctas * kWarps; i += 32) {
+    s += sh.sums[i].x;
+    t += sh.sums[i].y;
+  }
+#pragma unroll
+  for (int off = 16; off; off >>= 1) {
+    s += __shfl_xor_sync(kFull, s, off);
+    t += __shfl_xor_sync(kFull, t, off);
+  }
+  const Row r = finish_row(largest, s, t);
+  if (threadIdx.x == 0) write_row<T>(p, row, r);
+  if (!p.top) return;
+  const int count = sh.count;
+  if (count <= kCandidates) {
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+      const uint64_t mine = sh.keys[i];
+      int above = 0;
+      for (int j = 0; j < count; ++j) above += sh.keys[j] > mine;
+      if (above < p.top) write_top(p, row, r, above, logit_of((uint32_t)(mine >> 32)), (int)~(uint32_t)mine);
+    }
+    for (int i = count + threadIdx.x; i < p.top; i += kThreads) write_top(p, row, r, i, 0.0f, -1);
+    return;
+  }
+  uint64_t last = ~0ull;
+  for (int i = 0; i < p.top; ++i) {
+    uint64_t best = 0;
+    for (int a = threadIdx.x; a < p.actions; a += kThreads) {
+      const float v = to_f(x[a]);
+      if ((legal && !legal[a]) || !(v > -INFINITY)) continue;
+      const uint64_t key = key_of(v, a);
+      if (key < last && key > best) best = key;
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) best = max(best, __shfl_xor_sync(kFull, best, off));
+    if (lane == 0) sh.best[warp] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) best = max(best, sh.best[w]);
+    __syncthreads();
+    last = best;
+    if (threadIdx.x == 0) write_top(p, row, r, i, logit_of((uint32_t)(best >> 32)), (int)~(uint32_t)best);
+  }
+}
+
+// A long row's gradient: elements alone, so a CTA takes a piece of a row.
+constexpr int kPiece = 8192;
+template <typename T, bool Vector>
+__global__ void __launch_bounds__(kThreads) long_gradient_kernel(const __grid_constant__ Params p, int pieces) {
+  constexpr int W = Vector ? 16 / sizeof(T) : 1;
+  const int64_t row = blockIdx.x / pieces;
+  const int piece = blockIdx.x - (int)(row * pieces);
+  const T *x = static_cast<const T *>(p.logits) + row * p.stride;
+  const uint8_t *legal = p.legal ? p.legal + row * p.actions : nullptr;
+  T *grad = static_cast<T *>(p.grad) + row * p.actions;
+  const float top = p.max_logit[row], base = top == -INFINITY ? 0.0f : top;
+  const float log_sum = p.log_sum[row] * kLog2E;
+  const int a = p.action[row];
+  float g = 0.0f;
+  if (p.grad_log_prob && a >= 0 && a < p.actions && (!legal || legal[a]) && to_f(x[a]) != -INFINITY)
+    g = p.grad_log_prob[row] * p.inverse;
+  const float h = p.grad_entropy ? p.grad_entropy[row] * p.inverse : 0.0f;
+  const float offset = g + (h == 0.0f ? 0.0f : h * p.entropy[row]), slope = h * kLn2;
+  auto one = [&](float v, int i) {
+    const float u = max_nan((v - base) * p.scale - log_sum, kNothing);
+    float d = -exp2_fast(u) * fmaf(slope, u, offset);
+    if (i == a) d += g;
+    return v == -INFINITY ? 0.0f : d;
+  };
+  auto scalar = [&](int i) { grad[i] = from_f<T>(one(!legal || legal[i] ? to_f(x[i]) : -INFINITY, i)); };
+  const int head = Vector ? min(p.actions, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T)) : 0;
+  const int begin = head + piece * kPiece, whole = (p.actions - head) / W * W + head;
+  const int end = min(whole, begin + kPiece);
+  if (piece == 0 && (int)threadIdx.x < head) scalar(threadIdx.x);
+  if (piece == pieces - 1 && whole + (int)threadIdx.x < p.actions) scalar(whole + threadIdx.x);
+#pragma unroll 4
+  for (int i = begin + (int)threadIdx.x * W; i < end; i += kThreads * W) {
+    const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(x + i);
+    Vec<T, W> out;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      out.v[w] = from_f<T>(one(!legal || legal[i + w] ? to_f(q.v[w]) : -INFINITY, i + w));
+    *reinterpret_cast<Vec<T, W> *>(grad + i) = out;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+bool misaligned(const void *q, size_t a) { return (reinterpret_cast<uintptr_t>(q) & (a - 1)) != 0; }
+
+cudaError_t launched() {
+  g_log_probs_launches.fetch_add(1, std::memory_order_relaxed);
+  return cudaGetLastError();
+}
+
+template <typename T, int W, int V>
+cudaError_t launch_short(const Params &p, bool gradient, cudaStream_t st) {
+  const int64_t ctas = (p.rows * p.group + kThreads - 1) / kThreads;
+  if (gradient)
+    short_gradient_kernel<T, W, V><<<(unsigned)ctas, kThreads, 0, st>>>(p);
+  else
+    short_kernel<T, W, V><<<(unsigned)ctas, kThreads, 0, st>>>(p);
+  return launched();
+}
+
+// The fewest lanes that hold a row with 12 elements each, or 16 of a whole warp
+template <typename T, int W>
+cudaError_t short_rows(Params &p, bool gradient, cudaStream_t st) {
+  const int vectors = (p.actions + W - 1) / W;
+  p.group = 1;
+  while (p.group < 32 && (vectors + p.group - 1) / p.group * W > 12) p.group *= 2;
+  const int v = (vectors + p.group - 1) / p.group;
+  if (v * W <= 4) return launch_short<T, W, 4 / W>(p, gradient, st);
+  if (v * W <= 8) return launch_short<T, W, 8 / W>(p, gradient, st);
+  if (v * W <= 12) return launch_short<T, W, 12 / W>(p, gradient, st);
+  return launch_short<T, W, 16 / W>(p, gradient, st);
+}
+
+template <typename T>
+cudaError_t run(Params &p, bool gradient, int sms, cudaStream_t st) {
+  if (p.actions <= kMaxShort) {
+    // the widest loads that rows' places allow
+    auto fits = [&](int w) {
+      const uintptr_t all = reinterpret_cast<uintptr_t>(p.logits) | (uintptr_t)p.stride * sizeof(T) |
+                            reinterpret_cast<uintptr_t>(p.grad) | (uintptr_t)p.actions * sizeof(T);
+      return all % (w * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.legal) % w == 0;
+    };
+    if (fits(4)) return short_rows<T, 4>(p, gradient, st);
+    if (fits(2)) return short_rows<T, 2>(p, gradient, st);
+    return short_rows<T, 1>(p, gradient, st);
+  }
+  if (gradient) {
+    const int pieces = (p.actions + kPiece - 1) / kPiece;
+    if (p.rows * pieces > 0x7fffffff) return cudaErrorInvalidValue;
+    // vectors where a row and its gradient lie alike
+    const bool vector = !(((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad)) & 15) ||
+                          (p.rows > 1 && ((p.stride - p.actions) * sizeof(T) & 15)));
+    if (vector)
+      long_gradient_kernel<T, true><<<(unsigned)(p.rows * pieces), kThreads, 0, st>>>(p, pieces);
+    else
+      long_gradient_kernel<T, false><<<(unsigned)(p.rows * pieces), kThreads, 0, st>>>(p, pieces);
+    return launched();
+  }
+  // a cluster of CTAs while rows leave SMs without work and pieces keep four vectors a thread
+  int ctas = 1;
+  while (ctas < kMaxCluster && p.rows * ctas * 2 <= 2 * sms && p.actions / (ctas * 2) >= 4096) ctas *= 2;
+  if (p.rows * ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  if (ctas > 8) {
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(allowed.load(std::memory_order_acquire) & bit)) {
+      cudaError_t e = cudaFuncSetAttribute(long_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      allowed.fetch_or(bit, std::memory_order_release);
+    }
+  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.rows * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, long_kernel<T>, p);
+  if (e != cudaSuccess) return e;
+  return launched();
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  return n;
+}
+
+int dispatch(Params &p, int32_t dtype, bool gradient, void *stream) {
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count();
+  const cudaError_t e = dtype == 0   ? run<float>(p, gradient, sms, st)
+                        : dtype == 1 ? run<__nv_bfloat16>(p, gradient, sms, st)
+                                     : run<__half>(p, gradient, sms, st);
+  return e == cudaSuccess ? SCACCHI_OK : e == cudaErrorInvalidValue ? SCACCHI_EINVAL : SCACCHI_ECUDA;
+}
+
+bool rows_ok(const scacchi_log_prob_rows *r, int64_t num_rows, int32_t num_actions, int32_t dtype, double temperature) {
+  if (!r || num_rows < 0 || num_actions < 1 || num_actions > kMaxActions || dtype < 0 || dtype > 2 ||
+      !(temperature >= 1e-3 && temperature <= 1e3))
+    return false;
+  if (num_rows == 0) return true;
+  return num_rows <= (int64_t)1 << 31 && r->logits && r->action && r->stride >= num_actions &&
+         !misaligned(r->logits, dtype == 0 ? 4 : 2) && !misaligned(r->action, 4);
+}
+
+}  // namespace
+
+extern "C" {
+
+int scacchi_log_probs(const scacchi_log_prob_rows *rows, const scacchi_log_prob_out *out, int64_t num_rows,
+                      int32_t num_actions, int32_t dtype, double temperature, int32_t top, void *stream) {
+  if (!rows_ok(rows, num_rows, num_actions, dtype, temperature) || !out || top < 0 || top > kMaxTop)
+    return SCACCHI_EINVAL;
+  if (num_rows == 0) return SCACCHI_OK;
+  for (const void *q : {(const void *)out->log_prob, (const void *)out->entropy, (const void *)out->max_logit,
+                        (const void *)out->log_sum})
+    if (!q || misaligned(q, 4)) return SCACCHI_EINVAL;
+  if (top && (!out->top_log_prob || !out->top_action || misaligned(out->top_log_prob, 4) ||
+              misaligned(out->top_action, 4)))
+    return SCACCHI_EINVAL;
+  Params p = {};
+  p.logits = rows->logits;
+  p.legal = rows->legal;
+  p.action = rows->action;
+  p.log_prob = out->log_prob;
+  p.entropy = out->entropy;
+  p.max_logit = out->max_logit;
+  p.log_sum = out->log_sum;
+  p.top_log_prob = out->top_log_prob;
+  p.top_action = out->top_action;
+  p.rows = num_rows;
+  p.stride = rows->stride;
+  p.actions = num_actions;
+  p.top = top;
+  p.scale = (float)(1.44269504088896340736 / temperature);
+  p.inverse = (float)(1.0 / temperature);
+  return dispatch(p, dtype, false, stream);
+}
+
+int scacchi_log_probs_gradient(const scacchi_log_prob_rows *rows, const float *max_logit, const float *log_sum,
+                               const float *entropy, const float *grad_log_prob, const float *grad_entropy,
+                               int64_t num_rows, int32_t num_actions, int32_t dtype, double temperature,
+                               void *grad_logits, void *stream) {
+  if (!rows_ok(rows, num_rows, num_actions, dtype, temperature)) return SCACCHI_EINVAL;
+  if (num_rows == 0) return SCACCHI_OK;
+  if (!max_logit || !log_sum || !grad_logits || (grad_entropy && !entropy) || misaligned(max_logit, 4) ||
+      misaligned(log_sum, 4) || misaligned(entropy, 4) || misaligned(grad_log_prob, 4) ||
+      misaligned(grad_entropy, 4) || misaligned(grad_logits, dtype == 0 ? 4 : 2))
+    return SCACCHI_EINVAL;
+  Params p = {};
+  p.logits = rows->logits;
+  p.legal = rows->legal;
+  p.action = rows->action;
+  p.max_logit = const_cast<float *>(max_logit);
+  p.log_sum = const_cast<float *>(log_sum);
+  p.entropy = const_cast<float *>(entropy);
+  p.grad_log_prob = grad_log_prob;
+  p.grad_entropy = grad_entropy;
+  p.grad = grad_logits;
+  p.rows = num_rows;
+  p.stride = rows->stride;
+  p.actions = num_actions;
+  p.scale = (float)(1.44269504088896340736 / temperature);
+  p.inverse = (float)(1.0 / temperature);
+  return dispatch(p, dtype, true, stream);
+}
+
+uint64_t scacchi_log_probs_launch_count(void) { return g_log_probs_launches.load(std::memory_order_relaxed); }
+
+}  // extern "C"
