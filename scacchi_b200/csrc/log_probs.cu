@@ -268,160 +268,289 @@ __global__ void __launch_bounds__(kThreads) short_gradient_kernel(const __grid_c
 // long rows: a cluster each
 // ---------------------------------------------------------------------------
 
-// A row's elements by thread: vectors of W from the first 16-byte boundary
-// on, the head and the tail one by one, thread after thread across the
-// cluster.
-template <typename T, int W, typename F>
-__device__ __forceinline__ void each(const T *x, const uint8_t *legal, int actions, int index, int threads,
-                                     const F &f) {
-  const int head = min(actions, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-  const int vectors = (actions - head) / W, tail = head + vectors * W;
-  auto one = [&](int a) {
-    float v[1] = {!legal || legal[a] ? to_f(x[a]) : -INFINITY};
-    f(v, a);
-  };
-  // the head's and tail's elements go to the last threads, which may have a vector less
-  const int back = threads - 1 - index;
-  if (back < head) one(back);
-  if (back < actions - tail) one(tail + back);
-  constexpr int U = 4;
-  int v = index;
-  for (; v + (U - 1) * threads < vectors; v += U * threads) {
-    Vec<T, W> q[U];
+// A chunk of kVectors vectors a thread: their loads are in flight together,
+// and one comparison decides whether its sums change their base.
+constexpr int kVectors = 4;
+// What is below kFloor counts as -inf in a row whose maximum is above kLow: 2^((kFloor -
+// kLow) scale) is 0 at every temperature.
+constexpr float kFloor = -0x1p100f, kLow = -0x1p99f;
+
+template <typename T>
+__device__ __forceinline__ T minus_infinity() {
+  return from_f<T>(-INFINITY);
+}
+
+// A row's elements as the threads of its cluster take them: vectors from the
+// first 16-byte boundary on, thread after thread, and the head's and the
+// tail's elements one by one by the last threads, which may have a vector less.
+template <typename T>
+struct Slice {
+  static constexpr int W = 16 / sizeof(T);
+  const T *x;
+  const uint8_t *legal;
+  int actions, head, vectors, index, threads;
+
+  __device__ Slice(const Params &p, int64_t row, int index, int threads) : index(index), threads(threads) {
+    x = static_cast<const T *>(p.logits) + row * p.stride;
+    legal = p.legal ? p.legal + row * p.actions : nullptr;
+    actions = p.actions;
+    head = min(actions, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+    vectors = (actions - head) / W;
+  }
+  // the thread's odd element, or -1
+  __device__ int odd() const {
+    const int back = threads - 1 - index, tail = head + vectors * W;
+    return back < head ? back : back - head < actions - tail ? tail + back - head : -1;
+  }
+  __device__ int first(int v) const { return head + v * W; }
+  // chunk `v`'s vectors v, v + threads, ..., -inf where there is none or where the mask says so
+  __device__ void load(int v, Vec<T, W> (&q)[kVectors]) const {
 #pragma unroll
-    for (int k = 0; k < U; ++k) q[k] = *reinterpret_cast<const Vec<T, W> *>(x + head + (v + k * threads) * W);
+    for (int k = 0; k < kVectors; ++k) {
+      if (v + k * threads < vectors) {
+        q[k] = *reinterpret_cast<const Vec<T, W> *>(x + first(v + k * threads));
+      } else {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int a = head + (v + k * threads) * W;
-      float y[W];
+        for (int w = 0; w < W; ++w) q[k].v[w] = minus_infinity<T>();
+      }
+    }
+    if (legal) {
 #pragma unroll
-      for (int w = 0; w < W; ++w) y[w] = !legal || legal[a + w] ? to_f(q[k].v[w]) : -INFINITY;
-      f(y, a);
+      for (int k = 0; k < kVectors; ++k)
+        if (v + k * threads < vectors) mask(first(v + k * threads), q[k]);
     }
   }
-  for (; v < vectors; v += threads) {
-    const int a = head + v * W;
-    const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(x + a);
-    float y[W];
+  // the mask's bytes one by one, or four at a time where they lie so
+  __device__ void mask(int a, Vec<T, W> &q) const {
+    const uint8_t *m = legal + a;
+    uint32_t bits = 0;
+    if ((reinterpret_cast<uintptr_t>(m) & 3) == 0) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) y[w] = !legal || legal[a + w] ? to_f(q.v[w]) : -INFINITY;
-    f(y, a);
+      for (int w = 0; w < W; w += 4) {
+        const uint32_t four = *reinterpret_cast<const uint32_t *>(m + w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bits |= (four >> (8 * i) & 0xffu ? 1u : 0u) << (w + i);
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < W; ++w) bits |= (m[w] ? 1u : 0u) << w;
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      if (!(bits >> w & 1)) q.v[w] = minus_infinity<T>();
+  }
+  // -inf where the element is not kept
+  __device__ float element(int a) const { return !legal || legal[a] ? to_f(x[a]) : -INFINITY; }
+};
+
+// A chunk's elements in 32 bits, what is below kFloor raised to it, NaN kept
+template <typename T, int W>
+__device__ __forceinline__ void unpack(const Vec<T, W> (&q)[kVectors], float (&y)[W * kVectors]) {
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+      for (int w = 0; w < W; w += 2) {
+        const __nv_bfloat162 two = __hmax2_nan(__halves2bfloat162(q[k].v[w], q[k].v[w + 1]),
+                                               __float2bfloat162_rn(kFloor));
+        const uint32_t u = *reinterpret_cast<const uint32_t *>(&two);
+        y[k * W + w] = __uint_as_float(u << 16);
+        y[k * W + w + 1] = __uint_as_float(u & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < W; ++w) y[k * W + w] = max_nan(to_f(q[k].v[w]), kFloor);
+    }
   }
 }
 
+// Sums of a thread or of more: s = sum 2^v, t = sum v 2^v, v = (x - top) scale
+struct Sums {
+  float top, s, t;
+};
+__device__ __forceinline__ void rebase(Sums &a, float top, float scale) {
+  if (a.s != 0.0f) {
+    const float d = (a.top - top) * scale, f = exp2_fast(d);
+    a.t = f == 0.0f ? 0.0f : f * fmaf(d, a.s, a.t);
+    a.s *= f;
+  }
+  a.top = top;
+}
+
+template <int N>
+__device__ __forceinline__ void add_chunk(const float (&y)[N], float scale, Sums &a) {
+  float most = y[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) most = fmaxf(most, y[i]);
+  if (most > a.top) rebase(a, most, scale);
+  const float2 scale2 = make_float2(scale, scale), top2 = make_float2(-a.top, -a.top);
+  float2 s = make_float2(0.0f, 0.0f), t = s;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 v = __fmul2_rn(__fadd2_rn(make_float2(y[i], y[i + 1]), top2), scale2);
+    const float2 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+    s = __fadd2_rn(s, e);
+    t = __ffma2_rn(e, v, t);
+  }
+  a.s += s.x + s.y;
+  a.t += t.x + t.y;
+}
+
 struct Shared {
-  float maxima[kMaxGroups];
+  float4 maxima[kMaxGroups / 4];
   float2 sums[kMaxCluster * kWarps];
   uint64_t keys[kCandidates];
-  int count;
+  uint16_t reach[kThreads];
+  int count, reaching;
   float limit;
   uint64_t best[kWarps];
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) long_kernel(const __grid_constant__ Params p) {
-  constexpr int W = 16 / sizeof(T);
-  __shared__ Shared sh;
+// The groups' maxima to every CTA of the cluster; returns the row's
+__device__ __forceinline__ float exchange(Shared &sh, float top, int ctas, int rank, int groups) {
   cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
-  const int64_t row = blockIdx.x / ctas;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T *x = static_cast<const T *>(p.logits) + row * p.stride;
-  const uint8_t *legal = p.legal ? p.legal + row * p.actions : nullptr;
-  const int index = rank * kThreads + threadIdx.x, threads = ctas * kThreads;
-  if (threadIdx.x == 0) sh.count = 0;
-  // the cluster's CTAs have begun, and counts are set, before the first write into another's memory
-  if (ctas > 1) cluster.barrier_arrive();
-
-  float top = -INFINITY, s = 0.0f, t = 0.0f;
-  each<T, W>(x, legal, p.actions, index, threads, [&](auto &y, int) {
-    constexpr int N = sizeof(y) / sizeof(float);
-    float most = y[0];
-#pragma unroll
-    for (int w = 1; w < N; ++w) most = fmaxf(most, y[w]);
-    if (most > top) {
-      if (s != 0.0f) {
-        const float d = (top - most) * p.scale, f = exp2_fast(d);
-        t = f == 0.0f ? 0.0f : f * fmaf(d, s, t);
-        s *= f;
-      }
-      top = most;
-    }
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < N; ++w) {
-      const float u = exponent_of(y[w], base, p.scale), e = exp2_fast(u);
-      s += e;
-      t = fmaf(e, u, t);
-    }
-  });
-
-  // groups' maxima, to every CTA
-  const int width = ctas >= 8 ? 32 : 4 * ctas;  // threads of a group
-  const int per_cta = kThreads / width, groups = per_cta * ctas;
-  float most = top;
-  for (int off = width >> 1; off; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, off));
-  if (ctas > 1) cluster.barrier_wait();
+  const int width = ctas >= 8 ? 32 : 4 * ctas, per_cta = kThreads / width;  // threads of a group
+  for (int off = width >> 1; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
   if ((threadIdx.x & (width - 1)) == 0) {
     const int g = rank * per_cta + threadIdx.x / width;
     if (ctas == 1)
-      sh.maxima[g] = most;
+      reinterpret_cast<float *>(sh.maxima)[g] = top;
     else
-      for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&sh, c)->maxima[g] = most;
+      for (int c = 0; c < ctas; ++c) reinterpret_cast<float *>(cluster.map_shared_rank(&sh, c)->maxima)[g] = top;
   }
   if (ctas == 1)
     __syncthreads();
   else
     cluster.sync();
   float largest = -INFINITY;
-  for (int g = lane; g < groups; g += 32) largest = fmaxf(largest, sh.maxima[g]);
+  for (int g = threadIdx.x & 31; g < groups / 4; g += 32) {
+    const float4 m = sh.maxima[g];
+    largest = fmaxf(largest, fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)));
+  }
 #pragma unroll
   for (int off = 16; off; off >>= 1) largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, off));
+  return largest;
+}
+
+// The top-th largest of the groups' maxima, equal ones by their place
+__device__ __forceinline__ void find_limit(Shared &sh, int groups, int top) {
+  if ((int)threadIdx.x < groups) {
+    const float mine = reinterpret_cast<const float *>(sh.maxima)[threadIdx.x];
+    int above = 0;
+    for (int g = 0; g < groups / 4; ++g) {
+      const float4 m = sh.maxima[g];
+      const int i = 4 * g - (int)threadIdx.x;
+      above += m.x > mine || (m.x == mine && i < 0);
+      above += m.y > mine || (m.y == mine && i + 1 < 0);
+      above += m.z > mine || (m.z == mine && i + 2 < 0);
+      above += m.w > mine || (m.w == mine && i + 3 < 0);
+    }
+    if (above == top - 1) sh.limit = mine;
+  }
+}
+
+__device__ __forceinline__ void candidate(Shared *home, float v, float limit, int a) {
+  if (v >= limit && v > -INFINITY) {
+    const int at = atomicAdd(&home->count, 1);
+    if (at < kCandidates) home->keys[at] = key_of(v, a);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) long_kernel(const __grid_constant__ Params p) {
+  constexpr int W = Slice<T>::W;
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int64_t row = blockIdx.x / ctas;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Slice<T> slice(p, row, rank * kThreads + threadIdx.x, ctas * kThreads);
+  if (threadIdx.x == 0) sh.count = sh.reaching = 0;
+  // the cluster's CTAs have begun, and counts are set, before the first write into another's memory
+  if (ctas > 1) cluster.barrier_arrive();
+
+  const int odd = slice.odd();
+  Sums a = {-INFINITY, 0.0f, 0.0f};
+  if (odd >= 0) {
+    const float y = max_nan(slice.element(odd), kFloor);
+    a = Sums{y, 1.0f, 0.0f};
+    if (y != y) a = Sums{-INFINITY, y, y};
+  }
+  for (int v = slice.index; v < slice.vectors; v += kVectors * slice.threads) {
+    Vec<T, W> q[kVectors];
+    slice.load(v, q);
+    float y[W * kVectors];
+    unpack<T, W>(q, y);
+    add_chunk(y, p.scale, a);
+  }
+  const int groups = ctas >= 8 ? kWarps * ctas : 64;
+  if (ctas > 1) cluster.barrier_wait();
+  float largest = exchange(sh, a.top, ctas, rank, groups);
+  // a row masked throughout by low values, or with an infinity: element by element, as they are
+  const bool plain = largest >= kLow && largest < INFINITY;
+  if (!plain) {
+    a.top = odd >= 0 ? slice.element(odd) : -INFINITY;
+    for (int v = slice.index; v < slice.vectors; v += slice.threads)
+      for (int w = 0; w < W; ++w) a.top = fmaxf(a.top, slice.element(slice.first(v) + w));
+    if (ctas > 1)
+      cluster.sync();  // before the maxima are written again
+    else
+      __syncthreads();
+    largest = exchange(sh, a.top, ctas, rank, groups);
+    const float base = largest == -INFINITY ? 0.0f : largest;
+    a.s = a.t = 0.0f;
+    auto one = [&](float x) {
+      const float u = exponent_of(x, base, p.scale), e = exp2_fast(u);
+      a.s += e;
+      a.t = fmaf(e, u, a.t);
+    };
+    if (odd >= 0) one(slice.element(odd));
+    for (int v = slice.index; v < slice.vectors; v += slice.threads)
+      for (int w = 0; w < W; ++w) one(slice.element(slice.first(v) + w));
+  }
+  const float own = a.top;  // the largest of the thread's own elements
+  if (plain) rebase(a, largest, p.scale);
 
   Shared *home = ctas == 1 ? &sh : cluster.map_shared_rank(&sh, 0);
   if (p.top) {
-    // the top-th largest of the maxima, equal ones by their place
-    if (threadIdx.x < groups) {
-      const float mine = sh.maxima[threadIdx.x];
-      int above = 0;
-      for (int g = 0; g < groups; ++g) {
-        const float other = sh.maxima[g];
-        above += other > mine || (other == mine && g < (int)threadIdx.x);
-      }
-      if (above == p.top - 1) sh.limit = mine;
+    find_limit(sh, groups, p.top);
+    __syncthreads();
+    const float limit = plain && sh.limit <= kFloor ? -INFINITY : sh.limit;
+    // the threads that reach the limit, and their vectors over all threads of the CTA
+    if (own >= limit && own > -INFINITY) {
+      sh.reach[atomicAdd(&sh.reaching, 1)] = (uint16_t)threadIdx.x;
+      if (odd >= 0) candidate(home, slice.element(odd), limit, odd);
     }
     __syncthreads();
-    const float limit = sh.limit;
-    if (top >= limit && top > -INFINITY)
-      each<T, W>(x, legal, p.actions, index, threads, [&](auto &y, int a) {
-        constexpr int N = sizeof(y) / sizeof(float);
+    const int each = (slice.vectors + slice.threads - 1) / slice.threads, items = sh.reaching * each;
+    for (int i = threadIdx.x; i < items; i += kThreads) {
+      const int n = i / each, v = rank * kThreads + sh.reach[n] + (i - n * each) * slice.threads;
+      if (v >= slice.vectors) continue;
+      const int first = slice.first(v);
+      Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(slice.x + first);
+      if (slice.legal) slice.mask(first, q);
+      uint32_t high = 0;
 #pragma unroll
-        for (int w = 0; w < N; ++w)
-          if (y[w] >= limit && y[w] > -INFINITY) {
-            const int at = atomicAdd(&home->count, 1);
-            if (at < kCandidates) home->keys[at] = key_of(y[w], a + w);
-          }
-      });
-  }
-  // sums relative to the row's maximum, warp by warp
-  if (s != 0.0f) {
-    const float d = (top - largest) * p.scale, f = exp2_fast(d);
-    t = f == 0.0f ? 0.0f : f * fmaf(d, s, t);
-    s *= f;
+      for (int w = 0; w < W; ++w) high |= (to_f(q.v[w]) >= limit ? 1u : 0u) << w;
+      for (; high; high &= high - 1) {
+        const int w = __ffs(high) - 1;
+        candidate(home, slice.element(first + w), limit, first + w);
+      }
+    }
   }
 #pragma unroll
   for (int off = 16; off; off >>= 1) {
-    s += __shfl_xor_sync(kFull, s, off);
-    t += __shfl_xor_sync(kFull, t, off);
+    a.s += __shfl_xor_sync(kFull, a.s, off);
+    a.t += __shfl_xor_sync(kFull, a.t, off);
   }
-  if (lane == 0) home->sums[rank * kWarps + warp] = make_float2(s, t);
+  if (lane == 0) home->sums[rank * kWarps + warp] = make_float2(a.s, a.t);
   if (ctas == 1)
     __syncthreads();
   else
     cluster.sync();
   if (rank) return;
 
-  s = t = 0.0f;
+  float s = 0.0f, t = 0.0f;
   for (int i = lane; i < ctas * kWarps; i += 32) {
     s += sh.sums[i].x;
     t += sh.sums[i].y;
@@ -448,10 +577,10 @@ __global__ void __launch_bounds__(kThreads) long_kernel(const __grid_constant__ 
   uint64_t last = ~0ull;
   for (int i = 0; i < p.top; ++i) {
     uint64_t best = 0;
-    for (int a = threadIdx.x; a < p.actions; a += kThreads) {
-      const float v = to_f(x[a]);
-      if ((legal && !legal[a]) || !(v > -INFINITY)) continue;
-      const uint64_t key = key_of(v, a);
+    for (int k = threadIdx.x; k < p.actions; k += kThreads) {
+      const float v = slice.element(k);
+      if (!(v > -INFINITY)) continue;
+      const uint64_t key = key_of(v, k);
       if (key < last && key > best) best = key;
     }
 #pragma unroll

@@ -159,16 +159,16 @@ def _step_and_check(opt, weights, grads, *, lr, b1, b2, eps, decay, clip=None, k
         assert torch.equal(out.isfinite(), fin)
         x, tol, out = x[fin], tol[fin], out[fin]
         if tensor.dtype == torch.float32:
-            assert not bool(((out - x).abs() > tol).any()), float(((out - x).abs() / tol).max())
+            assert bool(((out - x).abs() <= tol).all()), float(((out - x).abs() / tol).max())
         elif key is None:
-            assert not bool(((out - x).abs() > tol + x.abs() * 2.0 ** -8 + 2.0 ** -134).any())
+            assert bool(((out - x).abs() <= tol + x.abs() * 2.0 ** -8 + 2.0 ** -134).all())
         else:
             r = (part(random) * 0x85eb & 0xffff)[fin]
             q = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -126))) - 7)
             assert _between((out * x.sign()).clamp(min=0), x.abs(), tol, q, r.double() / 65536)
     if opt.state_bits == 32:
-        assert not bool(((opt.first.double() - m).abs() > m_tol)[mask].any())
-        assert not bool(((opt.second.double() - v).abs() > v_tol * v + 2.0 ** -148)[mask].any())
+        assert bool(((opt.first.double() - m).abs() <= m_tol)[mask].all())
+        assert bool(((opt.second.double() - v).abs() <= v_tol * v + 2.0 ** -148)[mask].all())
         assert torch.equal(opt.first[~mask], old[0][~mask]) and torch.equal(opt.second[~mask], old[1][~mask])
         return
     c = opt.first.long()

@@ -85,7 +85,7 @@ def _near(got, want, tol, name):
     assert got.shape == want.shape, name
     fin = want.isfinite()
     assert torch.equal(got[~fin], want[~fin]), name
-    assert not bool(((got - want).abs() > tol)[fin].any()), (name, float(((got - want).abs() - tol)[fin].max()))
+    assert bool(((got - want).abs() <= tol)[fin].all()), (name, float(((got - want).abs() - tol)[fin].max()))
 
 
 def _check_top(out, d, top, T):
