@@ -275,94 +275,159 @@ constexpr int kVectors = 4;
 // kLow) scale) is 0 at every temperature.
 constexpr float kFloor = -0x1p100f, kLow = -0x1p99f;
 
+// 32 bits of -inf
 template <typename T>
-__device__ __forceinline__ T minus_infinity() {
-  return from_f<T>(-INFINITY);
-}
+constexpr uint32_t kMinusInfinity = std::is_same_v<T, float> ? 0xff800000u
+                                    : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
+
+// A chunk as it comes: vectors, and the mask's bytes beside them
+template <typename T, bool Masked>
+struct Raw {
+  uint4 q[kVectors];
+  uint32_t m[Masked ? kVectors : 1][4 / sizeof(T)];
+};
 
 // A row's elements as the threads of its cluster take them: vectors from the
 // first 16-byte boundary on, thread after thread, and the head's and the
 // tail's elements one by one by the last threads, which may have a vector less.
-template <typename T>
+template <typename T, bool Masked>
 struct Slice {
   static constexpr int W = 16 / sizeof(T);
   const T *x;
   const uint8_t *legal;
-  int actions, head, vectors, index, threads;
+  int actions, head, vectors;
 
-  __device__ Slice(const Params &p, int64_t row, int index, int threads) : index(index), threads(threads) {
+  __device__ Slice(const Params &p, int64_t row) {
     x = static_cast<const T *>(p.logits) + row * p.stride;
-    legal = p.legal ? p.legal + row * p.actions : nullptr;
+    legal = Masked ? p.legal + row * p.actions : nullptr;
     actions = p.actions;
     head = min(actions, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
     vectors = (actions - head) / W;
   }
   // the thread's odd element, or -1
-  __device__ int odd() const {
+  __device__ int odd(int index, int threads) const {
     const int back = threads - 1 - index, tail = head + vectors * W;
     return back < head ? back : back - head < actions - tail ? tail + back - head : -1;
   }
   __device__ int first(int v) const { return head + v * W; }
-  // chunk `v`'s vectors v, v + threads, ..., -inf where there is none or where the mask says so
-  __device__ void load(int v, Vec<T, W> (&q)[kVectors]) const {
+  // the mask's bytes of a vector: the words that hold them, shifted, where none of these reaches beyond the mask
+  __device__ void mask(const Params &p, int v, uint32_t (&m)[W / 4]) const {
+    const uint8_t *at = legal + first(v);
+    const int shift = (int)(reinterpret_cast<uintptr_t>(at) & 3);
+    const uint32_t *word = reinterpret_cast<const uint32_t *>(at - shift);
+    if (shift == 0) {
+#pragma unroll
+      for (int w = 0; w < W / 4; ++w) m[w] = word[w];
+    } else if (at - shift >= p.legal && at + W + 4 <= p.legal + p.rows * p.actions) {
+      uint32_t low = word[0];
+#pragma unroll
+      for (int w = 0; w < W / 4; ++w) {
+        const uint32_t high = word[w + 1];
+        m[w] = __funnelshift_r(low, high, 8 * shift);
+        low = high;
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < W; ++w) m[w / 4] = (w & 3 ? m[w / 4] : 0u) | (uint32_t)at[w] << (8 * (w & 3));
+    }
+  }
+  // vectors v, v + threads, ..., -inf where there is none
+  __device__ void load(const Params &p, int v, int threads, Raw<T, Masked> &raw) const {
+    const uint4 *at = reinterpret_cast<const uint4 *>(x + head) + v;
+    const uint32_t none = kMinusInfinity<T>;
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) {
-      if (v + k * threads < vectors) {
-        q[k] = *reinterpret_cast<const Vec<T, W> *>(x + first(v + k * threads));
-      } else {
-#pragma unroll
-        for (int w = 0; w < W; ++w) q[k].v[w] = minus_infinity<T>();
-      }
+      const bool there = v + k * threads < vectors;
+      raw.q[k] = there ? at[k * threads] : make_uint4(none, none, none, none);
+      if constexpr (Masked)
+        if (there) mask(p, v + k * threads, raw.m[k]);
     }
-    if (legal) {
-#pragma unroll
-      for (int k = 0; k < kVectors; ++k)
-        if (v + k * threads < vectors) mask(first(v + k * threads), q[k]);
-    }
-  }
-  // the mask's bytes one by one, or four at a time where they lie so
-  __device__ void mask(int a, Vec<T, W> &q) const {
-    const uint8_t *m = legal + a;
-    uint32_t bits = 0;
-    if ((reinterpret_cast<uintptr_t>(m) & 3) == 0) {
-#pragma unroll
-      for (int w = 0; w < W; w += 4) {
-        const uint32_t four = *reinterpret_cast<const uint32_t *>(m + w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bits |= (four >> (8 * i) & 0xffu ? 1u : 0u) << (w + i);
-      }
-    } else {
-#pragma unroll
-      for (int w = 0; w < W; ++w) bits |= (m[w] ? 1u : 0u) << w;
-    }
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-      if (!(bits >> w & 1)) q.v[w] = minus_infinity<T>();
   }
   // -inf where the element is not kept
-  __device__ float element(int a) const { return !legal || legal[a] ? to_f(x[a]) : -INFINITY; }
+  __device__ float element(int a) const { return !Masked || legal[a] ? to_f(x[a]) : -INFINITY; }
 };
 
-// A chunk's elements in 32 bits, what is below kFloor raised to it, NaN kept
-template <typename T, int W>
-__device__ __forceinline__ void unpack(const Vec<T, W> (&q)[kVectors], float (&y)[W * kVectors]) {
+// -inf where the mask's byte is 0
+template <typename T>
+__device__ __forceinline__ void apply(const uint32_t (&m)[4 / sizeof(T)], uint4 &q) {
+  uint32_t *word = reinterpret_cast<uint32_t *>(&q);
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k) {
-    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-#pragma unroll
-      for (int w = 0; w < W; w += 2) {
-        const __nv_bfloat162 two = __hmax2_nan(__halves2bfloat162(q[k].v[w], q[k].v[w + 1]),
-                                               __float2bfloat162_rn(kFloor));
-        const uint32_t u = *reinterpret_cast<const uint32_t *>(&two);
-        y[k * W + w] = __uint_as_float(u << 16);
-        y[k * W + w + 1] = __uint_as_float(u & 0xffff0000u);
-      }
-    } else {
-#pragma unroll
-      for (int w = 0; w < W; ++w) y[k * W + w] = max_nan(to_f(q[k].v[w]), kFloor);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t keep = sizeof(T) == 4 ? __byte_perm(__vcmpne4(m[0], 0u), 0u, 0x1111 * i)
+                                         : __byte_perm(__vcmpne4(m[sizeof(T) == 4 ? 0 : i / 2], 0u), 0u,
+                                                       i & 1 ? 0x3322 : 0x1100);
+    word[i] = (word[i] & keep) | (kMinusInfinity<T> & ~keep);
   }
 }
+
+// the largest of three, without those that are NaN
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// A pair (bfloat16, float16) or two words (float32) as floats
+template <typename T>
+__device__ __forceinline__ float2 floats(uint32_t u) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+}
+
+// A chunk as pairs of floats, what is below kFloor raised to it, NaN kept.
+// bfloat16 stays packed until a pair is needed, so that raising it and the
+// chunk's maximum take half an instruction an element.
+template <typename T>
+struct Chunk {
+  static constexpr int W = 16 / sizeof(T), N = W * kVectors;
+  float y[N];
+  __device__ explicit Chunk(const uint4 (&q)[kVectors]) {
+    const uint32_t *word = reinterpret_cast<const uint32_t *>(q);
+    if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = max_nan(__uint_as_float(word[i]), kFloor);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 two = floats<T>(word[i]);
+        y[2 * i] = max_nan(two.x, kFloor);
+        y[2 * i + 1] = max_nan(two.y, kFloor);
+      }
+    }
+  }
+  __device__ float2 pair(int i) const { return make_float2(y[2 * i], y[2 * i + 1]); }
+  __device__ float largest() const {
+    float m[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m[c] = fmaxf(y[c], y[c + 4]);
+#pragma unroll
+    for (int i = 8; i < N; i += 8)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) m[c] = max3(m[c], y[i + c], y[i + c + 4]);
+    return max3(m[0], m[1], fmaxf(m[2], m[3]));
+  }
+};
+template <>
+struct Chunk<__nv_bfloat16> {
+  static constexpr int W = 8, N = W * kVectors;
+  __nv_bfloat162 y[N / 2];
+  __device__ explicit Chunk(const uint4 (&q)[kVectors]) {
+    const __nv_bfloat162 floor = __float2bfloat162_rn(kFloor), *two = reinterpret_cast<const __nv_bfloat162 *>(q);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) y[i] = __hmax2_nan(two[i], floor);
+  }
+  __device__ float2 pair(int i) const { return floats<__nv_bfloat16>(*reinterpret_cast<const uint32_t *>(&y[i])); }
+  __device__ float largest() const {
+    __nv_bfloat162 m[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m[c] = __hmax2(y[c], y[c + 4]);
+#pragma unroll
+    for (int i = 8; i < N / 2; ++i) m[i & 3] = __hmax2(m[i & 3], y[i]);
+    const __nv_bfloat162 one = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    return fmaxf(__low2float(one), __high2float(one));
+  }
+};
 
 // Sums of a thread or of more: s = sum 2^v, t = sum v 2^v, v = (x - top) scale
 struct Sums {
@@ -377,23 +442,23 @@ __device__ __forceinline__ void rebase(Sums &a, float top, float scale) {
   a.top = top;
 }
 
-template <int N>
-__device__ __forceinline__ void add_chunk(const float (&y)[N], float scale, Sums &a) {
-  float most = y[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) most = fmaxf(most, y[i]);
+template <typename T>
+__device__ __forceinline__ void add_chunk(const Chunk<T> &y, float scale, Sums &a) {
+  const float most = y.largest();
   if (most > a.top) rebase(a, most, scale);
   const float2 scale2 = make_float2(scale, scale), top2 = make_float2(-a.top, -a.top);
-  float2 s = make_float2(0.0f, 0.0f), t = s;
+  float2 s[2] = {}, t[2] = {};
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float2 v = __fmul2_rn(__fadd2_rn(make_float2(y[i], y[i + 1]), top2), scale2);
+  for (int i = 0; i < Chunk<T>::N / 2; ++i) {
+    const float2 v = __fmul2_rn(__fadd2_rn(y.pair(i), top2), scale2);
     const float2 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
-    s = __fadd2_rn(s, e);
-    t = __ffma2_rn(e, v, t);
+    s[i & 1] = __fadd2_rn(s[i & 1], e);
+    t[i & 1] = __ffma2_rn(e, v, t[i & 1]);
   }
-  a.s += s.x + s.y;
-  a.t += t.x + t.y;
+  s[0] = __fadd2_rn(s[0], s[1]);
+  t[0] = __fadd2_rn(t[0], t[1]);
+  a.s += s[0].x + s[0].y;
+  a.t += t[0].x + t[0].y;
 }
 
 struct Shared {
@@ -401,7 +466,7 @@ struct Shared {
   float2 sums[kMaxCluster * kWarps];
   uint64_t keys[kCandidates];
   uint16_t reach[kThreads];
-  int count, reaching;
+  int count[2], reaching[2];  // of rows in turn
   float limit;
   uint64_t best[kWarps];
 };
@@ -449,107 +514,22 @@ __device__ __forceinline__ void find_limit(Shared &sh, int groups, int top) {
   }
 }
 
-__device__ __forceinline__ void candidate(Shared *home, float v, float limit, int a) {
+__device__ __forceinline__ void candidate(Shared *home, int turn, float v, float limit, int a) {
   if (v >= limit && v > -INFINITY) {
-    const int at = atomicAdd(&home->count, 1);
+    const int at = atomicAdd(&home->count[turn], 1);
     if (at < kCandidates) home->keys[at] = key_of(v, a);
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) long_kernel(const __grid_constant__ Params p) {
-  constexpr int W = Slice<T>::W;
-  __shared__ Shared sh;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
-  const int64_t row = blockIdx.x / ctas;
+// The row's numbers and its best actions, by the first CTA.  What it reads of
+// `sh` is written again after the next row's exchange, where all its threads meet.
+template <typename T, bool Masked>
+__device__ __forceinline__ void finish_long(const Params &p, Shared &sh, const Slice<T, Masked> &slice, int64_t row,
+                                            float largest, int turn, int ctas) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Slice<T> slice(p, row, rank * kThreads + threadIdx.x, ctas * kThreads);
-  if (threadIdx.x == 0) sh.count = sh.reaching = 0;
-  // the cluster's CTAs have begun, and counts are set, before the first write into another's memory
-  if (ctas > 1) cluster.barrier_arrive();
-
-  const int odd = slice.odd();
-  Sums a = {-INFINITY, 0.0f, 0.0f};
-  if (odd >= 0) {
-    const float y = max_nan(slice.element(odd), kFloor);
-    a = Sums{y, 1.0f, 0.0f};
-    if (y != y) a = Sums{-INFINITY, y, y};
-  }
-  for (int v = slice.index; v < slice.vectors; v += kVectors * slice.threads) {
-    Vec<T, W> q[kVectors];
-    slice.load(v, q);
-    float y[W * kVectors];
-    unpack<T, W>(q, y);
-    add_chunk(y, p.scale, a);
-  }
-  const int groups = ctas >= 8 ? kWarps * ctas : 64;
-  if (ctas > 1) cluster.barrier_wait();
-  float largest = exchange(sh, a.top, ctas, rank, groups);
-  // a row masked throughout by low values, or with an infinity: element by element, as they are
-  const bool plain = largest >= kLow && largest < INFINITY;
-  if (!plain) {
-    a.top = odd >= 0 ? slice.element(odd) : -INFINITY;
-    for (int v = slice.index; v < slice.vectors; v += slice.threads)
-      for (int w = 0; w < W; ++w) a.top = fmaxf(a.top, slice.element(slice.first(v) + w));
-    if (ctas > 1)
-      cluster.sync();  // before the maxima are written again
-    else
-      __syncthreads();
-    largest = exchange(sh, a.top, ctas, rank, groups);
-    const float base = largest == -INFINITY ? 0.0f : largest;
-    a.s = a.t = 0.0f;
-    auto one = [&](float x) {
-      const float u = exponent_of(x, base, p.scale), e = exp2_fast(u);
-      a.s += e;
-      a.t = fmaf(e, u, a.t);
-    };
-    if (odd >= 0) one(slice.element(odd));
-    for (int v = slice.index; v < slice.vectors; v += slice.threads)
-      for (int w = 0; w < W; ++w) one(slice.element(slice.first(v) + w));
-  }
-  const float own = a.top;  // the largest of the thread's own elements
-  if (plain) rebase(a, largest, p.scale);
-
-  Shared *home = ctas == 1 ? &sh : cluster.map_shared_rank(&sh, 0);
-  if (p.top) {
-    find_limit(sh, groups, p.top);
-    __syncthreads();
-    const float limit = plain && sh.limit <= kFloor ? -INFINITY : sh.limit;
-    // the threads that reach the limit, and their vectors over all threads of the CTA
-    if (own >= limit && own > -INFINITY) {
-      sh.reach[atomicAdd(&sh.reaching, 1)] = (uint16_t)threadIdx.x;
-      if (odd >= 0) candidate(home, slice.element(odd), limit, odd);
-    }
-    __syncthreads();
-    const int each = (slice.vectors + slice.threads - 1) / slice.threads, items = sh.reaching * each;
-    for (int i = threadIdx.x; i < items; i += kThreads) {
-      const int n = i / each, v = rank * kThreads + sh.reach[n] + (i - n * each) * slice.threads;
-      if (v >= slice.vectors) continue;
-      const int first = slice.first(v);
-      Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(slice.x + first);
-      if (slice.legal) slice.mask(first, q);
-      uint32_t high = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) high |= (to_f(q.v[w]) >= limit ? 1u : 0u) << w;
-      for (; high; high &= high - 1) {
-        const int w = __ffs(high) - 1;
-        candidate(home, slice.element(first + w), limit, first + w);
-      }
-    }
-  }
-#pragma unroll
-  for (int off = 16; off; off >>= 1) {
-    a.s += __shfl_xor_sync(kFull, a.s, off);
-    a.t += __shfl_xor_sync(kFull, a.t, off);
-  }
-  if (lane == 0) home->sums[rank * kWarps + warp] = make_float2(a.s, a.t);
-  if (ctas == 1)
-    __syncthreads();
-  else
-    cluster.sync();
-  if (rank) return;
-
+  const int count = p.top ? sh.count[turn] : 0;
+  // a warp without candidates has nothing to write
+  if (warp && 32 * warp >= count && 32 * warp >= p.top && count <= kCandidates) return;
   float s = 0.0f, t = 0.0f;
   for (int i = lane; i < ctas * kWarps; i += 32) {
     s += sh.sums[i].x;
@@ -563,7 +543,6 @@ __global__ void __launch_bounds__(kThreads, 4) long_kernel(const __grid_constant
   const Row r = finish_row(largest, s, t);
   if (threadIdx.x == 0) write_row<T>(p, row, r);
   if (!p.top) return;
-  const int count = sh.count;
   if (count <= kCandidates) {
     for (int i = threadIdx.x; i < count; i += kThreads) {
       const uint64_t mine = sh.keys[i];
@@ -592,6 +571,128 @@ __global__ void __launch_bounds__(kThreads, 4) long_kernel(const __grid_constant
     __syncthreads();
     last = best;
     if (threadIdx.x == 0) write_top(p, row, r, i, logit_of((uint32_t)(best >> 32)), (int)~(uint32_t)best);
+  }
+}
+
+// CTAs of an SM: two chunks and the masks' of a thread want registers
+template <bool Masked>
+constexpr int kLongCtas = Masked ? 2 : 3;
+
+// Clusters take row after row: the next chunk, the next row's first one among
+// them, is on its way while this one is added up.
+template <typename T, bool Masked>
+__global__ void __launch_bounds__(kThreads, kLongCtas<Masked>) long_kernel(const __grid_constant__ Params p) {
+  constexpr int W = 16 / sizeof(T);
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int index = rank * kThreads + threadIdx.x, threads = ctas * kThreads, step = kVectors * threads;
+  const int groups = ctas >= 8 ? kWarps * ctas : 64;
+  if (threadIdx.x < 2) sh.count[threadIdx.x] = sh.reaching[threadIdx.x] = 0;
+  // the cluster's CTAs have begun, and counts are set, before the first write into another's memory
+  if (ctas > 1) cluster.barrier_arrive();
+  Shared *home = ctas == 1 ? &sh : cluster.map_shared_rank(&sh, 0);
+
+  const int64_t rows_apart = gridDim.x / ctas;
+  int64_t row = blockIdx.x / ctas;
+  Slice<T, Masked> slice(p, row);
+  Raw<T, Masked> raw;
+  slice.load(p, index, threads, raw);
+  bool begun = ctas == 1;
+  for (int turn = 0; row < p.rows; turn ^= 1) {
+    const int64_t next_row = row + rows_apart;
+    const Slice<T, Masked> next(p, next_row < p.rows ? next_row : row);
+    const int odd = slice.odd(index, threads);
+    Sums a = {-INFINITY, 0.0f, 0.0f};
+    if (odd >= 0) {
+      const float y = max_nan(slice.element(odd), kFloor);
+      a = Sums{y, 1.0f, 0.0f};
+      if (y != y) a = Sums{-INFINITY, y, y};
+    }
+    int at = index;
+    do {
+      Raw<T, Masked> now = raw;
+      at += step;
+      // (chunks in full: a thread without vectors adds -inf)
+      if (at - index < slice.vectors)
+        slice.load(p, at, threads, raw);
+      else if (next_row < p.rows)
+        next.load(p, index, threads, raw);
+      if constexpr (Masked) {
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) apply<T>(now.m[k], now.q[k]);
+      }
+      add_chunk(Chunk<T>(now.q), p.scale, a);
+    } while (at - index < slice.vectors);
+
+    if (!begun) cluster.barrier_wait();
+    begun = true;
+    float largest = exchange(sh, a.top, ctas, rank, groups);
+    // a row masked throughout by low values, or with an infinity: element by element, as they are
+    const bool plain = largest >= kLow && largest < INFINITY;
+    if (!plain) {
+      a.top = odd >= 0 ? slice.element(odd) : -INFINITY;
+      for (int v = index; v < slice.vectors; v += threads)
+        for (int w = 0; w < W; ++w) a.top = fmaxf(a.top, slice.element(slice.first(v) + w));
+      if (ctas > 1)
+        cluster.sync();  // before the maxima are written again
+      else
+        __syncthreads();
+      largest = exchange(sh, a.top, ctas, rank, groups);
+      const float base = largest == -INFINITY ? 0.0f : largest;
+      a.s = a.t = 0.0f;
+      auto one = [&](float x) {
+        const float u = exponent_of(x, base, p.scale), e = exp2_fast(u);
+        a.s += e;
+        a.t = fmaf(e, u, a.t);
+      };
+      if (odd >= 0) one(slice.element(odd));
+      for (int v = index; v < slice.vectors; v += threads)
+        for (int w = 0; w < W; ++w) one(slice.element(slice.first(v) + w));
+    }
+    const float own = a.top;  // the largest of the thread's own elements
+    if (plain) rebase(a, largest, p.scale);
+    if (threadIdx.x == 0) sh.count[turn ^ 1] = sh.reaching[turn ^ 1] = 0;
+
+    if (p.top) {
+      find_limit(sh, groups, p.top);
+      __syncthreads();
+      const float limit = plain && sh.limit <= kFloor ? -INFINITY : sh.limit;
+      // the threads that reach the limit, and their vectors over all threads of the CTA
+      if (own >= limit && own > -INFINITY) {
+        sh.reach[atomicAdd(&sh.reaching[turn], 1)] = (uint16_t)threadIdx.x;
+        if (odd >= 0) candidate(home, turn, slice.element(odd), limit, odd);
+      }
+      __syncthreads();
+      const int each = (slice.vectors + threads - 1) / threads, items = sh.reaching[turn] * each;
+      for (int i = threadIdx.x; i < items; i += kThreads) {
+        const int n = i / each, v = rank * kThreads + sh.reach[n] + (i - n * each) * threads;
+        if (v >= slice.vectors) continue;
+        const int first = slice.first(v);
+        const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(slice.x + first);
+        uint32_t high = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) high |= (to_f(q.v[w]) >= limit ? 1u : 0u) << w;
+        for (; high; high &= high - 1) {
+          const int k = first + __ffs(high) - 1;
+          candidate(home, turn, slice.element(k), limit, k);
+        }
+      }
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+      a.s += __shfl_xor_sync(kFull, a.s, off);
+      a.t += __shfl_xor_sync(kFull, a.t, off);
+    }
+    if (lane == 0) home->sums[rank * kWarps + warp] = make_float2(a.s, a.t);
+    if (ctas == 1)
+      __syncthreads();
+    else
+      cluster.sync();
+    if (rank == 0) finish_long<T, Masked>(p, sh, slice, row, largest, turn, ctas);
+    row = next_row;
+    slice = next;
   }
 }
 
@@ -670,6 +771,38 @@ cudaError_t short_rows(Params &p, bool gradient, cudaStream_t st) {
   return launch_short<T, W, 16 / W>(p, gradient, st);
 }
 
+template <typename T, bool Masked>
+cudaError_t launch_long(const Params &p, int sms, cudaStream_t st) {
+  // a cluster of CTAs while rows leave SMs without work and pieces keep four vectors a thread
+  int ctas = 1;
+  while (ctas < kMaxCluster && p.rows * ctas * 2 <= 2 * sms && p.actions / (ctas * 2) >= 4096) ctas *= 2;
+  if (ctas > 8) {
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(allowed.load(std::memory_order_acquire) & bit)) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(long_kernel<T, Masked>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      allowed.fetch_or(bit, std::memory_order_release);
+    }
+  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.rows, std::max(1, kLongCtas<Masked> * sms / ctas)) * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, long_kernel<T, Masked>, p);
+  if (e != cudaSuccess) return e;
+  return launched();
+}
+
 template <typename T>
 cudaError_t run(Params &p, bool gradient, int sms, cudaStream_t st) {
   if (p.actions <= kMaxShort) {
@@ -695,34 +828,7 @@ cudaError_t run(Params &p, bool gradient, int sms, cudaStream_t st) {
       long_gradient_kernel<T, false><<<(unsigned)(p.rows * pieces), kThreads, 0, st>>>(p, pieces);
     return launched();
   }
-  // a cluster of CTAs while rows leave SMs without work and pieces keep four vectors a thread
-  int ctas = 1;
-  while (ctas < kMaxCluster && p.rows * ctas * 2 <= 2 * sms && p.actions / (ctas * 2) >= 4096) ctas *= 2;
-  if (p.rows * ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  if (ctas > 8) {
-    static std::atomic<uint64_t> allowed{0};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(allowed.load(std::memory_order_acquire) & bit)) {
-      cudaError_t e = cudaFuncSetAttribute(long_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-      allowed.fetch_or(bit, std::memory_order_release);
-    }
-  }
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.rows * ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, long_kernel<T>, p);
-  if (e != cudaSuccess) return e;
-  return launched();
+  return p.legal ? launch_long<T, true>(p, sms, st) : launch_long<T, false>(p, sms, st);
 }
 
 int sm_count() {
