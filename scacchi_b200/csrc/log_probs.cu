@@ -43,13 +43,17 @@ std::atomic<uint64_t> g_log_probs_launches{0};
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+// Threads of a long row's CTA: 4096 x 32000 bf16 58 us with 128, 67 with 256,
+// whose row ends hold up more warps, and 65 with 64.
+constexpr int kLong = 128;
+constexpr int kWarps = kLong / 32;
 constexpr int kMaxShort = 512;      // actions of a short row
 constexpr int kMaxActions = 262144;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxGroups = 128;
 constexpr int kCandidates = 512;
+constexpr int kParts = 8;           // of a thread's chunks, each with its maximum
 constexpr float kLog2E = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kNothing = -1.0e4f;  // 2^kNothing is 0, and 0 times it is 0
@@ -151,116 +155,255 @@ __device__ __forceinline__ void write_top(const Params &p, int64_t row, const Ro
   p.top_log_prob[row * p.top + rank] = a < 0 ? -INFINITY : (x - r.top) * p.inverse - r.log_sum;
 }
 
+template <int Bytes>
+__device__ __forceinline__ void copy_async(void *to, const void *from) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (Bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
+}
+
 // ---------------------------------------------------------------------------
-// short rows: p.group lanes each, V vectors of W elements a lane
+// short rows: p.group lanes each
 // ---------------------------------------------------------------------------
 
-template <typename T, int W, int V>
-__device__ __forceinline__ void load_short(const Params &p, int64_t row, int lane, bool live, float (&x)[V * W]) {
-  const T *logits = static_cast<const T *>(p.logits) + row * p.stride;
-  const uint8_t *legal = p.legal ? p.legal + row * p.actions : nullptr;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int a = (v * p.group + lane) * W;
-    if (live && a < p.actions) {
-      const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(logits + a);
-      Vec<uint8_t, W> keep;
-      if (legal) keep = *reinterpret_cast<const Vec<uint8_t, W> *>(legal + a);
-#pragma unroll
-      for (int w = 0; w < W; ++w) x[v * W + w] = !legal || keep.v[w] ? to_f(q.v[w]) : -INFINITY;
+// A warp takes a batch of rows, 32 / group of them, into shared memory and each
+// row's lanes read vectors of W elements of it: 82 actions have a lane to
+// themselves, so the row's ends (logarithms, divisions, results) cost a warp
+// once in 32 rows.  Neighbouring rows lie A elements apart; W is chosen with
+// A / W odd where A allows it, and reads meet no bank twice.
+//
+// A lane's elements form parts of about eight, whose maxima lie beside them:
+// the best k take k rounds over the parts and one part's elements.
+constexpr int kShortThreads = 128;
+constexpr int kShortWarps = kShortThreads / 32;
+constexpr int kPartElements = 8;
+
+struct Batch {  // of a warp, in bytes from its own shared memory's begin
+  int legal, maxima, results, bytes;
+  int vectors, parts;  // of a lane
+};
+
+template <int Size>
+__device__ __forceinline__ void stage(uint8_t *to, const uint8_t *from, int bytes) {
+  const int lane = threadIdx.x & 31, phase = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+  to += phase;
+  const int head = min(bytes, (16 - phase) & 15), body = (bytes - head) / 16, tail = head + 16 * body;
+  for (int i = lane; i < body; i += 32) copy_async<16>(to + head + 16 * i, from + head + 16 * i);
+  using Word = std::conditional_t<Size == 4, uint32_t, std::conditional_t<Size == 2, uint16_t, uint8_t>>;
+  if (lane * Size < head) *reinterpret_cast<Word *>(to + lane * Size) = *reinterpret_cast<const Word *>(from + lane * Size);
+  if (tail + lane * Size < bytes)
+    *reinterpret_cast<Word *>(to + tail + lane * Size) = *reinterpret_cast<const Word *>(from + tail + lane * Size);
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_constant__ Params p,
+                                                              const __grid_constant__ Batch b) {
+  extern __shared__ __align__(16) uint8_t shared_bytes[];
+  const int lane = threadIdx.x & 31, group = p.group, sub = lane & (group - 1), mine = lane / group;
+  uint8_t *own = shared_bytes + (threadIdx.x / 32) * b.bytes;
+  float *maxima = reinterpret_cast<float *>(own + b.maxima) + lane;  // of the lane's parts, 32 apart
+  const int rows = 32 / group, all = p.actions / W;                  // vectors of a row
+  const int64_t batches = (p.rows + rows - 1) / rows;
+  for (int64_t batch = (int64_t)blockIdx.x * kShortWarps + threadIdx.x / 32; batch < batches;
+       batch += (int64_t)gridDim.x * kShortWarps) {
+    const int64_t first = batch * rows;
+    const int count = (int)min((int64_t)rows, p.rows - first);
+    const T *from = static_cast<const T *>(p.logits) + first * p.stride;
+    const uint8_t *mask = p.legal ? p.legal + first * p.actions : nullptr;
+    int phase = 0;
+    if (p.stride == p.actions || count == 1) {
+      phase = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+      stage<sizeof(T)>(own, reinterpret_cast<const uint8_t *>(from), count * p.actions * (int)sizeof(T));
     } else {
-#pragma unroll
-      for (int w = 0; w < W; ++w) x[v * W + w] = -INFINITY;
+      for (int r = 0; r < count; ++r)
+        for (int i = lane; i < p.actions; i += 32) reinterpret_cast<T *>(own)[r * p.actions + i] = from[r * p.stride + i];
     }
-  }
-}
+    if (mask) stage<1>(own + b.legal, mask, count * p.actions);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    const bool live = mine < count;
+    const int64_t row = first + mine;
+    const int action = live ? p.action[row] : -1;
+    __syncwarp();
 
-template <typename T, int W, int V>
-__global__ void __launch_bounds__(kThreads) short_kernel(const __grid_constant__ Params p) {
-  constexpr int E = V * W;
-  const int group = p.group, lane = threadIdx.x & (group - 1);
-  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / group;
-  const bool live = row < p.rows;
-  float x[E];
-  load_short<T, W, V>(p, row, lane, live, x);
-  float top = -INFINITY;
+    Vec<T, W> *x = reinterpret_cast<Vec<T, W> *>(own + phase + (size_t)mine * p.actions * sizeof(T));
+    const Vec<uint8_t, W> *legal = reinterpret_cast<const Vec<uint8_t, W> *>(
+        own + b.legal + (reinterpret_cast<uintptr_t>(mask) & 15) + (size_t)mine * p.actions);
+    constexpr int kEach = kPartElements / W;  // vectors of a part
+    float top = -INFINITY;
+    if (live) {
+      for (int part = 0, v = sub; part < b.parts; ++part) {
+        float most = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < E; ++j) top = fmaxf(top, x[j]);
-  for (int off = group >> 1; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float s = 0.0f, t = 0.0f;
+        for (int k = 0; k < kEach; ++k, v += group) {
+          if (v >= all) break;
+          Vec<T, W> q = x[v];
+          if (mask) {
+            const Vec<uint8_t, W> keep = legal[v];
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const float u = exponent_of(x[j], base, p.scale), e = exp2_fast(u);
-    s += e;
-    t = fmaf(e, u, t);
-  }
-  for (int off = group >> 1; off; off >>= 1) {
-    s += __shfl_xor_sync(kFull, s, off);
-    t += __shfl_xor_sync(kFull, t, off);
-  }
-  const Row r = finish_row(top, s, t);
-  if (live && lane == 0) write_row<T>(p, row, r);
-  if (!p.top) return;
-  // a lane's best: the first of its largest, since its indices ascend
-  int removed = -1;
-  for (int rank = 0; rank < p.top; ++rank) {
-    float best = -INFINITY;
-    int at = -1;
+            for (int w = 0; w < W; ++w)
+              if (!keep.v[w]) q.v[w] = from_f<T>(-INFINITY);
+            x[v] = q;
+          }
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      if (j == removed) x[j] = -INFINITY;
-      if (x[j] > best) {
-        best = x[j];
-        at = j;
+          for (int w = 0; w < W; ++w) most = fmaxf(most, to_f(q.v[w]));
+        }
+        if (p.top) maxima[32 * part] = most;
+        top = fmaxf(top, most);
       }
     }
-    int a = at < 0 ? 0x7fffffff : ((at / W) * group + lane) * W + at % W;
-    const int mine = a;
+    for (int off = group >> 1; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float s = 0.0f, t = 0.0f;
+    if (live) {
+#pragma unroll 4
+      for (int v = sub; v < all; v += group) {
+        const Vec<T, W> q = x[v];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float u = exponent_of(to_f(q.v[w]), base, p.scale), e = exp2_fast(u);
+          s += e;
+          t = fmaf(e, u, t);
+        }
+      }
+    }
     for (int off = group >> 1; off; off >>= 1) {
-      const float other = __shfl_xor_sync(kFull, best, off);
-      const int oa = __shfl_xor_sync(kFull, a, off);
-      if (other > best || (other == best && oa < a)) {
-        best = other;
-        a = oa;
+      s += __shfl_xor_sync(kFull, s, off);
+      t += __shfl_xor_sync(kFull, t, off);
+    }
+    const Row r = finish_row(top, s, t);
+    __syncwarp();
+    if (live && sub == 0) {
+      float lp = 0.0f;
+      if (action >= 0 && action < p.actions) {
+        const float xa = to_f(reinterpret_cast<const T *>(x)[action]);
+        lp = xa == -INFINITY ? -INFINITY : (xa - top) * p.inverse - r.log_sum;
+      }
+      p.log_prob[row] = lp;
+      p.entropy[row] = r.entropy;
+      p.max_logit[row] = r.top;
+      p.log_sum[row] = r.log_sum;
+    }
+    if (p.top) {
+      float *values = reinterpret_cast<float *>(own + b.results);
+      int *places = reinterpret_cast<int *>(values + rows * p.top);
+      for (int rank = 0; rank < p.top; ++rank) {
+        // the first part with the lane's largest, since indices ascend
+        float best = -INFINITY;
+        int part = 0;
+        if (live) {
+          for (int i = 0; i < b.parts; ++i) {
+            const float most = maxima[32 * i];
+            if (most > best) {
+              best = most;
+              part = i;
+            }
+          }
+        }
+        int at = 0x7fffffff;
+        if (best > -INFINITY) {
+#pragma unroll
+          for (int k = kEach - 1; k >= 0; --k) {
+            const int v = sub + (part * kEach + k) * group;
+            if (v >= all) continue;
+            const Vec<T, W> q = x[v];
+#pragma unroll
+            for (int w = W - 1; w >= 0; --w)
+              if (to_f(q.v[w]) == best) at = v * W + w;
+          }
+        }
+        const int candidate = at;
+        for (int off = group >> 1; off; off >>= 1) {
+          const float other = __shfl_xor_sync(kFull, best, off);
+          const int place = __shfl_xor_sync(kFull, at, off);
+          if (other > best || (other == best && place < at)) {
+            best = other;
+            at = place;
+          }
+        }
+        if (live && at != 0x7fffffff && at == candidate) {  // taken out, and its part's maximum is the next one
+          reinterpret_cast<T *>(x)[at] = from_f<T>(-INFINITY);
+          float most = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < kEach; ++k) {
+            const int v = sub + (part * kEach + k) * group;
+            if (v >= all) break;
+            const Vec<T, W> q = x[v];
+#pragma unroll
+            for (int w = 0; w < W; ++w) most = fmaxf(most, to_f(q.v[w]));
+          }
+          maxima[32 * part] = most;
+        }
+        if (live && sub == 0) {
+          values[mine * p.top + rank] = at == 0x7fffffff ? -INFINITY : (best - top) * p.inverse - r.log_sum;
+          places[mine * p.top + rank] = at == 0x7fffffff ? -1 : at;
+        }
+      }
+      __syncwarp();
+      for (int i = lane; i < count * p.top; i += 32) {
+        p.top_log_prob[first * p.top + i] = values[i];
+        p.top_action[first * p.top + i] = places[i];
       }
     }
-    removed = a == mine ? at : -1;
-    if (live && lane == 0) write_top(p, row, r, rank, best, a == 0x7fffffff ? -1 : a);
+    __syncwarp();
   }
 }
 
-template <typename T, int W, int V>
-__global__ void __launch_bounds__(kThreads) short_gradient_kernel(const __grid_constant__ Params p) {
-  const int group = p.group, lane = threadIdx.x & (group - 1);
-  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / group;
-  if (row >= p.rows) return;
-  float x[V * W];
-  load_short<T, W, V>(p, row, lane, true, x);
-  const float top = p.max_logit[row], base = top == -INFINITY ? 0.0f : top;
-  const float log_sum = p.log_sum[row] * kLog2E;
+// The gradient of short rows: a CTA's first threads gather what its rows need,
+// then all take the rows' vectors in order.
+struct RowGradient {
+  float base, log_sum, offset, slope;
+  float g;
+  int action;
+};
+
+// of a row, with p_i = 2^v, v = (x - base) scale - log_sum: d_i = g [i = action] - p_i (offset + slope v)
+template <typename T>
+__device__ __forceinline__ RowGradient row_gradient(const Params &p, int64_t row) {
+  const float top = p.max_logit[row], log_sum = p.log_sum[row];
   const int a = p.action[row];
-  float g = 0.0f;
   const bool inside = a >= 0 && a < p.actions;
+  RowGradient r = {top == -INFINITY ? 0.0f : top, log_sum * kLog2E, 0.0f, 0.0f, 0.0f, inside ? a : -1};
   if (p.grad_log_prob && inside && (!p.legal || p.legal[row * p.actions + a]) &&
       to_f(static_cast<const T *>(p.logits)[row * p.stride + a]) != -INFINITY)
-    g = p.grad_log_prob[row] * p.inverse;
+    r.g = p.grad_log_prob[row] * p.inverse;
   const float h = p.grad_entropy ? p.grad_entropy[row] * p.inverse : 0.0f;
-  const float offset = g + (h == 0.0f ? 0.0f : h * p.entropy[row]), slope = h * kLn2;
-  T *grad = static_cast<T *>(p.grad) + row * p.actions;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int first = (v * group + lane) * W;
-    if (first >= p.actions) continue;
+  r.offset = r.g + (h == 0.0f ? 0.0f : h * p.entropy[row]);
+  r.slope = h * kLn2;
+  return r;
+}
+
+__device__ __forceinline__ float gradient_of(const RowGradient &r, float x, int i, float scale) {
+  const float v = max_nan((x - r.base) * scale - r.log_sum, kNothing);
+  const float d = -exp2_fast(v) * fmaf(r.slope, v, r.offset);
+  return x == -INFINITY ? 0.0f : i == r.action ? d + r.g : d;
+}
+
+constexpr int kMaxRows = 256;  // of a CTA
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads) short_gradient_kernel(const __grid_constant__ Params p, int rows,
+                                                                  uint32_t reciprocal) {
+  __shared__ RowGradient table[kMaxRows];
+  const int64_t first = (int64_t)blockIdx.x * rows;
+  const int count = (int)min((int64_t)rows, p.rows - first), all = p.actions / W;
+  if ((int)threadIdx.x < count) table[threadIdx.x] = row_gradient<T>(p, first + threadIdx.x);
+  __syncthreads();
+  const T *logits = static_cast<const T *>(p.logits) + first * p.stride;
+  const uint8_t *legal = p.legal ? p.legal + first * p.actions : nullptr;
+  T *grad = static_cast<T *>(p.grad) + first * p.actions;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count * all; i += kThreads) {
+    const int row = all == 1 ? i : (int)__umulhi((uint32_t)i, reciprocal), a = (i - row * all) * W;
+    const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(logits + row * p.stride + a);
+    Vec<uint8_t, W> keep;
+    if (legal) keep = *reinterpret_cast<const Vec<uint8_t, W> *>(legal + i * W);
+    const RowGradient r = table[row];
     Vec<T, W> out;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float u = max_nan((x[v * W + w] - base) * p.scale - log_sum, kNothing);
-      float d = -exp2_fast(u) * fmaf(slope, u, offset);
-      if (first + w == a) d += g;
-      out.v[w] = from_f<T>(x[v * W + w] == -INFINITY ? 0.0f : d);
-    }
-    *reinterpret_cast<Vec<T, W> *>(grad + first) = out;
+    for (int w = 0; w < W; ++w)
+      out.v[w] = from_f<T>(gradient_of(r, !legal || keep.v[w] ? to_f(q.v[w]) : -INFINITY, a + w, p.scale));
+    *reinterpret_cast<Vec<T, W> *>(grad + i * W) = out;
   }
 }
 
@@ -280,12 +423,28 @@ template <typename T>
 constexpr uint32_t kMinusInfinity = std::is_same_v<T, float> ? 0xff800000u
                                     : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
 
-// A chunk as it comes: vectors, and the mask's bytes beside them
+// Chunks on their way from memory: every thread copies its own vectors (and
+// the words that hold their masks' bytes) and reads them alone, so nothing
+// but its own copies is waited for.  Two stages: three measured the same.
 template <typename T, bool Masked>
-struct Raw {
-  uint4 q[kVectors];
-  uint32_t m[Masked ? kVectors : 1][4 / sizeof(T)];
+struct Ring {
+  static constexpr int kStages = 2, kWords = Masked ? 4 / sizeof(T) + 1 : 0;
+  uint4 q[kStages][kVectors][kLong];
+  uint32_t m[kStages][kVectors][Masked ? kWords : 1][Masked ? kLong : 1];
 };
+
+// -inf where the mask's byte is 0
+template <typename T>
+__device__ __forceinline__ void apply(const uint32_t (&m)[4 / sizeof(T)], uint4 &q) {
+  uint32_t *word = reinterpret_cast<uint32_t *>(&q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t keep = sizeof(T) == 4 ? __byte_perm(__vcmpne4(m[0], 0u), 0u, 0x1111 * i)
+                                         : __byte_perm(__vcmpne4(m[sizeof(T) == 4 ? 0 : i / 2], 0u), 0u,
+                                                       i & 1 ? 0x3322 : 0x1100);
+    word[i] = (word[i] & keep) | (kMinusInfinity<T> & ~keep);
+  }
+}
 
 // A row's elements as the threads of its cluster take them: vectors from the
 // first 16-byte boundary on, thread after thread, and the head's and the
@@ -310,55 +469,56 @@ struct Slice {
     return back < head ? back : back - head < actions - tail ? tail + back - head : -1;
   }
   __device__ int first(int v) const { return head + v * W; }
-  // the mask's bytes of a vector: the words that hold them, shifted, where none of these reaches beyond the mask
-  __device__ void mask(const Params &p, int v, uint32_t (&m)[W / 4]) const {
-    const uint8_t *at = legal + first(v);
-    const int shift = (int)(reinterpret_cast<uintptr_t>(at) & 3);
-    const uint32_t *word = reinterpret_cast<const uint32_t *>(at - shift);
-    if (shift == 0) {
-#pragma unroll
-      for (int w = 0; w < W / 4; ++w) m[w] = word[w];
-    } else if (at - shift >= p.legal && at + W + 4 <= p.legal + p.rows * p.actions) {
-      uint32_t low = word[0];
-#pragma unroll
-      for (int w = 0; w < W / 4; ++w) {
-        const uint32_t high = word[w + 1];
-        m[w] = __funnelshift_r(low, high, 8 * shift);
-        low = high;
-      }
-    } else {
-#pragma unroll
-      for (int w = 0; w < W; ++w) m[w / 4] = (w & 3 ? m[w / 4] : 0u) | (uint32_t)at[w] << (8 * (w & 3));
-    }
-  }
-  // vectors v, v + threads, ..., -inf where there is none
-  __device__ void load(const Params &p, int v, int threads, Raw<T, Masked> &raw) const {
+  // how far a vector's mask begins behind a word's
+  __device__ int shift(int v) const { return (int)(reinterpret_cast<uintptr_t>(legal + first(v)) & 3); }
+  // requests the vectors v, v + threads, ...; -inf where there is none
+  __device__ void request(const Params &p, int v, int threads, Ring<T, Masked> &ring, int stage) const {
     const uint4 *at = reinterpret_cast<const uint4 *>(x + head) + v;
     const uint32_t none = kMinusInfinity<T>;
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) {
-      const bool there = v + k * threads < vectors;
-      raw.q[k] = there ? at[k * threads] : make_uint4(none, none, none, none);
-      if constexpr (Masked)
-        if (there) mask(p, v + k * threads, raw.m[k]);
+      uint4 *to = &ring.q[stage][k][threadIdx.x];
+      if (v + k * threads >= vectors) {
+        *to = make_uint4(none, none, none, none);
+        continue;
+      }
+      copy_async<16>(to, at + k * threads);
+      if constexpr (Masked) {
+        const uint8_t *bytes = legal + first(v + k * threads), *word = bytes - shift(v + k * threads);
+        if (word >= p.legal && word + 4 * ring.kWords <= p.legal + p.rows * p.actions) {
+#pragma unroll
+          for (int w = 0; w < ring.kWords; ++w) copy_async<4>(&ring.m[stage][k][w][threadIdx.x], word + 4 * w);
+        } else {  // some of these words reach beyond the mask
+#pragma unroll
+          for (int w = 0; w < ring.kWords; ++w) {
+            uint32_t u = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (word + 4 * w + i >= bytes && word + 4 * w + i < bytes + W) u |= (uint32_t)word[4 * w + i] << (8 * i);
+            ring.m[stage][k][w][threadIdx.x] = u;
+          }
+        }
+      }
+    }
+  }
+  // what was requested, with -inf where the mask's byte is 0
+  __device__ void take(int v, int threads, const Ring<T, Masked> &ring, int stage, uint4 (&q)[kVectors]) const {
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+      q[k] = ring.q[stage][k][threadIdx.x];
+      if constexpr (Masked) {
+        const int bits = 8 * shift(v + k * threads);
+        uint32_t m[W / 4];
+#pragma unroll
+        for (int w = 0; w < W / 4; ++w)
+          m[w] = __funnelshift_r(ring.m[stage][k][w][threadIdx.x], ring.m[stage][k][w + 1][threadIdx.x], bits);
+        apply<T>(m, q[k]);
+      }
     }
   }
   // -inf where the element is not kept
   __device__ float element(int a) const { return !Masked || legal[a] ? to_f(x[a]) : -INFINITY; }
 };
-
-// -inf where the mask's byte is 0
-template <typename T>
-__device__ __forceinline__ void apply(const uint32_t (&m)[4 / sizeof(T)], uint4 &q) {
-  uint32_t *word = reinterpret_cast<uint32_t *>(&q);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t keep = sizeof(T) == 4 ? __byte_perm(__vcmpne4(m[0], 0u), 0u, 0x1111 * i)
-                                         : __byte_perm(__vcmpne4(m[sizeof(T) == 4 ? 0 : i / 2], 0u), 0u,
-                                                       i & 1 ? 0x3322 : 0x1100);
-    word[i] = (word[i] & keep) | (kMinusInfinity<T> & ~keep);
-  }
-}
 
 // the largest of three, without those that are NaN
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -442,8 +602,9 @@ __device__ __forceinline__ void rebase(Sums &a, float top, float scale) {
   a.top = top;
 }
 
+// returns the chunk's maximum
 template <typename T>
-__device__ __forceinline__ void add_chunk(const Chunk<T> &y, float scale, Sums &a) {
+__device__ __forceinline__ float add_chunk(const Chunk<T> &y, float scale, Sums &a) {
   const float most = y.largest();
   if (most > a.top) rebase(a, most, scale);
   const float2 scale2 = make_float2(scale, scale), top2 = make_float2(-a.top, -a.top);
@@ -459,13 +620,15 @@ __device__ __forceinline__ void add_chunk(const Chunk<T> &y, float scale, Sums &
   t[0] = __fadd2_rn(t[0], t[1]);
   a.s += s[0].x + s[0].y;
   a.t += t[0].x + t[0].y;
+  return most;
 }
 
 struct Shared {
   float4 maxima[kMaxGroups / 4];
   float2 sums[kMaxCluster * kWarps];
   uint64_t keys[kCandidates];
-  uint16_t reach[kThreads];
+  float parts[kParts][kLong];  // maxima of the threads' parts
+  uint16_t reach[kParts * kLong];
   int count[2], reaching[2];  // of rows in turn
   float limit;
   uint64_t best[kWarps];
@@ -474,7 +637,7 @@ struct Shared {
 // The groups' maxima to every CTA of the cluster; returns the row's
 __device__ __forceinline__ float exchange(Shared &sh, float top, int ctas, int rank, int groups) {
   cg::cluster_group cluster = cg::this_cluster();
-  const int width = ctas >= 8 ? 32 : 4 * ctas, per_cta = kThreads / width;  // threads of a group
+  const int per_cta = groups / ctas, width = kLong / per_cta;  // threads of a group
   for (int off = width >> 1; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
   if ((threadIdx.x & (width - 1)) == 0) {
     const int g = rank * per_cta + threadIdx.x / width;
@@ -544,19 +707,19 @@ __device__ __forceinline__ void finish_long(const Params &p, Shared &sh, const S
   if (threadIdx.x == 0) write_row<T>(p, row, r);
   if (!p.top) return;
   if (count <= kCandidates) {
-    for (int i = threadIdx.x; i < count; i += kThreads) {
+    for (int i = threadIdx.x; i < count; i += kLong) {
       const uint64_t mine = sh.keys[i];
       int above = 0;
       for (int j = 0; j < count; ++j) above += sh.keys[j] > mine;
       if (above < p.top) write_top(p, row, r, above, logit_of((uint32_t)(mine >> 32)), (int)~(uint32_t)mine);
     }
-    for (int i = count + threadIdx.x; i < p.top; i += kThreads) write_top(p, row, r, i, 0.0f, -1);
+    for (int i = count + threadIdx.x; i < p.top; i += kLong) write_top(p, row, r, i, 0.0f, -1);
     return;
   }
   uint64_t last = ~0ull;
   for (int i = 0; i < p.top; ++i) {
     uint64_t best = 0;
-    for (int k = threadIdx.x; k < p.actions; k += kThreads) {
+    for (int k = threadIdx.x; k < p.actions; k += kLong) {
       const float v = slice.element(k);
       if (!(v > -INFINITY)) continue;
       const uint64_t key = key_of(v, k);
@@ -574,35 +737,53 @@ __device__ __forceinline__ void finish_long(const Params &p, Shared &sh, const S
   }
 }
 
-// CTAs of an SM: two chunks and the masks' of a thread want registers
 template <bool Masked>
-constexpr int kLongCtas = Masked ? 2 : 3;
+constexpr int kLongCtas = Masked ? 5 : 6;  // of an SM: registers and, with masks, shared memory
 
-// Clusters take row after row: the next chunk, the next row's first one among
-// them, is on its way while this one is added up.
+// Clusters take row after row.  A thread's next chunks, the next row's among
+// them, are on their way while this one is added up and the row is finished.
 template <typename T, bool Masked>
-__global__ void __launch_bounds__(kThreads, kLongCtas<Masked>) long_kernel(const __grid_constant__ Params p) {
-  constexpr int W = 16 / sizeof(T);
+__global__ void __launch_bounds__(kLong, kLongCtas<Masked>) long_kernel(const __grid_constant__ Params p) {
+  constexpr int W = 16 / sizeof(T), kStages = Ring<T, Masked>::kStages;
+  extern __shared__ __align__(16) uint8_t ring_bytes[];
   __shared__ Shared sh;
+  Ring<T, Masked> &ring = *reinterpret_cast<Ring<T, Masked> *>(ring_bytes);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int index = rank * kThreads + threadIdx.x, threads = ctas * kThreads, step = kVectors * threads;
-  const int groups = ctas >= 8 ? kWarps * ctas : 64;
+  const int index = rank * kLong + threadIdx.x, threads = ctas * kLong, step = kVectors * threads;
+  const int groups = max(64, kWarps * ctas);
   if (threadIdx.x < 2) sh.count[threadIdx.x] = sh.reaching[threadIdx.x] = 0;
   // the cluster's CTAs have begun, and counts are set, before the first write into another's memory
   if (ctas > 1) cluster.barrier_arrive();
   Shared *home = ctas == 1 ? &sh : cluster.map_shared_rank(&sh, 0);
 
   const int64_t rows_apart = gridDim.x / ctas;
-  int64_t row = blockIdx.x / ctas;
-  Slice<T, Masked> slice(p, row);
-  Raw<T, Masked> raw;
-  slice.load(p, index, threads, raw);
+  // of every row: one that begins off a boundary may leave its last chunk empty
+  const int chunks = max(1, (p.actions / W + step - 1) / step), per_part = (chunks + kParts - 1) / kParts;
+  // what is requested next
+  int64_t ahead_row = blockIdx.x / ctas;
+  int ahead_chunk = 0, ahead_stage = 0, stage = 0;
+  Slice<T, Masked> ahead(p, ahead_row);
+  auto request = [&]() {
+    if (ahead_row < p.rows) {
+      ahead.request(p, index + ahead_chunk * step, threads, ring, ahead_stage);
+      if (++ahead_chunk == chunks) {
+        ahead_chunk = 0;
+        ahead_row += rows_apart;
+        if (ahead_row < p.rows) ahead = Slice<T, Masked>(p, ahead_row);
+      }
+    }
+    ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int i = 0; i + 1 < kStages; ++i) request();
+
   bool begun = ctas == 1;
-  for (int turn = 0; row < p.rows; turn ^= 1) {
-    const int64_t next_row = row + rows_apart;
-    const Slice<T, Masked> next(p, next_row < p.rows ? next_row : row);
+  int turn = 0;
+  for (int64_t row = blockIdx.x / ctas; row < p.rows; row += rows_apart, turn ^= 1) {
+    const Slice<T, Masked> slice(p, row);
     const int odd = slice.odd(index, threads);
     Sums a = {-INFINITY, 0.0f, 0.0f};
     if (odd >= 0) {
@@ -610,21 +791,22 @@ __global__ void __launch_bounds__(kThreads, kLongCtas<Masked>) long_kernel(const
       a = Sums{y, 1.0f, 0.0f};
       if (y != y) a = Sums{-INFINITY, y, y};
     }
-    int at = index;
-    do {
-      Raw<T, Masked> now = raw;
-      at += step;
-      // (chunks in full: a thread without vectors adds -inf)
-      if (at - index < slice.vectors)
-        slice.load(p, at, threads, raw);
-      else if (next_row < p.rows)
-        next.load(p, index, threads, raw);
-      if constexpr (Masked) {
-#pragma unroll
-        for (int k = 0; k < kVectors; ++k) apply<T>(now.m[k], now.q[k]);
+    float part = -INFINITY;
+#pragma unroll 1
+    for (int chunk = 0, left = per_part, to = 0; chunk < chunks; ++chunk) {
+      request();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      uint4 q[kVectors];
+      slice.take(index + chunk * step, threads, ring, stage, q);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      part = fmaxf(part, add_chunk(Chunk<T>(q), p.scale, a));
+      if (--left == 0 || chunk + 1 == chunks) {
+        if (p.top) sh.parts[to][threadIdx.x] = part;
+        ++to;
+        part = -INFINITY;
+        left = per_part;
       }
-      add_chunk(Chunk<T>(now.q), p.scale, a);
-    } while (at - index < slice.vectors);
+    }
 
     if (!begun) cluster.barrier_wait();
     begun = true;
@@ -633,8 +815,13 @@ __global__ void __launch_bounds__(kThreads, kLongCtas<Masked>) long_kernel(const
     const bool plain = largest >= kLow && largest < INFINITY;
     if (!plain) {
       a.top = odd >= 0 ? slice.element(odd) : -INFINITY;
-      for (int v = index; v < slice.vectors; v += threads)
-        for (int w = 0; w < W; ++w) a.top = fmaxf(a.top, slice.element(slice.first(v) + w));
+      for (int i = 0; i * per_part < chunks; ++i) {
+        part = -INFINITY;
+        for (int v = index + i * per_part * step; v < min(slice.vectors, (i + 1) * per_part * step); v += threads)
+          for (int w = 0; w < W; ++w) part = fmaxf(part, slice.element(slice.first(v) + w));
+        if (p.top) sh.parts[i][threadIdx.x] = part;
+        a.top = fmaxf(a.top, part);
+      }
       if (ctas > 1)
         cluster.sync();  // before the maxima are written again
       else
@@ -659,15 +846,18 @@ __global__ void __launch_bounds__(kThreads, kLongCtas<Masked>) long_kernel(const
       find_limit(sh, groups, p.top);
       __syncthreads();
       const float limit = plain && sh.limit <= kFloor ? -INFINITY : sh.limit;
-      // the threads that reach the limit, and their vectors over all threads of the CTA
+      // the parts that reach the limit, and their vectors over all threads of the CTA
       if (own >= limit && own > -INFINITY) {
-        sh.reach[atomicAdd(&sh.reaching[turn], 1)] = (uint16_t)threadIdx.x;
+        for (int i = 0; i * per_part < chunks; ++i)
+          if (sh.parts[i][threadIdx.x] >= limit)
+            sh.reach[atomicAdd(&sh.reaching[turn], 1)] = (uint16_t)(i * kLong + threadIdx.x);
         if (odd >= 0) candidate(home, turn, slice.element(odd), limit, odd);
       }
       __syncthreads();
-      const int each = (slice.vectors + threads - 1) / threads, items = sh.reaching[turn] * each;
-      for (int i = threadIdx.x; i < items; i += kThreads) {
-        const int n = i / each, v = rank * kThreads + sh.reach[n] + (i - n * each) * threads;
+      const int each = kVectors * per_part, items = sh.reaching[turn] * each;
+      for (int i = threadIdx.x; i < items; i += kLong) {
+        const int n = i / each, which = sh.reach[n];
+        const int v = rank * kLong + which % kLong + (which / kLong * each + i - n * each) * threads;
         if (v >= slice.vectors) continue;
         const int first = slice.first(v);
         const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(slice.x + first);
@@ -691,8 +881,6 @@ __global__ void __launch_bounds__(kThreads, kLongCtas<Masked>) long_kernel(const
     else
       cluster.sync();
     if (rank == 0) finish_long<T, Masked>(p, sh, slice, row, largest, turn, ctas);
-    row = next_row;
-    slice = next;
   }
 }
 
@@ -706,21 +894,8 @@ __global__ void __launch_bounds__(kThreads) long_gradient_kernel(const __grid_co
   const T *x = static_cast<const T *>(p.logits) + row * p.stride;
   const uint8_t *legal = p.legal ? p.legal + row * p.actions : nullptr;
   T *grad = static_cast<T *>(p.grad) + row * p.actions;
-  const float top = p.max_logit[row], base = top == -INFINITY ? 0.0f : top;
-  const float log_sum = p.log_sum[row] * kLog2E;
-  const int a = p.action[row];
-  float g = 0.0f;
-  if (p.grad_log_prob && a >= 0 && a < p.actions && (!legal || legal[a]) && to_f(x[a]) != -INFINITY)
-    g = p.grad_log_prob[row] * p.inverse;
-  const float h = p.grad_entropy ? p.grad_entropy[row] * p.inverse : 0.0f;
-  const float offset = g + (h == 0.0f ? 0.0f : h * p.entropy[row]), slope = h * kLn2;
-  auto one = [&](float v, int i) {
-    const float u = max_nan((v - base) * p.scale - log_sum, kNothing);
-    float d = -exp2_fast(u) * fmaf(slope, u, offset);
-    if (i == a) d += g;
-    return v == -INFINITY ? 0.0f : d;
-  };
-  auto scalar = [&](int i) { grad[i] = from_f<T>(one(!legal || legal[i] ? to_f(x[i]) : -INFINITY, i)); };
+  const RowGradient r = row_gradient<T>(p, row);
+  auto scalar = [&](int i) { grad[i] = from_f<T>(gradient_of(r, !legal || legal[i] ? to_f(x[i]) : -INFINITY, i, p.scale)); };
   const int head = Vector ? min(p.actions, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T)) : 0;
   const int begin = head + piece * kPiece, whole = (p.actions - head) / W * W + head;
   const int end = min(whole, begin + kPiece);
@@ -732,7 +907,7 @@ __global__ void __launch_bounds__(kThreads) long_gradient_kernel(const __grid_co
     Vec<T, W> out;
 #pragma unroll
     for (int w = 0; w < W; ++w)
-      out.v[w] = from_f<T>(one(!legal || legal[i + w] ? to_f(q.v[w]) : -INFINITY, i + w));
+      out.v[w] = from_f<T>(gradient_of(r, !legal || legal[i + w] ? to_f(q.v[w]) : -INFINITY, i + w, p.scale));
     *reinterpret_cast<Vec<T, W> *>(grad + i) = out;
   }
 }
@@ -748,27 +923,50 @@ cudaError_t launched() {
   return cudaGetLastError();
 }
 
-template <typename T, int W, int V>
-cudaError_t launch_short(const Params &p, bool gradient, cudaStream_t st) {
-  const int64_t ctas = (p.rows * p.group + kThreads - 1) / kThreads;
-  if (gradient)
-    short_gradient_kernel<T, W, V><<<(unsigned)ctas, kThreads, 0, st>>>(p);
-  else
-    short_kernel<T, W, V><<<(unsigned)ctas, kThreads, 0, st>>>(p);
-  return launched();
-}
-
-// The fewest lanes that hold a row with 12 elements each, or 16 of a whole warp
+// Rows and lanes of a batch: the fewest lanes a row with which reads of
+// neighbouring rows share no bank, a warp's rows stay within kBatchBytes, and
+// (when rows are few) every SM has eight warps' work.
+constexpr int kBatchBytes = 14 * 1024, kSharedBytes = 220 * 1024;
 template <typename T, int W>
-cudaError_t short_rows(Params &p, bool gradient, cudaStream_t st) {
-  const int vectors = (p.actions + W - 1) / W;
-  p.group = 1;
-  while (p.group < 32 && (vectors + p.group - 1) / p.group * W > 12) p.group *= 2;
-  const int v = (vectors + p.group - 1) / p.group;
-  if (v * W <= 4) return launch_short<T, W, 4 / W>(p, gradient, st);
-  if (v * W <= 8) return launch_short<T, W, 8 / W>(p, gradient, st);
-  if (v * W <= 12) return launch_short<T, W, 12 / W>(p, gradient, st);
-  return launch_short<T, W, 16 / W>(p, gradient, st);
+cudaError_t short_rows(Params &p, bool gradient, int sms, cudaStream_t st) {
+  const int all = p.actions / W;
+  if (gradient) {
+    const int rows = std::max(1, std::min(kMaxRows, 6144 / p.actions));
+    const int64_t ctas = (p.rows + rows - 1) / rows;
+    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    // i / all for i below 6144: the quotient's error i / 2^32 stays below 1 / all (all <= 512)
+    const uint32_t reciprocal = (uint32_t)((1ull << 32) / all + 1);
+    short_gradient_kernel<T, W><<<(unsigned)ctas, kThreads, 0, st>>>(p, rows, reciprocal);
+    return launched();
+  }
+  const int row_bytes = p.actions * ((int)sizeof(T) + (p.legal ? 1 : 0));
+  p.group = std::min(8, all & -all);
+  if (W * sizeof(T) < 16 && all % 2 == 0) p.group = std::min(8, p.group * 2);
+  while (p.group < 32 && (32 / p.group * row_bytes > kBatchBytes || p.rows * p.group < (int64_t)8 * 32 * sms)) p.group *= 2;
+  const int rows = 32 / p.group;
+  auto up = [](int n) { return (n + 15) / 16 * 16; };
+  Batch b;
+  b.vectors = (all + p.group - 1) / p.group;
+  b.parts = (b.vectors * W + kPartElements - 1) / kPartElements;
+  b.legal = up(rows * p.actions * (int)sizeof(T) + 16);
+  b.maxima = b.legal + (p.legal ? up(rows * p.actions + 16) : 0);
+  b.results = b.maxima + (p.top ? 128 * b.parts : 0);
+  b.bytes = b.results + up(8 * rows * p.top);
+  const int bytes = kShortWarps * b.bytes;
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(allowed.load(std::memory_order_acquire) & bit)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(short_kernel<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
+    if (e != cudaSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_release);
+  }
+  const int64_t batches = (p.rows + rows - 1) / rows, wanted = (batches + kShortWarps - 1) / kShortWarps;
+  const int64_t ctas = std::min<int64_t>(wanted, (int64_t)sms * std::min(12, kSharedBytes / (bytes + 1024)));
+  short_kernel<T, W><<<(unsigned)ctas, kShortThreads, bytes, st>>>(p, b);
+  return launched();
 }
 
 template <typename T, bool Masked>
@@ -776,17 +974,17 @@ cudaError_t launch_long(const Params &p, int sms, cudaStream_t st) {
   // a cluster of CTAs while rows leave SMs without work and pieces keep four vectors a thread
   int ctas = 1;
   while (ctas < kMaxCluster && p.rows * ctas * 2 <= 2 * sms && p.actions / (ctas * 2) >= 4096) ctas *= 2;
-  if (ctas > 8) {
-    static std::atomic<uint64_t> allowed{0};
-    int dev = 0;
-    if (cudaError_t e = cudaGetDevice(&dev)) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(allowed.load(std::memory_order_acquire) & bit)) {
-      const cudaError_t e =
-          cudaFuncSetAttribute(long_kernel<T, Masked>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-      allowed.fetch_or(bit, std::memory_order_release);
-    }
+  constexpr int kRing = (int)sizeof(Ring<T, Masked>);
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(allowed.load(std::memory_order_acquire) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(long_kernel<T, Masked>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(long_kernel<T, Masked>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+    if (e != cudaSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -794,7 +992,8 @@ cudaError_t launch_long(const Params &p, int sms, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.rows, std::max(1, kLongCtas<Masked> * sms / ctas)) * ctas));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kLong);
+  cfg.dynamicSmemBytes = kRing;
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -812,9 +1011,9 @@ cudaError_t run(Params &p, bool gradient, int sms, cudaStream_t st) {
                             reinterpret_cast<uintptr_t>(p.grad) | (uintptr_t)p.actions * sizeof(T);
       return all % (w * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.legal) % w == 0;
     };
-    if (fits(4)) return short_rows<T, 4>(p, gradient, st);
-    if (fits(2)) return short_rows<T, 2>(p, gradient, st);
-    return short_rows<T, 1>(p, gradient, st);
+    if (fits(4)) return short_rows<T, 4>(p, gradient, sms, st);
+    if (fits(2)) return short_rows<T, 2>(p, gradient, sms, st);
+    return short_rows<T, 1>(p, gradient, sms, st);
   }
   if (gradient) {
     const int pieces = (p.actions + kPiece - 1) / kPiece;
