@@ -48,6 +48,9 @@ constexpr int kThreads = 256;
 constexpr int kLong = 128;
 constexpr int kWarps = kLong / 32;
 constexpr int kMaxShort = 512;      // actions of a short row
+// and, where there are eight rows an SM at least, of a row that still goes that way: 20000 x 1000
+// bf16 with 20 best 57 us (131 as long rows), its gradient 22 (41); 5000 x 4000 62 (34) and 24 (15)
+constexpr int kMaxMany = 2048, kMaxManyGradient = 1024;
 constexpr int kMaxActions = 262144;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 16;
@@ -85,6 +88,14 @@ __device__ __forceinline__ T from_f(float v) {
   if constexpr (std::is_same_v<T, float>) return v;
   if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
   if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+}
+
+// a pair of bfloat16 or float16 as floats
+template <typename T>
+__device__ __forceinline__ float2 floats(uint32_t u) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&u));
 }
 
 template <typename T, int W>
@@ -181,13 +192,22 @@ constexpr int kShortWarps = kShortThreads / 32;
 constexpr int kPartElements = 8;
 
 struct Batch {  // of a warp, in bytes from its own shared memory's begin
+  int pitch, legal_pitch;  // of a row and of its mask
   int legal, maxima, results, bytes;
   int vectors, parts;  // of a lane
 };
 
+// Rows of `row` bytes, `pitch` apart in shared memory; they are one piece
+// there unless both are multiples of 16 bytes, and so is `from`
 template <int Size>
-__device__ __forceinline__ void stage(uint8_t *to, const uint8_t *from, int bytes) {
-  const int lane = threadIdx.x & 31, phase = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+__device__ __forceinline__ void stage(uint8_t *to, const uint8_t *from, int rows, int row, int pitch) {
+  const int lane = threadIdx.x & 31, bytes = rows * row;
+  if (pitch != row) {
+    const int each = row / 16;
+    for (int i = lane; i < rows * each; i += 32) copy_async<16>(to + 16 * i + i / each * (pitch - row), from + 16 * i);
+    return;
+  }
+  const int phase = (int)(reinterpret_cast<uintptr_t>(from) & 15);
   to += phase;
   const int head = min(bytes, (16 - phase) & 15), body = (bytes - head) / 16, tail = head + 16 * body;
   for (int i = lane; i < body; i += 32) copy_async<16>(to + head + 16 * i, from + head + 16 * i);
@@ -215,21 +235,21 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_const
     int phase = 0;
     if (p.stride == p.actions || count == 1) {
       phase = (int)(reinterpret_cast<uintptr_t>(from) & 15);
-      stage<sizeof(T)>(own, reinterpret_cast<const uint8_t *>(from), count * p.actions * (int)sizeof(T));
+      stage<sizeof(T)>(own, reinterpret_cast<const uint8_t *>(from), count, p.actions * (int)sizeof(T), b.pitch);
     } else {
       for (int r = 0; r < count; ++r)
-        for (int i = lane; i < p.actions; i += 32) reinterpret_cast<T *>(own)[r * p.actions + i] = from[r * p.stride + i];
+        for (int i = lane; i < p.actions; i += 32) reinterpret_cast<T *>(own + r * b.pitch)[i] = from[r * p.stride + i];
     }
-    if (mask) stage<1>(own + b.legal, mask, count * p.actions);
+    if (mask) stage<1>(own + b.legal, mask, count, p.actions, b.legal_pitch);
     asm volatile("cp.async.wait_all;" ::: "memory");
     const bool live = mine < count;
     const int64_t row = first + mine;
     const int action = live ? p.action[row] : -1;
     __syncwarp();
 
-    Vec<T, W> *x = reinterpret_cast<Vec<T, W> *>(own + phase + (size_t)mine * p.actions * sizeof(T));
+    Vec<T, W> *x = reinterpret_cast<Vec<T, W> *>(own + phase + mine * b.pitch);
     const Vec<uint8_t, W> *legal = reinterpret_cast<const Vec<uint8_t, W> *>(
-        own + b.legal + (reinterpret_cast<uintptr_t>(mask) & 15) + (size_t)mine * p.actions);
+        own + b.legal + (reinterpret_cast<uintptr_t>(mask) & 15) + mine * b.legal_pitch);
     constexpr int kEach = kPartElements / W;  // vectors of a part
     float top = -INFINITY;
     if (live) {
@@ -350,60 +370,143 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_const
   }
 }
 
-// The gradient of short rows: a CTA's first threads gather what its rows need,
-// then all take the rows' vectors in order.
+// What a row's gradient needs: with v = (x - base) scale - log_sum, p = 2^v,
+// d = p (offset + slope v), and g more at the action.  (offset and slope are
+// negative: p goes with them.)
 struct RowGradient {
   float base, log_sum, offset, slope;
   float g;
+  int action;  // -1 where it is not kept
+};
+// in two steps, whose loads depend on one another
+template <typename T>
+struct RowLoads {
+  float top, log_sum, entropy, g, h, x;
   int action;
+  bool kept;
+  __device__ __forceinline__ void first(const Params &p, int64_t row) {
+    top = p.max_logit[row];
+    log_sum = p.log_sum[row];
+    action = p.action[row];
+    g = p.grad_log_prob ? p.grad_log_prob[row] : 0.0f;
+    h = p.grad_entropy ? p.grad_entropy[row] : 0.0f;
+    entropy = p.grad_entropy ? p.entropy[row] : 0.0f;
+  }
+  __device__ __forceinline__ void second(const Params &p, int64_t row) {
+    kept = action >= 0 && action < p.actions;
+    x = kept ? to_f(static_cast<const T *>(p.logits)[row * p.stride + action]) : 0.0f;
+    if (kept && p.legal) kept = p.legal[row * p.actions + action];
+  }
+  __device__ __forceinline__ RowGradient finish(const Params &p) const {
+    const bool keep = kept && x != -INFINITY;
+    RowGradient r = {top, log_sum * kLog2E, 0.0f, -h * p.inverse * kLn2, keep ? g * p.inverse : 0.0f, keep ? action : -1};
+    if (top == -INFINITY) r.base = r.log_sum = 0.0f;
+    r.offset = -(r.g + (h == 0.0f ? 0.0f : h * p.inverse * entropy));
+    return r;
+  }
 };
 
-// of a row, with p_i = 2^v, v = (x - base) scale - log_sum: d_i = g [i = action] - p_i (offset + slope v)
-template <typename T>
-__device__ __forceinline__ RowGradient row_gradient(const Params &p, int64_t row) {
-  const float top = p.max_logit[row], log_sum = p.log_sum[row];
-  const int a = p.action[row];
-  const bool inside = a >= 0 && a < p.actions;
-  RowGradient r = {top == -INFINITY ? 0.0f : top, log_sum * kLog2E, 0.0f, 0.0f, 0.0f, inside ? a : -1};
-  if (p.grad_log_prob && inside && (!p.legal || p.legal[row * p.actions + a]) &&
-      to_f(static_cast<const T *>(p.logits)[row * p.stride + a]) != -INFINITY)
-    r.g = p.grad_log_prob[row] * p.inverse;
-  const float h = p.grad_entropy ? p.grad_entropy[row] * p.inverse : 0.0f;
-  r.offset = r.g + (h == 0.0f ? 0.0f : h * p.entropy[row]);
-  r.slope = h * kLn2;
-  return r;
+__device__ __forceinline__ float2 gradient_of(const RowGradient &r, float2 x, float scale) {
+  float2 v = __ffma2_rn(__fadd2_rn(x, make_float2(-r.base, -r.base)), make_float2(scale, scale),
+                        make_float2(-r.log_sum, -r.log_sum));
+  v = make_float2(max_nan(v.x, kNothing), max_nan(v.y, kNothing));
+  return __fmul2_rn(make_float2(exp2_fast(v.x), exp2_fast(v.y)),
+                    __ffma2_rn(make_float2(r.slope, r.slope), v, make_float2(r.offset, r.offset)));
+}
+__device__ __forceinline__ float gradient_of(const RowGradient &r, float x, float scale) {
+  const float v = max_nan(fmaf(x - r.base, scale, -r.log_sum), kNothing);
+  return exp2_fast(v) * fmaf(r.slope, v, r.offset);
 }
 
-__device__ __forceinline__ float gradient_of(const RowGradient &r, float x, int i, float scale) {
-  const float v = max_nan((x - r.base) * scale - r.log_sum, kNothing);
-  const float d = -exp2_fast(v) * fmaf(r.slope, v, r.offset);
-  return x == -INFINITY ? 0.0f : i == r.action ? d + r.g : d;
-}
-
-constexpr int kMaxRows = 256;  // of a CTA
-template <typename T, int W>
+// The gradient of short rows.  CTAs take groups of rows in turn, whole 16-byte
+// pieces of them in order where rows are dense (C cells of W elements each, a
+// cell within a row); a group's first threads gather what the next one's rows
+// need while this one is computed.
+constexpr int kMaxRows = 256;  // of a group
+constexpr int kGroupElements = 6144;
+template <typename T, int W, int C>
 __global__ void __launch_bounds__(kThreads) short_gradient_kernel(const __grid_constant__ Params p, int rows,
                                                                   uint32_t reciprocal) {
-  __shared__ RowGradient table[kMaxRows];
-  const int64_t first = (int64_t)blockIdx.x * rows;
-  const int count = (int)min((int64_t)rows, p.rows - first), all = p.actions / W;
-  if ((int)threadIdx.x < count) table[threadIdx.x] = row_gradient<T>(p, first + threadIdx.x);
+  constexpr int N = W * C;
+  __shared__ RowGradient tables[2][kMaxRows];
+  const int all = p.actions / W;  // cells of a row
+  const int64_t groups = (p.rows + rows - 1) / rows;
+  const bool gathers = (int)threadIdx.x < rows;
+  RowLoads<T> loads;
+  {
+    const int64_t row = (int64_t)blockIdx.x * rows + threadIdx.x;
+    if (gathers && row < p.rows) {
+      loads.first(p, row);
+      loads.second(p, row);
+      tables[0][threadIdx.x] = loads.finish(p);
+    }
+  }
   __syncthreads();
-  const T *logits = static_cast<const T *>(p.logits) + first * p.stride;
-  const uint8_t *legal = p.legal ? p.legal + first * p.actions : nullptr;
-  T *grad = static_cast<T *>(p.grad) + first * p.actions;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < count * all; i += kThreads) {
-    const int row = all == 1 ? i : (int)__umulhi((uint32_t)i, reciprocal), a = (i - row * all) * W;
-    const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(logits + row * p.stride + a);
-    Vec<uint8_t, W> keep;
-    if (legal) keep = *reinterpret_cast<const Vec<uint8_t, W> *>(legal + i * W);
-    const RowGradient r = table[row];
-    Vec<T, W> out;
+  int turn = 0;
+  for (int64_t group = blockIdx.x; group < groups; group += gridDim.x, turn ^= 1) {
+    const int64_t first = group * rows, next = (group + gridDim.x) * rows + threadIdx.x;
+    const int count = (int)min((int64_t)rows, p.rows - first), cells = count * all;
+    const RowGradient *table = tables[turn];
+    const T *logits = static_cast<const T *>(p.logits) + first * p.stride;
+    const uint8_t *legal = p.legal ? p.legal + first * p.actions : nullptr;
+    T *grad = static_cast<T *>(p.grad) + first * p.actions;
+    const bool gather = gathers && next < p.rows;
+    if (gather) loads.first(p, next);
+    for (int begin = 0; begin < cells; begin += kThreads * C) {
+      const int cell = begin + (int)threadIdx.x * C;
+      int row = all == 1 ? cell : (int)__umulhi((uint32_t)cell, reciprocal), at = cell - row * all;
+      Vec<T, N> q;
+      Vec<uint8_t, N> keep;
+      const bool whole = cell + C <= cells;
+      if (whole) {
+        q = *reinterpret_cast<const Vec<T, N> *>(C > 1 ? logits + cell * W : logits + row * p.stride + at * W);
+        if (legal) keep = *reinterpret_cast<const Vec<uint8_t, N> *>(legal + cell * W);
+      } else if (cell < cells) {
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-      out.v[w] = from_f<T>(gradient_of(r, !legal || keep.v[w] ? to_f(q.v[w]) : -INFINITY, a + w, p.scale));
-    *reinterpret_cast<Vec<T, W> *>(grad + i * W) = out;
+        for (int n = 0; n < N; ++n)
+          if (cell * W + n < cells * W) {
+            q.v[n] = C > 1 ? logits[cell * W + n] : logits[row * p.stride + at * W + n];
+            keep.v[n] = !legal || legal[cell * W + n];
+          }
+      }
+      if (begin == 0 && gather) loads.second(p, next);
+      if (cell >= cells) continue;
+      Vec<T, N> out;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const RowGradient r = table[row < count ? row : 0];
+        float d[W];
+        if constexpr (W % 2 == 0) {
+#pragma unroll
+          for (int w = 0; w < W; w += 2) {
+            const float2 two = gradient_of(r, make_float2(to_f(q.v[c * W + w]), to_f(q.v[c * W + w + 1])), p.scale);
+            d[w] = two.x;
+            d[w + 1] = two.y;
+          }
+        } else {
+          d[0] = gradient_of(r, to_f(q.v[c]), p.scale);
+        }
+        const int action = r.action - at * W;  // of the cell
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          if (w == action) d[w] += r.g;
+          out.v[c * W + w] = from_f<T>(legal && !keep.v[c * W + w] ? 0.0f : d[w]);
+        }
+        if (++at == all) {
+          at = 0;
+          ++row;
+        }
+      }
+      if (whole) {
+        *reinterpret_cast<Vec<T, N> *>(grad + cell * W) = out;
+      } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (cell * W + n < cells * W) grad[cell * W + n] = out.v[n];
+      }
+    }
+    if (gather) tables[turn ^ 1][threadIdx.x] = loads.finish(p);
+    __syncthreads();
   }
 }
 
@@ -469,6 +572,22 @@ struct Slice {
     return back < head ? back : back - head < actions - tail ? tail + back - head : -1;
   }
   __device__ int first(int v) const { return head + v * W; }
+  // the mask's bytes of the W elements from `a` on
+  __device__ void mask(const Params &p, int a, uint32_t (&m)[W / 4]) const {
+    const uint8_t *bytes = legal + a;
+    const int off = (int)(reinterpret_cast<uintptr_t>(bytes) & 3);
+    const uint32_t *word = reinterpret_cast<const uint32_t *>(bytes - off);
+    if (off == 0) {
+#pragma unroll
+      for (int w = 0; w < W / 4; ++w) m[w] = word[w];
+    } else if (bytes - off >= p.legal && bytes + W + 4 <= p.legal + p.rows * p.actions) {
+#pragma unroll
+      for (int w = 0; w < W / 4; ++w) m[w] = __funnelshift_r(word[w], word[w + 1], 8 * off);
+    } else {
+#pragma unroll
+      for (int w = 0; w < W; ++w) m[w / 4] = (w & 3 ? m[w / 4] : 0u) | (uint32_t)bytes[w] << (8 * (w & 3));
+    }
+  }
   // how far a vector's mask begins behind a word's
   __device__ int shift(int v) const { return (int)(reinterpret_cast<uintptr_t>(legal + first(v)) & 3); }
   // requests the vectors v, v + threads, ...; -inf where there is none
@@ -525,14 +644,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
-}
-
-// A pair (bfloat16, float16) or two words (float32) as floats
-template <typename T>
-__device__ __forceinline__ float2 floats(uint32_t u) {
-  if constexpr (std::is_same_v<T, __nv_bfloat16>)
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  return __half22float2(*reinterpret_cast<const __half2 *>(&u));
 }
 
 // A chunk as pairs of floats, what is below kFloor raised to it, NaN kept.
@@ -885,31 +996,78 @@ __global__ void __launch_bounds__(kLong, kLongCtas<Masked>) long_kernel(const __
 }
 
 // A long row's gradient: elements alone, so a CTA takes a piece of a row.
-constexpr int kPiece = 8192;
+// Vectors where a row and its gradient lie alike.
+constexpr int kAhead = 4;  // vectors of a thread, whose loads are in flight together
 template <typename T, bool Vector>
+constexpr int kPiece = kThreads * kAhead * (Vector ? 16 / (int)sizeof(T) : 4);
+template <typename T, bool Vector, bool Masked>
 __global__ void __launch_bounds__(kThreads) long_gradient_kernel(const __grid_constant__ Params p, int pieces) {
-  constexpr int W = Vector ? 16 / sizeof(T) : 1;
+  constexpr int W = 16 / sizeof(T);
   const int64_t row = blockIdx.x / pieces;
   const int piece = blockIdx.x - (int)(row * pieces);
-  const T *x = static_cast<const T *>(p.logits) + row * p.stride;
-  const uint8_t *legal = p.legal ? p.legal + row * p.actions : nullptr;
+  const Slice<T, Masked> slice(p, row);
+  const T *x = slice.x;
   T *grad = static_cast<T *>(p.grad) + row * p.actions;
-  const RowGradient r = row_gradient<T>(p, row);
-  auto scalar = [&](int i) { grad[i] = from_f<T>(gradient_of(r, !legal || legal[i] ? to_f(x[i]) : -INFINITY, i, p.scale)); };
-  const int head = Vector ? min(p.actions, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T)) : 0;
-  const int begin = head + piece * kPiece, whole = (p.actions - head) / W * W + head;
-  const int end = min(whole, begin + kPiece);
-  if (piece == 0 && (int)threadIdx.x < head) scalar(threadIdx.x);
-  if (piece == pieces - 1 && whole + (int)threadIdx.x < p.actions) scalar(whole + threadIdx.x);
-#pragma unroll 4
-  for (int i = begin + (int)threadIdx.x * W; i < end; i += kThreads * W) {
-    const Vec<T, W> q = *reinterpret_cast<const Vec<T, W> *>(x + i);
-    Vec<T, W> out;
+  const int head = Vector ? slice.head : 0, begin = head + piece * kPiece<T, Vector>;
+  const int whole = Vector ? slice.first(slice.vectors) : p.actions;
+  RowLoads<T> loads;
+  loads.first(p, row);
+  if constexpr (Vector) {
+    uint4 q[kAhead];
+    uint32_t m[Masked ? kAhead : 1][W / 4];
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-      out.v[w] = from_f<T>(gradient_of(r, !legal || legal[i + w] ? to_f(q.v[w]) : -INFINITY, i + w, p.scale));
-    *reinterpret_cast<Vec<T, W> *>(grad + i) = out;
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = begin + (k * kThreads + (int)threadIdx.x) * W;
+      if (i >= whole) continue;
+      q[k] = *reinterpret_cast<const uint4 *>(x + i);
+      if constexpr (Masked) slice.mask(p, i, m[k]);
+    }
+    loads.second(p, row);
+    const RowGradient r = loads.finish(p);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = begin + (k * kThreads + (int)threadIdx.x) * W;
+      if (i >= whole) continue;
+      if constexpr (Masked) apply<T>(m[k], q[k]);
+      uint32_t *word = reinterpret_cast<uint32_t *>(&q[k]);
+#pragma unroll
+      for (int w = 0; w < 4; w += sizeof(T) == 4 ? 2 : 1) {
+        if constexpr (sizeof(T) == 4) {
+          const float2 d = gradient_of(r, make_float2(__uint_as_float(word[w]), __uint_as_float(word[w + 1])), p.scale);
+          word[w] = __float_as_uint(d.x);
+          word[w + 1] = __float_as_uint(d.y);
+        } else {
+          const float2 d = gradient_of(r, floats<T>(word[w]), p.scale);
+          if constexpr (std::is_same_v<T, __half>)
+            *reinterpret_cast<__half2 *>(&word[w]) = __floats2half2_rn(d.x, d.y);
+          else
+            *reinterpret_cast<__nv_bfloat162 *>(&word[w]) = __floats2bfloat162_rn(d.x, d.y);
+        }
+      }
+      *reinterpret_cast<uint4 *>(grad + i) = q[k];
+    }
+  } else {
+    loads.second(p, row);
+    const RowGradient r = loads.finish(p);
+#pragma unroll 4
+    for (int k = 0; k < kPiece<T, Vector> / kThreads; ++k) {
+      const int i = begin + k * kThreads + (int)threadIdx.x;
+      if (i < whole) grad[i] = from_f<T>(gradient_of(r, slice.element(i), p.scale));
+    }
   }
+  const RowGradient r = loads.finish(p);
+  // the elements before the first vector and behind the last
+  if (Vector && piece == 0) {
+    const int i = (int)threadIdx.x < head ? (int)threadIdx.x : whole + (int)threadIdx.x - head;
+    if (i < head || (i >= whole && i < p.actions)) grad[i] = from_f<T>(gradient_of(r, slice.element(i), p.scale));
+  }
+  // the action's element once more, by one thread behind a barrier: testing every vector costs the others 10 %
+  const bool here = r.action >= 0 && (r.action < head || r.action >= whole
+                                          ? piece == 0
+                                          : (r.action - head) / kPiece<T, Vector> == piece);
+  if (!here) return;
+  __syncthreads();
+  if (threadIdx.x == 0) grad[r.action] = from_f<T>(gradient_of(r, loads.x, p.scale) + r.g);
 }
 
 // ---------------------------------------------------------------------------
@@ -926,30 +1084,40 @@ cudaError_t launched() {
 // Rows and lanes of a batch: the fewest lanes a row with which reads of
 // neighbouring rows share no bank, a warp's rows stay within kBatchBytes, and
 // (when rows are few) every SM has eight warps' work.
-constexpr int kBatchBytes = 14 * 1024, kSharedBytes = 220 * 1024;
+constexpr int kBatchBytes = 11 * 1024, kSharedBytes = 220 * 1024;
 template <typename T, int W>
 cudaError_t short_rows(Params &p, bool gradient, int sms, cudaStream_t st) {
   const int all = p.actions / W;
   if (gradient) {
-    const int rows = std::max(1, std::min(kMaxRows, 6144 / p.actions));
-    const int64_t ctas = (p.rows + rows - 1) / rows;
-    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-    // i / all for i below 6144: the quotient's error i / 2^32 stays below 1 / all (all <= 512)
+    // (whole eights of rows: a group then begins on a 16-byte boundary where the first does)
+    const int rows = std::max(8, std::min(kMaxRows, kGroupElements / p.actions / 8 * 8));
+    // cell / all for cells below 2^13 (8 rows of 512, or kGroupElements): the quotient's error cell / 2^32 stays below 1 / all
     const uint32_t reciprocal = (uint32_t)((1ull << 32) / all + 1);
-    short_gradient_kernel<T, W><<<(unsigned)ctas, kThreads, 0, st>>>(p, rows, reciprocal);
+    const unsigned ctas = (unsigned)std::min<int64_t>((p.rows + rows - 1) / rows, (int64_t)sms * 8);
+    constexpr int C = 16 / (W * (int)sizeof(T));
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.grad);
+    if (C > 1 && at % 16 == 0 && reinterpret_cast<uintptr_t>(p.legal) % (W * C) == 0 && p.stride == p.actions)
+      short_gradient_kernel<T, W, C><<<ctas, kThreads, 0, st>>>(p, rows, reciprocal);
+    else
+      short_gradient_kernel<T, W, 1><<<ctas, kThreads, 0, st>>>(p, rows, reciprocal);
     return launched();
   }
   const int row_bytes = p.actions * ((int)sizeof(T) + (p.legal ? 1 : 0));
-  p.group = std::min(8, all & -all);
-  if (W * sizeof(T) < 16 && all % 2 == 0) p.group = std::min(8, p.group * 2);
+  // rows of whole 16-byte pieces lie 16 bytes further apart where that is odd, others share banks
+  auto apart = [](const void *q, int64_t bytes) {
+    return bytes % 32 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 ? (int)bytes + 16 : (int)bytes;
+  };
+  Batch b;
+  b.pitch = apart(p.logits, (int64_t)p.actions * sizeof(T));
+  b.legal_pitch = apart(p.legal, p.actions);
+  p.group = b.pitch != p.actions * (int)sizeof(T) ? 1 : std::min(8, all & -all);
   while (p.group < 32 && (32 / p.group * row_bytes > kBatchBytes || p.rows * p.group < (int64_t)8 * 32 * sms)) p.group *= 2;
   const int rows = 32 / p.group;
   auto up = [](int n) { return (n + 15) / 16 * 16; };
-  Batch b;
   b.vectors = (all + p.group - 1) / p.group;
   b.parts = (b.vectors * W + kPartElements - 1) / kPartElements;
-  b.legal = up(rows * p.actions * (int)sizeof(T) + 16);
-  b.maxima = b.legal + (p.legal ? up(rows * p.actions + 16) : 0);
+  b.legal = up(rows * b.pitch + 16);
+  b.maxima = b.legal + (p.legal ? up(rows * b.legal_pitch + 16) : 0);
   b.results = b.maxima + (p.top ? 128 * b.parts : 0);
   b.bytes = b.results + up(8 * rows * p.top);
   const int bytes = kShortWarps * b.bytes;
@@ -966,6 +1134,14 @@ cudaError_t short_rows(Params &p, bool gradient, int sms, cudaStream_t st) {
   const int64_t batches = (p.rows + rows - 1) / rows, wanted = (batches + kShortWarps - 1) / kShortWarps;
   const int64_t ctas = std::min<int64_t>(wanted, (int64_t)sms * std::min(12, kSharedBytes / (bytes + 1024)));
   short_kernel<T, W><<<(unsigned)ctas, kShortThreads, bytes, st>>>(p, b);
+  return launched();
+}
+
+template <typename T, bool Vector, bool Masked>
+cudaError_t launch_gradient(const Params &p, cudaStream_t st) {
+  const int pieces = (p.actions + kPiece<T, Vector> - 1) / kPiece<T, Vector>;
+  if (p.rows * pieces > 0x7fffffff) return cudaErrorInvalidValue;
+  long_gradient_kernel<T, Vector, Masked><<<(unsigned)(p.rows * pieces), kThreads, 0, st>>>(p, pieces);
   return launched();
 }
 
@@ -1004,7 +1180,7 @@ cudaError_t launch_long(const Params &p, int sms, cudaStream_t st) {
 
 template <typename T>
 cudaError_t run(Params &p, bool gradient, int sms, cudaStream_t st) {
-  if (p.actions <= kMaxShort) {
+  if (p.actions <= kMaxShort || (p.actions <= (gradient ? kMaxManyGradient : kMaxMany) && p.rows >= (int64_t)8 * sms)) {
     // the widest loads that rows' places allow
     auto fits = [&](int w) {
       const uintptr_t all = reinterpret_cast<uintptr_t>(p.logits) | (uintptr_t)p.stride * sizeof(T) |
@@ -1016,16 +1192,10 @@ cudaError_t run(Params &p, bool gradient, int sms, cudaStream_t st) {
     return short_rows<T, 1>(p, gradient, sms, st);
   }
   if (gradient) {
-    const int pieces = (p.actions + kPiece - 1) / kPiece;
-    if (p.rows * pieces > 0x7fffffff) return cudaErrorInvalidValue;
-    // vectors where a row and its gradient lie alike
     const bool vector = !(((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.grad)) & 15) ||
                           (p.rows > 1 && ((p.stride - p.actions) * sizeof(T) & 15)));
-    if (vector)
-      long_gradient_kernel<T, true><<<(unsigned)(p.rows * pieces), kThreads, 0, st>>>(p, pieces);
-    else
-      long_gradient_kernel<T, false><<<(unsigned)(p.rows * pieces), kThreads, 0, st>>>(p, pieces);
-    return launched();
+    if (p.legal) return vector ? launch_gradient<T, true, true>(p, st) : launch_gradient<T, false, true>(p, st);
+    return vector ? launch_gradient<T, true, false>(p, st) : launch_gradient<T, false, false>(p, st);
   }
   return p.legal ? launch_long<T, true>(p, sms, st) : launch_long<T, false>(p, sms, st);
 }

@@ -129,7 +129,8 @@ def policy_log_probs_gradient(logits: torch.Tensor, action: torch.Tensor, out: L
     mask and temperature (its entropy, max_logit and log_sum are read).  The
     gradients are floating point of the rows' shape; either may be absent,
     not both.  An action without a log-probability (out of range, illegal,
-    -inf) has no gradient of it; illegal actions and those of -inf have 0.
+    -inf) has no gradient of it; illegal actions and those of -inf have 0
+    (in a row whose numbers are NaN the gradient may be NaN throughout).
 
     The gradient is returned, not recorded: ``logits.backward(gradient)``
     continues it.  float16 ends at 6e-8: put a loss scale into the gradients
