@@ -9,6 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libscacchi_b200.so")
+HOST = os.path.join(HERE, "_host.so")  # Python's calls of some operators (csrc/host.cpp)
 # (source, extra flags).  The search kernels are bit-reproducible against
 # the oracle: no implicit multiply-add contraction (they call fmaf()
 # explicitly where they want one), and the AdamW step's 8-bit codes against
@@ -40,6 +41,8 @@ def stale() -> bool:
 
 def build(force: bool = False, verbose: bool = False, out: str | None = None, defines: tuple = ()) -> str:
     out = out or LIB
+    if out == LIB:
+        build_host(force)
     if out == LIB and not force and not stale():
         return LIB
     objs = []
@@ -58,6 +61,27 @@ def build(force: bool = False, verbose: bool = False, out: str | None = None, de
             raise RuntimeError("nvcc failed")
     subprocess.run([nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", out, *objs], check=True)
     return out
+
+
+def build_host(force: bool = False) -> str:
+    """The extension module, by the host's compiler against torch's headers."""
+    src, header = os.path.join(CSRC, "host.cpp"), os.path.join(ROOT, "include", "scacchi_b200.h")
+    if not force and os.path.exists(HOST) and all(os.path.getmtime(p) <= os.path.getmtime(HOST) for p in (src, header)):
+        return HOST
+    import sysconfig
+
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc())) or "/usr/local/cuda"
+    part = f"{HOST}.{os.getpid()}"  # renamed when whole: several processes may build at once
+    subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{base}/include",
+                    f"-I{base}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
+                    f"-I{cuda}/include", src, "-o", part, f"-L{base}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+                    "-lc10", "-lc10_cuda", f"-Wl,-rpath,{base}/lib"], check=True)
+    os.replace(part, HOST)
+    return HOST
 
 
 if __name__ == "__main__":

@@ -207,6 +207,20 @@ def lib() -> C.CDLL:
     return handle
 
 
+@functools.lru_cache(maxsize=None)
+def host():
+    """The extension module bound to the library, built first if it is missing."""
+    if not os.path.exists(_build.HOST):
+        _build.build_host()
+    from . import _host
+
+    handle = lib()
+    _host.bind(*(C.cast(getattr(handle, n), C.c_void_p).value for n in (
+        "scacchi_log_probs", "scacchi_log_probs_gradient", "scacchi_gradient_norm",
+        "scacchi_gradient_norm_workspace_bytes", "scacchi_adamw_step", "scacchi_adamw_moments")))
+    return _host
+
+
 def check(rc: int, what: str) -> None:
     if rc == OK:
         return

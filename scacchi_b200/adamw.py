@@ -70,6 +70,9 @@ def gradient_norm(gradients: Iterable[torch.Tensor] | Mapping[str, torch.Tensor]
     captured into a CUDA graph.
     """
     grads = list(gradients.values() if isinstance(gradients, Mapping) else gradients)
+    done = _lib.host().gradient_norm(grads)
+    if done is not None:
+        return done
     if not grads:
         raise ValueError("gradient_norm needs at least one gradient")
     device = grads[0].device
@@ -168,7 +171,8 @@ class AdamW:
             if b[0] < a[1]:
                 raise ValueError(f"{a[2]} and {b[2]} share memory")
         words = (0, 0) if key is None else tuple(int(k) & 0xFFFFFFFF for k in np.asarray(key, np.uint32).reshape(2))
-        self.weights, self.device, self.state_bits, self.max_norm = dict(weights), device, state_bits, max_norm
+        self.weights, self.device, self.state_bits = dict(weights), device, state_bits
+        self.max_norm = None if max_norm is None else float(max_norm)
         self._names, self._tensors = tuple(weights), tuple(weights.values())
         self._shapes = [w.shape for w in self._tensors]
         self._table = table
@@ -226,6 +230,10 @@ class AdamW:
         call launches on the current stream, does not synchronise and can be
         captured into a CUDA graph.
         """
+        done = _lib.host().adamw_step(self._names, self._tensors, gradients, self._table.ctypes.data,
+                                      C.addressof(self._params), self.device.index, self.max_norm, norm, learning_rate)
+        if done is not None:
+            return done[0]
         grads = self._gradients(gradients)
         for name, t in (("norm", norm), ("learning_rate", learning_rate)):
             if isinstance(t, torch.Tensor) and (t.dtype != torch.float32 or t.numel() != 1 or t.device != self.device):
@@ -240,13 +248,17 @@ class AdamW:
 
     def _step(self, grads: list, norm, learning_rate):
         table = self._table
+        for name, w, row in zip(self._names, self._tensors, table):
+            if w.numel() != row["count"] or WEIGHT_DTYPES.get(w.dtype) != row["weight_dtype"] or not w.is_contiguous():
+                raise ValueError(f"{name} has changed its size, type or layout since AdamW was made")
         table["weight"] = [w.data_ptr() for w in self._tensors]
         table["gradient"] = [0 if g is None else g.data_ptr() for g in grads]
         table["gradient_dtype"] = [0 if g is None else GRADIENT_DTYPES[g.dtype] for g in grads]
         if self.max_norm is not None and norm is None:
             norm = _norm(table[[g is not None for g in grads]], self.device)
         params = _lib.AdamWStep.from_buffer_copy(self._params)
-        params.norm = None if norm is None else norm.data_ptr()
+        if norm is not None:
+            params.norm, params.max_norm = norm.data_ptr(), float(self.max_norm)
         if isinstance(learning_rate, torch.Tensor):
             params.learning_rate_at = learning_rate.data_ptr()
         elif learning_rate is not None:
@@ -273,6 +285,9 @@ class AdamW:
         their codes stand for, without rounding; those of 32 as float32."""
         if self.state_bits == 32:
             return self.first.clone(), self.second.sqrt()
+        done = _lib.host().adamw_moments(self.first, self.second, self.first_exponent, self.second_exponent)
+        if done is not None:
+            return done
         with torch.cuda.device(self.device):
             first = torch.empty(self.first.shape, dtype=torch.bfloat16, device=self.device)
             root = torch.empty_like(first)

@@ -52,8 +52,8 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;   // elements that share an exponent; tensors begin at whole blocks
 constexpr int kChunk = 4096;  // elements of a tensor that a CTA takes
-constexpr int kNormChunk = 16384;
-constexpr int kMaxPartials = 148 * 8;
+constexpr int kNormChunk = 8192;
+constexpr int kMaxPartials = 148 * 6;  // CTAs of a norm's launch
 constexpr int kMaxDtype = 2;
 
 // What a step's launches share, in device memory.
@@ -400,24 +400,41 @@ __device__ __forceinline__ double cta_sum(double v) {
 // not depend on the launch's shape.
 template <typename T>
 __device__ __forceinline__ double squares(const Entry &e, int64_t begin) {
-  constexpr int W = 16 / sizeof(T);
+  constexpr int W = 16 / sizeof(T), kAhead = 4;  // vectors of a thread in flight together
   const T *x = static_cast<const T *>(e.gradient);
   const int64_t end = min(e.count, begin + kNormChunk);
-  const bool aligned = e.kind & 16;
   double sum = 0.0;
-#pragma unroll 4
-  for (int64_t i = begin + (int)threadIdx.x * W; i < end; i += kThreads * W) {
-    float f[W];
-    load<T, W>(x, i, e.count, aligned && i + W <= e.count, f);
+  if (e.kind & 16) {
+    for (int64_t i = begin + (int)threadIdx.x * W; i < end; i += kAhead * kThreads * W) {
+      float f[kAhead][W];
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum = fma((double)f[w], (double)f[w], sum);
+      for (int k = 0; k < kAhead; ++k) {
+        const int64_t at = i + k * kThreads * W;
+        if (at < end)
+          load<T, W>(x, at, e.count, at + W <= e.count, f[k]);
+        else
+#pragma unroll
+          for (int w = 0; w < W; ++w) f[k][w] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum = fma((double)f[k][w], (double)f[k][w], sum);
+    }
+  } else {
+#pragma unroll 4
+    for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) {
+      const double f = (double)to_f(x[i]);
+      sum = fma(f, f, sum);
+    }
   }
   return sum;
 }
 
+constexpr int kNormCtas = 6;  // of an SM
 template <int N>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<N> table, int chunks,
-                                                        double *partial) {
+__global__ void __launch_bounds__(kThreads, kNormCtas) norm_kernel(const __grid_constant__ Table<N> table, int chunks,
+                                                                   double *partial) {
   double sum = 0.0;
   for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const Entry &e = table.entry[find(table, chunk)];
@@ -521,9 +538,7 @@ cudaError_t launch_norm(const Chunked &all, double *partial, int *partials, cuda
   static thread_local Table<N> table;
   size_t at = 0;
   while (const int chunks = fill(table, all, at)) {
-    const int launches_left = (int)((all.entries.size() - at + N - 1) / N);
     const int ctas = std::min(chunks, kMaxPartials);
-    (void)launches_left;
     norm_kernel<N><<<ctas, kThreads, 0, st>>>(table, chunks, partial + *partials);
     if (cudaError_t e = launched()) return e;
     *partials += ctas;

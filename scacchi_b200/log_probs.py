@@ -93,6 +93,9 @@ def policy_log_probs(logits: torch.Tensor, action: torch.Tensor, *, legal: torch
     is outside autograd.  The call launches on the current stream, does not
     synchronise and can be captured into a CUDA graph.
     """
+    done = _lib.host().log_probs(logits, action, legal, temperature, top)
+    if done is not None:
+        return LogProbs(*done)
     _check("policy_log_probs", logits, action, legal, temperature)
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top must be in [0, {MAX_TOP}], got {top}")
@@ -137,6 +140,10 @@ def policy_log_probs_gradient(logits: torch.Tensor, action: torch.Tensor, out: L
     where rows are many.  The call launches on the current stream, does not
     synchronise and can be captured into a CUDA graph.
     """
+    done = _lib.host().log_probs_gradient(logits, action, legal, temperature, out.max_logit, out.log_sum, out.entropy,
+                                          grad_log_prob, grad_entropy)
+    if done is not None:
+        return done
     _check("policy_log_probs_gradient", logits, action, legal, temperature)
     if grad_log_prob is None and grad_entropy is None:
         raise ValueError("pass grad_log_prob, grad_entropy or both")
