@@ -132,8 +132,8 @@ class AdamW:
         for name, b in (("beta1", beta1), ("beta2", beta2)):
             if not 0.0 <= b < 1.0:
                 raise ValueError(f"{name} must be in [0, 1), got {b}")
-        if not 0.0 <= eps <= 1e30:
-            raise ValueError(f"eps must be in [0, 1e30], got {eps}")
+        if not (eps == 0.0 or 1e-30 <= eps <= 1e30):
+            raise ValueError(f"eps must be 0 or in [1e-30, 1e30], got {eps}")
         if not math.isfinite(learning_rate):
             raise ValueError(f"learning_rate must be finite, got {learning_rate}")
         if max_norm is not None and not 0.0 < max_norm < math.inf:

@@ -51,7 +51,11 @@ std::atomic<uint64_t> g_adamw_launches{0};
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;   // elements that share an exponent; tensors begin at whole blocks
-constexpr int kChunk = 4096;  // elements of a tensor that a CTA takes
+// Elements of a tensor that a CTA takes.  Longer chunks put the CTAs of a
+// moment further apart in memory, and powers of two meet the same channels: a
+// step of 67.1 M bfloat16 weights with 8-bit moments 215 us with 4096, 237 with
+// 2048, 299 with 8192, 267 with 16384.
+constexpr int kChunk = 4096;
 constexpr int kNormChunk = 8192;
 constexpr int kMaxPartials = 148 * 6;  // CTAs of a norm's launch
 constexpr int kMaxDtype = 2;
@@ -114,190 +118,306 @@ __device__ __forceinline__ float to_f(T v) {
   if constexpr (std::is_same_v<T, __half>) return __half2float(v);
 }
 
-template <typename T, int W>
-struct alignas(sizeof(T) * W > 16 ? 16 : sizeof(T) * W) Vec {
-  T v[W];
-};
-
-// W elements at x[i], zero past `count`
-template <typename T, int W>
-__device__ __forceinline__ void load(const T *x, int64_t i, int64_t count, bool whole, float (&f)[W]) {
-  if (whole) {
-    const Vec<T, W> p = *reinterpret_cast<const Vec<T, W> *>(x + i);
-#pragma unroll
-    for (int w = 0; w < W; ++w) f[w] = to_f(p.v[w]);
-  } else {
-#pragma unroll
-    for (int w = 0; w < W; ++w) f[w] = i + w < count ? to_f(x[i + w]) : 0.0f;
-  }
-}
-
-// A weight's type: float32 as it is, bfloat16 to nearest or by random bits
+// Four elements as they lie in memory.  A tensor's whole vectors are loaded and
+// stored at once; what stands off a 16-byte boundary or at the tensor's end
+// goes element by element.  Nothing is converted on either way, so that a
+// thread's loads are all on their way before it waits for the first.
 template <typename T>
-__device__ __forceinline__ T to_weight(float w, bool stochastic, uint32_t random) {
-  if constexpr (std::is_same_v<T, float>) {
-    return w;
+using Four = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
+
+template <typename T>
+using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+template <typename T>
+__device__ __forceinline__ Four<T> load_slowly(const T *x, int64_t i, int64_t count) {
+  const Bits<T> *from = reinterpret_cast<const Bits<T> *>(x) + i;
+  const uint32_t a = i < count ? from[0] : 0, b = i + 1 < count ? from[1] : 0, c = i + 2 < count ? from[2] : 0,
+                 d = i + 3 < count ? from[3] : 0;
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(a, b, c, d);
+  else
+    return make_uint2(a | b << 16, c | d << 16);
+}
+template <typename T>
+__device__ __forceinline__ void store_slowly(T *x, int64_t i, int64_t count, const Four<T> &q) {
+  Bits<T> *to = reinterpret_cast<Bits<T> *>(x) + i;
+  if constexpr (sizeof(T) == 4) {
+    if (i < count) to[0] = q.x;
+    if (i + 1 < count) to[1] = q.y;
+    if (i + 2 < count) to[2] = q.z;
+    if (i + 3 < count) to[3] = q.w;
   } else {
-    if (!stochastic || w != w) return __float2bfloat16_rn(w);
-    return __ushort_as_bfloat16((unsigned short)((__float_as_uint(w) + (random * 0x85ebu & 0xffffu)) >> 16));
+    if (i < count) to[0] = (uint16_t)q.x;
+    if (i + 1 < count) to[1] = (uint16_t)(q.x >> 16);
+    if (i + 2 < count) to[2] = (uint16_t)q.y;
+    if (i + 3 < count) to[3] = (uint16_t)(q.y >> 16);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 pair_of(Four<T> q, int pair) {
+  if constexpr (sizeof(T) == 4) {
+    return pair ? make_float2(__uint_as_float(q.z), __uint_as_float(q.w))
+                : make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+  } else {
+    const uint32_t u = pair ? q.y : q.x;
+    if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
 }
 
-template <typename T, int W>
-__device__ __forceinline__ void store(T *x, int64_t i, int64_t count, bool whole, const Vec<T, W> &p) {
-  if (whole) {
-    *reinterpret_cast<Vec<T, W> *>(x + i) = p;
-  } else {
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-      if (i + w < count) x[i + w] = p.v[w];
+// one of the two sixteen bits of a word
+__device__ __forceinline__ uint32_t half_of(uint32_t word, int i) { return i & 1 ? word >> 16 : word & 0xffffu; }
+
+// A pair of weights as bfloat16: to nearest, or up where the random bits reach
+// (the upper halves of sums; a NaN would run over)
+__device__ __forceinline__ uint32_t to_pair(float a, float b, bool stochastic, uint32_t ra, uint32_t rb) {
+  if (!stochastic || a != a || b != b) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(a, b);
+    if (!stochastic) return *reinterpret_cast<const uint32_t *>(&two);
+    const uint32_t x = a != a ? 0x7fff0000u : __float_as_uint(a) + (ra * 0x85eb0000u >> 16);
+    const uint32_t y = b != b ? 0x7fff0000u : __float_as_uint(b) + (rb * 0x85eb0000u >> 16);
+    return __byte_perm(x, y, 0x7632);
   }
+  return __byte_perm(__float_as_uint(a) + (ra * 0x85eb0000u >> 16), __float_as_uint(b) + (rb * 0x85eb0000u >> 16), 0x7632);
+}
+template <typename T>
+__device__ __forceinline__ Four<T> to_weights(float2 a, float2 b, bool stochastic, uint2 random) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+  else
+    return make_uint2(to_pair(a.x, a.y, stochastic, half_of(random.x, 0), half_of(random.x, 1)),
+                      to_pair(b.x, b.y, stochastic, half_of(random.y, 0), half_of(random.y, 1)));
 }
 
 __device__ __forceinline__ float power_of_two(int field) { return __int_as_float(field << 23); }
 
-// Sixteen random bits of each of four elements, of which the first has index
-// 4 q among the moments
-__device__ __forceinline__ void random4(const State &s, int64_t q, uint32_t (&r)[4]) {
-  const sk_key k = sk_threefry(sk_key{s.key0, s.key1}, (uint32_t)(q >> 32), (uint32_t)q);
-  r[0] = k.k0 & 0xffffu;
-  r[1] = k.k0 >> 16;
-  r[2] = k.k1 & 0xffffu;
-  r[3] = k.k1 >> 16;
+// Sixteen random bits of each of four elements, two in a word, of which the
+// first has index 4 q among the moments
+__device__ __forceinline__ uint2 random4(const State &s, int64_t q) {
+  const sk_key k = sk_threefry(sk_key{s.key0, s.key1}, (uint32_t)((uint64_t)q >> 32), (uint32_t)q);
+  return make_uint2(k.k0, k.k1);
 }
 
-struct Element {
-  float m, v, root;
-};
-
-__device__ __forceinline__ Element moments_of(const Moments &p, float clip, float g, float m, float v) {
-  Element e;
-  g = g * clip;
-  e.m = m * p.b1 + g * p.b1c;
-  e.v = v * p.b2 + g * g * p.b2c;
-  e.root = sqrtf(e.v);
-  return e;
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 operator*(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 operator+(float2 a, float2 b) { return __fadd2_rn(a, b); }
 
-__device__ __forceinline__ float weight_of(const Moments &p, const State &s, float decay, float w, const Element &e) {
-  return w * decay - __fdividef(s.size * e.m, e.root * s.inv_root + p.eps);
+// m and v become the new moments, of which the root is returned
+__device__ __forceinline__ float2 moments_of(const Moments &p, float clip, float2 g, float2 &m, float2 &v) {
+  g = g * both(clip);
+  m = m * both(p.b1) + g * both(p.b1c);
+  v = v * both(p.b2) + g * g * both(p.b2c);
+  return make_float2(sqrtf(v.x), sqrtf(v.y));
+}
+__device__ __forceinline__ float2 weights_of(const Moments &p, const State &s, float decay, float2 w, float2 m, float2 root) {
+  const float2 den = __ffma2_rn(root, both(s.inv_root), both(p.eps));
+  return __ffma2_rn(w, both(decay), m * both(-s.size) * make_float2(reciprocal(den.x), reciprocal(den.y)));
 }
 
 // Moments of 32 bits: four elements of each array a thread and pass.
 template <typename PT, typename GT>
 __device__ __forceinline__ void step32(const Moments &p, const Entry &e, const State &s, int chunk) {
-  constexpr int W = 4, kPasses = kChunk / (kThreads * W);
-  float *first = static_cast<float *>(p.first) + e.offset, *second = static_cast<float *>(p.second) + e.offset;
+  constexpr int W = 4;
+  constexpr int kPasses = kChunk / (kThreads * W);
   PT *weight = static_cast<PT *>(e.weight);
   const GT *gradient = static_cast<const GT *>(e.gradient);
-  const bool aligned = e.kind & 16;
+  float4 *first = reinterpret_cast<float4 *>(static_cast<float *>(p.first) + e.offset);
+  float4 *second = reinterpret_cast<float4 *>(static_cast<float *>(p.second) + e.offset);
   const float decay = (float)(1.0 - s.learning_rate * e.weight_decay);
   if (s.skip) return;
 #pragma unroll 2
   for (int pass = 0; pass < kPasses; ++pass) {
     const int64_t i = (int64_t)chunk * kChunk + (pass * kThreads + (int)threadIdx.x) * W;
     if (i >= e.count) continue;
-    const bool whole = aligned && i + W <= e.count;
-    float g[W], w[W];
-    load<GT, W>(gradient, i, e.count, whole, g);
-    load<PT, W>(weight, i, e.count, whole, w);
-    Vec<float, W> m = *reinterpret_cast<const Vec<float, W> *>(first + i);
-    Vec<float, W> v = *reinterpret_cast<const Vec<float, W> *>(second + i);
-    uint32_t random[W] = {};
-    if constexpr (!std::is_same_v<PT, float>)
-      if (p.stochastic) random4(s, (e.offset + i) >> 2, random);
-    Vec<PT, W> out;
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const Element x = moments_of(p, s.clip, g[j], m.v[j], v.v[j]);
-      m.v[j] = x.m;
-      v.v[j] = x.v;
-      out.v[j] = to_weight<PT>(weight_of(p, s, decay, w[j], x), p.stochastic, random[j]);
+    const bool whole = (e.kind & 16) && i + W <= e.count;
+    Four<GT> g;
+    Four<PT> w;
+    if (whole) {
+      g = *reinterpret_cast<const Four<GT> *>(gradient + i);
+      w = *reinterpret_cast<const Four<PT> *>(weight + i);
+    } else {
+      g = load_slowly(gradient, i, e.count);
+      w = load_slowly(weight, i, e.count);
     }
-    *reinterpret_cast<Vec<float, W> *>(first + i) = m;
-    *reinterpret_cast<Vec<float, W> *>(second + i) = v;
-    store<PT, W>(weight, i, e.count, whole, out);
+    const float4 mq = first[i / W], vq = second[i / W];
+    uint2 random = {0, 0};
+    if constexpr (!std::is_same_v<PT, float>)
+      if (p.stochastic) random = random4(s, (e.offset + i) >> 2);
+    float2 m[2] = {{mq.x, mq.y}, {mq.z, mq.w}}, v[2] = {{vq.x, vq.y}, {vq.z, vq.w}}, next[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 root = moments_of(p, s.clip, pair_of<GT>(g, j), m[j], v[j]);
+      next[j] = weights_of(p, s, decay, pair_of<PT>(w, j), m[j], root);
+    }
+    first[i / W] = make_float4(m[0].x, m[0].y, m[1].x, m[1].y);
+    second[i / W] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    w = to_weights<PT>(next[0], next[1], p.stochastic, random);
+    if (whole)
+      *reinterpret_cast<Four<PT> *>(weight + i) = w;
+    else
+      store_slowly(weight, i, e.count, w);
   }
 }
 
-// 2^(field - 127), NaN where a block holds what is not finite
+// 2^(field - 126), NaN where a block holds what is not finite
 __device__ __forceinline__ float block_scale(uint32_t field) {
-  return __uint_as_float(field == 255u ? 0x7fc00000u : field << 23);
+  return __uint_as_float(field == 255u ? 0x7fc00000u : (field + 1) << 23);
 }
-__device__ __forceinline__ float decode_first(uint32_t code, float scale) {
-  return __uint_as_float(((code & 0x7fu) << 20) | ((code & 0x80u) << 24)) * 0x1p113f * scale;
+// Two of a word's four codes.  A code's fields are those of a float16 from its
+// exponent's lowest bit on, and that float16 is half the code's value below
+// the block's exponent.
+__device__ __forceinline__ float2 decode_first(uint32_t codes, int pair) {
+  const uint32_t up = __byte_perm(codes, 0u, pair ? 0x3424 : 0x1404);
+  const uint32_t h = (up >> 1 & 0x3f803f80u) | (up & 0x80008000u);
+  return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
-__device__ __forceinline__ float decode_root(uint32_t code, float scale) {
-  return __uint_as_float(code << 19) * 0x1p113f * scale;
+__device__ __forceinline__ float2 decode_root(uint32_t codes, int pair) {
+  const uint32_t h = __byte_perm(codes, 0u, pair ? 0x4342 : 0x4140) << 6;
+  return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
-// The exponent field of a block from the bits of its largest element, of
-// which every lane of the warp has its own largest: what is below 2^-100
-// rounds on the grid of 2^-100 (it stays exact in bfloat16), above 2^126
-// the largest codes hold it
-__device__ __forceinline__ uint32_t block_field(uint32_t bits) {
-  bits = __reduce_max_sync(kFull, bits);
+// The exponent field of a block from its largest element, of which every lane
+// of the warp has its own largest: what is below 2^-100 rounds on the grid of
+// 2^-100 (it stays exact in bfloat16), above 2^126 the largest codes hold it
+__device__ __forceinline__ uint32_t block_field(float most) {
+  const uint32_t bits = __reduce_max_sync(kFull, __float_as_uint(most));
   return bits >= 0x7f800000u ? 255u : min(max(bits >> 23, 27u), 253u);
 }
+// the larger of a and |b|, |c|, NaN where any is
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return y;
+}
+// byte 3 of each
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+template <int Bytes>
+__device__ __forceinline__ void copy_async(void *to, const void *from) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(Bytes) : "memory");
+}
 
-// Moments of 8 bits: a warp takes a block of 256, eight elements a lane.
+// A warp's block on its way from memory: a lane copies and reads its own places
+// alone, four elements of either half
+struct Staged {
+  uint4 gradient[2][32], weight[2][32];
+  uint32_t first[2][32], second[2][32];
+};
+
+// Moments of 8 bits: a warp takes block after block, the next one's data on
+// their way while this one is computed.  Pairs of floats throughout.
 template <typename PT, typename GT>
-__device__ __forceinline__ void step8(const Moments &p, const Entry &e, const State &s, int chunk) {
-  constexpr int W = 8, kWarps = kThreads / 32, kPasses = kChunk / (kWarps * kBlock);
+__device__ __forceinline__ void step8(const Moments &p, const Entry &e, const State &s, int chunk,
+                                      Staged (*shared)[kThreads / 32]) {
+  constexpr int W = 4, kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   PT *weight = static_cast<PT *>(e.weight);
   const GT *gradient = static_cast<const GT *>(e.gradient);
-  const bool aligned = e.kind & 16;
   const float decay = (float)(1.0 - s.learning_rate * e.weight_decay);
   if (s.skip) return;
-#pragma unroll 1
-  for (int pass = 0; pass < kPasses; ++pass) {
-    const int64_t start = (int64_t)chunk * kChunk + (pass * kWarps + warp) * kBlock;
-    if (start >= e.count) break;
-    const int64_t i = start + lane * W, block = (e.offset + start) / kBlock;
-    const bool whole = aligned && i + W <= e.count;
-    float g[W], w[W];
-    load<GT, W>(gradient, i, e.count, whole, g);
-    load<PT, W>(weight, i, e.count, whole, w);
-    uint2 *first = reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.first) + e.offset + i);
-    uint2 *second = reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.second) + e.offset + i);
-    const uint2 mc = *first, rc = *second;
-    const float m_scale = block_scale(p.first_exponent[block]), r_scale = block_scale(p.second_exponent[block]);
-    uint32_t random[W];
-    random4(s, (e.offset + i) >> 2, *reinterpret_cast<uint32_t(*)[4]>(random));
-    random4(s, ((e.offset + i) >> 2) + 1, *reinterpret_cast<uint32_t(*)[4]>(random + 4));
-    float m[W], r[W];
-    uint32_t m_most = 0, r_most = 0;
-    Vec<PT, W> out;
+  const int64_t begin = (int64_t)chunk * kChunk, end = min(e.count, begin + kChunk);
+  uint32_t fields[2] = {0, 0};  // of the block ahead
+  auto request = [&](int64_t start, int stage) {
+    if (start < end) {
+      Staged &to = shared[stage][warp];
+      const uint32_t *first = reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(p.first) + e.offset + start) + lane;
+      const uint32_t *second = reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(p.second) + e.offset + start) + lane;
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const uint32_t mb = (j < 4 ? mc.x : mc.y) >> (8 * (j & 3)) & 0xffu;
-      const uint32_t rb = (j < 4 ? rc.x : rc.y) >> (8 * (j & 3)) & 0xffu;
-      const float root = decode_root(rb, r_scale);
-      const Element x = moments_of(p, s.clip, g[j], decode_first(mb, m_scale), root * root);
-      m[j] = x.m;
-      r[j] = x.root;
-      m_most = max(m_most, __float_as_uint(x.m) & 0x7fffffffu);
-      r_most = max(r_most, __float_as_uint(x.root) & 0x7fffffffu);
-      out.v[j] = to_weight<PT>(weight_of(p, s, decay, w[j], x), p.stochastic, random[j]);
+      for (int h = 0; h < 2; ++h) {
+        const int64_t i = start + h * (kBlock / 2) + lane * W;
+        Four<GT> *g = reinterpret_cast<Four<GT> *>(&to.gradient[h][lane]);
+        Four<PT> *w = reinterpret_cast<Four<PT> *>(&to.weight[h][lane]);
+        if ((e.kind & 16) && start + kBlock <= e.count) {
+          copy_async<sizeof(Four<GT>)>(g, gradient + i);
+          copy_async<sizeof(Four<PT>)>(w, weight + i);
+        } else {
+          *g = load_slowly(gradient, i, e.count);
+          *w = load_slowly(weight, i, e.count);
+        }
+        copy_async<4>(&to.first[h][lane], first + h * (kBlock / 8));
+        copy_async<4>(&to.second[h][lane], second + h * (kBlock / 8));
+      }
+      fields[0] = p.first_exponent[(uint64_t)(e.offset + start) / kBlock];
+      fields[1] = p.second_exponent[(uint64_t)(e.offset + start) / kBlock];
     }
-    store<PT, W>(weight, i, e.count, whole, out);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  request(begin + warp * kBlock, 0);
+  int stage = 0;
+#pragma unroll 1
+  for (int64_t start = begin + warp * kBlock; start < end; start += kWarps * kBlock, stage ^= 1) {
+    const int64_t block = (uint64_t)(e.offset + start) / kBlock;
+    const uint32_t m_old = fields[0], r_old = fields[1];
+    request(start + kWarps * kBlock, stage ^ 1);
+    uint32_t *first = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.first) + e.offset + start) + lane;
+    uint32_t *second = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.second) + e.offset + start) + lane;
+    const bool whole = (e.kind & 16) && start + kBlock <= e.count;
+    const int64_t i = start + lane * W, other = i + kBlock / 2;
+    // (while the loads are on their way)
+    const uint2 random[2] = {random4(s, (e.offset + i) >> 2), random4(s, (e.offset + other) >> 2)};
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const Staged &now = shared[stage][warp];
+    Four<PT> w[2];
+    const float2 m_scale = both(block_scale(m_old)), r_scale = both(block_scale(r_old));
+    float2 m[2][2], r[2][2];
+    float m_most = 0.0f, r_most = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Four<GT> g = *reinterpret_cast<const Four<GT> *>(&now.gradient[h][lane]);
+      w[h] = *reinterpret_cast<const Four<PT> *>(&now.weight[h][lane]);
+      const uint32_t mc = now.first[h][lane], rc = now.second[h][lane];
+      float2 next[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 r0 = decode_root(rc, j) * r_scale;
+        float2 v = r0 * r0;
+        m[h][j] = decode_first(mc, j) * m_scale;
+        r[h][j] = moments_of(p, s.clip, pair_of<GT>(g, j), m[h][j], v);
+        m_most = max_of(m_most, m[h][j].x, m[h][j].y);
+        r_most = max_of(r_most, r[h][j].x, r[h][j].y);
+        next[j] = weights_of(p, s, decay, pair_of<PT>(w[h], j), m[h][j], r[h][j]);
+      }
+      w[h] = to_weights<PT>(next[0], next[1], p.stochastic, random[h]);
+    }
+    if (whole) {
+      *reinterpret_cast<Four<PT> *>(weight + i) = w[0];
+      *reinterpret_cast<Four<PT> *>(weight + other) = w[1];
+    } else {
+      store_slowly(weight, i, e.count, w[0]);
+      store_slowly(weight, other, e.count, w[1]);
+    }
     const uint32_t m_field = block_field(m_most), r_field = block_field(r_most);
     // 2^-e, then 2^-113: one factor would leave the range of floats
-    const float m_down = power_of_two(254 - (int)min(m_field, 253u)), r_down = power_of_two(254 - (int)min(r_field, 253u));
-    uint2 mo = {0, 0}, ro = {0, 0};
+    const float2 m_down = both(power_of_two(254 - (int)min(m_field, 253u)));
+    const float2 r_down = both(power_of_two(254 - (int)min(r_field, 253u)));
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const float y = fabsf(m[j]) * m_down * 0x1p-113f, z = r[j] * r_down * 0x1p-113f;
-      uint32_t mb = (__float_as_uint(y) + (random[j] << 4) + 8u) >> 20;
-      uint32_t rb = (__float_as_uint(z) + ((random[j] * 0x9e37u & 0xffffu) << 3) + 4u) >> 19;
-      mb = min(mb, 0x7eu) | (__float_as_uint(m[j]) >> 24 & 0x80u);
-      rb = min(max(rb, r[j] > 0.0f ? 1u : 0u), 0xffu);
-      (j < 4 ? mo.x : mo.y) |= mb << (8 * (j & 3));
-      (j < 4 ? ro.x : ro.y) |= rb << (8 * (j & 3));
+    for (int h = 0; h < 2; ++h) {
+      // sums whose upper byte is the code, the random bits below it: 16 (bits + 16 u + 8), 32 (bits + 8 u' + 4)
+      uint32_t mb[W], rb[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float2 y = m[h][j / 2] * m_down * both(0x1p-113f), z = r[h][j / 2] * r_down * both(0x1p-113f);
+        const uint32_t u = half_of(j < 2 ? random[h].x : random[h].y, j);
+        const uint32_t yb = __float_as_uint(j & 1 ? y.y : y.x), zb = __float_as_uint(j & 1 ? z.y : z.x);
+        mb[j] = (yb * 16u + (u * 256u + 128u)) | (yb & 0x80000000u);
+        rb[j] = zb * 32u + ((u * 0x9e370000u + 0x8000u) >> 8);
+      }
+      uint32_t mo = upper_bytes(mb[0], mb[1], mb[2], mb[3]), ro = upper_bytes(rb[0], rb[1], rb[2], rb[3]);
+      if (m_field == 253u) mo = __vminu4(mo & 0x7f7f7f7fu, 0x7e7e7e7eu) | (mo & 0x80808080u);  // beyond the largest code
+      if ((ro - 0x01010101u) & ~ro & 0x80808080u) {  // a byte of zero: the borrow reaches its upper bit
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          if ((j & 1 ? r[h][j / 2].y : r[h][j / 2].x) > 0.0f && !(ro >> (8 * j) & 0xffu)) ro |= 1u << (8 * j);
+      }
+      first[h * (kBlock / 8)] = mo;
+      second[h * (kBlock / 8)] = ro;
     }
-    *first = mo;
-    *second = ro;
     if (lane == 0) {
       p.first_exponent[block] = (uint8_t)m_field;
       p.second_exponent[block] = (uint8_t)r_field;
@@ -306,26 +426,29 @@ __device__ __forceinline__ void step8(const Moments &p, const Entry &e, const St
 }
 
 template <int Bits, typename PT, typename GT>
-__device__ __forceinline__ void step_chunk(const Moments &p, const Entry &e, const State &s, int chunk) {
+__device__ __forceinline__ void step_chunk(const Moments &p, const Entry &e, const State &s, int chunk,
+                                           Staged (*shared)[kThreads / 32]) {
   if constexpr (Bits == 32)
     step32<PT, GT>(p, e, s, chunk);
   else
-    step8<PT, GT>(p, e, s, chunk);
+    step8<PT, GT>(p, e, s, chunk, shared);
 }
 
 template <int Bits, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> table,
-                                                         const __grid_constant__ Moments p) {
+__global__ void __launch_bounds__(kThreads, Bits == 8 ? 4 : 5) adamw_kernel(const __grid_constant__ Table<N> table,
+                                                                           const __grid_constant__ Moments p) {
+  __shared__ Staged shared[Bits == 8 ? 2 : 1][Bits == 8 ? kThreads / 32 : 1];
+  Staged(*staged)[kThreads / 32] = reinterpret_cast<Staged(*)[kThreads / 32]>(&shared[0][0]);
   const Entry &e = table.entry[find(table, blockIdx.x)];
   const int chunk = blockIdx.x - e.first;
   const State s = *p.state;
   switch (e.kind & 15) {
-    case 0: return step_chunk<Bits, float, float>(p, e, s, chunk);
-    case 4: return step_chunk<Bits, float, __nv_bfloat16>(p, e, s, chunk);
-    case 8: return step_chunk<Bits, float, __half>(p, e, s, chunk);
-    case 1: return step_chunk<Bits, __nv_bfloat16, float>(p, e, s, chunk);
-    case 5: return step_chunk<Bits, __nv_bfloat16, __nv_bfloat16>(p, e, s, chunk);
-    case 9: return step_chunk<Bits, __nv_bfloat16, __half>(p, e, s, chunk);
+    case 0: return step_chunk<Bits, float, float>(p, e, s, chunk, staged);
+    case 4: return step_chunk<Bits, float, __nv_bfloat16>(p, e, s, chunk, staged);
+    case 8: return step_chunk<Bits, float, __half>(p, e, s, chunk, staged);
+    case 1: return step_chunk<Bits, __nv_bfloat16, float>(p, e, s, chunk, staged);
+    case 5: return step_chunk<Bits, __nv_bfloat16, __nv_bfloat16>(p, e, s, chunk, staged);
+    case 9: return step_chunk<Bits, __nv_bfloat16, __half>(p, e, s, chunk, staged);
   }
 }
 
@@ -366,16 +489,18 @@ __global__ void __launch_bounds__(kThreads) adamw_moments_kernel(const uint8_t *
   if (i >= count) return;
   const uint2 mc = *reinterpret_cast<const uint2 *>(first + i), rc = *reinterpret_cast<const uint2 *>(second + i);
   const float m_scale = block_scale(first_exponent[i / kBlock]), r_scale = block_scale(second_exponent[i / kBlock]);
-  Vec<__nv_bfloat16, 8> m, r;
+  uint4 m, r;
+  uint32_t *mw = reinterpret_cast<uint32_t *>(&m), *rw = reinterpret_cast<uint32_t *>(&r);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t mb = (j < 4 ? mc.x : mc.y) >> (8 * (j & 3)) & 0xffu;
-    const uint32_t rb = (j < 4 ? rc.x : rc.y) >> (8 * (j & 3)) & 0xffu;
-    m.v[j] = __float2bfloat16_rn(decode_first(mb, m_scale));
-    r.v[j] = __float2bfloat16_rn(decode_root(rb, r_scale));
+  for (int j = 0; j < 4; ++j) {
+    const float2 a = decode_first(j < 2 ? mc.x : mc.y, j & 1) * both(m_scale);
+    const float2 b = decode_root(j < 2 ? rc.x : rc.y, j & 1) * both(r_scale);
+    // (exact: the lower halves are zero)
+    mw[j] = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x7632);
+    rw[j] = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x7632);
   }
-  *reinterpret_cast<Vec<__nv_bfloat16, 8> *>(first_out + i) = m;
-  *reinterpret_cast<Vec<__nv_bfloat16, 8> *>(root_out + i) = r;
+  *reinterpret_cast<uint4 *>(first_out + i) = m;
+  *reinterpret_cast<uint4 *>(root_out + i) = r;
 }
 
 // ---------------------------------------------------------------------------
@@ -399,35 +524,38 @@ __device__ __forceinline__ double cta_sum(double v) {
 // gradient of 1e20 nor one of 1e-25 is lost, and the factor that clips does
 // not depend on the launch's shape.
 template <typename T>
+__device__ __forceinline__ double square_of(uint32_t word, double sum) {
+  if constexpr (std::is_same_v<T, float>) {
+    const double f = (double)__uint_as_float(word);
+    return fma(f, f, sum);
+  } else {
+    float2 two;
+    if constexpr (std::is_same_v<T, __half>)
+      two = __half22float2(*reinterpret_cast<const __half2 *>(&word));
+    else
+      two = make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
+    return fma((double)two.y, (double)two.y, fma((double)two.x, (double)two.x, sum));
+  }
+}
+template <typename T>
 __device__ __forceinline__ double squares(const Entry &e, int64_t begin) {
   constexpr int W = 16 / sizeof(T), kAhead = 4;  // vectors of a thread in flight together
-  const T *x = static_cast<const T *>(e.gradient);
-  const int64_t end = min(e.count, begin + kNormChunk);
+  const T *x = static_cast<const T *>(e.gradient) + begin;
+  const int count = (int)min((int64_t)kNormChunk, e.count - begin);
+  const int vectors = e.kind & 16 ? count / W : 0;
   double sum = 0.0;
-  if (e.kind & 16) {
-    for (int64_t i = begin + (int)threadIdx.x * W; i < end; i += kAhead * kThreads * W) {
-      float f[kAhead][W];
+  for (int i = threadIdx.x; i < vectors; i += kAhead * kThreads) {
+    uint4 q[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int64_t at = i + k * kThreads * W;
-        if (at < end)
-          load<T, W>(x, at, e.count, at + W <= e.count, f[k]);
-        else
+    for (int k = 0; k < kAhead; ++k)
+      q[k] = i + k * kThreads < vectors ? reinterpret_cast<const uint4 *>(x)[i + k * kThreads] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int w = 0; w < W; ++w) f[k][w] = 0.0f;
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-#pragma unroll
-        for (int w = 0; w < W; ++w) sum = fma((double)f[k][w], (double)f[k][w], sum);
-    }
-  } else {
-#pragma unroll 4
-    for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) {
-      const double f = (double)to_f(x[i]);
-      sum = fma(f, f, sum);
-    }
+    for (int k = 0; k < kAhead; ++k)
+      sum = square_of<T>(q[k].w, square_of<T>(q[k].z, square_of<T>(q[k].y, square_of<T>(q[k].x, sum))));
   }
+#pragma unroll 1
+  for (int i = vectors * W + (int)threadIdx.x; i < count; i += kThreads)
+    sum = fma((double)to_f(x[i]), (double)to_f(x[i]), sum);
   return sum;
 }
 
@@ -593,7 +721,7 @@ int scacchi_adamw_step(const scacchi_adamw *params, const scacchi_adamw_tensor *
   const scacchi_adamw &a = *params;
   const bool eight = a.state_bits == 8;
   if ((a.state_bits != 32 && !eight) || !(a.beta1 >= 0.0 && a.beta1 < 1.0) || !(a.beta2 >= 0.0 && a.beta2 < 1.0) ||
-      !(a.eps >= 0.0f && a.eps <= 1e30f) || !isfinite(a.learning_rate) || a.moments < 0 || a.moments % kBlock ||
+      !(a.eps == 0.0f || (a.eps >= 1e-30f && a.eps <= 1e30f)) || !isfinite(a.learning_rate) || a.moments < 0 || a.moments % kBlock ||
       !a.state || misaligned(a.state, 8) || misaligned(a.norm, 4) || misaligned(a.learning_rate_at, 4) ||
       (a.norm && !(a.max_norm > 0.0 && isfinite(a.max_norm))) || (eight && !a.stochastic))
     return SCACCHI_EINVAL;
