@@ -248,12 +248,13 @@ def test_clipping(cuda, bits):
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_more_tensors_than_a_launch_takes(cuda, bits):
-    sizes = [1 + (37 * i) % 700 for i in range(1100)]
+    sizes = [1 + (37 * i) % 250 for i in range(1100)]
+    key = KEY if bits == 8 else None
     weights = _tensors(sizes, "fp32", 1, 0.1)
-    opt = AdamW(weights, learning_rate=0.01, max_norm=1.0, state_bits=bits, key=KEY)
+    opt = AdamW(weights, learning_rate=0.01, max_norm=1.0, state_bits=bits, key=key)
     launches = _lib.lib().scacchi_adamw_launch_count()
     _step_and_check(opt, weights, _tensors(sizes, "bf16", 2, 0.1), lr=0.01, b1=0.9, b2=0.999, eps=1e-8, decay=0.0,
-                    clip=1.0, key=KEY)
+                    clip=1.0, key=key)
     assert _lib.lib().scacchi_adamw_launch_count() - launches == 3 + 1 + 1 + 3
 
 
@@ -413,6 +414,52 @@ def test_captured_steps_count_on(cuda, bits):
         results.append([norm, *weights.values(), opt.first, opt.second])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_plain_calls_and_the_python_way_agree(cuda, monkeypatch):
+    """Steps, norms and moments through the extension module and without it."""
+    class Nothing:
+        @staticmethod
+        def adamw_step(*args):
+            return None
+
+        gradient_norm = adamw_moments = adamw_step
+
+    def run():
+        res = []
+        for bits in (32, 8):
+            for clip in (None, 0.5):
+                weights = _tensors(SIZES, "bf16", 1, 0.1)
+                opt = AdamW(weights, learning_rate=0.01, weight_decay=0.1, max_norm=clip, state_bits=bits, key=KEY)
+                grads = _tensors(SIZES, "fp32", 2, 0.1)
+                grads["t4"] = None
+                norms = [opt.step(grads), opt.step(dict(list(grads.items())[3:]), learning_rate=0.1)]
+                if clip:
+                    norms.append(opt.step(grads, norm=torch.tensor(9.0, device="cuda")))
+                opt.step(grads, learning_rate=torch.tensor(0.03, device="cuda"))
+                res += [*norms, *weights.values(), *opt.moments(), opt.first, opt.second, torch.tensor(opt.steps())]
+                res.append(gradient_norm([g for g in grads.values() if g is not None]))
+        return res
+
+    fast = run()
+    host = _lib.host()
+    assert host.gradient_norm([torch.ones((3,), device="cuda")]) is not None
+    monkeypatch.setattr(_lib, "host", lambda: Nothing)
+    slow = run()
+    assert len(fast) == len(slow)
+    for a, b in zip(fast, slow):
+        assert a is None and b is None or a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+
+
+def test_a_large_tensor(cuda):
+    """Many CTAs, on either side of chunks' and blocks' ends."""
+    for n in (1 << 18, 300_001):
+        for bits, dtype in ((32, "fp32"), (8, "bf16"), (8, "fp32")):
+            weights = _tensors([n], dtype, 1, 0.1)
+            opt = AdamW(weights, learning_rate=0.01, state_bits=bits, max_norm=1.0, key=KEY)
+            for step in range(2):
+                _step_and_check(opt, weights, _tensors([n], "bf16", 2 + step, 1e-2), lr=0.01, b1=0.9, b2=0.999, eps=1e-8,
+                                decay=0.0, clip=1.0, key=KEY)
 
 
 def test_backward_through_a_stepped_weight_is_refused(cuda):

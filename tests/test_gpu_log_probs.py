@@ -23,6 +23,7 @@ import math
 import pytest
 import torch
 
+from scacchi_b200 import _lib
 from scacchi_b200.log_probs import policy_log_probs, policy_log_probs_gradient
 
 pytestmark = pytest.mark.gpu
@@ -161,6 +162,63 @@ def test_values_and_gradient(cuda, shape, dtype, legal):
         _check_gradient(logits, action, mask, T, out, d, g, h)
     _check_gradient(logits, action, mask, T, out, d, g, None)
     _check_gradient(logits, action, mask, T, out, d, None, h)
+
+
+# many rows: a lane each, rows of whole 16-byte pieces, batches and groups that the last rows do not fill, rows between
+# the short and the long ones
+MANY = [(40001, 82), (38017, 64), (38000, 8), (40003, 5), (9001, 128), (5003, 361), (1193, 513), (1200, 1000), (1185, 1024),
+        (1184, 1025), (1190, 2048), (1184, 2049)]
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_many_rows(cuda, shape, dtype):
+    N, A = shape
+    for legal in (False, True):
+        logits, action, mask = _inputs(N, A, dtype, legal)
+        out, d = _check(logits, action, mask, 0.9, 3)
+        g, h = torch.linspace(-1, 1, N, device="cuda"), torch.linspace(1, -0.5, N, device="cuda")
+        _check_gradient(logits, action, mask, 0.9, out, d, g, h)
+    wide, action, _ = _inputs(N, A + 3, dtype, False, seed=1)
+    logits = wide[:, 1:A + 1]
+    out, d = _check(logits, action, mask, 1.0, 2)
+    _check_gradient(logits, action, mask, 1.0, out, d, g, h)
+
+
+@pytest.mark.parametrize("A", [64, 82])
+def test_equal_logits_of_many_rows(cuda, A):
+    logits = torch.randint(0, 3, (40000, A), device="cuda").bfloat16()
+    logits[::3] = 1.0
+    _check(logits, torch.zeros(40000, dtype=torch.int32, device="cuda"), None, 1.0, 32)
+
+
+def test_plain_calls_and_the_python_way_agree(cuda, monkeypatch):
+    """Every call through the extension module and without it."""
+    class Nothing:
+        @staticmethod
+        def log_probs(*args):
+            return None
+
+        log_probs_gradient = log_probs
+
+    cases = [_inputs(N, A, d, legal) for N, A in ((64, 82), (7, 5000)) for d in sorted(DT) for legal in (False, True)]
+
+    def run():
+        res = []
+        for logits, action, mask in cases:
+            for top in (0, 4):
+                out = policy_log_probs(logits, action, legal=mask, temperature=0.7, top=top)
+                ones = torch.ones_like(out.entropy)
+                res += [*out, *(policy_log_probs_gradient(logits, action, out, grad_log_prob=g, grad_entropy=h,
+                                                          legal=mask, temperature=0.7)
+                                for g, h in ((ones, None), (None, ones), (ones, ones)))]
+        return res
+
+    fast = run()
+    assert sum(v is not None for v in [_lib.host().log_probs(c[0], c[1], c[2], 1.0, 2) for c in cases]) == len(cases)
+    monkeypatch.setattr(_lib, "host", lambda: Nothing)
+    for a, b in zip(fast, run()):
+        assert a is None and b is None or a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
 
 
 @pytest.mark.parametrize("dtype", sorted(DT))
