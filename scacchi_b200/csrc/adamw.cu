@@ -28,6 +28,17 @@
 // What is rounded to a code is computed without contraction (this file
 // compiles with -fmad=false), so that the definition in plain operations
 // gives the same codes.
+//
+// Device times, by graph replays: 50.4 M float32 weights and gradients with
+// 32-bit moments 212 us (6.7 TB/s, the copy's rate); 67.1 M bfloat16 weights and
+// gradients with moments of 8 bits 217 us (3.1 TB/s; 104 us at a copy's rate),
+// with float32 weights 202 us (4.6 TB/s); reading 8-bit moments out 62 us
+// (6.5 TB/s).  The norm of 67.1 M bfloat16 gradients 27 us (4.9 TB/s), of 50.4 M
+// float32 33 us (6.1 TB/s); 66 small tensors 6 us.
+//
+// 32-bit moments are bound by memory.  Those of 8 bits issue 90 instructions
+// an element on 60 to 70 % of the cycles: 19 are the random bits' (without
+// them a step took 8 % less), the rest decoding, the roots and encoding.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -204,7 +215,11 @@ __device__ __forceinline__ float reciprocal(float x) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 operator*(float2 a, float2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ float2 operator+(float2 a, float2 b) { return __fadd2_rn(a, b); }
+// (one by one: the compiler fuses a pair's sum with the product before it, and codes would differ from the
+// definition's here and there)
+__device__ __forceinline__ float2 operator+(float2 a, float2 b) {
+  return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
+}
 
 // m and v become the new moments, of which the root is returned
 __device__ __forceinline__ float2 moments_of(const Moments &p, float clip, float2 g, float2 &m, float2 &v) {

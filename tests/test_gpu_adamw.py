@@ -210,6 +210,36 @@ def test_steps(cuda, bits, weight, gradient, shift):
             _step_and_check(opt, weights, grads, lr=0.01, b1=0.9, b2=0.999, eps=1e-8, decay=decay, key=key)
 
 
+@pytest.mark.parametrize("gradient", sorted(DT))
+def test_moments_are_bit_for_bit_those_of_plain_operations(cuda, gradient):
+    """Every product and sum rounded by itself, so that what is rounded to a
+    code is the definition's: two fused sums in a million codes differ."""
+    w = _tensors([1 << 20], "fp32", 1, 0.1)
+    opt = AdamW(w, learning_rate=0.01, beta1=0.9, beta2=0.999)
+    eight = AdamW({"t0": w["t0"].clone()}, learning_rate=0.01, beta1=0.9, beta2=0.999, state_bits=8, key=KEY)
+    for step in range(3):
+        g = _tensors([1 << 20], gradient, 5 + step, 1e-2)
+        x = g["t0"].float()
+        first, second = opt.first * 0.9 + x * (1 - 0.9), opt.second * 0.999 + x * x * (1 - 0.999)
+        m0, v0 = _moments64(eight)
+        m = m0.float() * 0.9 + x * (1 - 0.9)
+        root = torch.sqrt(v0.float() * 0.999 + x * x * (1 - 0.999))
+        opt.step(g)
+        eight.step(g)
+        assert torch.equal(opt.first, first) and torch.equal(opt.second, second)
+        random = _random16(KEY, step + 1, 1 << 20)
+        for y, u, codes, exponent, shift in ((m.abs(), random, eight.first & 0x7f, eight.first_exponent, 20),
+                                             (root, random * 0x9e37 & 0xffff, eight.second, eight.second_exponent, 19)):
+            most = (y.view(-1, BLOCK).amax(-1).view(torch.int32) >> 23).clamp(27, 253)
+            assert torch.equal(exponent.int(), most)
+            unit = torch.exp2(127.0 - most.float()).repeat_interleave(BLOCK)
+            bits = (y * unit * 2.0 ** -113).view(torch.int32).long()
+            want = (bits + (u << shift - 16) + (1 << shift - 17)) >> shift
+            if shift == 19:
+                want = torch.maximum(want, (y > 0).long())
+            assert torch.equal(codes.long(), want)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_settings(cuda, bits):
     """Other betas, eps and rates, among them a rate given per step, as a number and on the device."""
