@@ -9,18 +9,32 @@
 //   dx_i     = (g ([i = a] - p_i) - h p_i (log p_i + entropy)) / T,
 //              p_i = e^(u_i - log s), for gradients g of log_prob, h of entropy
 //
-// Logits are read once.  Rows of up to 512 actions lie in the registers of a
-// few lanes.  Longer ones go through a CTA, or a cluster of them where rows
-// are few: every thread keeps the maximum of what it has seen and s and t
-// relative to it, and they are joined at the row's end.
+// Logits are read once.  Warps stage batches of short rows in shared memory
+// and give each row some lanes, one where 32 rows fit.  Longer rows go through
+// a CTA, or a cluster of them where rows are few: every thread keeps the
+// maximum of what it has seen and s and t relative to it, and they are joined
+// at the row's end.
 //
-// The best k come from the same maxima.  Split the row's threads into at least
-// 64 groups: of the groups' maxima the k-th largest, L, has k elements at or
-// above it, so the best k are among the elements >= L, and only threads whose
-// own maximum reaches L look at their elements again: for 64 groups of
+// The best k of a long row come from the same maxima.  Split its threads into
+// at least 64 groups: of the groups' maxima the k-th largest, L, has k elements
+// at or above it, so the best k are among the elements >= L, and only the parts
+// of threads whose maximum reaches L are looked at again: for 64 groups of
 // independent logits 64 ln(64 / (64 - k)) elements, 24 for k = 20.  They are
 // ranked by counting.  Where more than kCandidates elements reach L (many equal
 // ones) the CTA takes the maximum below the last one k times.
+//
+// Device times, by graph replays: 4096 rows of 32000 bf16 58 us (4.5 TB/s), with
+// the 20 best 69, with a mask 96 and 112; the same of fp32 86 us (6.1 TB/s) and
+// 101.  262144 rows of 82 fp32 20 us (4.3 TB/s), with the 4 best 33, with a mask
+// 28 and 46.  8 rows of 131071 fp32 with the 20 best 9 us.  Gradients: 4096 x
+// 32000 bf16 79 us (6.6 TB/s), with a mask 96; 262144 x 82 fp32 with a mask 46 us
+// (4.3 TB/s).
+//
+// Long rows of fp32 and long gradients are bound by memory.  Long bf16 rows
+// issue 9 instructions an element on 68 % of the cycles (the exponentials alone
+// are not the bound: without them 56 us for 61), their ends 1700 a row.  Short
+// rows issue 15 to 50 instructions for 32 elements (masks and best actions) on
+// 54 to 71 % of the cycles: shared memory leaves 14 to 23 warps an SM.
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -233,7 +247,8 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_const
     const T *from = static_cast<const T *>(p.logits) + first * p.stride;
     const uint8_t *mask = p.legal ? p.legal + first * p.actions : nullptr;
     int phase = 0;
-    if (p.stride == p.actions || count == 1) {
+    // (a single row of others may begin anywhere, but pieces of 16 bytes may not)
+    if (p.stride == p.actions || (count == 1 && b.pitch == p.actions * (int)sizeof(T))) {
       phase = (int)(reinterpret_cast<uintptr_t>(from) & 15);
       stage<sizeof(T)>(own, reinterpret_cast<const uint8_t *>(from), count, p.actions * (int)sizeof(T), b.pitch);
     } else {
@@ -519,8 +534,9 @@ __global__ void __launch_bounds__(kThreads, kGradientCtas) short_gradient_kernel
 // and one comparison decides whether its sums change their base.
 constexpr int kVectors = 4;
 // What is below kFloor counts as -inf in a row whose maximum is above kLow: 2^((kFloor -
-// kLow) scale) is 0 at every temperature.
-constexpr float kFloor = -0x1p100f, kLow = -0x1p99f;
+// kLow) scale) is 0 at every temperature.  A row whose maximum is above kHigh is not summed
+// this way either: exponents might end at -inf, and 0 times that is no number.
+constexpr float kFloor = -0x1p100f, kLow = -0x1p99f, kHigh = 0x1p99f;
 
 // 32 bits of -inf
 template <typename T>
@@ -923,8 +939,8 @@ __global__ void __launch_bounds__(kLong, kLongCtas<Masked>) long_kernel(const __
     if (!begun) cluster.barrier_wait();
     begun = true;
     float largest = exchange(sh, a.top, ctas, rank, groups);
-    // a row masked throughout by low values, or with an infinity: element by element, as they are
-    const bool plain = largest >= kLow && largest < INFINITY;
+    // a row masked throughout by low values, or with an infinity or near it: element by element, as they are
+    const bool plain = largest >= kLow && largest <= kHigh;
     if (!plain) {
       a.top = odd >= 0 ? slice.element(odd) : -INFINITY;
       for (int i = 0; i * per_part < chunks; ++i) {
@@ -1092,7 +1108,7 @@ cudaError_t short_rows(Params &p, bool gradient, int sms, cudaStream_t st) {
   if (gradient) {
     // (whole eights of rows: a group then begins on a 16-byte boundary where the first does)
     const int rows = std::max(8, std::min(kMaxRows, kGroupElements / p.actions / 8 * 8));
-    // cell / all for cells below 2^13 (8 rows of 512, or kGroupElements): the quotient's error cell / 2^32 stays below 1 / all
+    // cell / all for cells below 2^13 (8 rows of kMaxManyGradient, or kGroupElements): the quotient's error cell / 2^32 stays below 1 / all
     const uint32_t reciprocal = (uint32_t)((1ull << 32) / all + 1);
     const unsigned ctas = (unsigned)std::min<int64_t>((p.rows + rows - 1) / rows, (int64_t)sms * kGradientCtas);
     constexpr int C = 16 / (W * (int)sizeof(T));

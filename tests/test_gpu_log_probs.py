@@ -242,6 +242,32 @@ def test_strided_rows_and_offsets(cuda, shape, dtype):
     _check_gradient(logits, action, legal, 1.0, out, d, torch.ones(N, device="cuda"), None)
 
 
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("shape", [(40, 64), (1, 64), (3, 32), (38017, 64), (50, 512), (7, 8)], ids=str)
+def test_rows_of_whole_pieces_strided(cuda, shape, dtype):
+    """Rows of a multiple of 32 bytes, the first on a 16-byte boundary, others on none."""
+    N, A = shape
+    for pad in (1, 3, 8):
+        wide, action, mask = _inputs(N, A + pad, dtype, True, seed=pad)
+        logits, legal = wide[:, :A], mask[:, :A]
+        out, d = _check(logits, action.clamp(max=A), legal, 1.0, 3)
+        g = torch.linspace(-1, 1, N, device="cuda")
+        _check_gradient(logits, action.clamp(max=A), legal, 1.0, out, d, g, g)
+
+
+@pytest.mark.parametrize("A", [82, 700, 70000])
+def test_far_apart_logits(cuda, A):
+    """A maximum of 1e20 to 1e35 above ordinary logits: exponents of up to
+    1e38, which float32 holds, at every temperature's end."""
+    logits, action, _ = _inputs(8, A, "fp32", False)
+    action[:4] = A // 2
+    logits[:, A // 2] = torch.tensor([1e30, 1e35, 3e34, 1e20, -1e34, 6e29, 7e29, 2e32], device="cuda")
+    logits[1, 3] = -3e34
+    for T in (1e-3, 1.0, 1e3):
+        out, d = _check(logits, action, None, T, 5)
+        _check_gradient(logits, action, None, T, out, d, torch.ones(8, device="cuda"), torch.ones(8, device="cuda"))
+
+
 def test_transposed_logits_are_copied(cuda):
     logits, action, _ = _inputs(82, 64, "fp32", False)
     out, _ = _check(logits, action, None, 1.0, 2)
