@@ -31,14 +31,14 @@
 //
 // Device times, by graph replays: 50.4 M float32 weights and gradients with
 // 32-bit moments 212 us (6.7 TB/s, the copy's rate); 67.1 M bfloat16 weights and
-// gradients with moments of 8 bits 217 us (3.1 TB/s; 104 us at a copy's rate),
-// with float32 weights 202 us (4.6 TB/s); reading 8-bit moments out 62 us
+// gradients with moments of 8 bits 223 us (3.0 TB/s; 104 us at a copy's rate),
+// with float32 weights 210 us (4.5 TB/s); reading 8-bit moments out 62 us
 // (6.5 TB/s).  The norm of 67.1 M bfloat16 gradients 27 us (4.9 TB/s), of 50.4 M
 // float32 33 us (6.1 TB/s); 66 small tensors 6 us.
 //
-// 32-bit moments are bound by memory.  Those of 8 bits issue 90 instructions
-// an element on 60 to 70 % of the cycles: 19 are the random bits' (without
-// them a step took 8 % less), the rest decoding, the roots and encoding.
+// 32-bit moments are bound by memory.  Those of 8 bits issue 100 instructions
+// an element on 80 % of the cycles, the pipe of logic and additions 69 % busy: 19
+// are the random bits', the rest decoding, roots, quotients and encoding.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -228,9 +228,18 @@ __device__ __forceinline__ float2 moments_of(const Moments &p, float clip, float
   v = v * both(p.b2) + g * g * both(p.b2c);
   return make_float2(sqrtf(v.x), sqrtf(v.y));
 }
+// The quotient takes one step of Newton's method from the approximate
+// reciprocal, as exact as a division: bfloat16 weights round by random bits, and
+// what 32 bits lose shows there as whole steps.  (A root that is infinite would
+// make the residual no number.)
 __device__ __forceinline__ float2 weights_of(const Moments &p, const State &s, float decay, float2 w, float2 m, float2 root) {
-  const float2 den = __ffma2_rn(root, both(s.inv_root), both(p.eps));
-  return __ffma2_rn(w, both(decay), m * both(-s.size) * make_float2(reciprocal(den.x), reciprocal(den.y)));
+  float2 den = __ffma2_rn(root, both(s.inv_root), both(p.eps));
+  den = make_float2(fminf(den.x, 1e37f), fminf(den.y, 1e37f));
+  const float2 r = make_float2(reciprocal(den.x), reciprocal(den.y));
+  const float2 update = m * both(-s.size);
+  float2 q = update * r;
+  q = __ffma2_rn(__ffma2_rn(make_float2(-den.x, -den.y), q, update), r, q);
+  return __ffma2_rn(w, both(decay), q);
 }
 
 // Moments of 32 bits: four elements of each array a thread and pass.
