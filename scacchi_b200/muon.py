@@ -190,7 +190,7 @@ class NetworkMuon:
     gives the updated parameters, and raises ScacchiError where a wait of a
     step ran out (``check_waits``).  The stem, the 1x1 convolutions, the
     output vectors, biases and BatchNorm are not matrices to orthogonalise
-    and stay as they were given (train them with Adam beside it).
+    and stay as they were given (``adamw.NetworkAdamW`` steps them beside it).
     """
 
     def __init__(self, params: AZDirichletParams, *, learning_rate: float, beta: float = 0.95, nesterov: bool = True,
