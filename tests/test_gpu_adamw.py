@@ -492,6 +492,25 @@ def test_a_large_tensor(cuda):
                                 decay=0.0, clip=1.0, key=KEY)
 
 
+def test_offsets_past_32_bits(cuda):
+    """One step of gradients of 1 over more than 2^31 weights of 0: the first
+    moment is 0.1, the root sqrt(0.001), each on one of the codes beside it
+    (1/8 and 1/16 of their binades), the weight -0.01 to bfloat16."""
+    n = (1 << 31) + 5003
+    w = {"a": torch.zeros((n,), dtype=torch.bfloat16, device="cuda")}
+    g = {"a": torch.ones((n,), dtype=torch.bfloat16, device="cuda")}
+    opt = AdamW(w, learning_rate=0.01, state_bits=8, key=KEY)
+    assert abs(float(gradient_norm(g)) - math.sqrt(n)) <= U * math.sqrt(n)
+    opt.step(g)
+    first, root = opt.moments()
+    for part in (slice(0, 5000), slice(n - 5003, n)):
+        assert float((w["a"][part].double() + 0.01).abs().max()) <= 0.01 * 2.0 ** -7
+        assert float((first[part].double() / 0.1 - 1).abs().max()) <= 1 / 8
+        assert float((root[part].double() / math.sqrt(0.001) - 1).abs().max()) <= 1 / 16
+        assert abs(float(first[part].double().mean()) - 0.1) < 1e-3  # (5000 of at most 1/16 x 0.1 each: 6 sigma 5e-4)
+    assert not bool(first[n:].any()) and not bool(root[n:].any())
+
+
 def test_backward_through_a_stepped_weight_is_refused(cuda):
     w = torch.ones((8,), device="cuda", requires_grad=True)
     loss = (w * w).sum()

@@ -400,6 +400,31 @@ def test_shapes_types_and_empty_batches(cuda):
     assert not policy_log_probs_gradient(tracked, action, flat, grad_log_prob=flat.entropy).requires_grad
 
 
+@pytest.mark.parametrize("shape", [(66001, 32768), (26_300_003, 82)], ids=str)
+def test_offsets_past_32_bits(cuda, shape):
+    """The last of more than 2^31 logits."""
+    N, A = shape
+    assert N * A > 1 << 31
+    logits = torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    action = torch.arange(N, device="cuda", dtype=torch.int32) % A
+    legal = torch.ones(shape, dtype=torch.bool, device="cuda")
+    legal[-2, ::3] = False
+    out = policy_log_probs(logits, action, legal=legal, top=2)
+    last = slice(-5, None)
+    want, d = _definition(logits[last], action[last], legal[last], 1.0)
+    for name, (value, tol) in want.items():
+        _near(getattr(out, name)[last], value, tol, name)
+    _check_top(type(out)(*(v[last] for v in out)), d, 2, 1.0)
+    g = torch.ones(N, device="cuda")
+    grad = policy_log_probs_gradient(logits, action, out, grad_log_prob=g, grad_entropy=g, legal=legal)
+    few = policy_log_probs(logits[last], action[last], legal=legal[last])
+    small = policy_log_probs_gradient(logits[last], action[last], few, grad_log_prob=g[last], grad_entropy=g[last],
+                                      legal=legal[last])
+    # the row's numbers of either call are off by less than 1e-5 each, and one step of bfloat16
+    assert bool(((grad[last].float() - small.float()).abs() <= 1e-4 * small.float().abs() + 2.0 ** -8 * small.float().abs()
+                 + 1e-7).all())
+
+
 def test_repeats_bit_for_bit(cuda):
     for shape in ((4096, 82), (64, 20001), (2, 131071)):
         logits, action, mask = _inputs(*shape, "bf16", True)
