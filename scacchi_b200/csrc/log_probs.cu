@@ -68,7 +68,7 @@ constexpr int kMaxMany = 2048, kMaxManyGradient = 1024;
 constexpr int kMaxActions = 262144;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 16;
-constexpr int kMaxGroups = 128;
+constexpr int kMaxGroups = 64;  // of a row's threads: four warps of sixteen CTAs, or 64 of fewer
 constexpr int kCandidates = 512;
 constexpr int kParts = 8;           // of a thread's chunks, each with its maximum
 constexpr float kLog2E = 1.44269504088896341f;
