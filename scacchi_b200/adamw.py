@@ -249,8 +249,9 @@ class AdamW:
     def _step(self, grads: list, norm, learning_rate):
         table = self._table
         for name, w, row in zip(self._names, self._tensors, table):
-            if w.numel() != row["count"] or WEIGHT_DTYPES.get(w.dtype) != row["weight_dtype"] or not w.is_contiguous():
-                raise ValueError(f"{name} has changed its size, type or layout since AdamW was made")
+            if (w.device != self.device or w.numel() != row["count"] or not w.is_contiguous()
+                    or WEIGHT_DTYPES.get(w.dtype) != row["weight_dtype"]):
+                raise ValueError(f"{name} has changed its device, size, type or layout since AdamW was made")
         table["weight"] = [w.data_ptr() for w in self._tensors]
         table["gradient"] = [0 if g is None else g.data_ptr() for g in grads]
         table["gradient_dtype"] = [0 if g is None else GRADIENT_DTYPES[g.dtype] for g in grads]

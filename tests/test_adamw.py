@@ -145,3 +145,15 @@ def test_network_arrays_are_what_muon_leaves():
         return 0
 
     assert held == sum(size(getattr(params, f.name)) for f in dataclasses.fields(params))
+
+
+def test_a_weight_that_left_its_device_is_refused():
+    """``w.data = w.data.cpu()`` (a module moved behind the optimiser's back): its address is no longer the GPU's."""
+    launches = _lib.lib().scacchi_adamw_launch_count()
+    opt = AdamW.__new__(AdamW)
+    opt.device, opt.max_norm = torch.device("cuda", 0), None
+    opt._names, opt._tensors = ("a",), (torch.zeros(300),)
+    opt._table, opt._params = _table(), _params()
+    with pytest.raises(ValueError, match="a has changed its device"):
+        opt._step([torch.zeros(300)], None, None)
+    assert _lib.lib().scacchi_adamw_launch_count() == launches

@@ -600,3 +600,21 @@ def test_norm_refusals(cuda):
     for bad in ([good, good.cpu()], [good.double()], [good, good.int()]):
         with pytest.raises(ValueError):
             gradient_norm(bad)
+
+
+def test_weights_that_changed_are_refused(cuda):
+    """Moved to the CPU, of another size, type or layout: nothing is written."""
+    good = torch.ones((10, 10), device="cuda")
+    for change in (lambda t: t.cpu(), lambda t: t[:5], lambda t: t.bfloat16(), lambda t: t.t()):
+        w, other = torch.zeros((10, 10), device="cuda"), torch.zeros((3,), device="cuda")
+        opt = AdamW({"a": w, "b": other}, learning_rate=0.1)
+        w.data = change(w.data)
+        for grads in ({"a": good, "b": torch.ones((3,), device="cuda")}, {"b": torch.ones((3,), device="cuda")}):
+            with pytest.raises(ValueError, match="a has changed its device, size, type or layout|gradient of a"):
+                opt.step(grads)
+        assert opt.steps() == 0 and not bool(other.any()) and not bool(w.any())
+    # another storage on the same device is taken up
+    opt = AdamW({"a": w.data.t()}, learning_rate=0.1)
+    opt.weights["a"].data = torch.ones((10, 10), device="cuda")
+    opt.step({"a": good})
+    assert float(opt.weights["a"].max()) < 0.95
