@@ -622,8 +622,9 @@ typedef struct {
 } scacchi_adamw_tensor;
 
 /* norm[0] = sqrt(sum of squares) over all tensors, summed in 64 bits in a
- * fixed order.  workspace: scacchi_gradient_norm_workspace_bytes(num_tensors)
- * bytes, 8-byte aligned, of this call alone. */
+ * fixed order; at most 2^43 elements in all.  workspace:
+ * scacchi_gradient_norm_workspace_bytes(num_tensors) bytes, 8-byte aligned, of
+ * this call alone. */
 size_t scacchi_gradient_norm_workspace_bytes(int32_t num_tensors);
 int scacchi_gradient_norm(const scacchi_adamw_tensor *tensors, int32_t num_tensors, float *norm, void *workspace,
                           void *stream);

@@ -634,6 +634,8 @@ bool overlap(std::vector<Span> &own, const std::vector<Span> &read) {
   return false;
 }
 
+constexpr int64_t kMaxChunks = (int64_t)1 << 30;  // of a launch
+
 // The tensors that hold anything, each with its first chunk of `size`
 // elements
 struct Chunked {
@@ -645,8 +647,8 @@ bool chunked(const scacchi_adamw_tensor *tensors, int32_t n, int64_t size, Chunk
     const scacchi_adamw_tensor &t = tensors[i];
     if (t.count == 0 || !t.gradient) continue;
     const bool aligned = !misaligned(t.weight, 16) && !misaligned(t.gradient, 16);
-    const int64_t chunks = (t.count + size - 1) / size;
-    if (chunks > (int64_t)1 << 30) return false;
+    const int64_t chunks = (t.count - 1) / size + 1;
+    if (chunks > kMaxChunks) return false;
     out.entries.push_back(Entry{t.weight, t.gradient, t.count, t.offset, t.weight_decay,
                                 t.weight_dtype + 4 * t.gradient_dtype + (aligned ? 16 : 0), 0});
     out.chunks.push_back(chunks);
@@ -660,7 +662,7 @@ template <int N>
 int fill(Table<N> &table, const Chunked &all, size_t &at) {
   int64_t total = 0;
   table.tensors = 0;
-  while (at < all.entries.size() && table.tensors < N && total + all.chunks[at] <= ((int64_t)1 << 30)) {
+  while (at < all.entries.size() && table.tensors < N && total + all.chunks[at] <= kMaxChunks) {
     Entry &e = table.entry[table.tensors++];
     e = all.entries[at];
     e.first = (int32_t)total;
@@ -724,6 +726,11 @@ int scacchi_gradient_norm(const scacchi_adamw_tensor *tensors, int32_t num_tenso
   try {
     Chunked all;
     if (!chunked(tensors, num_tensors, kNormChunk, all)) return SCACCHI_EINVAL;
+    // the workspace holds the partials of launches with full tables: gradients that are listed
+    // again and again may fill a grid before its table
+    int64_t total = 0;
+    for (const int64_t chunks : all.chunks) total += chunks;
+    if (total > kMaxChunks) return SCACCHI_EINVAL;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     double *partial = static_cast<double *>(workspace);
     int partials = 0;

@@ -157,3 +157,13 @@ def test_a_weight_that_left_its_device_is_refused():
     with pytest.raises(ValueError, match="a has changed its device"):
         opt._step([torch.zeros(300)], None, None)
     assert _lib.lib().scacchi_adamw_launch_count() == launches
+
+
+def test_library_rejects_norms_of_more_than_the_workspace_holds():
+    """A gradient of 2^42 elements fills half of a launch's grid, and listed
+    three times two launches: more partial sums than three tensors have room for."""
+    launches = _lib.lib().scacchi_adamw_launch_count()
+    for n, count in ((3, 1 << 42), (2, (1 << 42) + 1), (1, (1 << 43) + 1), (1, (1 << 63) - 1)):
+        table = _table(*[(0, A, count, 0, 0.0, 0, 1)] * n)
+        assert _lib.lib().scacchi_gradient_norm(table.ctypes.data, n, 5 * A, 6 * A, None) == _lib.EINVAL
+    assert _lib.lib().scacchi_adamw_launch_count() == launches
