@@ -207,6 +207,14 @@ def lib() -> C.CDLL:
     return handle
 
 
+def bind_host(module, replaced: dict | None = None) -> None:
+    """Gives the extension module the library's entry points, or others' addresses by name."""
+    handle, names = lib(), ("scacchi_log_probs", "scacchi_log_probs_gradient", "scacchi_gradient_norm",
+                            "scacchi_gradient_norm_workspace_bytes", "scacchi_adamw_step", "scacchi_adamw_moments")
+    at = {n: C.cast(getattr(handle, n), C.c_void_p).value for n in names} | (replaced or {})
+    module.bind(*(at[n] for n in names), ScacchiError)
+
+
 @functools.lru_cache(maxsize=None)
 def host():
     """The extension module bound to the library, built first if it is missing."""
@@ -214,10 +222,7 @@ def host():
         _build.build_host()
     from . import _host
 
-    handle = lib()
-    _host.bind(*(C.cast(getattr(handle, n), C.c_void_p).value for n in (
-        "scacchi_log_probs", "scacchi_log_probs_gradient", "scacchi_gradient_norm",
-        "scacchi_gradient_norm_workspace_bytes", "scacchi_adamw_step", "scacchi_adamw_moments")))
+    bind_host(_host)
     return _host
 
 

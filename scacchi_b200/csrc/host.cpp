@@ -4,8 +4,10 @@
 //
 // Each function returns None where anything is not plain (another type,
 // layout, device or size, a value to refuse), and the caller's Python goes on
-// with its own checks, copies and errors; no argument is written then.  The
-// library's entry points come as addresses (bind).
+// with its own checks, copies and errors; no argument is written then.  What
+// fails in the library's launches is an error at once: some of a call's
+// launches may have run, and the call may not be made again.  The library's
+// entry points come as addresses (bind).
 //
 // 66 small tensors' AdamW step takes 56 us without this and 14 us with it,
 // the norm of 73 gradients 47 and 10, log-probabilities of 64 x 82 24 and 10.
@@ -18,6 +20,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <memory>
 #include <vector>
 
 #include "../../include/scacchi_b200.h"
@@ -31,7 +34,18 @@ struct Entries {
   decltype(&scacchi_gradient_norm_workspace_bytes) norm_bytes = nullptr;
   decltype(&scacchi_adamw_step) step = nullptr;
   decltype(&scacchi_adamw_moments) moments = nullptr;
+  PyObject *error = nullptr;  // the class of what is raised
 } g;
+
+struct Failed {};  // thrown with a Python error set
+
+// Whether the library took the call; false where it refused it, before any launch
+bool taken(int status, const char *what) {
+  if (status == SCACCHI_OK) return true;
+  if (status == SCACCHI_EINVAL) return false;
+  PyErr_Format(g.error, "%s: CUDA launch failed (status %d)", what, status);
+  throw Failed{};
+}
 
 constexpr int64_t kMaxActions = 262144, kMaxTop = 32;
 
@@ -114,7 +128,8 @@ PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t n) {
         static_cast<float *>(out[0].data_ptr()), static_cast<float *>(out[1].data_ptr()),
         static_cast<float *>(out[2].data_ptr()), static_cast<float *>(out[3].data_ptr()),
         top ? static_cast<float *>(out[4].data_ptr()) : nullptr, top ? static_cast<int32_t *>(out[5].data_ptr()) : nullptr};
-    if (g.log_probs(&r.rows, &at, r.num_rows, r.actions, r.dtype, temperature, (int32_t)top, stream_of(r.index)))
+    if (!taken(g.log_probs(&r.rows, &at, r.num_rows, r.actions, r.dtype, temperature, (int32_t)top,
+                           stream_of(r.index)), "log_probs"))
       Py_RETURN_NONE;
     PyObject *tuple = PyTuple_New(6);
     if (!tuple) return nullptr;
@@ -127,6 +142,8 @@ PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t n) {
       PyTuple_SET_ITEM(tuple, i, o);
     }
     return tuple;
+  } catch (const Failed &) {
+    return nullptr;
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -145,10 +162,12 @@ PyObject *log_probs_gradient(PyObject *, PyObject *const *args, Py_ssize_t n) {
         (args[8] != Py_None && args[6] == Py_None))
       Py_RETURN_NONE;
     at::Tensor out = empty(r.logits->sizes(), r.logits->scalar_type(), r.index);
-    if (g.gradient(&r.rows, at[0], at[1], at[2], at[3], at[4], r.num_rows, r.actions, r.dtype,
-                   PyFloat_AS_DOUBLE(args[3]), out.data_ptr(), stream_of(r.index)))
+    if (!taken(g.gradient(&r.rows, at[0], at[1], at[2], at[3], at[4], r.num_rows, r.actions, r.dtype,
+                          PyFloat_AS_DOUBLE(args[3]), out.data_ptr(), stream_of(r.index)), "log_probs_gradient"))
       Py_RETURN_NONE;
     return THPVariable_Wrap(out);
+  } catch (const Failed &) {
+    return nullptr;
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -159,7 +178,8 @@ PyObject *log_probs_gradient(PyObject *, PyObject *const *args, Py_ssize_t n) {
 at::Tensor norm_of(const scacchi_adamw_tensor *table, int32_t n, int index) {
   at::Tensor out = empty({}, at::kFloat, index);
   at::Tensor workspace = empty({(int64_t)(g.norm_bytes(n) + 7) / 8}, at::kDouble, index);
-  if (g.norm(table, n, static_cast<float *>(out.data_ptr()), workspace.data_ptr(), stream_of(index)))
+  if (!taken(g.norm(table, n, static_cast<float *>(out.data_ptr()), workspace.data_ptr(), stream_of(index)),
+             "gradient_norm"))
     return at::Tensor();
   return out;
 }
@@ -182,6 +202,8 @@ PyObject *gradient_norm(PyObject *, PyObject *list) {
     at::Tensor out = norm_of(table.data(), (int32_t)n, index);
     if (!out.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
+  } catch (const Failed &) {
+    return nullptr;
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -257,21 +279,25 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
       if (!norm.defined()) Py_RETURN_NONE;
     }
     params.norm = norm.defined() ? static_cast<const float *>(norm.data_ptr()) : nullptr;
-    if (g.step(&params, table.data(), (int32_t)count, stream_of(index))) Py_RETURN_NONE;
+    // (made before the step: nothing behind it may fail)
+    PyObject *o = norm.defined() ? THPVariable_Wrap(norm) : Py_NewRef(Py_None);
+    if (!o) return nullptr;
+    const auto release = [](PyObject *p) { Py_XDECREF(p); };
+    std::unique_ptr<PyObject, decltype(release)> tuple(PyTuple_New(1), release);
+    if (!tuple) {
+      Py_DECREF(o);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(tuple.get(), 0, o);
+    if (!taken(g.step(&params, table.data(), (int32_t)count, stream_of(index)), "adamw_step")) Py_RETURN_NONE;
     // a graph recorded before the step refuses to run backward through it
     for (Py_ssize_t i = 0; i < count; ++i) {
       const at::Tensor &w = THPVariable_Unpack(PyTuple_GET_ITEM(args[1], i));
       if (!w.is_inference()) w.unsafeGetTensorImpl()->bump_version();
     }
-    PyObject *o = norm.defined() ? THPVariable_Wrap(norm) : Py_NewRef(Py_None);
-    if (!o) return nullptr;
-    PyObject *tuple = PyTuple_New(1);
-    if (!tuple) {
-      Py_DECREF(o);
-      return nullptr;
-    }
-    PyTuple_SET_ITEM(tuple, 0, o);
-    return tuple;
+    return tuple.release();
+  } catch (const Failed &) {
+    return nullptr;
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -293,7 +319,8 @@ PyObject *adamw_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
     }
     if (size[1] != size[0] || size[2] != size[0] / SCACCHI_ADAMW_BLOCK || size[3] != size[2]) Py_RETURN_NONE;
     at::Tensor first = empty({size[0]}, at::kBFloat16, index), root = empty({size[0]}, at::kBFloat16, index);
-    if (g.moments(at[0], at[1], at[2], at[3], size[0], first.data_ptr(), root.data_ptr(), stream_of(index)))
+    if (!taken(g.moments(at[0], at[1], at[2], at[3], size[0], first.data_ptr(), root.data_ptr(), stream_of(index)),
+               "adamw_moments"))
       Py_RETURN_NONE;
     PyObject *a = THPVariable_Wrap(first), *b = a ? THPVariable_Wrap(root) : nullptr;
     PyObject *tuple = b ? PyTuple_New(2) : nullptr;
@@ -305,16 +332,18 @@ PyObject *adamw_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
     PyTuple_SET_ITEM(tuple, 0, a);
     PyTuple_SET_ITEM(tuple, 1, b);
     return tuple;
+  } catch (const Failed &) {
+    return nullptr;
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
   }
 }
 
-// (six addresses of the library's entry points)
+// (six addresses of the library's entry points, the class of errors)
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "bind takes six addresses");
+  if (n != 7 || !PyExceptionClass_Check(args[6])) {
+    PyErr_SetString(PyExc_TypeError, "bind takes six addresses and an exception's class");
     return nullptr;
   }
   void *at[6];
@@ -331,6 +360,7 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
   g.norm_bytes = reinterpret_cast<decltype(g.norm_bytes)>(at[3]);
   g.step = reinterpret_cast<decltype(g.step)>(at[4]);
   g.moments = reinterpret_cast<decltype(g.moments)>(at[5]);
+  Py_XSETREF(g.error, Py_NewRef(args[6]));
   Py_RETURN_NONE;
 }
 
