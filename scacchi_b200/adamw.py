@@ -122,6 +122,10 @@ class AdamW:
 
     A first moment that fades below 2^-17 of its block's largest is lost now
     and then; a root is never rounded to zero.
+
+    Squares of gradients above 1.8e19 are infinite in 32 bits: the weight then
+    rests (all but its decay), and 8-bit moments lose that block of 256, whose
+    weights are NaN from the next step on.  ``max_norm`` keeps gradients below.
     """
 
     def __init__(self, weights: Mapping[str, torch.Tensor], *, learning_rate: float, beta1: float = 0.9,

@@ -230,12 +230,13 @@ __device__ __forceinline__ float2 moments_of(const Moments &p, float clip, float
 }
 // The quotient takes one step of Newton's method from the approximate
 // reciprocal, as exact as a division: bfloat16 weights round by random bits, and
-// what 32 bits lose shows there as whole steps.  (A root that is infinite would
-// make the residual no number.)
+// what 32 bits lose shows there as whole steps.  An infinite root (of a square
+// beyond float32) has the reciprocal 0 and moves nothing; 1e37 in its place
+// keeps the residual a number.  A root that is NaN makes the reciprocal NaN.
 __device__ __forceinline__ float2 weights_of(const Moments &p, const State &s, float decay, float2 w, float2 m, float2 root) {
   float2 den = __ffma2_rn(root, both(s.inv_root), both(p.eps));
-  den = make_float2(fminf(den.x, 1e37f), fminf(den.y, 1e37f));
   const float2 r = make_float2(reciprocal(den.x), reciprocal(den.y));
+  den = make_float2(fminf(den.x, 1e37f), fminf(den.y, 1e37f));
   const float2 update = m * both(-s.size);
   float2 q = update * r;
   q = __ffma2_rn(__ffma2_rn(make_float2(-den.x, -den.y), q, update), r, q);

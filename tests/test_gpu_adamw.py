@@ -618,3 +618,49 @@ def test_weights_that_changed_are_refused(cuda):
     opt.weights["a"].data = torch.ones((10, 10), device="cuda")
     opt.step({"a": good})
     assert float(opt.weights["a"].max()) < 0.95
+
+
+@pytest.mark.parametrize("gradient", ["fp32", "bf16"])
+@pytest.mark.parametrize("weight", ["fp32", "bf16"])
+def test_a_square_beyond_float32_is_an_infinite_root(cuda, weight, gradient):
+    """A finite gradient whose square is infinite: its weight rests (m / inf
+    is 0) while the root is infinite, and in 8 bits its block of roots is NaN
+    from the next step on, and so are its weights."""
+    for bits in (32, 8):
+        w = {"a": torch.ones((1000,), device="cuda", dtype=DT[weight]), "b": torch.ones((10,), device="cuda")}
+        opt = AdamW(w, learning_rate=1e-3, state_bits=bits, key=KEY)
+        g = {"a": torch.ones((1000,), device="cuda", dtype=DT[gradient]), "b": torch.ones((10,), device="cuda")}
+        g["a"][300] = 3e38
+        opt.step(g)
+        assert float(w["a"][300]) == 1.0 and bool(w["a"].isfinite().all())
+        assert bool((w["a"].double() < 1.0 + 2.0 ** -24).all())
+        if bits == 8:
+            assert opt.second_exponent.tolist()[1] == 255 and 255 not in opt.first_exponent.tolist()
+        else:
+            assert math.isinf(float(opt.second[300])) and math.isfinite(float(opt.first[300]))
+        opt.step({k: torch.ones_like(v) for k, v in g.items()})
+        nan = w["a"].isnan()
+        if bits == 8:
+            assert bool(nan[256:512].all()) and not bool(nan[:256].any()) and not bool(nan[512:].any())
+        else:
+            assert not bool(nan.any()) and float(w["a"][300]) == 1.0
+        assert not bool(w["b"].isnan().any())
+
+
+def test_a_second_moment_that_is_no_number_shows_in_the_weight(cuda):
+    """A NaN that was loaded, and with beta2 = 0 one of infinity times 0."""
+    w = {"a": torch.ones((1000,), device="cuda")}
+    opt = AdamW(w, learning_rate=1e-3)
+    second = opt.second.clone()
+    second[7] = math.nan
+    opt.load_state_dict(dict(step=3, first=opt.first.clone(), second=second))
+    opt.step({"a": torch.ones((1000,), device="cuda")})
+    assert w["a"].isnan().nonzero().flatten().tolist() == [7]
+    w = {"a": torch.ones((1000,), device="cuda")}
+    opt = AdamW(w, learning_rate=1e-3, beta2=0.0)
+    g = torch.ones((1000,), device="cuda")
+    g[5] = 1e25
+    opt.step({"a": g})
+    assert bool(w["a"].isfinite().all())
+    opt.step({"a": torch.ones((1000,), device="cuda")})
+    assert w["a"].isnan().nonzero().flatten().tolist() == [5]
