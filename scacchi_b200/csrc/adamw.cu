@@ -430,11 +430,19 @@ __device__ __forceinline__ void step8(const Moments &p, const Entry &e, const St
         const float2 y = m[h][j / 2] * m_down * both(0x1p-113f), z = r[h][j / 2] * r_down * both(0x1p-113f);
         const uint32_t u = half_of(j < 2 ? random[h].x : random[h].y, j);
         const uint32_t yb = __float_as_uint(j & 1 ? y.y : y.x), zb = __float_as_uint(j & 1 ? z.y : z.x);
-        mb[j] = (yb * 16u + (u * 256u + 128u)) | (yb & 0x80000000u);
+        mb[j] = yb * 16u + (u * 256u + 128u) + (yb & 0x80000000u);
         rb[j] = zb * 32u + ((u * 0x9e370000u + 0x8000u) >> 8);
       }
-      uint32_t mo = upper_bytes(mb[0], mb[1], mb[2], mb[3]), ro = upper_bytes(rb[0], rb[1], rb[2], rb[3]);
-      if (m_field == 253u) mo = __vminu4(mo & 0x7f7f7f7fu, 0x7e7e7e7eu) | (mo & 0x80808080u);  // beyond the largest code
+      if (m_field == 253u) {  // beyond the largest code: before the sums' carry can reach the sign
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const float x = j & 1 ? m[h][j / 2].y : m[h][j / 2].x;
+          const uint32_t size = mb[j] - (__float_as_uint(x) & 0x80000000u);
+          mb[j] = min(size, 0x7effffffu) | (__float_as_uint(x) & 0x80000000u);
+        }
+      }
+      const uint32_t mo = upper_bytes(mb[0], mb[1], mb[2], mb[3]);
+      uint32_t ro = upper_bytes(rb[0], rb[1], rb[2], rb[3]);
       if ((ro - 0x01010101u) & ~ro & 0x80808080u) {  // a byte of zero: the borrow reaches its upper bit
 #pragma unroll
         for (int j = 0; j < W; ++j)

@@ -664,3 +664,20 @@ def test_a_second_moment_that_is_no_number_shows_in_the_weight(cuda):
     assert bool(w["a"].isfinite().all())
     opt.step({"a": torch.ones((1000,), device="cuda")})
     assert w["a"].isnan().nonzero().flatten().tolist() == [5]
+
+
+def test_the_largest_codes_keep_their_sign(cuda):
+    """First moments at the end of float32's range: 1.875 x 2^127 and above
+    would round to a code beyond the seven bits, and stay at the largest."""
+    n = 4 * BLOCK
+    w = {"a": torch.zeros((n,), device="cuda")}
+    opt = AdamW(w, learning_rate=0.0, beta1=0.0, state_bits=8, key=KEY)
+    g = torch.full((n,), 3.3e38, device="cuda")
+    g[BLOCK:2 * BLOCK] = torch.finfo(torch.float32).max
+    g[2 * BLOCK:] = 1.75 * 2.0 ** 127
+    g[::3] *= -1
+    opt.step({"a": g})
+    assert opt.first_exponent.tolist() == [253] * 4
+    want = torch.where(g < 0, 0xfe, 0x7e).to(torch.uint8)
+    assert torch.equal(opt.first, want)
+    assert torch.equal(opt.moments()[0].double(), g.sign().double() * 1.75 * 2.0 ** 127)
