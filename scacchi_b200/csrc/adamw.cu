@@ -570,18 +570,31 @@ __device__ __forceinline__ double square_of(uint32_t word, double sum) {
     return fma((double)two.y, (double)two.y, fma((double)two.x, (double)two.x, sum));
   }
 }
+// 16 bytes of elements, one by one where they begin off a boundary
 template <typename T>
+__device__ __forceinline__ uint4 vector_of(const T *x, bool aligned) {
+  if (aligned) return *reinterpret_cast<const uint4 *>(x);
+  constexpr int64_t N = 16 / sizeof(T);
+  if constexpr (sizeof(T) == 4) {
+    return load_slowly(x, 0, N);
+  } else {
+    const uint2 low = load_slowly(x, 0, N), high = load_slowly(x + 4, 0, N);
+    return make_uint4(low.x, low.y, high.x, high.y);
+  }
+}
+// (each element goes to the same thread whatever the tensor's alignment: the
+// order of the sum, and with it the norm's last bit, depends on sizes alone)
+template <typename T, bool Aligned>
 __device__ __forceinline__ double squares(const Entry &e, int64_t begin) {
   constexpr int W = 16 / sizeof(T), kAhead = 4;  // vectors of a thread in flight together
   const T *x = static_cast<const T *>(e.gradient) + begin;
-  const int count = (int)min((int64_t)kNormChunk, e.count - begin);
-  const int vectors = e.kind & 16 ? count / W : 0;
+  const int count = (int)min((int64_t)kNormChunk, e.count - begin), vectors = count / W;
   double sum = 0.0;
   for (int i = threadIdx.x; i < vectors; i += kAhead * kThreads) {
     uint4 q[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      q[k] = i + k * kThreads < vectors ? reinterpret_cast<const uint4 *>(x)[i + k * kThreads] : make_uint4(0, 0, 0, 0);
+      q[k] = i + k * kThreads < vectors ? vector_of(x + (i + k * kThreads) * W, Aligned) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       sum = square_of<T>(q[k].w, square_of<T>(q[k].z, square_of<T>(q[k].y, square_of<T>(q[k].x, sum))));
@@ -600,10 +613,13 @@ __global__ void __launch_bounds__(kThreads, kNormCtas) norm_kernel(const __grid_
   for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const Entry &e = table.entry[find(table, chunk)];
     const int64_t begin = (int64_t)(chunk - e.first) * kNormChunk;
-    switch (e.kind >> 2 & 3) {
-      case 0: sum += squares<float>(e, begin); break;
-      case 1: sum += squares<__nv_bfloat16>(e, begin); break;
-      default: sum += squares<__half>(e, begin); break;
+    switch (e.kind >> 2 & 7) {
+      case 0: sum += squares<float, false>(e, begin); break;
+      case 1: sum += squares<__nv_bfloat16, false>(e, begin); break;
+      case 2: sum += squares<__half, false>(e, begin); break;
+      case 4: sum += squares<float, true>(e, begin); break;
+      case 5: sum += squares<__nv_bfloat16, true>(e, begin); break;
+      default: sum += squares<__half, true>(e, begin); break;
     }
   }
   sum = cta_sum(sum);
@@ -645,17 +661,18 @@ bool overlap(std::vector<Span> &own, const std::vector<Span> &read) {
 
 constexpr int64_t kMaxChunks = (int64_t)1 << 30;  // of a launch
 
-// The tensors that hold anything, each with its first chunk of `size`
-// elements
+// The tensors that hold anything, each with its number of chunks
 struct Chunked {
   std::vector<Entry> entries;
   std::vector<int64_t> chunks;
 };
-bool chunked(const scacchi_adamw_tensor *tensors, int32_t n, int64_t size, Chunked &out) {
+// (`norm`: of gradients alone, weights are not looked at)
+bool chunked(const scacchi_adamw_tensor *tensors, int32_t n, bool norm, Chunked &out) {
+  const int64_t size = norm ? kNormChunk : kChunk;
   for (int32_t i = 0; i < n; ++i) {
     const scacchi_adamw_tensor &t = tensors[i];
     if (t.count == 0 || !t.gradient) continue;
-    const bool aligned = !misaligned(t.weight, 16) && !misaligned(t.gradient, 16);
+    const bool aligned = (norm || !misaligned(t.weight, 16)) && !misaligned(t.gradient, 16);
     const int64_t chunks = (t.count - 1) / size + 1;
     if (chunks > kMaxChunks) return false;
     out.entries.push_back(Entry{t.weight, t.gradient, t.count, t.offset, t.weight_decay,
@@ -734,7 +751,7 @@ int scacchi_gradient_norm(const scacchi_adamw_tensor *tensors, int32_t num_tenso
   }
   try {
     Chunked all;
-    if (!chunked(tensors, num_tensors, kNormChunk, all)) return SCACCHI_EINVAL;
+    if (!chunked(tensors, num_tensors, true, all)) return SCACCHI_EINVAL;
     // the workspace holds the partials of launches with full tables: gradients that are listed
     // again and again may fill a grid before its table
     int64_t total = 0;
@@ -796,7 +813,7 @@ int scacchi_adamw_step(const scacchi_adamw *params, const scacchi_adamw_tensor *
     if (a.norm) read.push_back(span(a.norm, 4));
     if (a.learning_rate_at) read.push_back(span(a.learning_rate_at, 4));
     Chunked all;
-    if (overlap(own, read) || !chunked(tensors, num_tensors, kChunk, all)) return SCACCHI_EINVAL;
+    if (overlap(own, read) || !chunked(tensors, num_tensors, false, all)) return SCACCHI_EINVAL;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     State *state = static_cast<State *>(a.state);
     adamw_begin_kernel<<<1, 1, 0, st>>>(Begin{state, a.norm, a.learning_rate_at, a.learning_rate, log(a.beta1),

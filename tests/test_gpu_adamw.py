@@ -681,3 +681,32 @@ def test_the_largest_codes_keep_their_sign(cuda):
     want = torch.where(g < 0, 0xfe, 0x7e).to(torch.uint8)
     assert torch.equal(opt.first, want)
     assert torch.equal(opt.moments()[0].double(), g.sign().double() * 1.75 * 2.0 ** 127)
+
+
+def _order_shows(dtype):
+    """Values whose squares' sum lies on a border of float32: 1 + 2^-23 +
+    2^-48 is the square of the middle between 1 and the next number, and 24
+    squares of 2^-54 count only where they meet each other before the 1."""
+    x = torch.zeros((8192,), dtype=torch.float32)
+    x[0], x[1001], x[2001], x[3001] = 1.0, 2.0 ** -12, 2.0 ** -12, 2.0 ** -24
+    tiny = [i for i in range(256, 8192, 256) if i % (4096 // dtype.itemsize)]
+    x[tiny] = 2.0 ** -27
+    return x.to(dtype).cuda()
+
+
+def _shifted(x, shift):
+    flat = torch.empty((x.numel() + shift,), dtype=x.dtype, device="cuda")
+    flat[shift:] = x
+    return flat[shift:]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norms_do_not_depend_on_alignment(cuda, dtype):
+    x = _order_shows(dtype)
+    want = gradient_norm([x])
+    for shift in range(1, 16 // x.element_size()):
+        assert torch.equal(gradient_norm([_shifted(x, shift)]), want)
+    # nor a step's own norm on where the weights lie
+    for shift in (0, 1):
+        w = _shifted(torch.zeros((8192,), device="cuda"), shift)
+        assert torch.equal(AdamW({"w": w}, learning_rate=0.1, max_norm=1.0).step({"w": x}), want)
