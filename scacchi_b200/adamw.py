@@ -277,7 +277,7 @@ class AdamW:
                              "weights do")
         _lib.check(rc, "adamw_step")
         # a graph recorded before the step refuses to run backward through it
-        torch.autograd.graph.increment_version(self._tensors)
+        torch.autograd.graph.increment_version([w for w, g in zip(self._tensors, grads) if g is not None])
         return norm
 
     def steps(self) -> int:

@@ -292,6 +292,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (!taken(g.step(&params, table.data(), (int32_t)count, stream_of(index)), "adamw_step")) Py_RETURN_NONE;
     // a graph recorded before the step refuses to run backward through it
     for (Py_ssize_t i = 0; i < count; ++i) {
+      if (!table[i].gradient) continue;
       const at::Tensor &w = THPVariable_Unpack(PyTuple_GET_ITEM(args[1], i));
       if (!w.is_inference()) w.unsafeGetTensorImpl()->bump_version();
     }

@@ -710,3 +710,17 @@ def test_norms_do_not_depend_on_alignment(cuda, dtype):
     for shift in (0, 1):
         w = _shifted(torch.zeros((8192,), device="cuda"), shift)
         assert torch.equal(AdamW({"w": w}, learning_rate=0.1, max_norm=1.0).step({"w": x}), want)
+
+
+@pytest.mark.parametrize("plain", [True, False])
+def test_backward_through_a_weight_that_was_not_stepped(cuda, plain):
+    """A weight without a gradient stays as it is, and so does a graph that it is in."""
+    a, b, c = (torch.ones((8,), device="cuda", requires_grad=True) for _ in range(3))
+    loss, other = (b * b).sum() + (c * c).sum(), (a * a).sum()
+    opt = AdamW({"a": a.detach(), "b": b.detach(), "c": c.detach()}, learning_rate=0.1)
+    g = torch.ones((8,), device="cuda") if plain else torch.ones((16,), device="cuda")[::2]
+    opt.step({"a": g, "c": None})
+    loss.backward()
+    assert torch.equal(b.grad, torch.full((8,), 2.0, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        other.backward()
