@@ -154,7 +154,7 @@ struct Row {
 
 __device__ __forceinline__ Row finish_row(float top, float s, float t) {
   Row r;
-  r.top = top;
+  r.top = s != s ? s : top;  // (maxima pass over what is no number, and +inf leaves a sum that is none)
   r.log_sum = logf(s);
   r.entropy = s == 0.0f ? 0.0f : r.log_sum - kLn2 * t / s;
   return r;

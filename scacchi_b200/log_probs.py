@@ -86,7 +86,8 @@ def policy_log_probs(logits: torch.Tensor, action: torch.Tensor, *, legal: torch
     any has entropy 0, ``max_logit`` and ``log_sum`` minus infinity; one
     whose logits all are the type's lowest value is uniform.  An illegal
     action's logit may hold anything; a NaN or +inf among the legal ones
-    makes the row's numbers NaN, its best actions unspecified.
+    makes the row's numbers NaN (a log-probability stays 0 or minus infinity
+    where the action has none), its best actions unspecified.
 
     ``max_logit`` and ``log_sum`` (log sum exp((x - max_logit) /
     temperature)) are what ``policy_log_probs_gradient`` needs.  The result
@@ -133,7 +134,8 @@ def policy_log_probs_gradient(logits: torch.Tensor, action: torch.Tensor, out: L
     gradients are floating point of the rows' shape; either may be absent,
     not both.  An action without a log-probability (out of range, illegal,
     -inf) has no gradient of it; illegal actions and those of -inf have 0
-    (in a row whose numbers are NaN the gradient may be NaN throughout).
+    (in a row whose numbers or gradients are not finite it may be NaN
+    throughout).
 
     The gradient is returned, not recorded: ``logits.backward(gradient)``
     continues it.  float16 ends at 6e-8: put a loss scale into the gradients

@@ -479,3 +479,33 @@ def test_refusals(cuda):
             policy_log_probs_gradient(x, k, out, grad_log_prob=bad)
         with pytest.raises(ValueError, match="max_logit"):
             policy_log_probs_gradient(x, k, out._replace(max_logit=bad), grad_log_prob=one)
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("shape", [(6, 82), (40000, 82), (6, 700), (1200, 1000), (6, 70000)], ids=str)
+@pytest.mark.parametrize("junk", [math.nan, math.inf])
+def test_all_numbers_of_a_row_with_a_legal_nan_or_infinity_are_nan(cuda, shape, dtype, junk):
+    """max_logit among them, beside other logits and where they are -inf; what
+    is said of actions out of range and of illegal ones holds there too."""
+    N, A = shape
+    logits, action, _ = _inputs(N, A, dtype, False)
+    legal = torch.ones((N, A), dtype=torch.bool, device="cuda")
+    legal[:, 1] = False
+    action[:5] = torch.tensor([0, A // 3, 0, -1, 1], dtype=torch.int32)
+    whole = policy_log_probs(logits, action, legal=legal)
+    logits[1] = -math.inf
+    logits[[0, 1, 3, 4], A // 3] = junk
+    for mask in (legal, None):
+        out = policy_log_probs(logits, action, legal=mask, top=2)
+        for name in ("entropy", "max_logit", "log_sum"):
+            assert bool(getattr(out, name)[[0, 1, 3, 4]].isnan().all()), name
+        assert out.log_prob[:2].isnan().all() and float(out.log_prob[3]) == 0.0
+    # (the last row's action is illegal with the mask)
+    out = policy_log_probs(logits, action, legal=legal)
+    assert float(out.log_prob[4]) == -math.inf
+    for a, b in zip(out[:4], whole[:4]):
+        assert torch.equal(a[5:], b[5:]) and torch.equal(a[2], b[2])
+    one = torch.ones(N, device="cuda")
+    grad = policy_log_probs_gradient(logits, action, out, grad_log_prob=one, grad_entropy=one, legal=legal)
+    assert bool(grad[[0, 1]].isnan().any(-1).all()) and bool(grad[2].isfinite().all())
+    assert bool(grad[5:].isfinite().all())
