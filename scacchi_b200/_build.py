@@ -20,7 +20,8 @@ UNITS = [(os.path.join(CSRC, "search.cu"), ["-fmad=false"]), (os.path.join(CSRC,
          (os.path.join(CSRC, "policy_loss.cu"), []), (os.path.join(CSRC, "muon.cu"), []),
          (os.path.join(CSRC, "adamw.cu"), ["-fmad=false"]), (os.path.join(CSRC, "log_probs.cu"), [])]
 SOURCES = [u[0] for u in UNITS]
-HEADERS = [os.path.join(CSRC, h) for h in ("smath.h", "threefry.h", "synthetic_env.h", "lane_cta.cuh", "tc05.cuh")] + [
+HEADERS = [os.path.join(CSRC, h) for h in ("smath.h", "threefry.h", "synthetic_env.h", "lane_cta.cuh", "tc05.cuh",
+                                            "row_log.cuh")] + [
     os.path.join(ROOT, "include", "scacchi_b200.h")]
 
 NVCC_FLAGS = ["-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo"]

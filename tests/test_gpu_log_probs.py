@@ -509,3 +509,44 @@ def test_all_numbers_of_a_row_with_a_legal_nan_or_infinity_are_nan(cuda, shape, 
     grad = policy_log_probs_gradient(logits, action, out, grad_log_prob=one, grad_entropy=one, legal=legal)
     assert bool(grad[[0, 1]].isnan().any(-1).all()) and bool(grad[2].isfinite().all())
     assert bool(grad[5:].isfinite().all())
+
+
+@pytest.mark.parametrize("A", [200, 600, 9000])
+@pytest.mark.parametrize("T", [1.0, 0.7, 3.0])
+def test_log_probs_are_rounded_once(cuda, A, T):
+    """n logits of 0, one u below them of e^-40 or less, the others -inf:
+    the sum is n in any type (n + e^-40 rounds to n in 32 bits), so log n, u /
+    T - log n and the entropy are off by their last rounding, 2^-24 of their
+    value, by the logarithm's 1.2e-10 of its own (the series' next term, 2e-11
+    twice, of at least 0.35) < 2^-32, and by 64-bit roundings and e^-40 (41 +
+    log n) < 2^-50."""
+    N = 180
+    n = 1 + torch.arange(N, device="cuda") % (A - 2)
+    logits = torch.where(torch.arange(A, device="cuda") < n[:, None], 0.0, -math.inf)
+    u = -40.0 * T - torch.arange(N, device="cuda") * 0.37
+    logits[:, A - 1] = u
+    action = torch.full((N,), A - 1, dtype=torch.int32, device="cuda")
+    action[::2] = 0
+    offset = torch.linspace(-3, 3, 13, device="cuda").round()[torch.arange(N, device="cuda") % 13]  # (0 is exact)
+    logits[:, :A - 1] += offset[:, None]
+    logits[:, A - 1] += offset
+    u = (logits[:, A - 1].double() - offset.double()) / T
+    out = policy_log_probs(logits, action, temperature=T, top=1)
+    log_n = n.double().log()
+    for name, want in (("log_sum", log_n), ("entropy", log_n), ("log_prob", torch.where(action == 0, -log_n, u - log_n))):
+        got = getattr(out, name).double()
+        assert bool(((got - want).abs() <= U * (1 + 2.0 ** -8) * want.abs() + 2.0 ** -50).all()), name
+    assert bool(((out.top_log_prob[:, 0].double() + log_n).abs() <= U * (1 + 2.0 ** -8) * log_n + 2.0 ** -50).all())
+
+
+@pytest.mark.parametrize("A", [82, 700, 20000])
+def test_log_probs_of_differences_beyond_float32(cuda, A):
+    """-3e38 below 3e38 at a temperature of 1000: 64 bits hold the difference,
+    and float32 holds its thousandth."""
+    logits = torch.zeros((4, A), device="cuda")
+    logits[:, 5] = 3e38
+    logits[:, 9] = -3e38
+    out = policy_log_probs(logits, torch.tensor([5, 9, 0, 9], device="cuda"), temperature=1e3)
+    want = [0.0, -6e35, -3e35, -6e35]
+    for a, b in zip(out.log_prob.tolist(), want):
+        assert abs(a - b) <= 4 * U * abs(b)
