@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import os
 import subprocess
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -41,11 +42,20 @@ def stale() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False, out: str | None = None, defines: tuple = ()) -> str:
+    """The library by nvcc alone, then the extension module, which needs
+    torch's and Python's headers: without them its calls go through Python."""
     out = out or LIB
+    if out != LIB or force or stale():
+        _build_library(out, verbose, defines)
     if out == LIB:
-        build_host(force)
-    if out == LIB and not force and not stale():
-        return LIB
+        try:
+            build_host(force)
+        except Exception as e:  # (no torch, no headers, no compiler)
+            warnings.warn(f"the extension module was not built: {e!r}", RuntimeWarning, stacklevel=2)
+    return out
+
+
+def _build_library(out: str, verbose: bool, defines: tuple) -> None:
     objs = []
     build_dir = os.path.join(HERE, "_build")
     os.makedirs(build_dir, exist_ok=True)
@@ -61,7 +71,6 @@ def build(force: bool = False, verbose: bool = False, out: str | None = None, de
         if p.wait() != 0:
             raise RuntimeError("nvcc failed")
     subprocess.run([nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", out, *objs], check=True)
-    return out
 
 
 def build_host(force: bool = False) -> str:
