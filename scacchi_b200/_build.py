@@ -4,13 +4,14 @@ from __future__ import annotations
 
 import os
 import subprocess
+import sys
+import threading
 import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libscacchi_b200.so")
-HOST = os.path.join(HERE, "_host.so")  # Python's calls of some operators (csrc/host.cpp)
 # (source, extra flags).  The search kernels are bit-reproducible against
 # the oracle: no implicit multiply-add contraction (they call fmaf()
 # explicitly where they want one), and the AdamW step's 8-bit codes against
@@ -73,25 +74,36 @@ def _build_library(out: str, verbose: bool, defines: tuple) -> None:
     subprocess.run([nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", out, *objs], check=True)
 
 
+def host_path() -> str:
+    """The extension module (csrc/host.cpp: Python's calls of some operators).
+    It holds to the C++ of the torch and the Python that it was built against,
+    so its name tells them: another torch finds none and builds its own."""
+    import torch
+
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    return os.path.join(HERE, f"_host.{sys.implementation.cache_tag}-torch{torch.__version__.replace("+", ".")}-abi{abi}.so")
+
+
 def build_host(force: bool = False) -> str:
     """The extension module, by the host's compiler against torch's headers."""
     src, header = os.path.join(CSRC, "host.cpp"), os.path.join(ROOT, "include", "scacchi_b200.h")
-    if not force and os.path.exists(HOST) and all(os.path.getmtime(p) <= os.path.getmtime(HOST) for p in (src, header)):
-        return HOST
+    path = host_path()
+    if not force and os.path.exists(path) and all(os.path.getmtime(p) <= os.path.getmtime(path) for p in (src, header)):
+        return path
     import sysconfig
 
     import torch
 
     base = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(nvcc())) or "/usr/local/cuda"
-    part = f"{HOST}.{os.getpid()}"  # renamed when whole: several processes may build at once
+    part = f"{path}.{os.getpid()}.{threading.get_ident()}"  # renamed when whole: several may build at once
     subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{base}/include",
                     f"-I{base}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
                     f"-I{cuda}/include", src, "-o", part, f"-L{base}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu",
                     "-lc10", "-lc10_cuda", f"-Wl,-rpath,{base}/lib"], check=True)
-    os.replace(part, HOST)
-    return HOST
+    os.replace(part, path)
+    return path
 
 
 if __name__ == "__main__":

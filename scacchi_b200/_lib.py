@@ -4,7 +4,10 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import importlib.machinery
+import importlib.util
 import os
+import warnings
 
 from . import _build
 
@@ -215,15 +218,35 @@ def bind_host(module, replaced: dict | None = None) -> None:
     module.bind(*(at[n] for n in names), ScacchiError)
 
 
+class PythonCalls:
+    """Stands in for the extension module: it declines every call, and Python's own way makes it."""
+
+    @staticmethod
+    def decline(*args) -> None:
+        return None
+
+    log_probs = log_probs_gradient = gradient_norm = adamw_step = adamw_moments = decline
+
+
 @functools.lru_cache(maxsize=None)
 def host():
-    """The extension module bound to the library, built first if it is missing."""
-    if not os.path.exists(_build.HOST):
-        _build.build_host()
-    from . import _host
+    """The extension module bound to the library, built first if it is missing.
 
-    bind_host(_host)
-    return _host
+    Where it cannot be built or loaded its calls go through Python, with the
+    same results and more of the host's time.
+    """
+    try:
+        path = _build.host_path()
+        if not os.path.exists(path):
+            _build.build_host()
+        loader = importlib.machinery.ExtensionFileLoader(f"{__package__}._host", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+        loader.exec_module(module)
+    except Exception as e:
+        warnings.warn(f"the extension module cannot be used, calls go through Python: {e!r}", RuntimeWarning, stacklevel=3)
+        return PythonCalls
+    bind_host(module)
+    return module
 
 
 def check(rc: int, what: str) -> None:

@@ -7,7 +7,9 @@ import sys
 
 import pytest
 
-from scacchi_b200 import _build
+import torch
+
+from scacchi_b200 import _build, _lib
 
 PATH = _build.__file__
 
@@ -72,3 +74,38 @@ assert len(seen) == 1 and "torch" in str(seen[0].message)
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
                          env={**os.environ, "PYTHONPATH": ""}, timeout=120)
     assert out.returncode == 0 and out.stdout == "library\n", out.stderr
+
+
+def test_the_extension_names_what_it_was_built_against(monkeypatch):
+    path = _build.host_path()
+    assert sys.implementation.cache_tag in path and torch.__version__.replace("+", ".") in path
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    assert _build.host_path() != path and "99.0" in _build.host_path()
+
+
+def _declines(module):
+    return all(getattr(module, n)(1, 2) is None for n in (
+        "log_probs", "log_probs_gradient", "gradient_norm", "adamw_step", "adamw_moments"))
+
+
+def test_without_a_compiler_calls_go_through_python(monkeypatch, tmp_path):
+    def fails(force=False):
+        raise FileNotFoundError("g++")
+
+    monkeypatch.setattr(_build, "host_path", lambda: str(tmp_path / "none.so"))
+    monkeypatch.setattr(_build, "build_host", fails)
+    with pytest.warns(RuntimeWarning, match="cannot be used.*g\\+\\+"):
+        assert _declines(_lib.host.__wrapped__())
+
+
+def test_an_extension_that_does_not_load_is_passed_over(monkeypatch, tmp_path):
+    broken = tmp_path / "broken.so"
+    broken.write_bytes(b"\x7fELF and no more")
+    monkeypatch.setattr(_build, "host_path", lambda: str(broken))
+    with pytest.warns(RuntimeWarning, match="cannot be used"):
+        assert _declines(_lib.host.__wrapped__())
+
+
+def test_the_extension_itself_loads():
+    assert _lib.host() is not _lib.PythonCalls
+    assert _lib.host().__name__ == "scacchi_b200._host"
