@@ -80,8 +80,8 @@ def host_path() -> str:
     so its name tells them: another torch finds none and builds its own."""
     import torch
 
-    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    return os.path.join(HERE, f"_host.{sys.implementation.cache_tag}-torch{torch.__version__.replace("+", ".")}-abi{abi}.so")
+    version, abi = torch.__version__.replace("+", "."), int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    return os.path.join(HERE, f"_host.{sys.implementation.cache_tag}-torch{version}-abi{abi}.so")
 
 
 def build_host(force: bool = False) -> str:

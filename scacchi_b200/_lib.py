@@ -243,7 +243,8 @@ def host():
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
         loader.exec_module(module)
     except Exception as e:
-        warnings.warn(f"the extension module cannot be used, calls go through Python: {e!r}", RuntimeWarning, stacklevel=3)
+        warnings.warn(f"the extension module cannot be used, calls go through Python: {e!r}", RuntimeWarning,
+                      stacklevel=3)
         return PythonCalls
     bind_host(module)
     return module
