@@ -75,6 +75,9 @@ def gradient_norm(gradients: Iterable[torch.Tensor] | Mapping[str, torch.Tensor]
         return done
     if not grads:
         raise ValueError("gradient_norm needs at least one gradient")
+    for g in grads:
+        if not isinstance(g, torch.Tensor):
+            raise ValueError(f"gradients must be tensors, got {type(g).__name__}")
     device = grads[0].device
     if device.type != "cuda":
         raise ValueError("gradient_norm runs on the GPU: pass gradients on a CUDA device")
@@ -207,6 +210,8 @@ class AdamW:
         for i, g in enumerate(grads):
             if g is None:
                 continue
+            if not isinstance(g, torch.Tensor):
+                raise ValueError(f"the gradient of {self._names[i]} must be a tensor, got {type(g).__name__}")
             if g.shape != self._shapes[i] or g.get_device() != index or g.dtype not in GRADIENT_DTYPES:
                 raise ValueError(f"the gradient of {self._names[i]} must be float32, bfloat16 or float16 "
                                  f"{tuple(self._shapes[i])} on {self.device}, got {g.dtype} {tuple(g.shape)} on "
@@ -243,6 +248,8 @@ class AdamW:
             if isinstance(t, torch.Tensor) and (t.dtype != torch.float32 or t.numel() != 1 or t.device != self.device):
                 raise ValueError(f"{name} must be one float32 on {self.device}, got {t.dtype} {tuple(t.shape)} on "
                                  f"{t.device}")
+        if norm is not None and not isinstance(norm, torch.Tensor):
+            raise ValueError(f"norm must be one float32 on {self.device}, got {type(norm).__name__}")
         if norm is not None and self.max_norm is None:
             raise ValueError("a norm is of use with max_norm alone")
         if torch.cuda.current_device() != self.device.index:

@@ -167,3 +167,16 @@ def test_library_rejects_norms_of_more_than_the_workspace_holds():
         table = _table(*[(0, A, count, 0, 0.0, 0, 1)] * n)
         assert _lib.lib().scacchi_gradient_norm(table.ctypes.data, n, 5 * A, 6 * A, None) == _lib.EINVAL
     assert _lib.lib().scacchi_adamw_launch_count() == launches
+
+
+def test_what_is_no_tensor_is_refused():
+    opt = AdamW.__new__(AdamW)
+    opt.device, opt.max_norm, opt._names, opt._shapes = torch.device("cuda", 0), 1.0, ("a",), [torch.Size([3])]
+    opt._tensors, opt._table, opt._params = (torch.zeros(3),), _table(), _params()
+    for bad in (np.zeros(3, np.float32), [0.0, 0.0, 0.0]):
+        with pytest.raises(ValueError, match="gradient of a must be a tensor"):
+            opt.step({"a": bad})
+        with pytest.raises(ValueError, match="must be tensors"):
+            gradient_norm([bad])
+    with pytest.raises(ValueError, match="norm must be one float32"):
+        opt.step({"a": None}, norm=5.0)
