@@ -258,7 +258,7 @@ class AdamW:
         return self._step(grads, norm, learning_rate)
 
     def _step(self, grads: list, norm, learning_rate):
-        table = self._table
+        table = self._table.copy()  # (the call lets other threads run, and they may step too)
         for name, w, row in zip(self._names, self._tensors, table):
             if (w.device != self.device or w.numel() != row["count"] or not w.is_contiguous()
                     or WEIGHT_DTYPES.get(w.dtype) != row["weight_dtype"]):

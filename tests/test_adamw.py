@@ -180,3 +180,23 @@ def test_what_is_no_tensor_is_refused():
             gradient_norm([bad])
     with pytest.raises(ValueError, match="norm must be one float32"):
         opt.step({"a": None}, norm=5.0)
+
+
+def test_a_call_has_a_table_of_its_own(monkeypatch):
+    """The library's call lets other threads run: what it reads is not written by another step."""
+    opt = AdamW.__new__(AdamW)
+    opt.device, opt.max_norm, opt._names, opt._tensors = torch.device("cpu"), None, ("a",), (torch.zeros(300),)
+    opt._table, opt._params = _table((0, 0, 300, 0, 0.0, 0, 0)), _params()
+    before, seen = opt._table.copy(), []
+
+    class Library:
+        @staticmethod
+        def scacchi_adamw_step(params, table, count, stream):
+            seen.append(table)
+            return _lib.EINVAL
+
+    monkeypatch.setattr(_lib, "lib", lambda: Library)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    with pytest.raises(ValueError, match="overlaps"):
+        opt._step([torch.zeros(300)], None, None)
+    assert seen[0] != opt._table.ctypes.data and np.array_equal(opt._table, before)
