@@ -574,6 +574,9 @@ int scacchi_muon_update(const scacchi_newton_schulz *params, const void *gradien
 int scacchi_muon_error(uint32_t *flags);
 uint64_t scacchi_muon_launch_count(void);
 
+#define SCACCHI_MAX_ACTIONS 262144     /* of a row of logits */
+#define SCACCHI_MAX_TOP 32             /* best actions of a row */
+
 /* Rows of logits and one action each.  logits hold num_actions elements a
  * row, rows `stride` elements apart; the others are dense. */
 typedef struct {

@@ -47,8 +47,6 @@ bool taken(int status, const char *what) {
   throw Failed{};
 }
 
-constexpr int64_t kMaxActions = 262144, kMaxTop = 32;
-
 int code_of(at::ScalarType t) {
   return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1;
 }
@@ -82,7 +80,7 @@ struct Rows {
     dtype = code_of(logits->scalar_type());
     if (index != c10::cuda::current_device() || dtype < 0 || !plain(x, index)) return false;
     const int64_t last = logits->size(-1);
-    if (last < 1 || last > kMaxActions) return false;
+    if (last < 1 || last > SCACCHI_MAX_ACTIONS) return false;
     actions = (int32_t)last;
     num_rows = logits->numel() / last;
     action = plain(a, index);
@@ -115,7 +113,7 @@ PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const double temperature = PyFloat_AS_DOUBLE(args[3]);
     int over = 0;
     const long top = PyLong_AsLongAndOverflow(args[4], &over);
-    if (over || top < 0 || top > kMaxTop) Py_RETURN_NONE;
+    if (over || top < 0 || top > SCACCHI_MAX_TOP) Py_RETURN_NONE;
     at::Tensor out[6];
     for (int i = 0; i < 4; ++i) out[i] = empty(r.lead(), at::kFloat, r.index);
     if (top) {

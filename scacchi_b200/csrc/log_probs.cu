@@ -66,8 +66,8 @@ constexpr int kMaxShort = 512;      // actions of a short row
 // and, where there are eight rows an SM at least, of a row that still goes that way: 20000 x 1000
 // bf16 with 20 best 57 us (131 as long rows), its gradient 22 (41); 5000 x 4000 62 (34) and 24 (15)
 constexpr int kMaxMany = 2048, kMaxManyGradient = 1024;
-constexpr int kMaxActions = 262144;
-constexpr int kMaxTop = 32;
+constexpr int kMaxActions = SCACCHI_MAX_ACTIONS;
+constexpr int kMaxTop = SCACCHI_MAX_TOP;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxGroups = 64;  // of a row's threads: four warps of sixteen CTAs, or 64 of fewer
 constexpr int kCandidates = 512;

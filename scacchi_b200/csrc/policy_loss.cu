@@ -71,7 +71,7 @@ constexpr int kMaxWarps = 8;  // of a long row's CTA
 static_assert(kLongThreads == 32 * kMaxWarps, "warps");
 constexpr int kMaxCluster = 16;
 constexpr int kMaxShort = 512;     // actions of a short row
-constexpr int kMaxActions = 262144;
+constexpr int kMaxActions = SCACCHI_MAX_ACTIONS;
 constexpr int kLongShared = 224 * 1024;  // of an SM, for the slices of its CTAs
 constexpr int kMaxPartials = 148 * 16;
 // What the 32-bit log-probability may be off by: terms within 2^-22 + 2.3 x

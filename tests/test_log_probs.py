@@ -2,12 +2,14 @@
 before any launch (no GPU needed)."""
 
 import ctypes as C
+import os
+import re
 
 import pytest
 import torch
 
-from scacchi_b200 import _lib
-from scacchi_b200.log_probs import LogProbs, policy_log_probs, policy_log_probs_gradient
+from scacchi_b200 import _build, _lib
+from scacchi_b200.log_probs import MAX_ACTIONS, MAX_TOP, LogProbs, policy_log_probs, policy_log_probs_gradient
 
 A = 1 << 20  # a made-up aligned address: a refused call reads none
 
@@ -83,3 +85,11 @@ def test_python_rejects_cpu_tensors():
 
 def test_struct_sizes():
     assert C.sizeof(_lib.LogProbRows) == 32 and C.sizeof(_lib.LogProbOut) == 48
+
+
+def test_limits_are_the_library_s():
+    header = open(os.path.join(_build.ROOT, "include", "scacchi_b200.h")).read()
+    for name, value in (("SCACCHI_MAX_ACTIONS", MAX_ACTIONS), ("SCACCHI_MAX_TOP", MAX_TOP)):
+        assert re.findall(rf"#define {name} (\d+)", header) == [str(value)]
+    assert _forward(rows=_rows(stride=MAX_ACTIONS + 1), actions=MAX_ACTIONS + 1) == _lib.EINVAL
+    assert _forward(top=MAX_TOP + 1) == _lib.EINVAL
