@@ -724,3 +724,37 @@ def test_backward_through_a_weight_that_was_not_stepped(cuda, plain):
     assert torch.equal(b.grad, torch.full((8,), 2.0, device="cuda"))
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         other.backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("weight", ["fp32", "bf16"])
+def test_launches_of_any_shape_change_no_bit(cuda, bits, weight):
+    """Two tensors beside 0, 40 and 600 others (tables of each size, the last
+    in two launches), stepped with them, each alone (the others without a
+    gradient), and with gradients off their boundaries."""
+    sizes = [5000, 300]
+    grads = [_tensors(sizes, "bf16", s, 0.1) for s in (5, 6)]
+
+    def run(more, alone=(None,), shift=0):
+        others = {f"o{i}": torch.ones((1 + 7 * i % 500,), device="cuda") for i in range(more)}
+        got = {}
+        for name in alone:
+            weights = {**_tensors(sizes, weight, 1, 0.1), **{k: v.clone() for k, v in others.items()}}
+            opt = AdamW(weights, learning_rate=0.01, state_bits=bits, key=KEY)
+            for g in grads:
+                given = {k: _shifted(v.reshape(-1), shift) for k, v in g.items() if name in (None, k)}
+                opt.step(given if name else {**given, **others})
+            for k in [name] if name else ["t0", "t1"]:
+                parts = [opt.views(opt.first)[k], opt.views(opt.second)[k], weights[k]]
+                if bits == 8:
+                    row = opt._table[opt._names.index(k)]
+                    at = slice(int(row["offset"]) // BLOCK, -(-int(row["offset"] + row["count"]) // BLOCK))
+                    parts += [opt.first_exponent[at], opt.second_exponent[at]]
+                got[k] = [p.clone() for p in parts]
+        return got
+
+    want = run(0)
+    for other in (run(40), run(600), run(0, ("t0", "t1")), run(600, ("t0", "t1")), run(0, shift=1), run(40, shift=5)):
+        for k, parts in want.items():
+            for a, b in zip(parts, other[k]):
+                assert torch.equal(a, b)
