@@ -613,13 +613,18 @@ __global__ void __launch_bounds__(kThreads, kNormCtas) norm_kernel(const __grid_
   for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const Entry &e = table.entry[find(table, chunk)];
     const int64_t begin = (int64_t)(chunk - e.first) * kNormChunk;
-    switch (e.kind >> 2 & 7) {
-      case 0: sum += squares<float, false>(e, begin); break;
-      case 1: sum += squares<__nv_bfloat16, false>(e, begin); break;
-      case 2: sum += squares<__half, false>(e, begin); break;
-      case 4: sum += squares<float, true>(e, begin); break;
-      case 5: sum += squares<__nv_bfloat16, true>(e, begin); break;
-      default: sum += squares<__half, true>(e, begin); break;
+    if (e.kind & 16) {
+      switch (e.kind >> 2 & 3) {
+        case 0: sum += squares<float, true>(e, begin); break;
+        case 1: sum += squares<__nv_bfloat16, true>(e, begin); break;
+        default: sum += squares<__half, true>(e, begin); break;
+      }
+    } else {
+      switch (e.kind >> 2 & 3) {
+        case 0: sum += squares<float, false>(e, begin); break;
+        case 1: sum += squares<__nv_bfloat16, false>(e, begin); break;
+        default: sum += squares<__half, false>(e, begin); break;
+      }
     }
   }
   sum = cta_sum(sum);
