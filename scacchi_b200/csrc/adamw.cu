@@ -418,6 +418,13 @@ __device__ __forceinline__ void step8(const Moments &p, const Entry &e, const St
       store_slowly(weight, other, e.count, w[1]);
     }
     const uint32_t m_field = block_field(m_most), r_field = block_field(r_most);
+    if (m_field == 253u) {  // what is beyond the largest code takes it: a sum's carry would reach the sign
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float2 &two = m[k / 2][k % 2];
+        two = make_float2(fminf(fmaxf(two.x, -0x1.cp127f), 0x1.cp127f), fminf(fmaxf(two.y, -0x1.cp127f), 0x1.cp127f));
+      }
+    }
     // 2^-e, then 2^-113: one factor would leave the range of floats
     const float2 m_down = both(power_of_two(254 - (int)min(m_field, 253u)));
     const float2 r_down = both(power_of_two(254 - (int)min(r_field, 253u)));
@@ -430,16 +437,8 @@ __device__ __forceinline__ void step8(const Moments &p, const Entry &e, const St
         const float2 y = m[h][j / 2] * m_down * both(0x1p-113f), z = r[h][j / 2] * r_down * both(0x1p-113f);
         const uint32_t u = half_of(j < 2 ? random[h].x : random[h].y, j);
         const uint32_t yb = __float_as_uint(j & 1 ? y.y : y.x), zb = __float_as_uint(j & 1 ? z.y : z.x);
-        mb[j] = yb * 16u + (u * 256u + 128u) + (yb & 0x80000000u);
+        mb[j] = (yb * 16u + (u * 256u + 128u)) | (yb & 0x80000000u);
         rb[j] = zb * 32u + ((u * 0x9e370000u + 0x8000u) >> 8);
-      }
-      if (m_field == 253u) {  // beyond the largest code: before the sums' carry can reach the sign
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const float x = j & 1 ? m[h][j / 2].y : m[h][j / 2].x;
-          const uint32_t size = mb[j] - (__float_as_uint(x) & 0x80000000u);
-          mb[j] = min(size, 0x7effffffu) | (__float_as_uint(x) & 0x80000000u);
-        }
       }
       const uint32_t mo = upper_bytes(mb[0], mb[1], mb[2], mb[3]);
       uint32_t ro = upper_bytes(rb[0], rb[1], rb[2], rb[3]);
