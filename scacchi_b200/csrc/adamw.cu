@@ -31,14 +31,17 @@
 //
 // Device times, by graph replays: 50.4 M float32 weights and gradients with
 // 32-bit moments 212 us (6.7 TB/s, the copy's rate); 67.1 M bfloat16 weights and
-// gradients with moments of 8 bits 223 us (3.0 TB/s; 104 us at a copy's rate),
-// with float32 weights 210 us (4.5 TB/s); reading 8-bit moments out 62 us
-// (6.5 TB/s).  The norm of 67.1 M bfloat16 gradients 27 us (4.9 TB/s), of 50.4 M
-// float32 33 us (6.1 TB/s); 66 small tensors 6 us.
+// gradients with moments of 8 bits 228 us (2.9 TB/s; 104 us at a copy's rate),
+// with float32 weights 206 us (4.6 TB/s); reading 8-bit moments out 62 us
+// (6.5 TB/s).  The norm of 67.1 M bfloat16 gradients 28 us (4.7 TB/s), of 50.4 M
+// float32 33 us (6.1 TB/s), off their 16-byte boundaries 39 us and (67.1 M) 45;
+// 66 small tensors 6 us.
 //
-// 32-bit moments are bound by memory.  Those of 8 bits issue 100 instructions
-// an element on 80 % of the cycles, the pipe of logic and additions 69 % busy: 19
-// are the random bits', the rest decoding, roots, quotients and encoding.
+// 32-bit moments are bound by memory.  Those of 8 bits are bound by the
+// instructions of this implementation, 101 an element (94 with float32 weights)
+// on 80 % of the cycles, the pipe of logic and additions 69 % busy: 19 are the
+// random bits', which the definition asks for, the rest decoding, roots, quotients
+// and encoding, of which nothing says that it takes so many.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

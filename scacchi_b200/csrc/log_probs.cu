@@ -23,11 +23,11 @@
 // ranked by counting.  Where more than kCandidates elements reach L (many equal
 // ones) the CTA takes the maximum below the last one k times.
 //
-// Device times, by graph replays: 4096 rows of 32000 bf16 58 us (4.5 TB/s), with
-// the 20 best 69, with a mask 96 and 112; the same of fp32 86 us (6.1 TB/s) and
-// 101.  262144 rows of 82 fp32 20 us (4.3 TB/s), with the 4 best 33, with a mask
-// 28 and 46.  8 rows of 131071 fp32 with the 20 best 9 us.  Gradients: 4096 x
-// 32000 bf16 79 us (6.6 TB/s), with a mask 96; 262144 x 82 fp32 with a mask 46 us
+// Device times, by graph replays: 4096 rows of 32000 bf16 59 us (4.5 TB/s), with
+// the 20 best 70, with a mask 96 and 112; of fp16 64 and 73; of fp32 86 us (6.1
+// TB/s) and 101.  262144 rows of 82 fp32 20 us (4.3 TB/s), with the 4 best 34, with
+// a mask 29 and 47.  8 rows of 131071 fp32 with the 20 best 8 us.  Gradients: 4096 x
+// 32000 bf16 79 us (6.6 TB/s), with a mask 95; 262144 x 82 fp32 with a mask 46 us
 // (4.3 TB/s).
 //
 // Long rows of fp32 and long gradients are bound by memory.  Long bf16 rows
@@ -63,8 +63,11 @@ constexpr int kThreads = 256;
 constexpr int kLong = 128;
 constexpr int kWarps = kLong / 32;
 constexpr int kMaxShort = 512;      // actions of a short row
-// and, where there are eight rows an SM at least, of a row that still goes that way: 20000 x 1000
-// bf16 with 20 best 57 us (131 as long rows), its gradient 22 (41); 5000 x 4000 62 (34) and 24 (15)
+// and, where there are eight rows an SM at least, of a row that still goes that way.  bf16 this way, and as
+// long rows, without best actions, with 4 and with 20: 20000 x 1000 17, 27 and 57 us (80, 124 and 135), x 2048
+// 32, 46 and 98 (80, 124 and 134), x 2500 37, 57 and 122 (81, 126 and 136), x 4000 63, 98 and 214 (82, 127 and
+// 136); 1184 x 1000 4, 7 and 16 (8, 11 and 12), x 2048 5, 8 and 17 (8, 11 and 12).  fp32 20000 x 2048 39, 66 and
+// 158 (69, 114 and 122).  Gradients: 20000 x 1000 bf16 24 (41), fp32 33 (41), 1184 x 1000 bf16 4.2 (3.8).
 constexpr int kMaxMany = 2048, kMaxManyGradient = 1024;
 constexpr int kMaxActions = SCACCHI_MAX_ACTIONS;
 constexpr int kMaxTop = SCACCHI_MAX_TOP;
@@ -831,6 +834,11 @@ __device__ __forceinline__ void candidate(Shared *home, int turn, float v, float
   }
 }
 
+// A row with more than kCandidates elements at the limit is read `top` times by
+// its cluster's first CTA: 4096 x 32000 bf16 of equal logits with 1, 5 and 20 best
+// 0.71, 0.99 and 2.6 ms (other logits with 20: 70 us), 8 x 131071 fp32 0.24, 0.40
+// and 1.0.
+//
 // The row's numbers and its best actions, by the first CTA.  What it reads of
 // `sh` is written again after the next row's exchange, where all its threads meet.
 template <typename T, bool Masked>
@@ -961,6 +969,7 @@ __global__ void __launch_bounds__(kLong, kLongCtas<Masked>) long_kernel(const __
     begun = true;
     float largest = exchange(sh, a.top, ctas, rank, groups);
     // a row masked throughout by low values, or with an infinity or near it: element by element, as they are
+    // (4096 x 32000 bf16 with a mask, of which one row in 64 has nothing left, 119 us for 96)
     const bool plain = largest >= kLow && largest <= kHigh;
     if (!plain) {
       a.top = odd >= 0 ? slice.element(odd) : -INFINITY;

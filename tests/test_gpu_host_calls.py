@@ -69,7 +69,7 @@ def test_what_the_library_refuses_is_left_to_python(failing):
 
 
 def _calls():
-    """(host function, arguments that it must decline, the public call) each; the Python way refuses or converts them."""
+    """(host function, arguments that it must decline, the public call, which refuses them) each."""
     x, k = torch.zeros((3, 5), device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
     out, one = policy_log_probs(x, k), torch.ones(3, device="cuda")
     legal = torch.ones((3, 5), dtype=torch.bool, device="cuda")
@@ -122,8 +122,10 @@ def test_steps_that_python_refuses_the_extension_declines(cuda):
                 norm, rate)
 
     bad = [(opt, dict(grads={"a": g})) for g in (good[:9], good.double(), good.cpu(), good.view(100), 1.0, w)]
-    bad += [(opt, dict(grads={"b": good})), (opt, dict(grads={"a": good, "b": good})), (opt, dict(grads={"a": good}, norm=one))]
-    bad += [(opt, dict(grads={"a": good}, rate=r)) for r in (math.nan, math.inf, one.cpu(), one.double(), good, w[0, 0])]
+    bad += [(opt, dict(grads=g)) for g in ({"b": good}, {"a": good, "b": good})]
+    bad += [(opt, dict(grads={"a": good}, norm=one))]
+    rates = (math.nan, math.inf, one.cpu(), one.double(), good, w[0, 0])
+    bad += [(opt, dict(grads={"a": good}, rate=r)) for r in rates]
     bad += [(clipped, dict(grads={"a": good}, norm=n)) for n in (one.cpu(), one.double(), good, 1.0)]
     for o, kw in bad:
         before = _lib.launch_count()
