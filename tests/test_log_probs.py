@@ -2,14 +2,12 @@
 before any launch (no GPU needed)."""
 
 import ctypes as C
-import os
-import re
 
 import pytest
 import torch
 
-from scacchi_b200 import _build, _lib
-from scacchi_b200.log_probs import MAX_ACTIONS, MAX_TOP, LogProbs, policy_log_probs, policy_log_probs_gradient
+from scacchi_b200 import _lib
+from scacchi_b200.log_probs import LogProbs, policy_log_probs, policy_log_probs_gradient
 
 A = 1 << 20  # a made-up aligned address: a refused call reads none
 
@@ -88,6 +86,12 @@ def test_struct_sizes():
 
 
 def test_limits_are_the_library_s():
+    import os
+    import re
+
+    from scacchi_b200 import _build
+    from scacchi_b200.log_probs import MAX_ACTIONS, MAX_TOP
+
     header = open(os.path.join(_build.ROOT, "include", "scacchi_b200.h")).read()
     for name, value in (("SCACCHI_MAX_ACTIONS", MAX_ACTIONS), ("SCACCHI_MAX_TOP", MAX_TOP)):
         assert re.findall(rf"#define {name} (\d+)", header) == [str(value)]
